@@ -1,0 +1,353 @@
+// Routing of rows (atoms, tokens) to experts: the choice of k of E experts by their logits, and the gates.
+//     key_e = logit_e + bias_e (fp32, one rounding); a logit or key of -inf closes the expert
+//     groups: the top_groups groups (of E / groups experts each) of largest key stay open
+//     chosen: the k largest keys, ties to the lowest index; expert -1 and gate 0 where no open expert is left
+//     score: softmax over the E logits, or sigmoid of each; gate_j = scale score_j / sum_chosen score, or scale score_j
+// The bias moves the choice only, not the gates.  It is added to the logits, of which both scores are monotone functions:
+// one rounded addition, so the choice does not depend on the order of a sum or the rounding of an exponential, and
+// saturated sigmoids do not tie.  Renormalised gates are a softmax over the chosen of the scores' logarithms (of the
+// logits, or of log sigmoid), so that scores that all underflow still give gates of sum scale.  A NaN logit is chosen
+// first and makes the gates NaN.
+// A row lies in LPR lanes, C consecutive logits each; k rounds of a maximum over the lanes' best keys (as integers of the
+// same order), the lowest lane with it giving its first such logit: no sort, no memory but the logits and the results.
+// Bound by the rounds' vector instructions for large k, by HBM for small k.
+#include "rowvec.h"
+
+#define MM_ROUTE_MAX_E 1024
+#define MM_ROUTE_MAX_K 32
+#define MM_ROUTE_MAX_G 64
+
+// larger key, larger integer; NaN above all, 0 for -inf (closed)
+__device__ __forceinline__ unsigned mm_route_key(float x) {
+  if (x != x) return 0xFFFFFFFFu;
+  if (x == -__builtin_inff()) return 0u;
+  const unsigned u = __float_as_uint(x + 0.f);   // -0 + 0 = +0: equal keys are equal integers
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+template <int CTRL>
+__device__ __forceinline__ unsigned mm_dpp_u(unsigned v) {
+  return (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
+}
+
+// maximum over the W lanes of a row, in every lane
+template <int W>
+__device__ __forceinline__ unsigned mm_route_max(unsigned v) {
+  if constexpr (W >= 2) v = max(v, mm_dpp_u<0xB1>(v));
+  if constexpr (W >= 4) v = max(v, mm_dpp_u<0x4E>(v));
+  if constexpr (W >= 8) v = max(v, mm_dpp_u<0x141>(v));
+  if constexpr (W >= 16) v = max(v, mm_dpp_u<0x140>(v));
+  if constexpr (W >= 32) v = max(v, (unsigned)__shfl_xor((int)v, 16));
+  if constexpr (W >= 64) v = max(v, (unsigned)__shfl_xor((int)v, 32));
+  return v;
+}
+
+// C consecutive values of a row from column c on, `none` past the last one
+template <typename T, int C>
+__device__ __forceinline__ void mm_route_load(const T* __restrict__ p, int c, int E, float none, float* v) {
+  constexpr int N = C < MMVec<T>::N ? C : MMVec<T>::N;
+  typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+#pragma unroll
+  for (int q = 0; q < C; q += N) {
+    if (c + q + N <= E) {
+      const vec x = *(const vec*)(p + c + q);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[q + i] = (float)x[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[q + i] = c + q + i < E ? (float)p[c + q + i] : none;
+    }
+  }
+}
+
+struct MMRoute {
+  long T, ldl;
+  int E, k, sigmoid, groups, top_groups, renorm;
+  float scale;
+};
+
+template <typename T, int LPR, int C>
+__global__ void __launch_bounds__(256) mm_route_fwd_kernel(MMRoute a, const T* __restrict__ logits,
+                                                           const float* __restrict__ bias, float* __restrict__ gates,
+                                                           int* __restrict__ experts) {
+  constexpr int RPB = 256 / LPR, KM = (MM_ROUTE_MAX_K + LPR - 1) / LPR;   // rows per workgroup, results per lane
+  __shared__ unsigned s_best[RPB][MM_ROUTE_MAX_G], s_open[RPB][2];
+  const int lane = threadIdx.x & (LPR - 1), sub = threadIdx.x / LPR, c0 = lane * C;
+  const long row = (long)blockIdx.x * RPB + sub;
+  const bool ok = row < a.T;
+  const long r = ok ? row : a.T - 1;
+  const float none = -__builtin_inff();
+  float x[C];
+  unsigned key[C];
+  mm_route_load<T, C>(logits + r * a.ldl, c0, a.E, none, x);
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const float b = bias && c0 + i < a.E ? bias[c0 + i] : 0.f;
+    key[i] = x[i] == none ? 0u : mm_route_key(x[i] + b);
+  }
+  if (a.groups > 1) {
+    const int gs = a.E / a.groups, g0 = c0 / gs, rem = c0 - g0 * gs;
+    for (int q = lane; q < a.groups; q += LPR) s_best[sub][q] = 0;
+    if (lane < 2) s_open[sub][lane] = 0;
+    mm_wave_lds_sync();
+    int g = g0, m = rem;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      if (c0 + i < a.E) atomicMax(&s_best[sub][g], key[i]);
+      if (++m == gs) { m = 0; ++g; }
+    }
+    mm_wave_lds_sync();
+    for (int q = lane; q < a.groups; q += LPR) {
+      const unsigned mine = s_best[sub][q];
+      int before = 0;
+      for (int o = 0; o < a.groups; ++o) {
+        const unsigned other = s_best[sub][o];
+        before += other > mine || (other == mine && o < q);
+      }
+      if (before < a.top_groups) atomicOr(&s_open[sub][q >> 5], 1u << (q & 31));
+    }
+    mm_wave_lds_sync();
+    const unsigned open0 = s_open[sub][0], open1 = s_open[sub][1];
+    g = g0;
+    m = rem;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      if (!((g < 32 ? open0 : open1) >> (g & 31) & 1)) key[i] = 0;
+      if (++m == gs) { m = 0; ++g; }
+    }
+  }
+  // softmax over all experts, where the gates keep its normalisation
+  float top = 0.f, whole = 1.f;
+  if (!a.renorm && !a.sigmoid) {
+    top = none;
+#pragma unroll
+    for (int i = 0; i < C; ++i) top = fmaxf(top, x[i]);
+    top = mm_lanes_max<LPR>(top);
+    whole = 0.f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) whole += expf(x[i] - top);   // rows with nothing open have no gate that uses it
+    whole = mm_lanes_sum<LPR>(whole);
+  }
+  unsigned best = 0;
+#pragma unroll
+  for (int i = 0; i < C; ++i) best = max(best, key[i]);
+  float xj[KM];
+  int ej[KM];
+#pragma unroll
+  for (int q = 0; q < KM; ++q) {
+    xj[q] = none;
+    ej[q] = -1;
+  }
+  const int first_lane = (threadIdx.x & 63) & ~(LPR - 1);
+  for (int j = 0; j < a.k; ++j) {
+    const unsigned m = mm_route_max<LPR>(best);
+    if (__ballot(m != 0) == 0) break;   // no row of the wave has an open expert left
+    const unsigned long long have = __ballot(best == m) >> first_lane;
+    const int src = __ffsll((unsigned long long)have) - 1;   // the lane of this row with the lowest such index
+    // every lane's first logit of its best key
+    float xb = 0.f;
+    int ib = 0;
+#pragma unroll
+    for (int i = C - 1; i >= 0; --i)
+      if (key[i] == best) {
+        xb = x[i];
+        ib = i;
+      }
+    const float xw = __shfl(xb, src, LPR);
+    const int ew = __shfl(c0 + ib, src, LPR);
+    if (m != 0) {
+#pragma unroll
+      for (int q = 0; q < KM; ++q)
+        if (j == q * LPR + lane) {
+          xj[q] = xw;
+          ej[q] = ew;
+        }
+    }
+    if (lane == src) {
+      best = 0;
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        if (i == ib) key[i] = 0;
+        best = max(best, key[i]);
+      }
+    }
+  }
+  float gj[KM];
+  if (a.renorm) {
+    float m = none, sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < KM; ++q) {
+      gj[q] = a.sigmoid ? fminf(xj[q], 0.f) - log1pf(expf(-fabsf(xj[q]))) : xj[q];
+      if (xj[q] != xj[q]) gj[q] = xj[q];   // fminf drops a NaN
+      if (ej[q] >= 0) m = fmaxf(m, gj[q]);
+    }
+    m = mm_lanes_max<LPR>(m);
+#pragma unroll
+    for (int q = 0; q < KM; ++q) {
+      gj[q] = ej[q] >= 0 ? expf(gj[q] - m) : 0.f;
+      sum += gj[q];
+    }
+    sum = mm_lanes_sum<LPR>(sum);
+#pragma unroll
+    for (int q = 0; q < KM; ++q) gj[q] = gj[q] / sum;
+  } else {
+#pragma unroll
+    for (int q = 0; q < KM; ++q) gj[q] = a.sigmoid ? 1.f / (1.f + expf(-xj[q])) : expf(xj[q] - top) / whole;
+  }
+  if (!ok) return;
+#pragma unroll
+  for (int q = 0; q < KM; ++q) {
+    const int j = q * LPR + lane;
+    if (j >= a.k) continue;
+    gates[row * a.k + j] = ej[q] >= 0 ? a.scale * gj[q] : 0.f;
+    experts[row * a.k + j] = ej[q];
+  }
+}
+
+// dlogits from dgates, the gates and the chosen experts.  With w_j = gate_j / scale, over the chosen of a row:
+//   renormalised       d log score_j = gate_j (dgate_j - sum_i w_i dgate_i)
+//   sigmoid, plain     d log score_j = gate_j dgate_j
+//   softmax, plain     dl_e = [e chosen] gate_e dgate_e - p_e sum_j gate_j dgate_j,  p over all E logits
+// and d log score / dl = 1 (softmax, renormalised) or 1 - sigmoid(l).  The E values of a row are put together in LDS and
+// written once; the logits are read where a formula has them.  Bound by HBM.
+template <typename T, int LPR, int C>
+__global__ void __launch_bounds__(256) mm_route_bwd_kernel(MMRoute a, const T* __restrict__ logits,
+                                                           const float* __restrict__ gates,
+                                                           const int* __restrict__ experts,
+                                                           const float* __restrict__ dgates, T* __restrict__ dlogits) {
+  constexpr int RPB = 256 / LPR, KM = (MM_ROUTE_MAX_K + LPR - 1) / LPR;
+  __shared__ float s_d[RPB][LPR * C];
+  const int lane = threadIdx.x & (LPR - 1), sub = threadIdx.x / LPR, c0 = lane * C;
+  const long row = (long)blockIdx.x * RPB + sub;
+  const bool ok = row < a.T;
+  const long r = ok ? row : a.T - 1;
+  const bool plain_softmax = !a.renorm && !a.sigmoid;
+  float x[C];
+  if (plain_softmax) mm_route_load<T, C>(logits + r * a.ldl, c0, a.E, -__builtin_inff(), x);
+  float d[KM], g[KM], sum = 0.f;
+  int e[KM];
+#pragma unroll
+  for (int q = 0; q < KM; ++q) {
+    const int j = q * LPR + lane;
+    e[q] = j < a.k ? experts[r * a.k + j] : -1;
+    const bool used = (unsigned)e[q] < (unsigned)a.E;
+    g[q] = used ? gates[r * a.k + j] : 0.f;
+    d[q] = used ? dgates[r * a.k + j] : 0.f;
+    if (!used) e[q] = -1;
+    sum = fmaf(g[q], d[q], sum);
+  }
+  sum = mm_lanes_sum<LPR>(sum);
+#pragma unroll
+  for (int q = 0; q < KM; ++q) {
+    d[q] = g[q] * (a.renorm ? d[q] - sum / a.scale : d[q]);
+    if (a.sigmoid && e[q] >= 0) d[q] /= 1.f + expf((float)logits[r * a.ldl + e[q]]);
+  }
+  float v[C];
+  if (plain_softmax) {
+    float top = -__builtin_inff(), whole = 0.f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) top = fmaxf(top, x[i]);
+    top = mm_lanes_max<LPR>(top);
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      v[i] = expf(x[i] - top);
+      whole += v[i];
+    }
+    whole = mm_lanes_sum<LPR>(whole);
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = x[i] == -__builtin_inff() ? 0.f : -(v[i] / whole) * sum;
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i) s_d[sub][c0 + i] = v[i];
+  mm_wave_lds_sync();
+#pragma unroll
+  for (int q = 0; q < KM; ++q)
+    if (e[q] >= 0) s_d[sub][e[q]] += d[q];   // the chosen of a row are different experts
+  mm_wave_lds_sync();
+  if (!ok) return;
+#pragma unroll
+  for (int i = 0; i < C; ++i) v[i] = s_d[sub][c0 + i];
+  T* __restrict__ o = dlogits + row * a.E;
+  constexpr int N = C < MMVec<T>::N ? C : MMVec<T>::N;
+  typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+#pragma unroll
+  for (int q = 0; q < C; q += N) {
+    if (c0 + q + N <= a.E) {
+      vec y;
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] = (T)v[q + i];
+      *(vec*)(o + c0 + q) = y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c0 + q + i < a.E) o[c0 + q + i] = (T)v[q + i];
+    }
+  }
+}
+
+namespace {
+int route_args(const char* name, int dtype, long T, int E, int k, int scoring, int groups, int top_groups, long ldl,
+               float scale, MMRoute* a, int renorm) {
+  auto bad = [&](const char* what, int code) {
+    mm::set_error(std::string(name) + ": " + what);
+    return code;
+  };
+  if (dtype < MM_F32 || dtype > MM_F16) return bad("bad dtype", MM_EINVAL);
+  if (T < 0 || E < 1 || k < 1 || k > E || ldl < E) return bad("bad sizes", MM_EINVAL);
+  if (scoring != 0 && scoring != 1) return bad("scoring must be 0 (softmax) or 1 (sigmoid)", MM_EINVAL);
+  if (groups < 1 || E % groups || top_groups < 1 || top_groups > groups) return bad("bad groups", MM_EINVAL);
+  if (!(scale != 0.f)) return bad("scale must not be 0", MM_EINVAL);
+  if (E > MM_ROUTE_MAX_E) return bad("more than 1024 experts are not supported", MM_ERANGE);
+  if (k > MM_ROUTE_MAX_K) return bad("more than 32 experts a row are not supported", MM_ERANGE);
+  if (groups > MM_ROUTE_MAX_G) return bad("more than 64 groups are not supported", MM_ERANGE);
+  if (T > 2147483647L * 4) return bad("too many rows", MM_ERANGE);
+  *a = MMRoute{T, ldl, E, k, scoring, groups, top_groups, renorm != 0, scale};
+  return MM_OK;
+}
+}  // namespace
+
+// lanes a row and logits a lane by E: few lanes keep the rounds' lane maxima short and let a wave work on many rows,
+// until a lane's own logits cost more
+#define MM_ROUTE_SHAPES(X)  \
+  if (E <= 16) { X(4, 4) }  \
+  else if (E <= 32) { X(8, 4) } \
+  else if (E <= 64) { X(16, 4) } \
+  else if (E <= 128) { X(16, 8) } \
+  else if (E <= 256) { X(16, 16) } \
+  else if (E <= 512) { X(32, 16) } \
+  else { X(64, 16) }
+
+extern "C" int mm_route_fwd(const void* logits, long ldl, int dtype, long T, int E, int k, int scoring,
+                            const float* bias, int groups, int top_groups, int renorm, float scale, float* gates,
+                            int* experts, hipStream_t stream) {
+  MMRoute a;
+  const int rc = route_args("mm_route_fwd", dtype, T, E, k, scoring, groups, top_groups, ldl, scale, &a, renorm);
+  if (rc != MM_OK || T == 0) return rc;
+#define X(l, c)                                                                                               \
+  hipLaunchKernelGGL((mm_route_fwd_kernel<T_, l, c>), dim3((unsigned)((a.T + 256 / l - 1) / (256 / l))), dim3(256), 0, \
+                     stream, a, (const T_*)logits, bias, gates, experts);
+  if (dtype == MM_F32) { using T_ = float; MM_ROUTE_SHAPES(X) }
+  else if (dtype == MM_BF16) { using T_ = __bf16; MM_ROUTE_SHAPES(X) }
+  else { using T_ = _Float16; MM_ROUTE_SHAPES(X) }
+#undef X
+  return mm::launch_status("mm_route_fwd");
+}
+
+extern "C" int mm_route_bwd(const void* logits, long ldl, int dtype, long T, int E, int k, int scoring, int renorm,
+                            float scale, const float* gates, const int* experts, const float* dgates, void* dlogits,
+                            hipStream_t stream) {
+  MMRoute a;
+  const int rc = route_args("mm_route_bwd", dtype, T, E, k, scoring, 1, 1, ldl, scale, &a, renorm);
+  if (rc != MM_OK || T == 0) return rc;
+#define X(l, c)                                                                                               \
+  hipLaunchKernelGGL((mm_route_bwd_kernel<T_, l, c>), dim3((unsigned)((a.T + 256 / l - 1) / (256 / l))), dim3(256), 0, \
+                     stream, a, (const T_*)logits, gates, experts, dgates, (T_*)dlogits);
+  if (dtype == MM_F32) { using T_ = float; MM_ROUTE_SHAPES(X) }
+  else if (dtype == MM_BF16) { using T_ = __bf16; MM_ROUTE_SHAPES(X) }
+  else { using T_ = _Float16; MM_ROUTE_SHAPES(X) }
+#undef X
+  return mm::launch_status("mm_route_bwd");
+}

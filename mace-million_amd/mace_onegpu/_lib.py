@@ -89,6 +89,18 @@ SIGNATURES = {
     "mm_pair_forces_skin": [L, P, P, P, P, P, P],
     "mm_chunk_forces": [I, I, P, P, P, P, P, P, P],
     "mm_chunk_edge_index": [L, P, P, P, I, P, P, P],
+    # mixtures of expert blocks: layer norm, routing, the experts' products
+    "mm_layernorm_fwd": [P, L, I, L, I, P, P, I, F, P, L, P, P, P],
+    "mm_layernorm_workspace": [L, I, I, P],
+    "mm_layernorm_bwd": [P, L, P, L, I, L, I, P, I, P, P, P, L, P, P, P, P],
+    "mm_route_fwd": [P, L, I, L, I, I, I, P, I, I, I, F, P, P, P],
+    "mm_route_bwd": [P, L, I, L, I, I, I, I, F, P, P, P, P, P],
+    "mm_expert_plan_scratch": [I, I, P],
+    "mm_expert_plan": [P, I, I, P, P, P, P],
+    "mm_expert_rows": [P, L, L, I, I, I, I, I, I, P, I, I, P, P, P, P],
+    "mm_expert_combine": [P, P, P, I, L, I, I, I, I, P, P],
+    "mm_expert_combine_bwd": [P, P, P, P, L, L, I, L, I, I, I, I, P, P, P],
+    "mm_expert_wgrad": [P, L, L, P, L, L, I, I, I, I, I, I, I, P, P, P, P, P],
     # tables
     "mm_radial_mlp_f64": [I, P, P, P, P, P, I, I, I, D, I, D, P, P],
     "mm_spline_coeffs": [P, I, I, D, D, I, I, P, P],
