@@ -365,10 +365,12 @@ int mm_expert_combine(const float* rows, const float* gates, const int* experts,
  * (0 without an expert); each nullable */
 int mm_expert_combine_bwd(const float* rows, const float* gates, const int* experts, const void* x, long st, long sm,
                           int dtype, long T, int k, int M, int N, int E, void* dx, float* dgates, mm_stream_t stream);
-/* dW [E, D, F] = sum over the slots of e and the components of gate x^T dy; 0 for an expert without slots */
+/* dW [E, D, F] = sum over the slots of e and the components of gate x^T dy; 0 for an expert without slots; workspace of
+ * mm_expert_wgrad_workspace bytes (0: null) */
+int mm_expert_wgrad_workspace(int S, int M, int D, int F, int E, size_t* bytes /* HOST */);
 int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, long yt, long ym, int dtype, int S, int k, int M,
                     int D, int F, int E, const float* gates, const int* offsets, const int* order, void* dW,
-                    mm_stream_t stream);
+                    float* workspace, mm_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------- utilities */
 int mm_fill_f32(float* p, long n, float v, mm_stream_t stream);

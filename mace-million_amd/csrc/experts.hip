@@ -8,6 +8,8 @@
 // A slot whose expert lies outside [0, E) takes part nowhere.
 #include "rowvec.h"
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
 #define MM_EXPERT_MAX_E 1024
 #define MM_PLAN_WAVE 1024   // slots per wave of the plan kernels
 
@@ -160,6 +162,164 @@ __device__ __forceinline__ MMTile mm_expert_tile(const int* __restrict__ offsets
   return MMTile{-1, 0, 0};
 }
 
+// ------------------------------------------------------------------------------------------------ matrix products
+// Operands of v_mfma_f32_16x16x32 (fp32 sums): lane (i, g) = (lane & 15, lane >> 4) holds the values k = 8 g .. 8 g + 7 of
+// row (column) i.  16-bit types: one product.  float: three bf16 planes x = x0 + x1 + x2 (x0 = bf16(x), x1 = bf16(x - x0),
+// x2 = bf16(x - x0 - x1), |x - x0 - x1 - x2| <= 2^-27 |x|) and the six products a_i b_j with i + j <= 2; those left out
+// are below 3 * 2^-24 |a b|.  96 matrix cycles for 16 x 16 x 32 against 256 in fp32 products.
+template <typename T>
+struct MMFrag {
+  typedef T vec __attribute__((ext_vector_type(8)));
+  vec v;
+};
+template <>
+struct MMFrag<float> {
+  bf16x8 v[3];
+};
+
+__device__ __forceinline__ void mm_mma(floatx4& c, const MMFrag<__bf16>& a, const MMFrag<__bf16>& b) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mm_mma(floatx4& c, const MMFrag<_Float16>& a, const MMFrag<_Float16>& b) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mm_mma(floatx4& c, const MMFrag<float>& a, const MMFrag<float>& b) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[2], b.v[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[1], b.v[1], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[0], b.v[2], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[1], b.v[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[0], b.v[1], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[0], b.v[0], c, 0, 0, 0);
+}
+
+__device__ __forceinline__ MMFrag<float> mm_split(const float* x) {
+  MMFrag<float> f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __bf16 h = (__bf16)x[i];
+    const float r = x[i] - (float)h;
+    const __bf16 l = (__bf16)r;
+    f.v[0][i] = h;
+    f.v[1][i] = l;
+    f.v[2][i] = (__bf16)(r - (float)l);
+  }
+  return f;
+}
+
+// Tiles in LDS, in units of 16 bytes.  MM_TILE_K<T> values of the summed index a stage.
+//   KC (the summed index contiguous in memory): a row of 8 units (128 bytes), unit u of row r at 8 r + (u ^ (r & 7)): the
+//   16 rows of an operand read spread over all banks.
+//   NC (the other index contiguous): a row per value of the summed index, UPR units; unit u of row q at UPR q + (u ^ s(q)),
+//   s(q) chosen so that the rows read together lie in different banks.  16-bit operands come out of it by transposing
+//   reads (ds_read_b64_tr_b16: 16 lanes give the addresses of a 4 x 16 block, four lanes a row, and lane i receives its
+//   column i), float operands value by value.
+// Staged by loads straight into LDS (16 bytes a lane, the wave's units in order, so the swizzle is in the addresses of
+// the sources) where the units are aligned, else through registers.
+template <typename T>
+constexpr int MM_TILE_K = 128 / sizeof(T);
+
+typedef __attribute__((address_space(3))) void* mm_lds_ptr;
+typedef const __attribute__((address_space(1))) void* mm_global_ptr;
+
+__device__ uint4 mm_zero_unit;   // source of units outside the operands (zero-initialised, never written)
+
+template <typename T, int UPR>
+__device__ __forceinline__ int mm_nc_swizzle(int q) {
+  if constexpr (sizeof(T) == 2) return ((q & 3) | (q >> 3 & 1) << 2) << 1 & (UPR - 1);
+  else return (q >> 3 & 3) << 2 & (UPR - 1);
+}
+
+// operand rows n0 + i, values 32 s + 8 g .. of a KC tile
+template <typename T>
+__device__ __forceinline__ MMFrag<T> mm_frag_kc(const uint4* tile, int n0, int s, int lane) {
+  const int r = n0 + (lane & 15), g = lane >> 4;
+  if constexpr (sizeof(T) == 2) {
+    MMFrag<T> f;
+    f.v = __builtin_bit_cast(typename MMFrag<T>::vec, tile[8 * r + ((4 * s + g) ^ (r & 7))]);
+    return f;
+  } else {
+    float x[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const floatx4 v = __builtin_bit_cast(floatx4, tile[8 * r + ((2 * g + h) ^ (r & 7))]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * h + i] = v[i];
+    }
+    return mm_split(x);
+  }
+}
+
+// operand columns n0 + i, values 32 s + 8 g .. of an NC tile
+template <typename T, int UPR>
+__device__ __forceinline__ MMFrag<T> mm_frag_nc(const uint4* tile, int n0, int s, int lane) {
+  const int i = lane & 15, g = lane >> 4;
+  if constexpr (sizeof(T) == 2) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    s4 h[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int q = 32 * s + 8 * g + 4 * b + (i >> 2);
+      const char* p = (const char*)&tile[UPR * q + ((n0 / 8 + (i >> 1 & 1)) ^ mm_nc_swizzle<T, UPR>(q))] + 8 * (i & 1);
+      h[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
+    }
+    MMFrag<T> f;
+    f.v = __builtin_bit_cast(typename MMFrag<T>::vec, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    return f;
+  } else {
+    float x[8];
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const int q = 8 * g + b, n = n0 + i;
+      x[b] = ((const float*)&tile[UPR * q + ((n >> 2) ^ mm_nc_swizzle<T, UPR>(q))])[n & 3];
+    }
+    return mm_split(x);
+  }
+}
+
+// A thread's share of staging one tile: NU units, unit number tid + 256 j.  DMA: straight into LDS.
+template <typename T, int NU, bool DMA>
+struct MMStage {
+  uint4 v[DMA ? 1 : NU];
+
+  // unit j from p (left = values of T left at p; none: zeros)
+  __device__ __forceinline__ void load(uint4* tile, int j, const T* p, int left) {
+    constexpr int N = MMVec<T>::N;
+    if constexpr (DMA) {
+      const void* src = left > 0 ? (const void*)p : (const void*)&mm_zero_unit;
+      __builtin_amdgcn_global_load_lds((mm_global_ptr)src, (mm_lds_ptr)(tile + 256 * j + (threadIdx.x & ~63)), 16, 0, 0);
+    } else {
+      typename MMVec<T>::type x;
+      if (left >= N) {
+        x = *(const typename MMVec<T>::type*)p;
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = i < left ? p[i] : (T)0.f;
+      }
+      v[j] = __builtin_bit_cast(uint4, x);
+    }
+  }
+  __device__ __forceinline__ void put(uint4* tile) {
+    if constexpr (!DMA) {
+#pragma unroll
+      for (int j = 0; j < NU; ++j) tile[256 * j + threadIdx.x] = v[j];
+    }
+  }
+};
+
+// every load into LDS of this wave has arrived, and every wave's (and its LDS accesses are done)
+__device__ __forceinline__ void mm_stage_done() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// Workgroups are dealt out to the 8 XCDs in turn: number them so that an XCD gets consecutive work, whose operands its L2
+// then holds.
+__device__ __forceinline__ int mm_xcd_order(int b, int n) {
+  const int per = n / 8, rest = n % 8, x = b % 8, i = b / 8;
+  return x < rest ? x * (per + 1) + i : x * per + rest + i;
+}
+
 // ------------------------------------------------------------------------------------------------ rows
 struct MMRows {
   const void *in, *W;
@@ -169,51 +329,93 @@ struct MMRows {
   int k, M, K, N, E;
 };
 
-// 64 x 64 tiles, 4 x 4 values a thread, fp32 products and sums.  TRANS: W[e] is [N][K], else [K][N].
-template <typename T, bool TRANS>
-__global__ void __launch_bounds__(256) mm_expert_rows_kernel(MMRows a) {
-  __shared__ float As[16][68], Bs[16][68];
-  __shared__ long s_in[64], s_out[64];
-  const MMTile t = mm_expert_tile(a.offsets, a.E, a.M, 64, blockIdx.x);
+// A workgroup: a tile of 128 rows of one expert by 128 columns, its 4 waves 64 x 64 each, two stages in LDS: the next stage
+// is on its way while this one is multiplied.  The weights are the first operand, so that a lane ends with 4 consecutive
+// columns of a row.  TRANS: W[e] is [N][K], else [K][N].
+template <typename T, bool TRANS, bool DMA>
+__global__ void __launch_bounds__(256, 2) mm_expert_rows_kernel(MMRows a, int tiles_n) {
+  constexpr int BK = MM_TILE_K<T>, N = MMVec<T>::N, UPR = 128 / N, KS = BK / 32;
+  __shared__ uint4 As[2][1024], Bs[2][1024];
+  __shared__ long s_out[128];
+  const int at = mm_xcd_order(blockIdx.x, gridDim.x), n0 = at % tiles_n * 128;
+  const MMTile t = mm_expert_tile(a.offsets, a.E, a.M, 128, at / tiles_n);
   if (t.e < 0) return;
-  const int tid = threadIdx.x, n0 = blockIdx.y * 64;
-  if (tid < 64) {
-    const int r = t.row0 + min(tid, t.rows - 1), p = r / a.M, m = r - p * a.M;
-    const int slot = a.order[a.offsets[t.e] + p];
-    s_in[tid] = (slot / a.k) * a.st + m * a.sm;
-    s_out[tid] = ((long)slot * a.M + m) * a.N;
-  }
-  __syncthreads();
-  const T* __restrict__ in = (const T*)a.in;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const T* __restrict__ W = (const T*)a.W + (size_t)t.e * a.K * a.N;
-  float acc[4][4] = {};
-  const int tr = tid >> 4, tc = tid & 15;
-  for (int k0 = 0; k0 < a.K; k0 += 16) {
+  const int* __restrict__ list = a.order + a.offsets[t.e];
+  if (tid < 128) {
+    const int r = t.row0 + min(tid, t.rows - 1), p = r / a.M, m = r - p * a.M;
+    s_out[tid] = ((long)list[p] * a.M + m) * a.N;
+  }
+  // sources of this thread's units: row pu / 8 of the tile, unit (pu & 7) ^ (row & 7)
+  const T *pa[4], *pb[4];
+  int kb[4], nb[4];   // B: TRANS: columns n0 + row, k as A's; else k row and values left in that row
+  const int ka = ((tid & 7) ^ (tid >> 3 & 7)) * N;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int kk = tid & 15, r = (tid >> 4) + 16 * q;
-      As[kk][r] = k0 + kk < a.K ? (float)in[s_in[r] + k0 + kk] : 0.f;
-      if (TRANS) {
-        const int n = n0 + r;
-        Bs[kk][r] = k0 + kk < a.K && n < a.N ? (float)W[(size_t)n * a.K + k0 + kk] : 0.f;
-      } else {
-        const int kb = (tid >> 6) + 4 * q, n = n0 + (tid & 63);
-        Bs[kb][tid & 63] = k0 + kb < a.K && n < a.N ? (float)W[(size_t)(k0 + kb) * a.N + n] : 0.f;
-      }
+  for (int j = 0; j < 4; ++j) {
+    const int pu = tid + 256 * j, row = pu >> 3;
+    const int r = t.row0 + min(row, t.rows - 1), p = r / a.M, m = r - p * a.M;
+    pa[j] = (const T*)a.in + (long)(list[p] / a.k) * a.st + m * a.sm + ka;
+    if constexpr (TRANS) {
+      const int n = n0 + row;
+      nb[j] = n < a.N;
+      kb[j] = ka;
+      pb[j] = W + (size_t)min(n, a.N - 1) * a.K + ka;
+    } else {
+      const int q = pu / UPR, u = (pu % UPR) ^ mm_nc_swizzle<T, UPR>(q);
+      kb[j] = q;
+      nb[j] = a.N - n0 - u * N;
+      pb[j] = W + (size_t)q * a.N + n0 + u * N;
     }
-    __syncthreads();
+  }
+  MMStage<T, 4, DMA> sa, sb;
+  auto load = [&](int k0, int buf) {
 #pragma unroll
-    for (int kk = 0; kk < 16; ++kk)
+    for (int j = 0; j < 4; ++j) sa.load(As[buf], j, pa[j] + k0, a.K - k0 - ka);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (TRANS) sb.load(Bs[buf], j, pb[j] + k0, nb[j] ? a.K - k0 - kb[j] : 0);
+      else sb.load(Bs[buf], j, pb[j] + (size_t)k0 * a.N, k0 + kb[j] < a.K ? nb[j] : 0);
+    }
+  };
+  floatx4 acc[4][4] = {};   // [columns][rows]
+  const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+  load(0, 0);
+  sa.put(As[0]);
+  sb.put(Bs[0]);
+  mm_stage_done();
+  int buf = 0;
+  for (int k0 = 0; k0 < a.K; k0 += BK) {
+    const bool more = k0 + BK < a.K;
+    if (more) load(k0 + BK, buf ^ 1);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      MMFrag<T> fa[4], fb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (TRANS) fb[i] = mm_frag_kc<T>(Bs[buf], wn + 16 * i, s, lane);
+        else fb[i] = mm_frag_nc<T, UPR>(Bs[buf], wn + 16 * i, s, lane);
+        fa[i] = mm_frag_kc<T>(As[buf], wm + 16 * i, s, lane);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(As[kk][tr * 4 + i], Bs[kk][tc * 4 + j], acc[i][j]);
-    __syncthreads();
+        for (int j = 0; j < 4; ++j) mm_mma(acc[i][j], fb[i], fa[j]);
+    }
+    if (more) {
+      sa.put(As[buf ^ 1]);
+      sb.put(Bs[buf ^ 1]);
+    }
+    mm_stage_done();
+    buf ^= 1;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (tr * 4 + i >= t.rows) continue;
-    mm_store_vec(a.out + s_out[tr * 4 + i], n0 + tc * 4, a.N, acc[i]);
+  for (int j = 0; j < 4; ++j) {
+    const int m = wm + 16 * j + (lane & 15);
+    if (m >= t.rows) continue;
+    float* __restrict__ o = a.out + s_out[m];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mm_store_vec(o, n0 + wn + 16 * i + 4 * (lane >> 4), a.N, (const float*)&acc[i][j]);
   }
 }
 
@@ -302,45 +504,147 @@ struct MMWgrad {
   int k, M, D, F, E;
 };
 
-// a workgroup: one 64 x 64 tile of dW[e] over all rows of expert e, 16 rows at a time in the order of the plan
-template <typename T>
-__global__ void __launch_bounds__(256) mm_expert_wgrad_kernel(MMWgrad a) {
-  __shared__ float Xs[16][68], Ys[16][68];
-  const int e = blockIdx.z, d0 = blockIdx.x * 64, f0 = blockIdx.y * 64, tid = threadIdx.x;
-  const int first = a.offsets[e], rows = (a.offsets[e + 1] - first) * a.M;
-  float acc[4][4] = {};
-  const int tr = tid >> 4, tc = tid & 15;
-  for (int r0 = 0; r0 < rows; r0 += 16) {
+// A workgroup: a 128 x 128 tile of dW[e] over a chunk of the expert's rows (SPLIT: chunks of `chunk` rows, each into its own
+// fp32 partial sums, which mm_expert_wgrad_sum_kernel adds in order; else all rows, straight into dW).  x goes into LDS as
+// it is, dy through registers times its gate: in 16-bit types that rounds gate x dy to the type, an error of the size that
+// dy's own rounding has.  Rows past the end are zeros on both sides.
+#define MM_WG_ROWS 512   // rows whose offsets are kept in LDS at a time
+
+template <typename T, bool SPLIT, bool DMA>
+__global__ void __launch_bounds__(256, 2) mm_expert_wgrad_kernel(MMWgrad a, int chunk, int tiles_f, int tiles_df,
+                                                                 float* __restrict__ part) {
+  constexpr int BK = MM_TILE_K<T>, N = MMVec<T>::N, UPR = 128 / N, KS = BK / 32;
+  __shared__ uint4 Xs[2][1024], Ys[2][1024];
+  __shared__ long s_x[MM_WG_ROWS], s_y[MM_WG_ROWS];
+  __shared__ float s_g[MM_WG_ROWS];
+  const int at = mm_xcd_order(blockIdx.x, gridDim.x), tile = at / tiles_df, df = at % tiles_df;
+  MMTile t;
+  if constexpr (SPLIT) t = mm_expert_tile(a.offsets, a.E, a.M, chunk, tile);
+  else t = MMTile{tile, 0, (a.offsets[tile + 1] - a.offsets[tile]) * a.M};
+  if (t.e < 0) return;
+  const int d0 = df / tiles_f * 128, f0 = df % tiles_f * 128;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int* __restrict__ list = a.order + a.offsets[t.e];
+  int q[4], left_d[4], left_f[4], col[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int rr = (tid >> 6) + 4 * q, c = tid & 63, r = r0 + rr;
-      float xv = 0.f, yv = 0.f;
-      if (r < rows) {
-        const int p = r / a.M, m = r - p * a.M, slot = a.order[first + p];
-        const long t = slot / a.k;
-        if (d0 + c < a.D) xv = (float)((const T*)a.x)[t * a.xt + m * a.xm + d0 + c];
-        if (f0 + c < a.F) yv = (float)((const T*)a.dy)[t * a.yt + m * a.ym + f0 + c] * (a.gates ? a.gates[slot] : 1.f);
+  for (int j = 0; j < 4; ++j) {
+    const int pu = tid + 256 * j;
+    q[j] = pu / UPR;
+    col[j] = ((pu % UPR) ^ mm_nc_swizzle<T, UPR>(q[j])) * N;
+    left_d[j] = a.D - d0 - col[j];
+    left_f[j] = a.F - f0 - col[j];
+  }
+  MMStage<T, 4, DMA> sx;
+  MMStage<T, 4, false> sy;
+  float gy[4];
+  auto load = [&](int r0, int buf) {   // rows r0 .. r0 + BK of the chunk, within one block of offsets
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in = r0 + q[j] < t.rows;
+      const int r = (r0 + q[j]) & (MM_WG_ROWS - 1);
+      sx.load(Xs[buf], j, (const T*)a.x + (in ? s_x[r] : 0) + d0 + col[j], in ? left_d[j] : 0);
+      sy.load(Ys[buf], j, (const T*)a.dy + (in ? s_y[r] : 0) + f0 + col[j], in ? left_f[j] : 0);
+      gy[j] = in ? s_g[r] : 0.f;
+    }
+  };
+  auto put = [&](int buf) {
+    sx.put(Xs[buf]);
+    if (a.gates) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        typename MMVec<T>::type v = __builtin_bit_cast(typename MMVec<T>::type, sy.v[j]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (T)(gy[j] * (float)v[i]);
+        sy.v[j] = __builtin_bit_cast(uint4, v);
       }
-      Xs[rr][c] = xv;
-      Ys[rr][c] = yv;
+    }
+    sy.put(Ys[buf]);
+  };
+  auto rows_of = [&](int r0) {
+    for (int i = tid; i < MM_WG_ROWS && r0 + i < t.rows; i += 256) {
+      const int r = t.row0 + r0 + i, p = r / a.M, m = r - p * a.M, slot = list[p];
+      const long tok = slot / a.k;
+      s_x[i] = tok * a.xt + m * a.xm;
+      s_y[i] = tok * a.yt + m * a.ym;
+      s_g[i] = a.gates ? a.gates[slot] : 1.f;
     }
     __syncthreads();
+  };
+  floatx4 acc[4][4] = {};   // [f][d]
+  const int wd = (wave & 1) * 64, wf = (wave >> 1) * 64;
+  if (t.rows > 0) {
+    rows_of(0);
+    load(0, 0);
+    put(0);
+    mm_stage_done();
+  }
+  int buf = 0;
+  for (int r0 = 0; r0 < t.rows; r0 += BK) {
+    const int next = r0 + BK;
+    const bool more = next < t.rows;
+    if (more) {
+      if (next % MM_WG_ROWS == 0) rows_of(next);   // the previous block's offsets are used up (barrier of the last step)
+      load(next, buf ^ 1);
+    }
 #pragma unroll
-    for (int kk = 0; kk < 16; ++kk)
+    for (int s = 0; s < KS; ++s) {
+      MMFrag<T> fd[4], ff[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ff[i] = mm_frag_nc<T, UPR>(Ys[buf], wf + 16 * i, s, lane);
+        fd[i] = mm_frag_nc<T, UPR>(Xs[buf], wd + 16 * i, s, lane);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(Xs[kk][tr * 4 + i], Ys[kk][tc * 4 + j], acc[i][j]);
-    __syncthreads();
-  }
-  T* __restrict__ o = (T*)a.dW + (size_t)e * a.D * a.F;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = d0 + tr * 4 + i, f = f0 + tc * 4 + j;
-      if (d < a.D && f < a.F) o[(size_t)d * a.F + f] = (T)acc[i][j];
+        for (int j = 0; j < 4; ++j) mm_mma(acc[i][j], ff[i], fd[j]);
     }
+    if (more) put(buf ^ 1);
+    mm_stage_done();
+    buf ^= 1;
+  }
+  const size_t base = SPLIT ? (size_t)tile * a.D * a.F : (size_t)t.e * a.D * a.F;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int d = d0 + wd + 16 * j + (lane & 15);
+    if (d >= a.D) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int f = f0 + wf + 16 * i + 4 * (lane >> 4);
+      if constexpr (SPLIT) {
+        mm_store_vec(part + base + (size_t)d * a.F, f, a.F, (const float*)&acc[i][j]);
+      } else {
+        T* __restrict__ o = (T*)a.dW + base + (size_t)d * a.F;
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (f + v < a.F) o[f + v] = (T)acc[i][j][v];
+      }
+    }
+  }
+}
+
+// dW[e] = the partial sums of the expert's chunks, in order
+template <typename T>
+__global__ void __launch_bounds__(256) mm_expert_wgrad_sum_kernel(MMWgrad a, int chunk, const float* __restrict__ part) {
+  const int lane = threadIdx.x & 63, e = blockIdx.y;
+  int first = 0;   // chunks of the experts before e
+  for (int o = lane; o < e; o += 64) first += ((a.offsets[o + 1] - a.offsets[o]) * a.M + chunk - 1) / chunk;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) first += __shfl_xor(first, d);
+  const int n = ((a.offsets[e + 1] - a.offsets[e]) * a.M + chunk - 1) / chunk;
+  const long size = (long)a.D * a.F, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= size) return;
+  float t[4] = {};
+  for (int c = 0; c < n; ++c) {
+    const float* __restrict__ p = part + (size_t)(first + c) * size;
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (i + v < size) t[v] += p[i + v];
+  }
+  T* __restrict__ o = (T*)a.dW + (size_t)e * size;
+#pragma unroll
+  for (int v = 0; v < 4; ++v)
+    if (i + v < size) o[i + v] = (T)t[v];
 }
 
 // ------------------------------------------------------------------------------------------------ entry points
@@ -349,6 +653,19 @@ constexpr int kPlanTile = 4 * MM_PLAN_WAVE;
 
 // waves of the one workgroup that plans S slots of E experts (its counters fit 64 KB of LDS); 0: several workgroups
 int plan_waves(int S, int E) { return S <= 4 * MM_PLAN_WAVE ? 4 : S <= 16 * MM_PLAN_WAVE && E <= 512 ? 16 : 0; }
+
+// base of a matrix whose 16-byte units can be loaded straight into LDS
+bool aligned(const void* p) { return (size_t)p % 16 == 0; }
+
+// Rows per chunk of dW's sums; 0: no chunks.  A card of 256 CUs takes 512 workgroups at a time: with at least that many
+// (expert, tile) pairs none are made; else chunks for about 1024 workgroups, of 256 rows or more (a chunk's partial sums
+// are 64 KB per tile to write and read, 256 rows of both operands 128 KB or more).
+int wgrad_chunk(long rows, int D, int F, int E) {
+  const long tiles = (long)((D + 127) / 128) * ((F + 127) / 128);
+  if (E * tiles >= 512 || rows < 512) return 0;
+  const long c = (rows * tiles + 1023) / 1024;
+  return (int)(c < 256 ? 256 : (c + 63) / 64 * 64);
+}
 
 int range_error(const char* name, const char* what) {
   mm::set_error(std::string(name) + ": " + what);
@@ -392,15 +709,22 @@ extern "C" int mm_expert_rows(const void* in, long st, long sm, int dtype, int S
                               hipStream_t stream) {
   MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");
   MM_CHECK_ARG(S >= 0 && k >= 1 && M >= 1 && K >= 1 && N >= 1 && E >= 1 && st >= 0 && sm >= 0, "bad sizes");
-  if ((long)S * M > 2147483647L - 64) return range_error("mm_expert_rows", "2^31 rows or more are not supported");
+  if ((long)S * M > 2147483647L - 128) return range_error("mm_expert_rows", "2^31 rows or more are not supported");
   if (S == 0) return MM_OK;
   const MMRows a{in, W, offsets, order, out, st, sm, k, M, K, N, E};
+  const int tiles_n = (N + 127) / 128;
   // every expert's list may end in a cut tile
-  const dim3 grid((unsigned)(((long)S * M + 63) / 64 + (E < S ? E : S)), (unsigned)((N + 63) / 64));
-  if (transposed)
-    MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_rows_kernel<T, true>), grid, dim3(256), 0, stream, a));
-  else
-    MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_rows_kernel<T, false>), grid, dim3(256), 0, stream, a));
+  const long wg = (((long)S * M + 127) / 128 + (E < S ? E : S)) * tiles_n;
+  if (wg > 2147483647L) return range_error("mm_expert_rows", "output too large for one launch");
+  const int unit = dtype == MM_F32 ? 4 : 8;
+  const bool dma = aligned(in) && aligned(W) && st % unit == 0 && (M == 1 || sm % unit == 0) &&
+                   K % unit == 0 && (transposed || N % unit == 0);
+#define CALL(trans, dma) \
+  MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_rows_kernel<T, trans, dma>), dim3((unsigned)wg), dim3(256), 0, stream, a, \
+                                        tiles_n))
+  if (transposed) { if (dma) CALL(true, true); else CALL(true, false); }
+  else { if (dma) CALL(false, true); else CALL(false, false); }
+#undef CALL
   return mm::launch_status("mm_expert_rows");
 }
 
@@ -439,16 +763,37 @@ extern "C" int mm_expert_combine_bwd(const float* rows, const float* gates, cons
   return mm::launch_status("mm_expert_combine_bwd");
 }
 
+extern "C" int mm_expert_wgrad_workspace(int S, int M, int D, int F, int E, size_t* bytes) {
+  MM_CHECK_ARG(S >= 0 && M >= 1 && D >= 1 && F >= 1 && E >= 1 && bytes, "bad sizes");
+  const long rows = (long)S * M, c = wgrad_chunk(rows, D, F, E);
+  *bytes = c ? (size_t)(rows / c + (E < S ? E : S)) * D * F * sizeof(float) : 0;
+  return MM_OK;
+}
+
 extern "C" int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, long yt, long ym, int dtype, int S,
                                int k, int M, int D, int F, int E, const float* gates, const int* offsets,
-                               const int* order, void* dW, hipStream_t stream) {
+                               const int* order, void* dW, float* workspace, hipStream_t stream) {
   MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");
   MM_CHECK_ARG(S >= 0 && k >= 1 && M >= 1 && D >= 1 && F >= 1 && E >= 1, "bad sizes");
   MM_CHECK_ARG(xt >= 0 && xm >= 0 && yt >= 0 && ym >= 0, "bad strides");
   if (E > MM_EXPERT_MAX_E) return range_error("mm_expert_wgrad", "more than 1024 experts are not supported");
-  if ((long)S * M > 2147483647L - 64) return range_error("mm_expert_wgrad", "2^31 rows or more are not supported");
+  if ((long)S * M > 2147483647L - 128) return range_error("mm_expert_wgrad", "2^31 rows or more are not supported");
   const MMWgrad a{x, dy, gates, offsets, order, dW, xt, xm, yt, ym, k, M, D, F, E};
-  const dim3 grid((D + 63) / 64, (F + 63) / 64, E);
-  MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_wgrad_kernel<T>), grid, dim3(256), 0, stream, a));
+  const int chunk = wgrad_chunk((long)S * M, D, F, E), tiles_f = (F + 127) / 128, tiles_df = (D + 127) / 128 * tiles_f;
+  MM_CHECK_ARG(!chunk || workspace, "workspace is null");
+  const int unit = dtype == MM_F32 ? 4 : 8;
+  const bool dma = aligned(x) && xt % unit == 0 && (M == 1 || xm % unit == 0) && D % unit == 0;
+  const long wg = (chunk ? (long)S * M / chunk + (E < S ? E : S) : E) * tiles_df;
+  if (wg > 2147483647L) return range_error("mm_expert_wgrad", "output too large for one launch");
+#define CALL(split, dma)                                                                                            \
+  MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_wgrad_kernel<T, split, dma>), dim3((unsigned)wg), dim3(256), 0, stream, \
+                                        a, chunk, tiles_f, tiles_df, workspace))
+  if (chunk) { if (dma) CALL(true, true); else CALL(true, false); }
+  else { if (dma) CALL(false, true); else CALL(false, false); }
+#undef CALL
+  if (chunk)
+    MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_wgrad_sum_kernel<T>),
+                                          dim3((unsigned)(((long)D * F + 1023) / 1024), E), dim3(256), 0, stream, a, chunk,
+                                          workspace));
   return mm::launch_status("mm_expert_wgrad");
 }

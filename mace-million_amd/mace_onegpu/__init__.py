@@ -9,6 +9,8 @@ Module map (mirrors the reference package mace_onegpu, same module paths for the
   md                MDRunner: velocity-Verlet MD with a skin neighbour list (the standalone MD-loop shape)
   make_threepass_model  writes the pickled ThreePassMLIAP model file that pair_style mliap unified loads
   fast_layers       per-chunk layer pipelines on the HIP kernels
+  layer_norm        layer_norm, LayerNorm: forward and backward kernels over the last axis
+  experts           mixtures of expert weight blocks: route, plan_experts, expert_linear
   lammps_data       periodic-image ML-IAP data object (one GPU stands in for LAMMPS' ghost exchange)
   model, o3, codegen, systems, _lib   architecture, couplings, kernel generator, inputs, C-ABI binding
 """

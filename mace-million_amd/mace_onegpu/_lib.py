@@ -100,7 +100,8 @@ SIGNATURES = {
     "mm_expert_rows": [P, L, L, I, I, I, I, I, I, P, I, I, P, P, P, P],
     "mm_expert_combine": [P, P, P, I, L, I, I, I, I, P, P],
     "mm_expert_combine_bwd": [P, P, P, P, L, L, I, L, I, I, I, I, P, P, P],
-    "mm_expert_wgrad": [P, L, L, P, L, L, I, I, I, I, I, I, I, P, P, P, P, P],
+    "mm_expert_wgrad_workspace": [I, I, I, I, I, P],
+    "mm_expert_wgrad": [P, L, L, P, L, L, I, I, I, I, I, I, I, P, P, P, P, P, P],
     # tables
     "mm_radial_mlp_f64": [I, P, P, P, P, P, I, I, I, D, I, D, P, P],
     "mm_spline_coeffs": [P, I, I, D, D, I, I, P, P],

@@ -194,8 +194,11 @@ class _ExpertLinearFn(torch.autograd.Function):
                              stream())
             K.mm_expert_combine_bwd(rows, gates, plan.experts, x, xt, xm, code, T, k, M, D, E, dx, dg, stream())
         if nw:
+            n = ctypes.c_size_t(0)
+            K.mm_expert_wgrad_workspace(T * k, M, D, F, E, ctypes.byref(n))
+            ws = torch.empty(n.value // 4, dtype=torch.float32, device=x.device) if n.value else None
             K.mm_expert_wgrad(x, xt, xm, dy, yt, ym, code, T * k, k, M, D, F, E, gates, plan.offsets, plan.order, dw,
-                              stream())
+                              ws, stream())
         return dx, dw, dg, None, None
 
 
@@ -231,7 +234,7 @@ def expert_linear(x, weight, plan, gates=None):
     flat = x.dim() == 2
     if flat:
         x = x[:, None, :]
-    if T * k * x.shape[1] > INT32_MAX - 64:
+    if T * k * x.shape[1] > INT32_MAX - 128:
         raise ValueError(f"{T * k * x.shape[1]} rows: 2^31 or more are not supported")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, gates)):
         y = _ExpertLinearFn.apply(x, weight, gates, plan, code)
