@@ -3,6 +3,7 @@
     python mace-million_amd/build.py            (also called by __graft_entry__.build())
 
 Output: mace-million_amd/lib/libmace_million_amd.so (git-ignored; it travels with the tree to the GPU box),
+lib/mm_torch_ops.so: the PyTorch functions of the operators with autograd nodes (host C++ against the installed torch),
 lib/kernel_ops.json: the fp32 operations per thread that the straight-line generated symmetric-contraction kernels
 execute, counted from their gfx950 assembly (bench.py reports their FLOP rates from it), and lib/jit/: the
 channelwise TP kernels of the path tables in o3.PREBUILT_JIT_TP_TABLES (mace_onegpu/tp_jit.py).
@@ -83,6 +84,38 @@ def _count_ops(name):
     return {k: codegen.asm_valu_flops(text, k) for k in COUNTED[name]}
 
 
+TORCH_OPS = os.path.join(LIB_DIR, "mm_torch_ops.so")
+
+
+def _build_torch_ops():
+    """lib/mm_torch_ops.so: csrc/torch/ops.cpp, host C++ against the installed torch (linked by _link_torch_ops)."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    obj = os.path.join(OBJ, "torch_ops.o")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I" + os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include"),
+           "-I" + sysconfig.get_paths()["include"], "-c", os.path.join(CSRC, "torch", "ops.cpp"), "-o", obj]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    return obj, os.path.join(root, "lib")
+
+
+def _link_torch_ops(obj, torch_lib):
+    tmp = TORCH_OPS + ".tmp"
+    cmd = ["g++", "-shared", "-o", tmp, obj, "-L" + LIB_DIR, "-l:" + os.path.basename(LIB), "-L" + torch_lib, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+           "-ltorch", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_OPS)
+
+
 def build(jobs=None, verbose=True):
     generate()
     os.makedirs(OBJ, exist_ok=True)
@@ -96,12 +129,14 @@ def build(jobs=None, verbose=True):
         counts = [ex.submit(_count_ops, n) for n in COUNTED]
         # the kernels of the tables that FusedConvTP builds on first use, made ahead for the listed tables
         jit = [ex.submit(tp_jit.build, o3.tp_table(list(a), b, c), True) for a, b, c in o3.PREBUILT_JIT_TP_TABLES]
+        torch_ops = ex.submit(_build_torch_ops)
         objs = list(ex.map(_compile, srcs))
         ops = {}
         for c in counts:
             ops.update(c.result())
         for j in jit:
             j.result()
+        torch_ops = torch_ops.result()
     import json
     with open(OPS_JSON, "w") as fh:
         json.dump(ops, fh, indent=1)
@@ -111,6 +146,7 @@ def build(jobs=None, verbose=True):
     if r.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _link_torch_ops(*torch_ops)
     shutil.rmtree(OBJ, ignore_errors=True)
     if verbose:
         print(f"built {LIB} from {len(srcs)} sources")

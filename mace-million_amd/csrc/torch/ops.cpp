@@ -1,0 +1,389 @@
+// PyTorch functions of the layer norm, routing and expert kernels: argument checks, output and workspace tensors, the
+// calls of the C ABI on torch's current stream, and their place in autograd.
+//
+// In C++ because small calls are bound by the host: with the forward and backward as Python functions, a training call took
+// 130 - 210 us whatever its kernels took, most of it the hand-over of the interpreter to autograd's thread and back.
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <ATen/ops/empty.h>
+#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPStream.h>
+
+#include <optional>
+#include <sstream>
+#include <string>
+#include <tuple>
+
+#include "../../../include/mace_million_amd.h"
+
+namespace {
+namespace py = pybind11;
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+constexpr long kInt32Max = 2147483647L;
+constexpr int kMaxDim = 16384, kMaxExperts = 1024, kMaxK = 32, kMaxGroups = 64;
+
+template <typename... A>
+std::string text(const A&... a) {
+  std::ostringstream s;
+  (s << ... << a);
+  return s.str();
+}
+
+void done(int rc) {
+  if (rc != 0) throw std::runtime_error(mm_last_error());
+}
+
+mm_stream_t stream() { return (mm_stream_t)c10::hip::getCurrentHIPStream().stream(); }
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+float* fptr(const Tensor& t) { return (float*)ptr(t); }
+int* iptr(const Tensor& t) { return (int*)ptr(t); }
+
+const char* type_name(at::ScalarType t) { return c10::toString(t); }
+
+// dtype code of a floating tensor of the current GPU
+int check_gpu(const Tensor& t, const char* name) {
+  if (!t.is_cuda()) throw py::type_error(text(name, " must be a GPU tensor"));
+  if (t.device().index() != c10::hip::current_device())
+    throw py::value_error(text(name, " is on ", t.device(), ", the current device is cuda:",
+                               (int)c10::hip::current_device()));
+  switch (t.scalar_type()) {
+    case at::kFloat: return 0;
+    case at::kBFloat16: return 1;
+    case at::kHalf: return 2;
+    default:
+      throw py::type_error(text(name, " must be float32, bfloat16 or float16, got ", type_name(t.scalar_type())));
+  }
+}
+
+Tensor f32(at::IntArrayRef size, const Tensor& like) { return at::empty(size, like.options().dtype(at::kFloat)); }
+Tensor i32(at::IntArrayRef size, const Tensor& like) { return at::empty(size, like.options().dtype(at::kInt)); }
+
+// Autograd takes absent tensors as empty optionals.
+using Maybe = std::optional<Tensor>;
+Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); }
+Tensor value(const Maybe& t) { return t ? *t : Tensor(); }
+
+bool needs_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// Gradients that raise when they are differentiated again, instead of passing for constants.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_(true);
+  auto error = std::make_shared<torch::autograd::DelayedError>(text(what, " can be differentiated once only"),
+                                                               (int64_t)grads.size());
+  return (*error)(std::move(grads));
+}
+
+// t as rows with a contiguous last axis, and the distance of rows
+std::pair<Tensor, long> as_rows(Tensor t) {
+  const long D = t.size(-1);
+  if (t.dim() != 2) t = t.reshape({-1, D});
+  if (D > 1 && t.stride(1) != 1) t = t.contiguous();
+  return {t, t.size(0) > 1 ? t.stride(0) : D};
+}
+
+// ------------------------------------------------------------------------------------------------ layer norm
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& w, const Maybe& b, double eps, int64_t code,
+                        int64_t p_code) {
+    const Tensor weight = value(w), bias = value(b);
+    Tensor stats;
+    auto [x2, ldx] = as_rows(x);
+    Tensor y = run(x, x2, ldx, weight, bias, eps, (int)code, (int)p_code, &stats);
+    ctx->save_for_backward({x2, weight, stats});
+    ctx->saved_data["bias"] = bias.defined();
+    ctx->saved_data["codes"] = code * 4 + p_code;
+    ctx->saved_data["ldx"] = (int64_t)ldx;
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return y;
+  }
+
+  static Tensor run(const Tensor& x, const Tensor& x2, long ldx, const Tensor& weight, const Tensor& bias, double eps,
+                    int code, int p_code, Tensor* stats) {
+    const long rows = x2.size(0), D = x2.size(1);
+    Tensor y = at::empty(x.sizes(), x.options());
+    const Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+    if (stats) *stats = f32({2, rows}, x);
+    float* mean = stats ? fptr(*stats) : nullptr;
+    done(mm_layernorm_fwd(ptr(x2), ldx, code, rows, (int)D, ptr(w), ptr(b), p_code, (float)eps, ptr(y), D, mean,
+                          mean ? mean + rows : nullptr, stream()));
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
+    const int64_t codes = ctx->saved_data["codes"].toInt();
+    const int code = (int)(codes / 4), p_code = (int)(codes % 4);
+    const long rows = x.size(0), D = x.size(1), ldx = ctx->saved_data["ldx"].toInt();
+    auto [dy, lddy] = as_rows(grads[0]);
+    Tensor dx, dw, db, ws;
+    if (ctx->needs_input_grad(0)) dx = at::empty(ctx->saved_data["shape"].toIntVector(), x.options());
+    const auto p_type = p_code == 0 ? at::kFloat : x.scalar_type();
+    const int at_bias = weight.defined() ? 2 : 1;   // autograd counts the tensors that are there
+    if (weight.defined() && ctx->needs_input_grad(1)) dw = at::empty({D}, x.options().dtype(p_type));
+    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(at_bias)) db = at::empty({D}, x.options().dtype(p_type));
+    if (dw.defined() || db.defined()) {
+      size_t bytes = 0;
+      done(mm_layernorm_workspace(rows, (int)D, code, &bytes));
+      ws = f32({(int64_t)(bytes / sizeof(float))}, x);
+    }
+    const Tensor w = weight.defined() ? weight.contiguous() : weight;
+    const float* mean = fptr(stats);
+    done(mm_layernorm_bwd(ptr(dy), lddy, ptr(x), ldx, code, rows, (int)D, ptr(w), p_code, mean, mean + rows, ptr(dx), D,
+                          ptr(dw), ptr(db), fptr(ws), stream()));
+    return once({dx, dw, db, Tensor(), Tensor(), Tensor()}, "layer_norm");
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, double eps) {
+  const int code = check_gpu(x, "x");
+  if (x.dim() < 1 || x.size(-1) == 0)
+    throw py::value_error(text("x must be [..., D] with D > 0, got ", x.sizes()));
+  const long D = x.size(-1);
+  if (D > kMaxDim)
+    throw py::value_error(text("rows of more than ", kMaxDim, " values are not supported, got ", D));
+  int p_code = code;
+  auto param = [&](const Maybe& p, const char* name) {
+    if (!p) return Tensor();
+    p_code = check_gpu(*p, name);
+    if (p_code != code && p_code != 0)
+      throw py::type_error(text(name, " must be ", type_name(x.scalar_type()), " (as x) or float32, got ",
+                                type_name(p->scalar_type())));
+    if (p->dim() != 1 || p->size(0) != D) throw py::value_error(text(name, " must be [", D, "], got ", p->sizes()));
+    return *p;
+  };
+  const Tensor w = param(weight, "weight"), b = param(bias, "bias");
+  if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
+    throw py::type_error(text("weight and bias must have one type, got ", type_name(w.scalar_type()), " and ",
+                              type_name(b.scalar_type())));
+  if (needs_grad({&x, &w, &b})) return LayerNormFn::apply(x, maybe(w), maybe(b), eps, (int64_t)code, (int64_t)p_code);
+  auto [x2, ldx] = as_rows(x);
+  return LayerNormFn::run(x, x2, ldx, w, b, eps, code, p_code, nullptr);
+}
+
+// ------------------------------------------------------------------------------------------------ routing
+struct RouteFn : torch::autograd::Function<RouteFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Maybe& bias, int64_t code, int64_t k,
+                               int64_t scoring, int64_t groups, int64_t top_groups, int64_t renorm, double scale) {
+    const Tensor x = rows(logits);
+    auto [gates, experts] = run(x, value(bias), code, k, scoring, groups, top_groups, renorm, scale);
+    ctx->save_for_backward({x, gates, experts});
+    ctx->saved_data["args"] = std::vector<int64_t>{code, scoring, renorm};
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({experts});
+    return {gates, experts};
+  }
+
+  static Tensor rows(const Tensor& t) {
+    const bool ok = (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+    return ok ? t : t.contiguous();
+  }
+
+  static long distance(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+  static std::pair<Tensor, Tensor> run(const Tensor& x, const Tensor& bias, int64_t code, int64_t k, int64_t scoring,
+                                       int64_t groups, int64_t top_groups, int64_t renorm, double scale) {
+    const long T = x.size(0), E = x.size(1);
+    Tensor gates = f32({T, k}, x), experts = i32({T, k}, x);
+    done(mm_route_fwd(ptr(x), distance(x), (int)code, T, (int)E, (int)k, (int)scoring, fptr(bias), (int)groups,
+                      (int)top_groups, (int)renorm, (float)scale, fptr(gates), iptr(experts), stream()));
+    return {gates, experts};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &gates = saved[1], &experts = saved[2];
+    const auto args = ctx->saved_data["args"].toIntVector();
+    const long T = x.size(0), E = x.size(1), k = gates.size(1);
+    const Tensor dg = grads[0].contiguous();
+    Tensor dl = at::empty({T, E}, x.options());
+    done(mm_route_bwd(ptr(x), distance(x), (int)args[0], T, (int)E, (int)k, (int)args[1], (int)args[2],
+                      (float)ctx->saved_data["scale"].toDouble(), fptr(gates), iptr(experts), fptr(dg), ptr(dl), stream()));
+    variable_list out(9);
+    out[0] = dl;
+    return once(out, "route");
+  }
+};
+
+std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::string& scoring,
+                                 const Maybe& bias, int64_t groups, std::optional<int64_t> top,
+                                 bool renormalize, double scale) {
+  const int code = check_gpu(logits, "logits");
+  if (logits.dim() != 2 || logits.size(1) == 0)
+    throw py::value_error(text("logits must be [rows, experts], got ", logits.sizes()));
+  const long E = logits.size(1), most = std::min<long>(E, kMaxK);
+  if (E > kMaxExperts) throw py::value_error(text("at most ", kMaxExperts, " experts are supported, got ", E));
+  if (k < 1 || k > most) throw py::value_error(text("k must be 1 .. ", most, ", got ", k));
+  if (scoring != "softmax" && scoring != "sigmoid")
+    throw py::value_error(text("scoring must be 'softmax' or 'sigmoid', got '", scoring, "'"));
+  if (groups < 1 || groups > kMaxGroups || E % groups)
+    throw py::value_error(text("groups must divide the ", E, " experts and be at most ", kMaxGroups, ", got ", groups));
+  const int64_t top_groups = top.value_or(groups);
+  if (top_groups < 1 || top_groups > groups)
+    throw py::value_error(text("top_groups must be 1 .. ", groups, ", got ", top_groups));
+  if (!((float)scale != 0.f) || !std::isfinite((float)scale))
+    throw py::value_error(text("scale must be finite and not 0, got ", scale));
+  Tensor b;
+  if (bias) {
+    check_gpu(*bias, "bias");
+    if (bias->scalar_type() != at::kFloat)
+      throw py::type_error(text("bias must be float32, got ", type_name(bias->scalar_type())));
+    if (bias->dim() != 1 || bias->size(0) != E)
+      throw py::value_error(text("bias must be [", E, "], got ", bias->sizes()));
+    b = bias->detach().contiguous();
+  }
+  const int64_t s = scoring == "sigmoid", r = renormalize;
+  if (needs_grad({&logits})) {
+    const variable_list out = RouteFn::apply(logits, maybe(b), (int64_t)code, k, s, groups, top_groups, r, scale);
+    return {out[0], out[1]};
+  }
+  auto [gates, experts] = RouteFn::run(RouteFn::rows(logits), b, code, k, s, groups, top_groups, r, scale);
+  return {gates, experts};
+}
+
+// ------------------------------------------------------------------------------------------------ plan
+// (experts as int32, offsets, order)
+std::tuple<Tensor, Tensor, Tensor> plan_experts(const Tensor& experts, int64_t E) {
+  if (!experts.is_cuda()) throw py::type_error("experts must be a GPU tensor");
+  if (experts.scalar_type() != at::kInt && experts.scalar_type() != at::kLong)
+    throw py::type_error(text("experts must be int32 or int64, got ", type_name(experts.scalar_type())));
+  if (experts.device().index() != c10::hip::current_device())
+    throw py::value_error(text("experts is on ", experts.device(), ", the current device is cuda:",
+                               (int)c10::hip::current_device()));
+  if (experts.dim() != 2 || experts.size(1) == 0)
+    throw py::value_error(text("experts must be [rows, k], got ", experts.sizes()));
+  if (E < 1 || E > kMaxExperts) throw py::value_error(text("n_experts must be 1 .. ", kMaxExperts, ", got ", E));
+  const long S = experts.numel();
+  if (S > kInt32Max) throw py::value_error(text("more than 2^31 - 1 slots (", S, ")"));
+  // values outside int32 must not wrap into the range of the experts
+  const Tensor e = (experts.scalar_type() == at::kLong ? experts.clamp(-1, E).to(at::kInt) : experts).contiguous();
+  long scratch = 0;
+  done(mm_expert_plan_scratch((int)S, (int)E, &scratch));
+  const Tensor buf = i32({S + E + 1 + scratch}, e);
+  int* p = iptr(buf);
+  done(mm_expert_plan(iptr(e), (int)S, (int)E, p, p + E + 1, scratch ? p + E + 1 + S : nullptr, stream()));
+  return {e, buf.narrow(0, 0, E + 1), buf.narrow(0, E + 1, S)};
+}
+
+// ------------------------------------------------------------------------------------------------ products
+struct Sizes { long T, M, D, F, E, k; };
+
+Tensor inner(const Tensor& t) { return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; }
+
+struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Maybe& gates,
+                        const Tensor& experts, const Tensor& offsets, const Tensor& order, int64_t code) {
+    const Tensor w = weight.contiguous(), g = gates ? gates->contiguous() : Tensor();
+    ctx->save_for_backward({x, w, g, experts, offsets, order});
+    ctx->saved_data["code"] = code;
+    return run(x, w, g, experts, offsets, order, (int)code);
+  }
+
+  static Sizes sizes(const Tensor& x, const Tensor& w, const Tensor& experts) {
+    return Sizes{x.size(0), x.size(1), x.size(2), w.size(2), w.size(0), experts.size(1)};
+  }
+
+  static Tensor run(const Tensor& x0, const Tensor& w, const Tensor& gates, const Tensor& experts, const Tensor& offsets,
+                    const Tensor& order, int code) {
+    const Sizes n = sizes(x0, w, experts);
+    const Tensor x = inner(x0);
+    Tensor y = at::empty({n.T, n.M, n.F}, x.options()), rows = f32({n.T * n.k, n.M, n.F}, x);
+    done(mm_expert_rows(ptr(x), x.stride(0), x.stride(1), code, (int)(n.T * n.k), (int)n.k, (int)n.M, (int)n.D, (int)n.F,
+                        ptr(w), 0, (int)n.E, iptr(offsets), iptr(order), fptr(rows), stream()));
+    done(mm_expert_combine(fptr(rows), fptr(gates), iptr(experts), code, n.T, (int)n.k, (int)n.M, (int)n.F, (int)n.E,
+                           ptr(y), stream()));
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor x = inner(saved[0]), &w = saved[1], &gates = saved[2], &experts = saved[3], &offsets = saved[4],
+                 &order = saved[5];
+    const Tensor dy = inner(grads[0]);
+    const int code = (int)ctx->saved_data["code"].toInt();
+    const Sizes n = sizes(x, w, experts);
+    const int S = (int)(n.T * n.k), k = (int)n.k, M = (int)n.M, D = (int)n.D, F = (int)n.F, E = (int)n.E;
+    Tensor dx, dw, dg;
+    if (ctx->needs_input_grad(0)) dx = at::empty({n.T, n.M, n.D}, x.options());
+    if (ctx->needs_input_grad(1)) dw = at::empty({n.E, n.D, n.F}, x.options());
+    if (gates.defined() && ctx->needs_input_grad(2)) dg = f32({n.T, n.k}, x);
+    if (dx.defined() || dg.defined()) {
+      const Tensor rows = f32({S, M, D}, x);
+      done(mm_expert_rows(ptr(dy), dy.stride(0), dy.stride(1), code, S, k, M, F, D, ptr(w), 1, E, iptr(offsets),
+                          iptr(order), fptr(rows), stream()));
+      done(mm_expert_combine_bwd(fptr(rows), fptr(gates), iptr(experts), ptr(x), x.stride(0), x.stride(1), code, n.T, k, M,
+                                 D, E, ptr(dx), fptr(dg), stream()));
+    }
+    if (dw.defined()) {
+      size_t bytes = 0;
+      done(mm_expert_wgrad_workspace(S, M, D, F, E, &bytes));
+      Tensor ws;
+      if (bytes) ws = f32({(int64_t)(bytes / sizeof(float))}, x);
+      done(mm_expert_wgrad(ptr(x), x.stride(0), x.stride(1), ptr(dy), dy.stride(0), dy.stride(1), code, S, k, M, D, F, E,
+                           fptr(gates), iptr(offsets), iptr(order), ptr(dw), fptr(ws), stream()));
+    }
+    variable_list out(7);
+    out[0] = dx;
+    out[1] = dw;
+    out[2] = dg;
+    return once(out, "expert_linear");
+  }
+};
+
+Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates, const Tensor& experts,
+                     const Tensor& offsets, const Tensor& order) {
+  const int code = check_gpu(x0, "x");
+  if (check_gpu(weight, "weight") != code)
+    throw py::type_error(text("weight must be ", type_name(x0.scalar_type()), " (as x), got ",
+                              type_name(weight.scalar_type())));
+  if ((x0.dim() != 2 && x0.dim() != 3) || weight.dim() != 3)
+    throw py::value_error(text("x must be [rows, D] or [rows, components, D] and weight [experts, D, F], got ",
+                               x0.sizes(), " and ", weight.sizes()));
+  const long T = experts.size(0), k = experts.size(1), E = offsets.size(0) - 1;
+  if (x0.size(0) != T) throw py::value_error(text("x has ", x0.size(0), " rows, the plan ", T));
+  if (weight.size(0) != E || weight.size(1) != x0.size(-1) || weight.size(1) == 0 || weight.size(2) == 0)
+    throw py::value_error(text("weight must be [", E, ", ", x0.size(-1), ", F], got ", weight.sizes()));
+  if (x0.dim() == 3 && x0.size(1) == 0) throw py::value_error("x has no components");
+  if (weight.size(1) > kInt32Max || weight.size(2) > kInt32Max) throw py::value_error("weight blocks are too large");
+  Tensor g;
+  if (gates) {
+    g = *gates;
+    check_gpu(g, "gates");
+    if (g.scalar_type() != at::kFloat)
+      throw py::type_error(text("gates must be float32, got ", type_name(g.scalar_type())));
+    if (g.dim() != 2 || g.size(0) != T || g.size(1) != k)
+      throw py::value_error(text("gates must be [", T, ", ", k, "], got ", g.sizes()));
+  }
+  if (experts.device() != x0.device()) throw py::value_error("x and the plan must be on one device");
+  const bool flat = x0.dim() == 2;
+  const Tensor x = flat ? x0.unsqueeze(1) : x0;
+  if (T * k * x.size(1) > kInt32Max - 128)
+    throw py::value_error(text(T * k * x.size(1), " rows: 2^31 or more are not supported"));
+  const Tensor y = needs_grad({&x, &weight, &g})
+                       ? ExpertLinearFn::apply(x, weight, maybe(g), experts, offsets, order, (int64_t)code)
+                       : ExpertLinearFn::run(x, weight.contiguous(), g.defined() ? g.contiguous() : g, experts, offsets,
+                                             order, code);
+  return flat ? y.squeeze(1) : y;
+}
+}  // namespace
+
+PYBIND11_MODULE(mm_torch_ops, m) {
+  m.def("version", []() { return mm_version(); });
+  m.def("layer_norm", &layer_norm);
+  m.def("route", &route);
+  m.def("plan_experts", &plan_experts);
+  m.def("expert_linear", &expert_linear);
+}

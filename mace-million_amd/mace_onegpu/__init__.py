@@ -12,6 +12,6 @@ Module map (mirrors the reference package mace_onegpu, same module paths for the
   layer_norm        layer_norm, LayerNorm: forward and backward kernels over the last axis
   experts           mixtures of expert weight blocks: route, plan_experts, expert_linear
   lammps_data       periodic-image ML-IAP data object (one GPU stands in for LAMMPS' ghost exchange)
-  model, o3, codegen, systems, _lib   architecture, couplings, kernel generator, inputs, C-ABI binding
+  model, o3, codegen, systems, _lib, _ops   architecture, couplings, kernel generator, inputs, C-ABI and torch bindings
 """
 __version__ = "0.1.0"

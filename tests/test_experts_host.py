@@ -99,6 +99,6 @@ def test_cpu_tensors_are_refused():
     x = torch.zeros(4, 8)
     e = torch.zeros(4, 2, dtype=torch.int32)
     for call in (lambda: layer_norm(x), lambda: route(x, 2), lambda: plan_experts(e, 8),
-                 lambda: expert_linear(x, torch.zeros(8, 8, 8), ExpertPlan(e, 8, None, None))):
+                 lambda: expert_linear(x, torch.zeros(8, 8, 8), ExpertPlan(e, 8, e[0], e[0]))):
         with pytest.raises(TypeError, match="GPU tensor"):
             call()

@@ -61,3 +61,36 @@ def test_plan_and_products():
                              ((x, w, plan, g[:, :1]), ValueError, "gates must be")]:
         with pytest.raises(err, match=match):
             expert_linear(*args)
+
+
+def test_second_derivatives_are_refused():
+    """Gradients are taken once: differentiating them again raises, it does not pass them off as constants."""
+    from mace_onegpu.experts import expert_linear, plan_experts, route
+    from mace_onegpu.layer_norm import layer_norm
+    x = torch.randn(5, 8, generator=torch.Generator().manual_seed(0)).cuda().requires_grad_()
+    w = torch.randn(4, 8, 8, generator=torch.Generator().manual_seed(1)).cuda()
+    plan = plan_experts(torch.randint(0, 4, (5, 2)).cuda(), 4)
+    for f in (lambda: layer_norm(x), lambda: route(x, 2)[0], lambda: expert_linear(x, w, plan)):
+        (dx,) = torch.autograd.grad(f().square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once only"):
+            dx.square().sum().backward()
+
+
+def test_each_gradient_alone():
+    """Only some inputs ask for a gradient: it is the same one as when all do."""
+    from mace_onegpu.experts import expert_linear, plan_experts
+    from mace_onegpu.layer_norm import layer_norm
+    g = torch.Generator().manual_seed(2)
+    x, w, b = (torch.randn(*s, generator=g).cuda() for s in ((30, 24), (24,), (24,)))
+    blocks, gates = torch.randn(4, 24, 16, generator=g).cuda(), torch.rand(30, 2, generator=g).cuda()
+    plan = plan_experts(torch.randint(0, 4, (30, 2), generator=g).cuda(), 4)
+    for f, args in ((layer_norm, (x, w, b)), (lambda a, c, d: expert_linear(a, c, plan, d), (x, blocks, gates))):
+        every = [t.clone().requires_grad_() for t in args]
+        want = torch.autograd.grad(f(*every).square().sum(), every)
+        for i in range(3):
+            one = [t.clone().requires_grad_(q == i) for q, t in enumerate(args)]
+            (got,) = torch.autograd.grad(f(*one).square().sum(), one[i])
+            assert torch.equal(got, want[i])
+    bias = b.clone().requires_grad_()
+    (got,) = torch.autograd.grad(layer_norm(x, None, bias).sum(), bias)       # a bias without a weight
+    assert torch.equal(got, torch.full_like(b, 30.0))
