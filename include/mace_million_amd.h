@@ -350,14 +350,18 @@ int mm_route_fwd(const void* logits, long ldl, int dtype, long T, int E, int k, 
 /* dlogits [T, E] (all of it written) of the gates and experts that mm_route_fwd gave */
 int mm_route_bwd(const void* logits, long ldl, int dtype, long T, int E, int k, int scoring, int renorm, float scale,
                  const float* gates, const int* experts, const float* dgates, void* dlogits, mm_stream_t stream);
-/* slots 0 .. S - 1 sorted by expert, stable: those of expert e are order[offsets[e] .. offsets[e + 1]); experts outside
- * [0, E) are left out (order then ends before S).  scratch: as many ints as mm_expert_plan_scratch says (0: null) */
+/* slots 0 .. S - 1 sorted by expert, stable: those of expert e are order[offsets[e] .. offsets[e + 1]), those with an
+ * expert outside [0, E) order[offsets[E] .. S).  scratch: as many ints as mm_expert_plan_scratch says (0: null) */
 int mm_expert_plan_scratch(int S, int E, long* ints /* HOST */);
 int mm_expert_plan(const int* experts, int S, int E, int* offsets, int* order, int* scratch, mm_stream_t stream);
 /* out [S, M, N] (slots without an expert are not written): out[s, m] = in[s / k, m] @ W[e], W [E, K, N], or [E, N, K] with
  * `transposed`; in at (row, component) offset row st + component sm; S M < 2^31 */
 int mm_expert_rows(const void* in, long st, long sm, int dtype, int S, int k, int M, int K, int N, const void* W,
                    int transposed, int E, const int* offsets, const int* order, float* out, mm_stream_t stream);
+/* y [T, M, F] = sum_j gates[t, j] x[t, m] @ W[experts[t, j]] (W [E, D, F]) in one launch without a plan, for few rows;
+ * T, M <= 65535 */
+int mm_expert_few(const void* x, long st, long sm, int dtype, int T, int k, int M, int D, int F, const void* W, int E,
+                  const float* gates, const int* experts, void* y, mm_stream_t stream);
 /* y [T, M, N] = sum_j gates[t, j] rows[t k + j] (gates null: ones) over the slots with an expert in [0, E) */
 int mm_expert_combine(const float* rows, const float* gates, const int* experts, int dtype, long T, int k, int M, int N,
                       int E, void* y, mm_stream_t stream);

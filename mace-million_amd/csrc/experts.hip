@@ -13,126 +13,181 @@
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 #define MM_EXPERT_MAX_E 1024
-#define MM_PLAN_WAVE 1024   // slots per wave of the plan kernels
 
 // ------------------------------------------------------------------------------------------------ plan
-// counts[e][tile]: slots of expert e in the tile of 4 waves
-__global__ void __launch_bounds__(256) mm_plan_count_kernel(const int* __restrict__ experts, int S, int E, int tiles,
-                                                            int* __restrict__ counts) {
-  extern __shared__ int h[];
-  for (int e = threadIdx.x; e < E; e += 256) h[e] = 0;
-  __syncthreads();
-  for (int r = 0; r < 4 * MM_PLAN_WAVE; r += 256) {
-    const long s = (long)blockIdx.x * (4 * MM_PLAN_WAVE) + r + threadIdx.x;
-    if (s >= S) break;
-    const int e = experts[s];
-    if ((unsigned)e < (unsigned)E) atomicAdd(&h[e], 1);
+// A stable counting sort by expert; slots without an expert are bucket E, at the end of the order.  Tiles of 4,096 slots,
+// each in the registers of one workgroup (16 a thread, loaded together).  Up to MM_PLAN_ONE tiles: one launch, whose
+// workgroups count the other tiles' slots as well.  Beyond: the tiles' counts, then the scatter, whose workgroups add up
+// the counts of all tiles themselves as long as that is at most MM_PLAN_SUM loads a thread; else a launch between them
+// takes the prefix sums.
+#define MM_PLAN_TILE 4096
+#define MM_PLAN_ONE 4
+#define MM_PLAN_SUM 128
+
+// buckets of four consecutive slots of a tile, number 4 i of it on; -1 past the end
+__device__ __forceinline__ int4 mm_plan_load(const int* __restrict__ experts, int S, int E, int tile, int i4) {
+  const long s = (long)tile * MM_PLAN_TILE + 4 * i4;
+  int v[4] = {-1, -1, -1, -1};
+  if (s + 4 <= S) {
+    typedef int i4 __attribute__((ext_vector_type(4), aligned(4)));
+    const i4 x = *(const i4*)(experts + s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (unsigned)x[i] < (unsigned)E ? x[i] : E;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (s + i < S) v[i] = (unsigned)experts[s + i] < (unsigned)E ? experts[s + i] : E;
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < E; e += 256) counts[(size_t)e * tiles + blockIdx.x] = h[e];
+  return make_int4(v[0], v[1], v[2], v[3]);
 }
 
-// one workgroup per expert: exclusive prefix sum over the tiles, and the total
-__global__ void __launch_bounds__(256) mm_plan_scan_kernel(int* __restrict__ counts, int tiles,
-                                                           int* __restrict__ totals) {
-  __shared__ int s[4];
-  int* __restrict__ row = counts + (size_t)blockIdx.x * tiles;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ void mm_plan_count(const int4& v, int* h) {
+  if (v.x >= 0) atomicAdd(&h[v.x], 1);
+  if (v.y >= 0) atomicAdd(&h[v.y], 1);
+  if (v.z >= 0) atomicAdd(&h[v.z], 1);
+  if (v.w >= 0) atomicAdd(&h[v.w], 1);
+}
+
+// counts[tile][bucket]
+__global__ void __launch_bounds__(1024) mm_plan_count_kernel(const int* __restrict__ experts, int S, int E,
+                                                             int* __restrict__ counts) {
+  extern __shared__ int h[];
+  const int4 v = mm_plan_load(experts, S, E, blockIdx.x, threadIdx.x);
+  for (int i = threadIdx.x; i <= E; i += 1024) h[i] = 0;
+  __syncthreads();
+  mm_plan_count(v, h);
+  __syncthreads();
+  for (int i = threadIdx.x; i <= E; i += 1024) counts[(size_t)blockIdx.x * (E + 1) + i] = h[i];
+}
+
+// one wave per bucket: its counts become exclusive prefix sums over the tiles, and the total
+__global__ void __launch_bounds__(64) mm_plan_scan_kernel(int* __restrict__ counts, int tiles, int E,
+                                                          int* __restrict__ totals) {
+  const int e = blockIdx.x, lane = threadIdx.x;
   int carry = 0;
-  for (int t0 = 0; t0 < tiles; t0 += 256) {
-    const int t = t0 + threadIdx.x;
-    const int v = t < tiles ? row[t] : 0;
+  for (int t0 = 0; t0 < tiles; t0 += 64) {
+    const int t = t0 + lane;
+    const int v = t < tiles ? counts[(size_t)t * (E + 1) + e] : 0;
     int inc = v;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int u = __shfl_up(inc, d);
       if (lane >= d) inc += u;
     }
-    if (lane == 63) s[wave] = inc;
-    __syncthreads();
-    int before = carry;
-    for (int w = 0; w < wave; ++w) before += s[w];
-    if (t < tiles) row[t] = before + inc - v;
-    carry += s[0] + s[1] + s[2] + s[3];
-    __syncthreads();
+    if (t < tiles) counts[(size_t)t * (E + 1) + e] = carry + inc - v;
+    carry += __shfl(inc, 63);
   }
-  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+  if (lane == 0) totals[e] = carry;
 }
 
-// Scatter of a tile of NW waves: the waves count their slots, then each ranks 64 consecutive slots at a time among equal
-// experts with one ballot per bit, on top of its counters.  SINGLE: the tile is the whole list, nothing was counted.
-template <int NW, bool SINGLE>
-__global__ void __launch_bounds__(64 * NW) mm_plan_kernel(const int* __restrict__ experts, int S, int E, int bits,
-                                                          int tiles, const int* __restrict__ counts,
+// threads of th side by side over the buckets (a power of two); the rest go over the tiles
+__host__ __device__ inline int mm_plan_across(int buckets, int th) {
+  int p = 1;
+  while (p < buckets && p < th) p <<= 1;
+  return p;
+}
+
+// One tile.  Each of the NW waves ranks its share of the slots, 64 consecutive ones at a time: one ballot per bit of the
+// bucket finds the equals, the first of which takes places for all of them from the wave's counters.  Then the counters
+// become places in the order.  Bound by the latency of these rounds, so as many waves as the counters leave room for
+// share them (4 instead of 16: 12.6 us instead of the figure below for 4,000 slots of 89 experts).  MODE 0: the other tiles are counted here; 1: the counts of all
+// tiles are added up here; 2: counts are prefix sums, with the totals.  BITS: of the largest bucket, or more.
+template <int MODE, int NW, int BITS>
+__global__ void __launch_bounds__(64 * NW) mm_plan_kernel(const int* __restrict__ experts, int S, int E, int tiles,
+                                                          const int* __restrict__ counts,
                                                           const int* __restrict__ totals, int* __restrict__ offsets,
                                                           int* __restrict__ order) {
+  constexpr int TH = 64 * NW, SHARE = MM_PLAN_TILE / NW;
   extern __shared__ int sm[];
-  int* cnt = sm;            // [NW][E]
-  int* base = sm + NW * E;  // [E]
+  __shared__ int s_e[MM_PLAN_TILE], s_at[MM_PLAN_TILE];
+  const int B = E + 1;                                          // buckets
+  int *cnt = sm, *total = sm + NW * B, *before = total + B;     // [NW][B], [B], [B]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const long s0 = (long)blockIdx.x * (NW * MM_PLAN_WAVE) + wave * MM_PLAN_WAVE + lane;
-  for (int i = tid; i < NW * E; i += 64 * NW) cnt[i] = 0;
+  for (int i = tid; i < (NW + 2) * B; i += TH) sm[i] = 0;
+  for (int i = tid; i < MM_PLAN_TILE / 4; i += TH) ((int4*)s_e)[i] = mm_plan_load(experts, S, E, blockIdx.x, i);
   __syncthreads();
-  for (int r = 0; r < MM_PLAN_WAVE; r += 64) {
-    const int e = s0 + r < S ? experts[s0 + r] : -1;
-    if ((unsigned)e < (unsigned)E) atomicAdd(&cnt[wave * E + e], 1);
-  }
-  __syncthreads();
-  for (int e = tid; e < E; e += 64 * NW) {
-    int t = 0;
-    if constexpr (SINGLE) {
-      for (int w = 0; w < NW; ++w) t += cnt[w * E + e];
-    } else {
-      t = totals[e];
+  if constexpr (MODE == 0) {
+    for (int c = 0; c < tiles; ++c) {
+      if (c == (int)blockIdx.x) continue;
+      int* to = c < (int)blockIdx.x ? before : total;   // total: the tiles after this one, for now
+      for (int i = tid; i < MM_PLAN_TILE / 4; i += TH) mm_plan_count(mm_plan_load(experts, S, E, c, i), to);
     }
-    base[e] = t;
+  }
+  if constexpr (MODE == 1) {
+    const int P = mm_plan_across(B, TH), G = TH / P, grp = tid / P;
+    for (int i = tid % P; i < B; i += P) {
+      int t = 0, f = 0;
+#pragma unroll 8
+      for (int c = grp; c < tiles; c += G) {
+        const int v = counts[(size_t)c * B + i];
+        t += v;
+        f += c < (int)blockIdx.x ? v : 0;
+      }
+      atomicAdd(&total[i], t);
+      atomicAdd(&before[i], f);
+    }
+  }
+  if constexpr (MODE == 2)
+    for (int i = tid; i < B; i += TH) {
+      total[i] = totals[i];
+      before[i] = counts[(size_t)blockIdx.x * B + i];
+    }
+  const int here = min(MM_PLAN_TILE, S - (int)blockIdx.x * MM_PLAN_TILE);   // slots of this tile
+  const int end = min((wave + 1) * SHARE, here);
+  // (the leaders' adds of one round are to different counters, those of successive rounds in order)
+  for (int i = wave * SHARE + lane; i - lane < end; i += 64) {
+    const int e = s_e[i];
+    unsigned long long same = __ballot(e >= 0);
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
+      const unsigned long long m = __ballot((e >> b) & 1);
+      same &= (e >> b) & 1 ? m : ~m;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1)), first = __ffsll(same) - 1;
+    int at = 0;
+    if (e >= 0 && rank == 0) at = atomicAdd(&cnt[wave * B + e], (int)__popcll(same));
+    at = __shfl(at, first & 63);
+    s_at[i] = at + rank;
   }
   __syncthreads();
-  if (wave == 0) {   // exclusive prefix sum of the experts' totals
+  if (wave == 0) {   // exclusive prefix sum of the buckets' totals
     int carry = 0;
-    for (int e0 = 0; e0 < E; e0 += 64) {
-      const int e = e0 + lane, v = e < E ? base[e] : 0;
+    for (int e0 = 0; e0 < B; e0 += 64) {
+      const int i = e0 + lane;
+      int v = 0;
+      if (i < B) {
+        v = total[i];
+        if constexpr (MODE == 0) {
+          v += before[i];
+#pragma unroll
+          for (int w = 0; w < NW; ++w) v += cnt[w * B + i];
+        }
+      }
       int inc = v;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
         const int u = __shfl_up(inc, d);
         if (lane >= d) inc += u;
       }
-      if (e < E) {
-        base[e] = carry + inc - v;
-        if (blockIdx.x == 0) offsets[e] = carry + inc - v;
+      if (i < B) {
+        total[i] = carry + inc - v;
+        if (blockIdx.x == 0) offsets[i] = carry + inc - v;   // offsets[E] = slots with an expert
       }
       carry += __shfl(inc, 63);
     }
-    if (blockIdx.x == 0 && lane == 0) offsets[E] = carry;
   }
   __syncthreads();
-  for (int e = tid; e < E; e += 64 * NW) {
-    int at = base[e];
-    if constexpr (!SINGLE) at += counts[(size_t)e * tiles + blockIdx.x];
+  for (int i = tid; i < B; i += TH) {
+    int at = total[i] + before[i];
+#pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const int c = cnt[w * E + e];
-      cnt[w * E + e] = at;
+      const int c = cnt[w * B + i];
+      cnt[w * B + i] = at;
       at += c;
     }
   }
   __syncthreads();
-  for (int r = 0; r < MM_PLAN_WAVE; r += 64) {
-    const int e = s0 + r < S ? experts[s0 + r] : -1;
-    const bool ok = (unsigned)e < (unsigned)E;
-    unsigned long long same = __ballot(ok);
-    if (same == 0) continue;
-    for (int b = 0; b < bits; ++b) {
-      const unsigned long long m = __ballot((e >> b) & 1);
-      same &= (e >> b) & 1 ? m : ~m;
-    }
-    const int before = __popcll(same & ((1ull << lane) - 1));
-    const int at = ok ? cnt[wave * E + e] : 0;
-    mm_wave_lds_sync();
-    if (ok && before == 0) cnt[wave * E + e] = at + __popcll(same);
-    mm_wave_lds_sync();
-    if (ok) order[at + before] = (int)(s0 + r);
-  }
+  for (int i = tid; i < here; i += TH) order[cnt[i / SHARE * B + s_e[i]] + s_at[i]] = blockIdx.x * MM_PLAN_TILE + i;
 }
 
 // ------------------------------------------------------------------------------------------------ tiles of an expert
@@ -140,10 +195,26 @@ struct MMTile {
   int e, row0, rows;   // expert, first of its rows (slots x M), rows in the tile; e < 0: no such tile
 };
 
-// The tile-th tile of BM rows of the experts' row lists one after the other (every expert's list ends in a cut tile);
-// every wave finds it by itself, 64 experts at a time.
-__device__ __forceinline__ MMTile mm_expert_tile(const int* __restrict__ offsets, int E, int M, int BM, int tile) {
+// Workgroup b of `per` for each of the tiles of BM rows that the experts' row lists have (every list ends in a cut tile):
+// its tile, and its number within it.  Every wave finds them by itself, 64 experts at a time.  Workgroups are dealt out to
+// the 8 XCDs in turn; the work is numbered so that an XCD gets consecutive pieces, whose operands its L2 then holds.
+__device__ __forceinline__ MMTile mm_expert_tile(const int* __restrict__ offsets, int E, int M, int BM, int per, int b,
+                                                 int* part, int* number) {
   const int lane = threadIdx.x & 63;
+  int all = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) {
+    const int e = e0 + lane;
+    all += e < E ? ((offsets[e + 1] - offsets[e]) * M + BM - 1) / BM : 0;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
+  all *= per;
+  if (b >= all) return MMTile{-1, 0, 0};
+  const int share = all / 8, rest = all % 8, x = b % 8;
+  const int at = x * share + min(x, rest) + b / 8;
+  int tile = at / per;
+  *part = at - tile * per;
+  *number = tile;
   for (int e0 = 0; e0 < E; e0 += 64) {
     const int e = e0 + lane;
     const int rows = e < E ? (offsets[e + 1] - offsets[e]) * M : 0, n = (rows + BM - 1) / BM;
@@ -363,13 +434,6 @@ __device__ __forceinline__ void mm_stage_done() {
   __syncthreads();
 }
 
-// Workgroups are dealt out to the 8 XCDs in turn: number them so that an XCD gets consecutive work, whose operands its L2
-// then holds.
-__device__ __forceinline__ int mm_xcd_order(int b, int n) {
-  const int per = n / 8, rest = n % 8, x = b % 8, i = b / 8;
-  return x < rest ? x * (per + 1) + i : x * per + rest + i;
-}
-
 // ------------------------------------------------------------------------------------------------ rows
 struct MMRows {
   const void *in, *W;
@@ -389,9 +453,10 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mm_expert_rows_kernel(MMRows 
   extern __shared__ uint4 mm_lds[];
   uint4 *As = mm_lds, *Bs = As + 2 * BM * 8;             // [2][BM * 8], [2][BN * 8]
   long* s_out = (long*)(Bs + 2 * BN * 8);                // [BM]
-  const int at = mm_xcd_order(blockIdx.x, gridDim.x), n0 = at % tiles_n * BN;
-  const MMTile t = mm_expert_tile(a.offsets, a.E, a.M, BM, at / tiles_n);
+  int part, number;
+  const MMTile t = mm_expert_tile(a.offsets, a.E, a.M, BM, tiles_n, blockIdx.x, &part, &number);
   if (t.e < 0) return;
+  const int n0 = part * BN;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const T* __restrict__ W = (const T*)a.W + (size_t)t.e * a.K * a.N;
   const int* __restrict__ list = a.order + a.offsets[t.e];
@@ -468,6 +533,60 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mm_expert_rows_kernel(MMRows 
 #pragma unroll
     for (int i = 0; i < FN; ++i) mm_store_vec(o, n0 + wn + 16 * i + 4 * (lane >> 4), a.N, (const float*)&acc[i][j]);
   }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// y[t, m] straight from the choices of row t, without a plan: a workgroup takes LC vectors of columns, its other threads
+// share the sum over d, W is read once per row, coalesced along the columns, fp32 sums.  Bound by latency: the sum over d is
+// split as far as the workgroup goes, and the columns over many workgroups.
+struct MMFew {
+  const void *x, *W;
+  const float* gates;
+  const int* experts;
+  long st, sm;
+  int k, M, D, F, E;
+};
+
+template <typename T, int LC>
+__global__ void __launch_bounds__(256) mm_expert_few_kernel(MMFew a, T* __restrict__ y) {
+  constexpr int N = MMVec<T>::N, G = 256 / LC;
+  __shared__ float red[4][LC * N];
+  const long t = blockIdx.y;
+  const int m = blockIdx.z, lc = threadIdx.x % LC, gd = threadIdx.x / LC, f = (blockIdx.x * LC + lc) * N;
+  const T* __restrict__ x = (const T*)a.x + t * a.st + m * a.sm;
+  float acc[N] = {};
+  for (int j = 0; j < a.k; ++j) {
+    const int e = a.experts[t * a.k + j];
+    if ((unsigned)e >= (unsigned)a.E) continue;
+    const float g = a.gates ? a.gates[t * a.k + j] : 1.f;
+    const T* __restrict__ W = (const T*)a.W + (size_t)e * a.D * a.F;
+    float sum[N] = {};
+    if (f < a.F) {
+#pragma unroll 8
+      for (int d = gd; d < a.D; d += G) {
+        float w[N];
+        mm_load_vec(W + (size_t)d * a.F, f, a.F, w);
+        const float xv = (float)x[d];
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] = fmaf(xv, w[i], sum[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = fmaf(g, sum[i], acc[i]);
+  }
+  // over the threads of a wave with the same columns, then over the waves
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int d = LC; d < 64; d <<= 1) acc[i] += __shfl_xor(acc[i], d);
+    if ((threadIdx.x & 63) < LC) red[threadIdx.x >> 6][lc * N + i] = acc[i];
+  }
+  __syncthreads();
+  if (threadIdx.x >= LC || f >= a.F) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    acc[i] = red[0][lc * N + i] + red[1][lc * N + i] + red[2][lc * N + i] + red[3][lc * N + i];
+  mm_store_vec(y + (t * a.M + m) * a.F, f, a.F, acc);
 }
 
 // ------------------------------------------------------------------------------------------------ rows -> y
@@ -611,11 +730,18 @@ __global__ void __launch_bounds__(64 * WD * WF, 2) mm_expert_wgrad_kernel(MMWgra
   uint4 *Xs = mm_lds, *Ys = Xs + 2 * BD * 8;             // [2][BD * 8], [2][BF * 8]
   long *s_x = (long*)(Ys + 2 * BF * 8), *s_y = s_x + MM_WG_ROWS;
   float* s_g = (float*)(s_y + MM_WG_ROWS);
-  const int at = mm_xcd_order(blockIdx.x, gridDim.x), tile = at / tiles_df, df = at % tiles_df;
+  int df, tile;
   MMTile t;
-  if constexpr (SPLIT) t = mm_expert_tile(a.offsets, a.E, a.M, chunk, tile);
-  else t = MMTile{tile, 0, (a.offsets[tile + 1] - a.offsets[tile]) * a.M};
-  if (t.e < 0) return;
+  if constexpr (SPLIT) {
+    t = mm_expert_tile(a.offsets, a.E, a.M, chunk, tiles_df, blockIdx.x, &df, &tile);
+    if (t.e < 0) return;
+  } else {   // an XCD gets every 8th expert: lists of different lengths, each read by one XCD
+    const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
+    tile = i / tiles_df * 8 + x;
+    df = i % tiles_df;
+    if (tile >= a.E) return;
+    t = MMTile{tile, 0, (a.offsets[tile + 1] - a.offsets[tile]) * a.M};
+  }
   const int d0 = df / tiles_f * BD, f0 = df % tiles_f * BF;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int* __restrict__ list = a.order + a.offsets[t.e];
@@ -723,17 +849,17 @@ __global__ void __launch_bounds__(256) mm_expert_wgrad_sum_kernel(MMWgrad a, int
   const int n = ((a.offsets[e + 1] - a.offsets[e]) * a.M + chunk - 1) / chunk;
   const long size = (long)a.D * a.F, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= size) return;
+  const float* __restrict__ p = part + (size_t)first * size + i;
+  const int left = (int)min(size - i, 4L);
   float t[4] = {};
+#pragma unroll 8
   for (int c = 0; c < n; ++c) {
-    const float* __restrict__ p = part + (size_t)(first + c) * size;
+    float v[4];
+    mm_load4(p + c * size, 0, left, v);
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
-      if (i + v < size) t[v] += p[i + v];
+    for (int q = 0; q < 4; ++q) t[q] += v[q];
   }
-  T* __restrict__ o = (T*)a.dW + (size_t)e * size;
-#pragma unroll
-  for (int v = 0; v < 4; ++v)
-    if (i + v < size) o[i + v] = (T)t[v];
+  mm_store4((T*)a.dW + (size_t)e * size + i, 0, left, t);
 }
 
 // ------------------------------------------------------------------------------------------------ entry points
@@ -742,11 +868,6 @@ int range_error(const char* name, const char* what) {
   mm::set_error(std::string(name) + ": " + what);
   return MM_ERANGE;
 }
-
-constexpr int kPlanTile = 4 * MM_PLAN_WAVE;
-
-// waves of the one workgroup that plans S slots of E experts (its counters fit 64 KB of LDS); 0: several workgroups
-int plan_waves(int S, int E) { return S <= 4 * MM_PLAN_WAVE ? 4 : S <= 16 * MM_PLAN_WAVE && E <= 512 ? 16 : 0; }
 
 // Tiles of 256 x 256 where the experts' lists and the columns fill them: twice the products per value loaded, but a cut
 // tile at the end of every list.
@@ -796,7 +917,7 @@ int launch_rows(const MMRows& a, int S, bool big, hipStream_t stream) {
 template <typename T, bool SPLIT, bool DMA, int BD, int BF, int WD, int WF>
 int launch_wgrad_tile(const MMWgrad& a, int S, int chunk, float* part, hipStream_t stream) {
   const int tiles_f = (a.F + BF - 1) / BF, tiles_df = (a.D + BD - 1) / BD * tiles_f;
-  const long wg = (SPLIT ? (long)S * a.M / chunk + (a.E < S ? a.E : S) : a.E) * tiles_df;
+  const long wg = (SPLIT ? (long)S * a.M / chunk + (a.E < S ? a.E : S) : (a.E + 7L) / 8 * 8) * tiles_df;
   if (wg > 2147483647L) return range_error("mm_expert_wgrad", "output too large for one launch");
   constexpr auto kernel = mm_expert_wgrad_kernel<T, SPLIT, DMA, BD, BF, WD, WF>;
   constexpr int lds = wgrad_lds<BD, BF>();
@@ -830,7 +951,8 @@ int wgrad_chunk(long rows, int D, int F, int E) {
 
 extern "C" int mm_expert_plan_scratch(int S, int E, long* ints) {
   MM_CHECK_ARG(S >= 0 && E >= 1 && ints, "bad sizes");
-  *ints = plan_waves(S, E) ? 0 : (long)E * ((S + (long)kPlanTile - 1) / kPlanTile + 1);
+  const long tiles = ((long)S + MM_PLAN_TILE - 1) / MM_PLAN_TILE;
+  *ints = tiles <= MM_PLAN_ONE ? 0 : (E + 1L) * (tiles + 1);   // counts, totals
   return MM_OK;
 }
 
@@ -838,24 +960,31 @@ extern "C" int mm_expert_plan(const int* experts, int S, int E, int* offsets, in
                               hipStream_t stream) {
   MM_CHECK_ARG(S >= 0 && E >= 1, "bad sizes");
   if (E > MM_EXPERT_MAX_E) return range_error("mm_expert_plan", "more than 1024 experts are not supported");
-  int bits = 0;
-  while (bits < 31 && (E - 1) >> bits) ++bits;
-  const int waves = plan_waves(S, E);
-  if (waves == 4)
-    hipLaunchKernelGGL((mm_plan_kernel<4, true>), dim3(1), dim3(256), 5 * E * sizeof(int), stream, experts, S, E, bits,
-                       1, nullptr, nullptr, offsets, order);
-  else if (waves)
-    hipLaunchKernelGGL((mm_plan_kernel<16, true>), dim3(1), dim3(1024), 17 * E * sizeof(int), stream, experts, S, E,
-                       bits, 1, nullptr, nullptr, offsets, order);
-  if (waves) return mm::launch_status("mm_expert_plan");
-  MM_CHECK_ARG(scratch, "scratch is null");
-  const int tiles = (int)((S + (long)kPlanTile - 1) / kPlanTile);
-  int *counts = scratch, *totals = scratch + (size_t)E * tiles;
-  hipLaunchKernelGGL(mm_plan_count_kernel, dim3(tiles), dim3(256), E * sizeof(int), stream, experts, S, E, tiles,
-                     counts);
-  hipLaunchKernelGGL(mm_plan_scan_kernel, dim3(E), dim3(256), 0, stream, counts, tiles, totals);
-  hipLaunchKernelGGL((mm_plan_kernel<4, false>), dim3(tiles), dim3(256), 5 * E * sizeof(int), stream, experts, S, E,
-                     bits, tiles, counts, totals, offsets, order);
+  const int tiles = (int)(((long)S + MM_PLAN_TILE - 1) / MM_PLAN_TILE), one = tiles <= MM_PLAN_ONE;
+  MM_CHECK_ARG(one || scratch, "scratch is null");
+  // 16 waves while their counters fit 64 KB of LDS beside the tile, else 4
+  const int nw = E < 400 ? 16 : 4, th = 64 * nw, across = mm_plan_across(E + 1, th);
+  const int lds = (nw + 2) * (E + 1) * (int)sizeof(int);
+  int *counts = scratch, *totals = scratch + (size_t)tiles * (E + 1);
+  if (!one)
+    hipLaunchKernelGGL(mm_plan_count_kernel, dim3(tiles), dim3(1024), (E + 1) * sizeof(int), stream, experts, S, E,
+                       counts);
+  const bool sums = ((long)tiles * across + th - 1) / th * ((E + across) / across) <= MM_PLAN_SUM;
+  if (!one && !sums)
+    hipLaunchKernelGGL(mm_plan_scan_kernel, dim3(E + 1), dim3(64), 0, stream, counts, tiles, E, totals);
+#define CALL(mode, nw, bits)                                                                                        \
+  hipLaunchKernelGGL((mm_plan_kernel<mode, nw, bits>), dim3(tiles ? tiles : 1), dim3(64 * nw), lds, stream, experts, S, \
+                     E, tiles, counts, totals, offsets, order)
+#define CALLS(mode)                      \
+  if (nw == 4) CALL(mode, 4, 11);        \
+  else if (E < 16) CALL(mode, 16, 4);    \
+  else if (E < 128) CALL(mode, 16, 7);   \
+  else CALL(mode, 16, 9);
+  if (one) { CALLS(0) }
+  else if (sums) { CALLS(1) }
+  else { CALLS(2) }
+#undef CALLS
+#undef CALL
   return mm::launch_status("mm_expert_plan");
 }
 
@@ -880,6 +1009,24 @@ extern "C" int mm_expert_rows(const void* in, long st, long sm, int dtype, int S
   else { if (dma) { CALL(false, true) } else { CALL(false, false) } }
 #undef CALL
   return rc;
+}
+
+extern "C" int mm_expert_few(const void* x, long st, long sm, int dtype, int T, int k, int M, int D, int F,
+                             const void* W, int E, const float* gates, const int* experts, void* y,
+                             hipStream_t stream) {
+  MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");
+  MM_CHECK_ARG(T >= 0 && k >= 1 && M >= 1 && D >= 1 && F >= 1 && E >= 1 && st >= 0 && sm >= 0, "bad sizes");
+  if (T > 65535 || M > 65535) return range_error("mm_expert_few", "more than 65535 rows or components are not supported");
+  if (T == 0) return MM_OK;
+  const MMFew a{x, W, gates, experts, st, sm, k, M, D, F, E};
+#define CALL(T_)                                                                                             \
+  hipLaunchKernelGGL((mm_expert_few_kernel<T_, 4>), dim3((F + 4 * MMVec<T_>::N - 1) / (4 * MMVec<T_>::N), T, M), \
+                     dim3(256), 0, stream, a, (T_*)y)
+  if (dtype == MM_F32) CALL(float);
+  else if (dtype == MM_BF16) CALL(__bf16);
+  else CALL(_Float16);
+#undef CALL
+  return mm::launch_status("mm_expert_few");
 }
 
 extern "C" int mm_expert_combine(const float* rows, const float* gates, const int* experts, int dtype, long T, int k,

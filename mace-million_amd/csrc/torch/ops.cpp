@@ -8,6 +8,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ops/empty.h>
+#include <ATen/ops/sub.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
@@ -255,8 +256,28 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::str
 }
 
 // ------------------------------------------------------------------------------------------------ plan
-// (experts as int32, offsets, order)
-std::tuple<Tensor, Tensor, Tensor> plan_experts(const Tensor& experts, int64_t E) {
+// The sorted lists of long lists of slots are made with the plan; few slots may do without (few_rows), theirs are made
+// when something first asks for them.
+constexpr long kPlanNow = 1024;
+
+struct Plan {
+  Tensor experts, offsets, order;
+  long T, k, E;
+
+  void lists() {
+    if (offsets.defined()) return;
+    const long S = T * k;
+    long scratch = 0;
+    done(mm_expert_plan_scratch((int)S, (int)E, &scratch));
+    const Tensor buf = i32({S + E + 1 + scratch}, experts);
+    int* p = iptr(buf);
+    done(mm_expert_plan(iptr(experts), (int)S, (int)E, p, p + E + 1, scratch ? p + E + 1 + S : nullptr, stream()));
+    offsets = buf.narrow(0, 0, E + 1);
+    order = buf.narrow(0, E + 1, S);
+  }
+};
+
+std::shared_ptr<Plan> plan_experts(const Tensor& experts, int64_t E) {
   if (!experts.is_cuda()) throw py::type_error("experts must be a GPU tensor");
   if (experts.scalar_type() != at::kInt && experts.scalar_type() != at::kLong)
     throw py::type_error(text("experts must be int32 or int64, got ", type_name(experts.scalar_type())));
@@ -268,18 +289,27 @@ std::tuple<Tensor, Tensor, Tensor> plan_experts(const Tensor& experts, int64_t E
   if (E < 1 || E > kMaxExperts) throw py::value_error(text("n_experts must be 1 .. ", kMaxExperts, ", got ", E));
   const long S = experts.numel();
   if (S > kInt32Max) throw py::value_error(text("more than 2^31 - 1 slots (", S, ")"));
+  auto p = std::make_shared<Plan>();
   // values outside int32 must not wrap into the range of the experts
-  const Tensor e = (experts.scalar_type() == at::kLong ? experts.clamp(-1, E).to(at::kInt) : experts).contiguous();
-  long scratch = 0;
-  done(mm_expert_plan_scratch((int)S, (int)E, &scratch));
-  const Tensor buf = i32({S + E + 1 + scratch}, e);
-  int* p = iptr(buf);
-  done(mm_expert_plan(iptr(e), (int)S, (int)E, p, p + E + 1, scratch ? p + E + 1 + S : nullptr, stream()));
-  return {e, buf.narrow(0, 0, E + 1), buf.narrow(0, E + 1, S)};
+  p->experts = (experts.scalar_type() == at::kLong ? experts.clamp(-1, E).to(at::kInt) : experts).contiguous();
+  p->T = experts.size(0);
+  p->k = experts.size(1);
+  p->E = E;
+  if (S > kPlanNow) p->lists();
+  return p;
 }
 
 // ------------------------------------------------------------------------------------------------ products
 struct Sizes { long T, M, D, F, E, k; };
+
+// Whether rows go straight through their blocks (mm_expert_few), without a plan and without joining slots: while the blocks'
+// bytes that they read, mostly from the L2s, stay below 64 MB.  Measured (us, straight against sorted): 128 -> 128 float, 2
+// of 8 experts: 1 row 3.6 / 19, 128 rows (17 MB) 4.4 / 21; 1024 -> 1024 bfloat16, 4 of 64: 1 row 17 / 26, 8 rows (67 MB)
+// 33 / 32, 16 rows 36 / 35, 64 rows 126 / 36; the same in float: 4 rows (67 MB) 26 / 75.
+bool few_rows(const Sizes& n, int code) {
+  const double bytes = (double)n.T * n.M * n.k * n.D * n.F * (code == 0 ? 4 : 2);
+  return bytes <= 64e6 && n.T <= 65535 && n.M <= 65535;
+}
 
 Tensor inner(const Tensor& t) { return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; }
 
@@ -300,7 +330,13 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
                     const Tensor& order, int code) {
     const Sizes n = sizes(x0, w, experts);
     const Tensor x = inner(x0);
-    Tensor y = at::empty({n.T, n.M, n.F}, x.options()), rows = f32({n.T * n.k, n.M, n.F}, x);
+    Tensor y = at::empty({n.T, n.M, n.F}, x.options());
+    if (few_rows(n, code)) {
+      done(mm_expert_few(ptr(x), x.stride(0), x.stride(1), code, (int)n.T, (int)n.k, (int)n.M, (int)n.D, (int)n.F, ptr(w),
+                         (int)n.E, fptr(gates), iptr(experts), ptr(y), stream()));
+      return y;
+    }
+    Tensor rows = f32({n.T * n.k, n.M, n.F}, x);
     done(mm_expert_rows(ptr(x), x.stride(0), x.stride(1), code, (int)(n.T * n.k), (int)n.k, (int)n.M, (int)n.D, (int)n.F,
                         ptr(w), 0, (int)n.E, iptr(offsets), iptr(order), fptr(rows), stream()));
     done(mm_expert_combine(fptr(rows), fptr(gates), iptr(experts), code, n.T, (int)n.k, (int)n.M, (int)n.F, (int)n.E,
@@ -343,8 +379,7 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
   }
 };
 
-Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates, const Tensor& experts,
-                     const Tensor& offsets, const Tensor& order) {
+Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates, const std::shared_ptr<Plan>& plan) {
   const int code = check_gpu(x0, "x");
   if (check_gpu(weight, "weight") != code)
     throw py::type_error(text("weight must be ", type_name(x0.scalar_type()), " (as x), got ",
@@ -352,7 +387,8 @@ Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates,
   if ((x0.dim() != 2 && x0.dim() != 3) || weight.dim() != 3)
     throw py::value_error(text("x must be [rows, D] or [rows, components, D] and weight [experts, D, F], got ",
                                x0.sizes(), " and ", weight.sizes()));
-  const long T = experts.size(0), k = experts.size(1), E = offsets.size(0) - 1;
+  if (!plan) throw py::type_error("plan must be an ExpertPlan (plan_experts)");
+  const long T = plan->T, k = plan->k, E = plan->E;
   if (x0.size(0) != T) throw py::value_error(text("x has ", x0.size(0), " rows, the plan ", T));
   if (weight.size(0) != E || weight.size(1) != x0.size(-1) || weight.size(1) == 0 || weight.size(2) == 0)
     throw py::value_error(text("weight must be [", E, ", ", x0.size(-1), ", F], got ", weight.sizes()));
@@ -367,15 +403,17 @@ Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates,
     if (g.dim() != 2 || g.size(0) != T || g.size(1) != k)
       throw py::value_error(text("gates must be [", T, ", ", k, "], got ", g.sizes()));
   }
+  const Tensor& experts = plan->experts;
   if (experts.device() != x0.device()) throw py::value_error("x and the plan must be on one device");
   const bool flat = x0.dim() == 2;
   const Tensor x = flat ? x0.unsqueeze(1) : x0;
   if (T * k * x.size(1) > kInt32Max - 128)
     throw py::value_error(text(T * k * x.size(1), " rows: 2^31 or more are not supported"));
-  const Tensor y = needs_grad({&x, &weight, &g})
-                       ? ExpertLinearFn::apply(x, weight, maybe(g), experts, offsets, order, (int64_t)code)
-                       : ExpertLinearFn::run(x, weight.contiguous(), g.defined() ? g.contiguous() : g, experts, offsets,
-                                             order, code);
+  const bool grad = needs_grad({&x, &weight, &g});
+  if (grad || !few_rows({T, x.size(1), x.size(2), weight.size(2), E, k}, code)) plan->lists();
+  const Tensor y = grad ? ExpertLinearFn::apply(x, weight, maybe(g), experts, plan->offsets, plan->order, (int64_t)code)
+                        : ExpertLinearFn::run(x, weight.contiguous(), g.defined() ? g.contiguous() : g, experts,
+                                              plan->offsets, plan->order, code);
   return flat ? y.squeeze(1) : y;
 }
 }  // namespace
@@ -384,6 +422,15 @@ PYBIND11_MODULE(mm_torch_ops, m) {
   m.def("version", []() { return mm_version(); });
   m.def("layer_norm", &layer_norm);
   m.def("route", &route);
+  py::class_<Plan, std::shared_ptr<Plan>>(m, "ExpertPlan")
+      .def_property_readonly("experts", [](Plan& p) { return p.experts; })
+      .def_property_readonly("n_experts", [](Plan& p) { return p.E; })
+      .def_property_readonly("offsets", [](Plan& p) { return p.lists(), p.offsets; })
+      .def_property_readonly("order", [](Plan& p) { return p.lists(), p.order; })
+      .def_property_readonly("counts", [](Plan& p) {
+        p.lists();
+        return at::sub(p.offsets.narrow(0, 1, p.E), p.offsets.narrow(0, 0, p.E));
+      });
   m.def("plan_experts", &plan_experts);
   m.def("expert_linear", &expert_linear);
 }

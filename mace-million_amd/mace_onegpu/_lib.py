@@ -98,6 +98,7 @@ SIGNATURES = {
     "mm_expert_plan_scratch": [I, I, P],
     "mm_expert_plan": [P, I, I, P, P, P, P],
     "mm_expert_rows": [P, L, L, I, I, I, I, I, I, P, I, I, P, P, P, P],
+    "mm_expert_few": [P, L, L, I, I, I, I, I, I, P, I, P, P, P, P],
     "mm_expert_combine": [P, P, P, I, L, I, I, I, I, P, P],
     "mm_expert_combine_bwd": [P, P, P, P, L, L, I, L, I, I, I, I, P, P, P],
     "mm_expert_wgrad_workspace": [I, I, I, I, I, P],

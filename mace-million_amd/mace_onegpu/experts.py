@@ -33,24 +33,16 @@ def route(logits, k, scoring="softmax", bias=None, groups=1, top_groups=None, re
     return ops().route(logits, k, scoring, bias, groups, top_groups, renormalize, scale)
 
 
-class ExpertPlan:
-    """The slots s = t k + j of experts [T, k] sorted by expert: those of expert e are order[offsets[e] : offsets[e + 1]],
-    in ascending order.  Slots with an expert outside [0, n_experts) are in no list (order ends before them).  Made by
-    plan_experts, and not changed afterwards: the kernels trust it."""
-
-    def __init__(self, experts, n_experts, offsets, order):
-        self.experts, self.n_experts, self.offsets, self.order = experts, n_experts, offsets, order
-
-    @property
-    def counts(self):
-        """Slots of each expert, int32 [n_experts] (its load, for a balance bias)."""
-        return self.offsets[1:] - self.offsets[:-1]
-
-
 def plan_experts(experts, n_experts):
-    """The ExpertPlan of experts [T, k] (int32 or int64; -1 for none), n_experts up to 1024: a stable counting sort."""
-    experts, offsets, order = ops().plan_experts(experts, n_experts)
-    return ExpertPlan(experts, int(n_experts), offsets, order)
+    """The plan of experts [T, k] (int32 or int64; -1 for none), n_experts up to 1024, for expert_linear: a stable counting
+    sort of the slots s = t k + j by expert.  Its fields (tensors are not to be changed: the kernels trust them):
+
+    experts int32 [T, k], n_experts
+    order int32 [T k], offsets int32 [n_experts + 1]: the slots of expert e are order[offsets[e] : offsets[e + 1]], in
+        ascending order; slots with an expert outside [0, n_experts) come after them, from offsets[n_experts] on.  For up
+        to 1024 slots the sort waits until something needs it: few rows do without.
+    counts int32 [n_experts]: slots of each expert (its load, for a balance bias)"""
+    return ops().plan_experts(experts, n_experts)
 
 
 def expert_linear(x, weight, plan, gates=None):
@@ -60,6 +52,4 @@ def expert_linear(x, weight, plan, gates=None):
     ir_mul features is read in place).  weight [E, D, F], of x's type; gates float32 [T, k] (None: ones).  Returns
     [T, (M,) F] of x's type.  Differentiable in x, weight and gates.  float32 products are taken from three bfloat16 parts
     of each operand at float32 accuracy (as the model's linears do); operands beyond 3.38e38 give NaN."""
-    if not isinstance(plan, ExpertPlan):
-        raise TypeError("plan must be an ExpertPlan (plan_experts)")
-    return ops().expert_linear(x, weight, gates, plan.experts, plan.offsets, plan.order)
+    return ops().expert_linear(x, weight, gates, plan)

@@ -36,6 +36,20 @@ def test_plan_is_a_stable_sort(T, k, E):
         assert torch.equal(plan.order[:n].cpu().long(), torch.sort(keys, stable=True).indices[:n])
 
 
+@pytest.mark.parametrize("T,k,E", [(700001, 4, 8), (300000, 1, 1024), (1500000, 2, 64)])
+def test_plan_of_long_lists(T, k, E):
+    """Lists whose tiles' counts are summed by a launch of their own, against a stable sort on the GPU."""
+    from mace_onegpu.experts import plan_experts
+    g = torch.Generator(device="cuda").manual_seed(T)
+    e = torch.randint(-1, E, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    plan = plan_experts(e, E)
+    keys = torch.where(e < 0, E, e).reshape(-1)
+    counts = torch.bincount(keys, minlength=E + 1)
+    assert torch.equal(plan.counts.long(), counts[:E]) and int(plan.offsets[-1]) == int(counts[:E].sum())
+    n = int(plan.offsets[-1])
+    assert torch.equal(plan.order[:n].long(), torch.sort(keys, stable=True).indices[:n])
+
+
 # ------------------------------------------------------------------------------------------------ products
 def _reference(x, w, experts, gates, dy):
     """(results, sums of magnitudes) of [T, M, D] inputs, 64 bits."""
