@@ -354,6 +354,17 @@ int mm_route_bwd(const void* logits, long ldl, int dtype, long T, int E, int k, 
  * expert outside [0, E) order[offsets[E] .. S).  scratch: as many ints as mm_expert_plan_scratch says (0: null) */
 int mm_expert_plan_scratch(int S, int E, long* ints /* HOST */);
 int mm_expert_plan(const int* experts, int S, int E, int* offsets, int* order, int* scratch, mm_stream_t stream);
+/* The rows 0 .. T - 1 of two choices each sorted by the pair of their experts, E <= 21: pair i of (E + 1)(E + 2) / 2 has
+ * the rows from order[offsets[i]] on, the last one to T; pairs e1 <= e2 in ascending order of (e1, e2), an expert outside
+ * [0, E) counting as E.  scratch: of mm_expert_plan_scratch(T, (E + 1)(E + 2) / 2 - 1, ...) ints */
+int mm_expert_plan_pairs(const int* experts, int T, int E, int* offsets, int* order, int* scratch, mm_stream_t stream);
+/* out [T, M, N] (of in's type, rows without an expert 0) = sum over the k = 1 or 2 choices of gate in[t, m] @ W[e] (W as in
+ * mm_expert_rows), joined before they are written; offsets and order of mm_expert_plan (k = 1) or mm_expert_plan_pairs
+ * (k = 2).  dgates [T, k] nullable: with in = dy and W transposed, sum_m <x[t, m], dy[t, m] @ W[e]^T>, N <= 128 (out then
+ * nullable).  M <= 64 */
+int mm_expert_joined(const void* in, long st, long sm, int dtype, int T, int k, int M, int K, int N, const void* W,
+                     int transposed, int E, const float* gates, const int* experts, const int* offsets,
+                     const int* order, void* out, const void* x, long xt, long xm, float* dgates, mm_stream_t stream);
 /* out [S, M, N] (slots without an expert are not written): out[s, m] = in[s / k, m] @ W[e], W [E, K, N], or [E, N, K] with
  * `transposed`; in at (row, component) offset row st + component sm; S M < 2^31 */
 int mm_expert_rows(const void* in, long st, long sm, int dtype, int S, int k, int M, int K, int N, const void* W,

@@ -13,6 +13,7 @@
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 #define MM_EXPERT_MAX_E 1024
+#define MM_PAIRS_MAX_E 21   // 253 pairs
 
 // ------------------------------------------------------------------------------------------------ plan
 // A stable counting sort by expert; slots without an expert are bucket E, at the end of the order.  Tiles of 4,096 slots,
@@ -24,11 +25,30 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 #define MM_PLAN_ONE 4
 #define MM_PLAN_SUM 128
 
-// buckets of four consecutive slots of a tile, number 4 i of it on; -1 past the end
-__device__ __forceinline__ int4 mm_plan_load(const int* __restrict__ experts, int S, int E, int tile, int i4) {
+// Bucket of a pair of choices among E experts and none (number E), in any order: rows e1 <= e2 of a triangle, the pair of
+// no expert at all last.
+__host__ __device__ inline int mm_pair_bucket(int e1, int e2, int E) {
+  const int lo = e1 < e2 ? e1 : e2, hi = e1 < e2 ? e2 : e1;
+  return lo * (E + 1) - lo * (lo - 1) / 2 + hi - lo;
+}
+__host__ __device__ inline int mm_pair_buckets(int E) { return (E + 1) * (E + 2) / 2; }
+
+// Buckets of four consecutive slots of a tile, number 4 i of it on; -1 past the end.  PAIRS: of rows with two choices each,
+// E being the number of buckets less one.
+template <bool PAIRS>
+__device__ __forceinline__ int4 mm_plan_load(const int* __restrict__ experts, int S, int E, int pairs_of, int tile,
+                                             int i4) {
   const long s = (long)tile * MM_PLAN_TILE + 4 * i4;
   int v[4] = {-1, -1, -1, -1};
-  if (s + 4 <= S) {
+  if constexpr (PAIRS) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (s + i < S) {
+        const int a = experts[2 * (s + i)], b = experts[2 * (s + i) + 1];
+        v[i] = mm_pair_bucket((unsigned)a < (unsigned)pairs_of ? a : pairs_of,
+                              (unsigned)b < (unsigned)pairs_of ? b : pairs_of, pairs_of);
+      }
+  } else if (s + 4 <= S) {
     typedef int i4 __attribute__((ext_vector_type(4), aligned(4)));
     const i4 x = *(const i4*)(experts + s);
 #pragma unroll
@@ -49,10 +69,11 @@ __device__ __forceinline__ void mm_plan_count(const int4& v, int* h) {
 }
 
 // counts[tile][bucket]
-__global__ void __launch_bounds__(1024) mm_plan_count_kernel(const int* __restrict__ experts, int S, int E,
+template <bool PAIRS>
+__global__ void __launch_bounds__(1024) mm_plan_count_kernel(const int* __restrict__ experts, int S, int E, int pairs_of,
                                                              int* __restrict__ counts) {
   extern __shared__ int h[];
-  const int4 v = mm_plan_load(experts, S, E, blockIdx.x, threadIdx.x);
+  const int4 v = mm_plan_load<PAIRS>(experts, S, E, pairs_of, blockIdx.x, threadIdx.x);
   for (int i = threadIdx.x; i <= E; i += 1024) h[i] = 0;
   __syncthreads();
   mm_plan_count(v, h);
@@ -92,8 +113,8 @@ __host__ __device__ inline int mm_plan_across(int buckets, int th) {
 // become places in the order.  Bound by the latency of these rounds, so as many waves as the counters leave room for
 // share them (4 instead of 16: 12.6 us instead of the figure below for 4,000 slots of 89 experts).  MODE 0: the other tiles are counted here; 1: the counts of all
 // tiles are added up here; 2: counts are prefix sums, with the totals.  BITS: of the largest bucket, or more.
-template <int MODE, int NW, int BITS>
-__global__ void __launch_bounds__(64 * NW) mm_plan_kernel(const int* __restrict__ experts, int S, int E, int tiles,
+template <int MODE, int NW, int BITS, bool PAIRS>
+__global__ void __launch_bounds__(64 * NW) mm_plan_kernel(const int* __restrict__ experts, int S, int E, int pairs_of, int tiles,
                                                           const int* __restrict__ counts,
                                                           const int* __restrict__ totals, int* __restrict__ offsets,
                                                           int* __restrict__ order) {
@@ -104,13 +125,13 @@ __global__ void __launch_bounds__(64 * NW) mm_plan_kernel(const int* __restrict_
   int *cnt = sm, *total = sm + NW * B, *before = total + B;     // [NW][B], [B], [B]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int i = tid; i < (NW + 2) * B; i += TH) sm[i] = 0;
-  for (int i = tid; i < MM_PLAN_TILE / 4; i += TH) ((int4*)s_e)[i] = mm_plan_load(experts, S, E, blockIdx.x, i);
+  for (int i = tid; i < MM_PLAN_TILE / 4; i += TH) ((int4*)s_e)[i] = mm_plan_load<PAIRS>(experts, S, E, pairs_of, blockIdx.x, i);
   __syncthreads();
   if constexpr (MODE == 0) {
     for (int c = 0; c < tiles; ++c) {
       if (c == (int)blockIdx.x) continue;
       int* to = c < (int)blockIdx.x ? before : total;   // total: the tiles after this one, for now
-      for (int i = tid; i < MM_PLAN_TILE / 4; i += TH) mm_plan_count(mm_plan_load(experts, S, E, c, i), to);
+      for (int i = tid; i < MM_PLAN_TILE / 4; i += TH) mm_plan_count(mm_plan_load<PAIRS>(experts, S, E, pairs_of, c, i), to);
     }
   }
   if constexpr (MODE == 1) {
@@ -195,17 +216,20 @@ struct MMTile {
   int e, row0, rows;   // expert, first of its rows (slots x M), rows in the tile; e < 0: no such tile
 };
 
-// Workgroup b of `per` for each of the tiles of BM rows that the experts' row lists have (every list ends in a cut tile):
-// its tile, and its number within it.  Every wave finds them by itself, 64 experts at a time.  Workgroups are dealt out to
-// the 8 XCDs in turn; the work is numbered so that an XCD gets consecutive pieces, whose operands its L2 then holds.
-__device__ __forceinline__ MMTile mm_expert_tile(const int* __restrict__ offsets, int E, int M, int BM, int per, int b,
-                                                 int* part, int* number) {
+// Workgroup b of `per` for each of the tiles of BM rows that the row lists of the buckets have (every list ends in a cut
+// tile); list i: entries offsets[i] .. offsets[i + 1], the last one to `end`, M rows each.  Every wave finds its tile by
+// itself, 64 lists at a time.  Workgroups are dealt out to the 8 XCDs in turn; the work is numbered so that an XCD gets
+// consecutive pieces, whose operands its L2 then holds.
+__device__ __forceinline__ MMTile mm_expert_tile(const int* __restrict__ offsets, int lists, int end, int M, int BM,
+                                                 int per, int b, int* part, int* number) {
   const int lane = threadIdx.x & 63;
+  auto rows_of = [&](int i) {
+    if (i >= lists) return 0;
+    return ((i + 1 < lists ? offsets[i + 1] : end) - offsets[i]) * M;
+  };
   int all = 0;
-  for (int e0 = 0; e0 < E; e0 += 64) {
-    const int e = e0 + lane;
-    all += e < E ? ((offsets[e + 1] - offsets[e]) * M + BM - 1) / BM : 0;
-  }
+#pragma unroll 4
+  for (int i = lane; i - lane < lists; i += 64) all += (rows_of(i) + BM - 1) / BM;
 #pragma unroll
   for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
   all *= per;
@@ -215,9 +239,8 @@ __device__ __forceinline__ MMTile mm_expert_tile(const int* __restrict__ offsets
   int tile = at / per;
   *part = at - tile * per;
   *number = tile;
-  for (int e0 = 0; e0 < E; e0 += 64) {
-    const int e = e0 + lane;
-    const int rows = e < E ? (offsets[e + 1] - offsets[e]) * M : 0, n = (rows + BM - 1) / BM;
+  for (int i0 = 0; i0 < lists; i0 += 64) {
+    const int rows = rows_of(i0 + lane), n = (rows + BM - 1) / BM;
     int inc = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -228,7 +251,7 @@ __device__ __forceinline__ MMTile mm_expert_tile(const int* __restrict__ offsets
     if (past) {
       const int src = __ffsll(past) - 1;
       const int first = (tile - __shfl(inc - n, src)) * BM, total = __shfl(rows, src);
-      return MMTile{e0 + src, first, min(BM, total - first)};
+      return MMTile{i0 + src, first, min(BM, total - first)};
     }
     tile -= __shfl(inc, 63);
   }
@@ -275,16 +298,18 @@ struct MMRaw<float> {
   float x[8];
 };
 
-template <typename T>
-__device__ __forceinline__ MMFrag<T> mm_operand(const MMRaw<T>& r) {
+// float operands may be scaled on the way
+template <typename T, bool SCALED = false>
+__device__ __forceinline__ MMFrag<T> mm_operand(const MMRaw<T>& r, float scale = 1.f) {
   if constexpr (sizeof(T) == 2) {
     return r.f;
   } else {
     MMFrag<float> f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const __bf16 h = (__bf16)r.x[i];
-      const float d = r.x[i] - (float)h;
+      const float x = SCALED ? scale * r.x[i] : r.x[i];
+      const __bf16 h = (__bf16)x;
+      const float d = x - (float)h;
       const __bf16 l = (__bf16)d;
       f.v[0][i] = h;
       f.v[1][i] = l;
@@ -294,11 +319,12 @@ __device__ __forceinline__ MMFrag<T> mm_operand(const MMRaw<T>& r) {
   }
 }
 
-// acc[i][j] += a(s, i) b(s, j) over the KS steps of a stage: operands b are read two ahead of their products and turned
+// acc[i][j] += a(s, i) b(s, j) scale[j] over the KS steps of a stage (SCALED: float only): operands b are read two ahead of their products and turned
 // into planes one ahead, the next step's operands a over the last products of this one.  The scheduling barriers keep the
 // reads there: left alone, the compiler reads two operands, waits for them and multiplies.
-template <typename T, int FN, int FM, int KS, typename A, typename B>
-__device__ __forceinline__ void mm_products(floatx4 (&acc)[FN][FM], A a, B b) {
+template <typename T, int FN, int FM, int KS, bool SCALED = false, typename A, typename B>
+__device__ __forceinline__ void mm_products(floatx4 (&acc)[FN][FM], A a, B b, const float* scale = nullptr) {
+  auto second = [&](const MMRaw<T>& r, int j) { return mm_operand<T, SCALED>(r, SCALED ? scale[j] : 1.f); };
   constexpr int Q = KS * FM;
   MMFrag<T> fa[KS > 1 ? 2 : 1][FN], fb[2];
   MMRaw<T> rb[3];
@@ -310,17 +336,21 @@ __device__ __forceinline__ void mm_products(floatx4 (&acc)[FN][FM], A a, B b) {
     rb[1] = b(1 / FM, 1 % FM);
 #pragma unroll
     for (int i = 0; i < FN; ++i) fa[0][i] = mm_operand(ra[i]);
-    fb[0] = mm_operand(rb[0]);
+    fb[0] = second(rb[0], 0);
   }
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
     const int s = q / FM, j = q % FM;
     if (q + 2 < Q) rb[(q + 2) % 3] = b((q + 2) / FM, (q + 2) % FM);
     if constexpr (KS > 1) {
-      if (s + 1 < KS && j >= FM - FN) fa[(s + 1) & 1][j - (FM - FN)] = mm_operand(a(s + 1, j - (FM - FN)));
+      if (s + 1 < KS) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+          if ((FN < FM ? i + FM - FN : i * FM / FN) == j) fa[(s + 1) & 1][i] = mm_operand(a(s + 1, i));
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (q + 1 < Q) fb[(q + 1) & 1] = mm_operand(rb[(q + 1) % 3]);
+    if (q + 1 < Q) fb[(q + 1) & 1] = second(rb[(q + 1) % 3], (q + 1) % FM);
 #pragma unroll
     for (int i = 0; i < FN; ++i) mm_mma(acc[i][j], fa[KS > 1 ? s & 1 : 0][i], fb[q & 1]);
     __builtin_amdgcn_sched_barrier(0);
@@ -454,7 +484,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mm_expert_rows_kernel(MMRows 
   uint4 *As = mm_lds, *Bs = As + 2 * BM * 8;             // [2][BM * 8], [2][BN * 8]
   long* s_out = (long*)(Bs + 2 * BN * 8);                // [BM]
   int part, number;
-  const MMTile t = mm_expert_tile(a.offsets, a.E, a.M, BM, tiles_n, blockIdx.x, &part, &number);
+  const MMTile t = mm_expert_tile(a.offsets, a.E, a.offsets[a.E], a.M, BM, tiles_n, blockIdx.x, &part, &number);
   if (t.e < 0) return;
   const int n0 = part * BN;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -535,6 +565,177 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mm_expert_rows_kernel(MMRows 
   }
 }
 
+// ------------------------------------------------------------------------------------------------ joined rows
+// All k <= 2 choices of a row in one workgroup: rows sorted by the set of their experts (the plan of the slots for k = 1, of
+// the pairs for k = 2) share both blocks, so that the products of a row are joined in registers and written once, in its
+// type, where the path through slots writes k fp32 rows and reads them again.  Rows without an expert are written as
+// zeros.  DG (k = 1): with the rows of dy and W[e]^T, also dgates[t] = sum over m of <x[t, m], (dy W^T)[t, m]>; a tile
+// holds whole rows t (all M components) and all columns.
+struct MMJoined {
+  const void *in, *W, *x;
+  const float* gates;
+  const int *experts, *offsets, *order;   // offsets [buckets]: where each set's rows begin
+  void* out;
+  float* dgates;
+  long st, sm, xt, xm;
+  int T, M, K, N, E, buckets;
+};
+
+template <typename T, bool TRANS, bool DMA, int J, bool DG, int BM>
+__global__ void __launch_bounds__(256, 2) mm_expert_joined_kernel(MMJoined a, int tiles_n) {
+  constexpr int BN = 128, WM = 2, WN = 2, TH = 256, BK = MM_TILE_K<T>, N = MMVec<T>::N, UPR = BN / N;
+  constexpr int KS = BK / 32, UA = BM * 8 / TH, UB = BN * 8 / TH, FM = BM / WM / 16, FN = BN / WN / 16;
+  __shared__ uint4 As[2 * BM * 8], Bs[2 * BN * 8];
+  __shared__ long s_out[BM], s_x[DG ? BM : 1];
+  __shared__ float s_g[J][BM], s_dg[DG ? WN : 1][BM];
+  int part, number;
+  const int rows_of_tile = BM / a.M * a.M;
+  const MMTile t = mm_expert_tile(a.offsets, a.buckets, a.T, a.M, rows_of_tile, tiles_n, blockIdx.x, &part, &number);
+  if (t.e < 0) return;
+  const int n0 = part * BN;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int e[J];   // this set's experts, a.E: none
+  if constexpr (J == 1) {
+    e[0] = t.e;
+  } else {
+    int lo = 0, rest = t.e;
+    while (rest >= a.E + 1 - lo) rest -= a.E + 1 - lo++;
+    e[0] = lo;
+    e[1] = lo + rest;
+  }
+  const int* __restrict__ list = a.order + a.offsets[t.e];
+  if (tid < BM) {
+    const int r = t.row0 + min(tid, t.rows - 1), p = r / a.M, m = r - p * a.M, tok = list[p];
+    s_out[tid] = ((long)tok * a.M + m) * a.N;
+    if constexpr (DG) s_x[tid] = tok * a.xt + m * a.xm;
+    if constexpr (J == 1) {
+      s_g[0][tid] = a.gates ? a.gates[tok] : 1.f;
+    } else {
+      const int first = a.experts[2 * (long)tok], swap = ((unsigned)first < (unsigned)a.E ? first : a.E) != e[0];
+      s_g[0][tid] = a.gates ? a.gates[2 * (long)tok + swap] : 1.f;
+      s_g[1][tid] = a.gates ? a.gates[2 * (long)tok + (1 - swap)] : 1.f;
+    }
+  }
+  const int ka = ((tid & 7) ^ (tid >> 3 & 7)) * N;
+  const T *pa[UA];
+  int kb[UB], nb[UB];
+  long ob[UB];
+#pragma unroll
+  for (int j = 0; j < UA; ++j) {
+    const int row = (tid + TH * j) >> 3;
+    const int r = t.row0 + min(row, t.rows - 1), p = r / a.M, m = r - p * a.M;
+    pa[j] = (const T*)a.in + (long)list[p] * a.st + m * a.sm + ka;
+  }
+#pragma unroll
+  for (int j = 0; j < UB; ++j) {
+    const int pu = tid + TH * j;
+    if constexpr (TRANS) {
+      const int n = n0 + (pu >> 3);
+      nb[j] = n < a.N;
+      kb[j] = ka;
+      ob[j] = (long)min(n, a.N - 1) * a.K + ka;
+    } else {
+      const int q = pu / UPR, u = (pu % UPR) ^ mm_nc_swizzle<T, UPR>(q);
+      kb[j] = q;
+      nb[j] = a.N - n0 - u * N;
+      ob[j] = (long)q * a.N + n0 + u * N;
+    }
+  }
+  MMStage<T, TH, UA, DMA> sa;
+  MMStage<T, TH, UB, DMA> sb;
+  auto load = [&](int c, int k0, int buf) {
+    const T* __restrict__ W = (const T*)a.W + (size_t)e[c] * a.K * a.N;
+#pragma unroll
+    for (int j = 0; j < UA; ++j) sa.load(As + buf * BM * 8, j, pa[j] + k0, a.K - k0 - ka);
+#pragma unroll
+    for (int j = 0; j < UB; ++j) {
+      if constexpr (TRANS) sb.load(Bs + buf * BN * 8, j, W + ob[j] + k0, nb[j] ? a.K - k0 - kb[j] : 0);
+      else sb.load(Bs + buf * BN * 8, j, W + ob[j] + (size_t)k0 * a.N, k0 + kb[j] < a.K ? nb[j] : 0);
+    }
+  };
+  auto put = [&](int buf) {
+    sa.put(As + buf * BM * 8);
+    sb.put(Bs + buf * BN * 8);
+  };
+  // The gates: on the rows' values as they become operands (float without DG: one more rounding of 2^-24), or on each
+  // choice's products, in sums of their own (16 bits, where the operands' rounding would show; DG, which needs the
+  // products without the gates).
+  constexpr bool SCALED = sizeof(T) == 4 && !DG, SUM = !SCALED;
+  floatx4 acc[FN][FM] = {}, sum[SUM ? FN : 1][SUM ? FM : 1] = {};
+  const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+  int buf = 0;
+  if (e[0] < a.E) {   // the choices without an expert are the last ones
+    load(0, 0, 0);
+    put(0);
+  }
+  mm_stage_done();
+#pragma unroll 1
+  for (int c = 0; c < J; ++c) {
+    if (e[c] >= a.E) break;
+    float gs[FM];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) gs[j] = s_g[c][wm + 16 * j + (lane & 15)];
+    for (int k0 = 0; k0 < a.K; k0 += BK) {
+      const bool same = k0 + BK < a.K, more = same || (c + 1 < J && e[c + 1 < J ? c + 1 : c] < a.E);
+      if (more) load(same ? c : c + 1, same ? k0 + BK : 0, buf ^ 1);
+      const uint4 *A = As + buf * BM * 8, *B = Bs + buf * BN * 8;
+      mm_products<T, FN, FM, KS, SCALED>(
+          acc,
+          [&](int s, int i) {
+            if constexpr (TRANS) return mm_read_kc<T>(B, wn + 16 * i, s, lane);
+            else return mm_read_nc<T, UPR>(B, wn + 16 * i, s, lane);
+          },
+          [&](int s, int j) { return mm_read_kc<T>(A, wm + 16 * j, s, lane); }, gs);
+      if (more) put(buf ^ 1);
+      mm_stage_done();
+      buf ^= 1;
+    }
+    if constexpr (SUM) {
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        const int m = wm + 16 * j + (lane & 15);
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+          if constexpr (DG) {
+            float xv[4];
+            mm_load4((const T*)a.x + s_x[m], n0 + wn + 16 * i + 4 * (lane >> 4), a.N, xv);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) dot = fmaf(xv[q], acc[i][j][q], dot);
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) sum[i][j][q] = fmaf(gs[j], acc[i][j][q], sum[i][j][q]);
+          acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+        if constexpr (DG) {
+          dot += __shfl_xor(dot, 16);
+          dot += __shfl_xor(dot, 32);
+          if (lane < 16) s_dg[wave / WM][m] = dot;
+        }
+      }
+    }
+    if constexpr (DG) {
+      __syncthreads();
+      if (tid < t.rows / a.M) {
+        float d = 0.f;
+        for (int m = tid * a.M; m < (tid + 1) * a.M; ++m) d += s_dg[0][m] + s_dg[1][m];
+        a.dgates[list[t.row0 / a.M + tid]] = d;
+      }
+      __syncthreads();
+    }
+  }
+  if constexpr (DG)
+    if (e[0] >= a.E && tid < t.rows / a.M) a.dgates[list[t.row0 / a.M + tid]] = 0.f;
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    const int m = wm + 16 * j + (lane & 15);
+    if (m >= t.rows || !a.out) continue;
+    T* __restrict__ o = (T*)a.out + s_out[m];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) mm_store4(o, n0 + wn + 16 * i + 4 * (lane >> 4), a.N, (const float*)&(SUM ? sum[SUM ? i : 0][SUM ? j : 0] : acc[i][j]));
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ few rows
 // y[t, m] straight from the choices of row t, without a plan: a workgroup takes LC vectors of columns, its other threads
 // share the sum over d, W is read once per row, coalesced along the columns, fp32 sums.  Bound by latency: the sum over d is
@@ -596,31 +797,6 @@ struct MMCombine {
   long T;
   int k, M, N, E;
 };
-
-template <typename T>
-__device__ __forceinline__ void mm_store4(T* __restrict__ p, int c, int N, const float* v) {
-  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  if (c + 4 <= N) {
-    *(vec*)(p + c) = vec{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (c + q < N) p[c + q] = (T)v[q];
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void mm_load4(const T* __restrict__ p, int c, int N, float* v) {
-  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  if (c + 4 <= N) {
-    const vec x = *(const vec*)(p + c);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = (float)x[q];
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = c + q < N ? (float)p[c + q] : 0.f;
-  }
-}
 
 // one vector of y a thread
 template <typename T>
@@ -733,7 +909,7 @@ __global__ void __launch_bounds__(64 * WD * WF, 2) mm_expert_wgrad_kernel(MMWgra
   int df, tile;
   MMTile t;
   if constexpr (SPLIT) {
-    t = mm_expert_tile(a.offsets, a.E, a.M, chunk, tiles_df, blockIdx.x, &df, &tile);
+    t = mm_expert_tile(a.offsets, a.E, a.offsets[a.E], a.M, chunk, tiles_df, blockIdx.x, &df, &tile);
     if (t.e < 0) return;
   } else {   // an XCD gets every 8th expert: lists of different lengths, each read by one XCD
     const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
@@ -956,10 +1132,11 @@ extern "C" int mm_expert_plan_scratch(int S, int E, long* ints) {
   return MM_OK;
 }
 
-extern "C" int mm_expert_plan(const int* experts, int S, int E, int* offsets, int* order, int* scratch,
-                              hipStream_t stream) {
-  MM_CHECK_ARG(S >= 0 && E >= 1, "bad sizes");
-  if (E > MM_EXPERT_MAX_E) return range_error("mm_expert_plan", "more than 1024 experts are not supported");
+namespace {
+// buckets 0 .. E; PAIRS: of S rows with two of pairs_of experts each, E + 1 = mm_pair_buckets(pairs_of)
+template <bool PAIRS>
+int launch_plan(const char* name, const int* experts, int S, int E, int pairs_of, int* offsets, int* order, int* scratch,
+                hipStream_t stream) {
   const int tiles = (int)(((long)S + MM_PLAN_TILE - 1) / MM_PLAN_TILE), one = tiles <= MM_PLAN_ONE;
   MM_CHECK_ARG(one || scratch, "scratch is null");
   // 16 waves while their counters fit 64 KB of LDS beside the tile, else 4
@@ -967,14 +1144,14 @@ extern "C" int mm_expert_plan(const int* experts, int S, int E, int* offsets, in
   const int lds = (nw + 2) * (E + 1) * (int)sizeof(int);
   int *counts = scratch, *totals = scratch + (size_t)tiles * (E + 1);
   if (!one)
-    hipLaunchKernelGGL(mm_plan_count_kernel, dim3(tiles), dim3(1024), (E + 1) * sizeof(int), stream, experts, S, E,
-                       counts);
+    hipLaunchKernelGGL(mm_plan_count_kernel<PAIRS>, dim3(tiles), dim3(1024), (E + 1) * sizeof(int), stream, experts, S, E,
+                       pairs_of, counts);
   const bool sums = ((long)tiles * across + th - 1) / th * ((E + across) / across) <= MM_PLAN_SUM;
   if (!one && !sums)
     hipLaunchKernelGGL(mm_plan_scan_kernel, dim3(E + 1), dim3(64), 0, stream, counts, tiles, E, totals);
-#define CALL(mode, nw, bits)                                                                                        \
-  hipLaunchKernelGGL((mm_plan_kernel<mode, nw, bits>), dim3(tiles ? tiles : 1), dim3(64 * nw), lds, stream, experts, S, \
-                     E, tiles, counts, totals, offsets, order)
+#define CALL(mode, nw, bits)                                                                                            \
+  hipLaunchKernelGGL((mm_plan_kernel<mode, nw, bits, PAIRS>), dim3(tiles ? tiles : 1), dim3(64 * nw), lds, stream, experts, \
+                     S, E, pairs_of, tiles, counts, totals, offsets, order)
 #define CALLS(mode)                      \
   if (nw == 4) CALL(mode, 4, 11);        \
   else if (E < 16) CALL(mode, 16, 4);    \
@@ -985,7 +1162,24 @@ extern "C" int mm_expert_plan(const int* experts, int S, int E, int* offsets, in
   else { CALLS(2) }
 #undef CALLS
 #undef CALL
-  return mm::launch_status("mm_expert_plan");
+  return mm::launch_status(name);
+}
+}  // namespace
+
+extern "C" int mm_expert_plan(const int* experts, int S, int E, int* offsets, int* order, int* scratch,
+                              hipStream_t stream) {
+  MM_CHECK_ARG(S >= 0 && E >= 1, "bad sizes");
+  if (E > MM_EXPERT_MAX_E) return range_error("mm_expert_plan", "more than 1024 experts are not supported");
+  MM_CHECK_ARG(S <= MM_PLAN_ONE * MM_PLAN_TILE || scratch, "scratch is null");
+  return launch_plan<false>("mm_expert_plan", experts, S, E, 0, offsets, order, scratch, stream);
+}
+
+extern "C" int mm_expert_plan_pairs(const int* experts, int T, int E, int* offsets, int* order, int* scratch,
+                                    hipStream_t stream) {
+  MM_CHECK_ARG(T >= 0 && E >= 1, "bad sizes");
+  if (E > MM_PAIRS_MAX_E) return range_error("mm_expert_plan_pairs", "pairs of more than 21 experts are not supported");
+  MM_CHECK_ARG(T <= MM_PLAN_ONE * MM_PLAN_TILE || scratch, "scratch is null");
+  return launch_plan<true>("mm_expert_plan_pairs", experts, T, mm_pair_buckets(E) - 1, E, offsets, order, scratch, stream);
 }
 
 extern "C" int mm_expert_rows(const void* in, long st, long sm, int dtype, int S, int k, int M, int K, int N,
@@ -1027,6 +1221,43 @@ extern "C" int mm_expert_few(const void* x, long st, long sm, int dtype, int T, 
   else CALL(_Float16);
 #undef CALL
   return mm::launch_status("mm_expert_few");
+}
+
+extern "C" int mm_expert_joined(const void* in, long st, long sm, int dtype, int T, int k, int M, int K, int N,
+                                const void* W, int transposed, int E, const float* gates, const int* experts,
+                                const int* offsets, const int* order, void* out, const void* x, long xt, long xm,
+                                float* dgates, hipStream_t stream) {
+  MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");
+  MM_CHECK_ARG(T >= 0 && M >= 1 && K >= 1 && N >= 1 && E >= 1 && st >= 0 && sm >= 0, "bad sizes");
+  MM_CHECK_ARG(k == 1 || k == 2, "k must be 1 or 2");
+  MM_CHECK_ARG(!dgates || (k == 1 && transposed && x && xt >= 0 && xm >= 0 && N <= 128),
+               "dgates needs one choice, the transposed blocks, x and at most 128 columns");
+  if (M > 64) return range_error("mm_expert_joined", "more than 64 components are not supported");
+  if (k == 2 && E > MM_PAIRS_MAX_E)
+    return range_error("mm_expert_joined", "pairs of more than 21 experts are not supported");
+  if ((long)T * M > 2147483647L - 128) return range_error("mm_expert_joined", "2^31 rows or more are not supported");
+  if (T == 0) return MM_OK;
+  const int buckets = k == 1 ? E + 1 : mm_pair_buckets(E), tiles_n = (N + 127) / 128, tile = (dtype == MM_F32 ? 128 : 64) / M;   // rows t a tile
+  const long wg = (((long)T + tile - 1) / tile + (buckets < T ? buckets : T)) * tiles_n;
+  if (wg > 2147483647L) return range_error("mm_expert_joined", "output too large for one launch");
+  const MMJoined a{in, W, x, gates, experts, offsets, order, out, dgates, st, sm, xt, xm, T, M, K, N, E, buckets};
+  const int unit = dtype == MM_F32 ? 4 : 8;
+  const bool dma = aligned(in) && aligned(W) && st % unit == 0 && (M == 1 || sm % unit == 0) && K % unit == 0 &&
+                   (transposed || N % unit == 0);
+#define CALL4(trans, dma, j, dg) \
+  MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_joined_kernel<T_, trans, dma, j, dg, sizeof(T_) == 4 ? 128 : 64>), dim3((unsigned)wg), dim3(256), 0, \
+                                        stream, a, tiles_n))
+#define CALL3(trans, j, dg) if (dma) { CALL4(trans, true, j, dg); } else { CALL4(trans, false, j, dg); }
+#define CALL2(j) \
+  if (transposed) { CALL3(true, j, false) } \
+  else { CALL3(false, j, false) }
+  if (dgates) { CALL3(true, 1, true) }
+  else if (k == 1) { CALL2(1) }
+  else { CALL2(2) }
+#undef CALL2
+#undef CALL3
+#undef CALL4
+  return mm::launch_status("mm_expert_joined");
 }
 
 extern "C" int mm_expert_combine(const float* rows, const float* gates, const int* experts, int dtype, long T, int k,
@@ -1097,7 +1328,7 @@ extern "C" int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, 
 #undef CALL
   if (rc != MM_OK) return rc;
   if (chunk)
-    MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_wgrad_sum_kernel<T>),
+    MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_wgrad_sum_kernel<T_>),
                                           dim3((unsigned)(((long)D * F + 1023) / 1024), E), dim3(256), 0, stream, a, chunk,
                                           workspace));
   return mm::launch_status("mm_expert_wgrad");

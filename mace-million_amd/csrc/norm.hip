@@ -250,9 +250,9 @@ extern "C" int mm_layernorm_fwd(const void* x, long ldx, int dtype, long rows, i
   const long rpb = norm_rows_per_wg(lpr), n = (rows + rpb - 1) / rpb;
   const dim3 grid((unsigned)(n < 4096 ? n : 4096));
 #define X(i, l, v)                                                                                              \
-  if constexpr (l * v * MMVec<T>::N <= MM_NORM_MAX_D) if (sh == i)                                              \
-    hipLaunchKernelGGL((mm_layernorm_fwd_kernel<T, l, v>), grid, dim3(l > 256 ? l : 256), 0, stream, (const T*)x, \
-                       ldx, rows, D, w, b, p_dtype == MM_F32, eps, (T*)y, ldy, mean, rstd);
+  if constexpr (l * v * MMVec<T_>::N <= MM_NORM_MAX_D) if (sh == i)                                              \
+    hipLaunchKernelGGL((mm_layernorm_fwd_kernel<T_, l, v>), grid, dim3(l > 256 ? l : 256), 0, stream, (const T_*)x, \
+                       ldx, rows, D, w, b, p_dtype == MM_F32, eps, (T_*)y, ldy, mean, rstd);
   MM_DISPATCH(dtype, MM_NORM_SHAPES(X));
 #undef X
   return mm::launch_status("mm_layernorm_fwd");
@@ -278,9 +278,9 @@ extern "C" int mm_layernorm_bwd(const void* dy, long lddy, const void* x, long l
   const int sh = shape_of(D, dtype), n = bwd_workgroups(rows, kShapes[sh].lpr);
   float* part = dw || db ? workspace : nullptr;
 #define X(i, l, v)                                                                                               \
-  if constexpr (l * v * MMVec<T>::N <= MM_NORM_MAX_D) if (sh == i)                                               \
-    hipLaunchKernelGGL((mm_layernorm_bwd_kernel<T, l, v>), dim3(n), dim3(l > 256 ? l : 256), 0, stream,          \
-                       (const T*)dy, lddy, (const T*)x, ldx, rows, D, w, p_dtype == MM_F32, mean, rstd, (T*)dx,  \
+  if constexpr (l * v * MMVec<T_>::N <= MM_NORM_MAX_D) if (sh == i)                                               \
+    hipLaunchKernelGGL((mm_layernorm_bwd_kernel<T_, l, v>), dim3(n), dim3(l > 256 ? l : 256), 0, stream,          \
+                       (const T_*)dy, lddy, (const T_*)x, ldx, rows, D, w, p_dtype == MM_F32, mean, rstd, (T_*)dx,  \
                        lddx, part);
   if (n && (dx || part)) MM_DISPATCH(dtype, MM_NORM_SHAPES(X));
 #undef X

@@ -42,6 +42,16 @@ __device__ __forceinline__ unsigned mm_route_max(unsigned v) {
   return v;
 }
 
+// exp(x) for x <= 0 (NaN stays NaN) to 2 units in the last place: 2^(x log2 e) with the rounding error of the product put
+// back to first order.  A softmax over a whole row takes one per logit, and expf twice the instructions.
+__device__ __forceinline__ float mm_exp_neg(float x) {
+  x = x < -150.f ? -150.f : x;   // 0 either way
+  const float t = x * 1.44269504088896340736f;
+  const float lo = fmaf(x, 1.92596299112661746887e-8f, fmaf(x, 1.44269504088896340736f, -t));
+  const float p = __builtin_amdgcn_exp2f(t);
+  return fmaf(p, lo * 0.693147180559945309417f, p);
+}
+
 // C consecutive values of a row from column c on, `none` past the last one
 template <typename T, int C>
 __device__ __forceinline__ void mm_route_load(const T* __restrict__ p, int c, int E, float none, float* v) {
@@ -66,11 +76,12 @@ struct MMRoute {
   float scale;
 };
 
-template <typename T, int LPR, int C>
+// KM: results a lane keeps (choice q LPR + lane), enough for k
+template <typename T, int LPR, int C, int KM>
 __global__ void __launch_bounds__(256) mm_route_fwd_kernel(MMRoute a, const T* __restrict__ logits,
                                                            const float* __restrict__ bias, float* __restrict__ gates,
                                                            int* __restrict__ experts) {
-  constexpr int RPB = 256 / LPR, KM = (MM_ROUTE_MAX_K + LPR - 1) / LPR;   // rows per workgroup, results per lane
+  constexpr int RPB = 256 / LPR;   // rows per workgroup
   __shared__ unsigned s_best[RPB][MM_ROUTE_MAX_G], s_open[RPB][2];
   const int lane = threadIdx.x & (LPR - 1), sub = threadIdx.x / LPR, c0 = lane * C;
   const long row = (long)blockIdx.x * RPB + sub;
@@ -90,11 +101,19 @@ __global__ void __launch_bounds__(256) mm_route_fwd_kernel(MMRoute a, const T* _
     for (int q = lane; q < a.groups; q += LPR) s_best[sub][q] = 0;
     if (lane < 2) s_open[sub][lane] = 0;
     mm_wave_lds_sync();
+    const bool whole = gs % C == 0;   // a lane's logits belong to one group
     int g = g0, m = rem;
+    if (whole) {
+      unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      if (c0 + i < a.E) atomicMax(&s_best[sub][g], key[i]);
-      if (++m == gs) { m = 0; ++g; }
+      for (int i = 0; i < C; ++i) top = max(top, key[i]);
+      if (c0 < a.E) atomicMax(&s_best[sub][g], top);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        if (c0 + i < a.E) atomicMax(&s_best[sub][g], key[i]);
+        if (++m == gs) { m = 0; ++g; }
+      }
     }
     mm_wave_lds_sync();
     for (int q = lane; q < a.groups; q += LPR) {
@@ -110,10 +129,16 @@ __global__ void __launch_bounds__(256) mm_route_fwd_kernel(MMRoute a, const T* _
     const unsigned open0 = s_open[sub][0], open1 = s_open[sub][1];
     g = g0;
     m = rem;
+    if (whole) {
+      const bool shut = !((g < 32 ? open0 : open1) >> (g & 31) & 1);
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      if (!((g < 32 ? open0 : open1) >> (g & 31) & 1)) key[i] = 0;
-      if (++m == gs) { m = 0; ++g; }
+      for (int i = 0; i < C; ++i) key[i] = shut ? 0 : key[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        if (!((g < 32 ? open0 : open1) >> (g & 31) & 1)) key[i] = 0;
+        if (++m == gs) { m = 0; ++g; }
+      }
     }
   }
   // softmax over all experts, where the gates keep its normalisation
@@ -125,53 +150,40 @@ __global__ void __launch_bounds__(256) mm_route_fwd_kernel(MMRoute a, const T* _
     top = mm_lanes_max<LPR>(top);
     whole = 0.f;
 #pragma unroll
-    for (int i = 0; i < C; ++i) whole += expf(x[i] - top);   // rows with nothing open have no gate that uses it
+    for (int i = 0; i < C; ++i) whole += mm_exp_neg(x[i] - top);   // rows with nothing open have no gate that uses it
     whole = mm_lanes_sum<LPR>(whole);
   }
   unsigned best = 0;
 #pragma unroll
   for (int i = 0; i < C; ++i) best = max(best, key[i]);
-  float xj[KM];
   int ej[KM];
 #pragma unroll
-  for (int q = 0; q < KM; ++q) {
-    xj[q] = none;
-    ej[q] = -1;
-  }
+  for (int q = 0; q < KM; ++q) ej[q] = -1;
   const int first_lane = (threadIdx.x & 63) & ~(LPR - 1);
   for (int j = 0; j < a.k; ++j) {
     const unsigned m = mm_route_max<LPR>(best);
     if (__ballot(m != 0) == 0) break;   // no row of the wave has an open expert left
     const unsigned long long have = __ballot(best == m) >> first_lane;
     const int src = __ffsll((unsigned long long)have) - 1;   // the lane of this row with the lowest such index
-    // every lane's first logit of its best key
-    float xb = 0.f;
-    int ib = 0;
+    int ib = 0;                                              // every lane's first logit of its best key
 #pragma unroll
-    for (int i = C - 1; i >= 0; --i)
-      if (key[i] == best) {
-        xb = x[i];
-        ib = i;
-      }
-    const float xw = __shfl(xb, src, LPR);
+    for (int i = C - 1; i >= 0; --i) ib = key[i] == best ? i : ib;
     const int ew = __shfl(c0 + ib, src, LPR);
-    if (m != 0) {
 #pragma unroll
-      for (int q = 0; q < KM; ++q)
-        if (j == q * LPR + lane) {
-          xj[q] = xw;
-          ej[q] = ew;
-        }
-    }
+    for (int q = 0; q < KM; ++q)
+      if (m != 0 && j == q * LPR + lane) ej[q] = ew;
     if (lane == src) {
       best = 0;
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        if (i == ib) key[i] = 0;
+        key[i] = i == ib ? 0 : key[i];
         best = max(best, key[i]);
       }
     }
   }
+  float xj[KM];
+#pragma unroll
+  for (int q = 0; q < KM; ++q) xj[q] = ej[q] >= 0 ? (float)logits[r * a.ldl + ej[q]] : none;
   float gj[KM];
   if (a.renorm) {
     float m = none, sum = 0.f;
@@ -210,12 +222,12 @@ __global__ void __launch_bounds__(256) mm_route_fwd_kernel(MMRoute a, const T* _
 //   softmax, plain     dl_e = [e chosen] gate_e dgate_e - p_e sum_j gate_j dgate_j,  p over all E logits
 // and d log score / dl = 1 (softmax, renormalised) or 1 - sigmoid(l).  The E values of a row are put together in LDS and
 // written once; the logits are read where a formula has them.  Bound by HBM.
-template <typename T, int LPR, int C>
+template <typename T, int LPR, int C, int KM>
 __global__ void __launch_bounds__(256) mm_route_bwd_kernel(MMRoute a, const T* __restrict__ logits,
                                                            const float* __restrict__ gates,
                                                            const int* __restrict__ experts,
                                                            const float* __restrict__ dgates, T* __restrict__ dlogits) {
-  constexpr int RPB = 256 / LPR, KM = (MM_ROUTE_MAX_K + LPR - 1) / LPR;
+  constexpr int RPB = 256 / LPR;
   __shared__ float s_d[RPB][LPR * C];
   const int lane = threadIdx.x & (LPR - 1), sub = threadIdx.x / LPR, c0 = lane * C;
   const long row = (long)blockIdx.x * RPB + sub;
@@ -250,7 +262,7 @@ __global__ void __launch_bounds__(256) mm_route_bwd_kernel(MMRoute a, const T* _
     top = mm_lanes_max<LPR>(top);
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      v[i] = expf(x[i] - top);
+      v[i] = mm_exp_neg(x[i] - top);
       whole += v[i];
     }
     whole = mm_lanes_sum<LPR>(whole);
@@ -310,15 +322,16 @@ int route_args(const char* name, int dtype, long T, int E, int k, int scoring, i
 }  // namespace
 
 // lanes a row and logits a lane by E: few lanes keep the rounds' lane maxima short and let a wave work on many rows,
-// until a lane's own logits cost more
+// until a lane's own logits cost more; one result a lane where k allows it
+#define MM_ROUTE_K(X, l, c) if (k <= l) { X(l, c, 1) } else { X(l, c, ((MM_ROUTE_MAX_K + l - 1) / l)) }
 #define MM_ROUTE_SHAPES(X)  \
-  if (E <= 16) { X(4, 4) }  \
-  else if (E <= 32) { X(8, 4) } \
-  else if (E <= 64) { X(16, 4) } \
-  else if (E <= 128) { X(16, 8) } \
-  else if (E <= 256) { X(16, 16) } \
-  else if (E <= 512) { X(32, 16) } \
-  else { X(64, 16) }
+  if (E <= 16) { MM_ROUTE_K(X, 4, 4) }  \
+  else if (E <= 32) { MM_ROUTE_K(X, 8, 4) } \
+  else if (E <= 64) { MM_ROUTE_K(X, 16, 4) } \
+  else if (E <= 128) { MM_ROUTE_K(X, 16, 8) } \
+  else if (E <= 256) { MM_ROUTE_K(X, 16, 16) } \
+  else if (E <= 512) { X(32, 16, 1) } \
+  else { X(64, 16, 1) }
 
 extern "C" int mm_route_fwd(const void* logits, long ldl, int dtype, long T, int E, int k, int scoring,
                             const float* bias, int groups, int top_groups, int renorm, float scale, float* gates,
@@ -326,8 +339,8 @@ extern "C" int mm_route_fwd(const void* logits, long ldl, int dtype, long T, int
   MMRoute a;
   const int rc = route_args("mm_route_fwd", dtype, T, E, k, scoring, groups, top_groups, ldl, scale, &a, renorm);
   if (rc != MM_OK || T == 0) return rc;
-#define X(l, c)                                                                                               \
-  hipLaunchKernelGGL((mm_route_fwd_kernel<T_, l, c>), dim3((unsigned)((a.T + 256 / l - 1) / (256 / l))), dim3(256), 0, \
+#define X(l, c, km)                                                                                             \
+  hipLaunchKernelGGL((mm_route_fwd_kernel<T_, l, c, km>), dim3((unsigned)((a.T + 256 / l - 1) / (256 / l))), dim3(256), 0, \
                      stream, a, (const T_*)logits, bias, gates, experts);
   if (dtype == MM_F32) { using T_ = float; MM_ROUTE_SHAPES(X) }
   else if (dtype == MM_BF16) { using T_ = __bf16; MM_ROUTE_SHAPES(X) }
@@ -342,8 +355,8 @@ extern "C" int mm_route_bwd(const void* logits, long ldl, int dtype, long T, int
   MMRoute a;
   const int rc = route_args("mm_route_bwd", dtype, T, E, k, scoring, 1, 1, ldl, scale, &a, renorm);
   if (rc != MM_OK || T == 0) return rc;
-#define X(l, c)                                                                                               \
-  hipLaunchKernelGGL((mm_route_bwd_kernel<T_, l, c>), dim3((unsigned)((a.T + 256 / l - 1) / (256 / l))), dim3(256), 0, \
+#define X(l, c, km)                                                                                             \
+  hipLaunchKernelGGL((mm_route_bwd_kernel<T_, l, c, km>), dim3((unsigned)((a.T + 256 / l - 1) / (256 / l))), dim3(256), 0, \
                      stream, a, (const T_*)logits, gates, experts, dgates, (T_*)dlogits);
   if (dtype == MM_F32) { using T_ = float; MM_ROUTE_SHAPES(X) }
   else if (dtype == MM_BF16) { using T_ = __bf16; MM_ROUTE_SHAPES(X) }

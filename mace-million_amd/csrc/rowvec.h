@@ -7,12 +7,12 @@
 #define MM_BF16 1
 #define MM_F16 2
 
-// Calls fn<T>() for the element type of a dtype argument.
+// CALL with T_ as the element type of a dtype argument.
 #define MM_DISPATCH(dtype, CALL)                     \
   do {                                               \
-    if ((dtype) == MM_F32) { using T = float; CALL; }      \
-    else if ((dtype) == MM_BF16) { using T = __bf16; CALL; } \
-    else { using T = _Float16; CALL; }               \
+    if ((dtype) == MM_F32) { using T_ = float; CALL; }      \
+    else if ((dtype) == MM_BF16) { using T_ = __bf16; CALL; } \
+    else { using T_ = _Float16; CALL; }               \
   } while (0)
 
 // 16 bytes of T, known to be aligned to one element only
@@ -48,6 +48,32 @@ __device__ __forceinline__ void mm_store_vec(T* __restrict__ p, int c, int D, co
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (c + i < D) p[c + i] = (T)v[i];
+  }
+}
+
+// four values, likewise
+template <typename T>
+__device__ __forceinline__ void mm_store4(T* __restrict__ p, int c, int N, const float* v) {
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (c + 4 <= N) {
+    *(vec*)(p + c) = vec{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (c + q < N) p[c + q] = (T)v[q];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void mm_load4(const T* __restrict__ p, int c, int N, float* v) {
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (c + 4 <= N) {
+    const vec x = *(const vec*)(p + c);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = (float)x[q];
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = c + q < N ? (float)p[c + q] : 0.f;
   }
 }
 

@@ -10,8 +10,12 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/sub.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
+#include <cmath>
+#include <memory>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -256,24 +260,46 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::str
 }
 
 // ------------------------------------------------------------------------------------------------ plan
-// The sorted lists of long lists of slots are made with the plan; few slots may do without (few_rows), theirs are made
-// when something first asks for them.
-constexpr long kPlanNow = 1024;
+struct Lists { Tensor offsets, order; };
+
+Lists make_lists(const Tensor& experts, long E) {
+  const long S = experts.numel();
+  long scratch = 0;
+  done(mm_expert_plan_scratch((int)S, (int)E, &scratch));
+  const Tensor buf = i32({S + E + 1 + scratch}, experts);
+  int* p = iptr(buf);
+  done(mm_expert_plan(iptr(experts), (int)S, (int)E, p, p + E + 1, scratch ? p + E + 1 + S : nullptr, stream()));
+  return {buf.narrow(0, 0, E + 1), buf.narrow(0, E + 1, S)};
+}
+
+// rows of two choices sorted by the pair of their experts
+Lists make_pairs(const Tensor& experts, long E) {
+  const long T = experts.size(0), buckets = (E + 1) * (E + 2) / 2;
+  long scratch = 0;
+  done(mm_expert_plan_scratch((int)T, (int)buckets - 1, &scratch));
+  const Tensor buf = i32({T + buckets + scratch}, experts);
+  int* p = iptr(buf);
+  done(mm_expert_plan_pairs(iptr(experts), (int)T, (int)E, p, p + buckets, scratch ? p + buckets + T : nullptr, stream()));
+  return {buf.narrow(0, 0, buckets), buf.narrow(0, buckets, T)};
+}
+
+// Up to kPlanLater slots the sort waits until something needs it: few rows do without.  Under graph capture nothing waits,
+// so that a captured plan is sorted by every replay; lists that a capture needs of an older plan are its own and are not
+// kept (they hold nothing until a replay).
+constexpr long kPlanLater = 1024;
+
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
 struct Plan {
-  Tensor experts, offsets, order;
+  Tensor experts;
   long T, k, E;
+  Lists kept;
 
-  void lists() {
-    if (offsets.defined()) return;
-    const long S = T * k;
-    long scratch = 0;
-    done(mm_expert_plan_scratch((int)S, (int)E, &scratch));
-    const Tensor buf = i32({S + E + 1 + scratch}, experts);
-    int* p = iptr(buf);
-    done(mm_expert_plan(iptr(experts), (int)S, (int)E, p, p + E + 1, scratch ? p + E + 1 + S : nullptr, stream()));
-    offsets = buf.narrow(0, 0, E + 1);
-    order = buf.narrow(0, E + 1, S);
+  Lists lists() {
+    if (kept.offsets.defined()) return kept;
+    const Lists made = make_lists(experts, E);
+    if (!capturing()) kept = made;
+    return made;
   }
 };
 
@@ -295,7 +321,7 @@ std::shared_ptr<Plan> plan_experts(const Tensor& experts, int64_t E) {
   p->T = experts.size(0);
   p->k = experts.size(1);
   p->E = E;
-  if (S > kPlanNow) p->lists();
+  if (S > kPlanLater || capturing()) p->kept = make_lists(p->experts, E);
   return p;
 }
 
@@ -313,34 +339,54 @@ bool few_rows(const Sizes& n, int code) {
 
 Tensor inner(const Tensor& t) { return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; }
 
+// Whether the choices of a row are joined in one workgroup (mm_expert_joined) instead of through fp32 rows of the slots.
+// One choice: always (65,536 rows, 8 experts, us, joined / slots: 128 -> 128 float 34 / 46, bfloat16 16 / 29; 16,384 rows
+// 1024 -> 1024 float 259 / 270, bfloat16 59 / 99).  Two choices: 16-bit types where every pair of experts fills tiles of
+// rows and the slots' rows are 32 M values or more, which pays for the pairs' plan of 15 us (65,536 rows 256 -> 256: 52 / 84;
+// 98,304 rows 128 -> 128: 39 / 56; float, where splitting operands bounds the small tiles: 89 / 97, 1024 -> 1024 521 / 484).
+bool join_rows(const Sizes& n, int code) {
+  if (n.M > 64) return false;
+  if (n.k == 1) return true;
+  const long pairs = (n.E + 1) * (n.E + 2) / 2;
+  return n.k == 2 && code != 0 && n.E <= 21 && n.T * n.M >= 128 * pairs && 2 * n.T * n.M * n.F >= 32000000;
+}
+
 struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Maybe& gates,
-                        const Tensor& experts, const Tensor& offsets, const Tensor& order, int64_t code) {
+                        const std::shared_ptr<Plan>& plan, int64_t code) {
     const Tensor w = weight.contiguous(), g = gates ? gates->contiguous() : Tensor();
-    ctx->save_for_backward({x, w, g, experts, offsets, order});
+    const Lists l = plan->lists();   // the backward's
+    ctx->save_for_backward({x, w, g, plan->experts, l.offsets, l.order});
     ctx->saved_data["code"] = code;
-    return run(x, w, g, experts, offsets, order, (int)code);
+    return run(x, w, g, plan->experts, [&]() { return l; }, (int)code);
   }
 
   static Sizes sizes(const Tensor& x, const Tensor& w, const Tensor& experts) {
     return Sizes{x.size(0), x.size(1), x.size(2), w.size(2), w.size(0), experts.size(1)};
   }
 
-  static Tensor run(const Tensor& x0, const Tensor& w, const Tensor& gates, const Tensor& experts, const Tensor& offsets,
-                    const Tensor& order, int code) {
+  template <typename L>
+  static Tensor run(const Tensor& x0, const Tensor& w, const Tensor& gates, const Tensor& experts, L lists, int code) {
     const Sizes n = sizes(x0, w, experts);
     const Tensor x = inner(x0);
     Tensor y = at::empty({n.T, n.M, n.F}, x.options());
+    const int T = (int)n.T, k = (int)n.k, M = (int)n.M, D = (int)n.D, F = (int)n.F, E = (int)n.E;
     if (few_rows(n, code)) {
-      done(mm_expert_few(ptr(x), x.stride(0), x.stride(1), code, (int)n.T, (int)n.k, (int)n.M, (int)n.D, (int)n.F, ptr(w),
-                         (int)n.E, fptr(gates), iptr(experts), ptr(y), stream()));
+      done(mm_expert_few(ptr(x), x.stride(0), x.stride(1), code, T, k, M, D, F, ptr(w), E, fptr(gates),
+                         iptr(experts), ptr(y), stream()));
       return y;
     }
-    Tensor rows = f32({n.T * n.k, n.M, n.F}, x);
-    done(mm_expert_rows(ptr(x), x.stride(0), x.stride(1), code, (int)(n.T * n.k), (int)n.k, (int)n.M, (int)n.D, (int)n.F,
-                        ptr(w), 0, (int)n.E, iptr(offsets), iptr(order), fptr(rows), stream()));
-    done(mm_expert_combine(fptr(rows), fptr(gates), iptr(experts), code, n.T, (int)n.k, (int)n.M, (int)n.F, (int)n.E,
-                           ptr(y), stream()));
+    if (join_rows(n, code)) {
+      const Lists l = k == 2 ? make_pairs(experts, E) : lists();
+      done(mm_expert_joined(ptr(x), x.stride(0), x.stride(1), code, T, k, M, D, F, ptr(w), 0, E, fptr(gates),
+                            iptr(experts), iptr(l.offsets), iptr(l.order), ptr(y), nullptr, 0, 0, nullptr, stream()));
+      return y;
+    }
+    const Lists l = lists();
+    const Tensor rows = f32({n.T * n.k, n.M, n.F}, x);
+    done(mm_expert_rows(ptr(x), x.stride(0), x.stride(1), code, T * k, k, M, D, F, ptr(w), 0, E, iptr(l.offsets),
+                        iptr(l.order), fptr(rows), stream()));
+    done(mm_expert_combine(fptr(rows), fptr(gates), iptr(experts), code, n.T, k, M, F, E, ptr(y), stream()));
     return y;
   }
 
@@ -356,7 +402,12 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
     if (ctx->needs_input_grad(0)) dx = at::empty({n.T, n.M, n.D}, x.options());
     if (ctx->needs_input_grad(1)) dw = at::empty({n.E, n.D, n.F}, x.options());
     if (gates.defined() && ctx->needs_input_grad(2)) dg = f32({n.T, n.k}, x);
-    if (dx.defined() || dg.defined()) {
+    if ((dx.defined() || dg.defined()) && k == 1 && M <= 64 && (D <= 128 || !dg.defined())) {
+      // one choice: dx and dgates straight from the products (128 -> 128, 65,536 rows, us: bfloat16 21 / 36, float 41 / 55)
+      done(mm_expert_joined(ptr(dy), dy.stride(0), dy.stride(1), code, (int)n.T, 1, M, F, D, ptr(w), 1, E, fptr(gates),
+                            iptr(experts), iptr(offsets), iptr(order), ptr(dx), ptr(x), x.stride(0), x.stride(1),
+                            fptr(dg), stream()));
+    } else if (dx.defined() || dg.defined()) {
       const Tensor rows = f32({S, M, D}, x);
       done(mm_expert_rows(ptr(dy), dy.stride(0), dy.stride(1), code, S, k, M, F, D, ptr(w), 1, E, iptr(offsets),
                           iptr(order), fptr(rows), stream()));
@@ -371,7 +422,7 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
       done(mm_expert_wgrad(ptr(x), x.stride(0), x.stride(1), ptr(dy), dy.stride(0), dy.stride(1), code, S, k, M, D, F, E,
                            fptr(gates), iptr(offsets), iptr(order), ptr(dw), fptr(ws), stream()));
     }
-    variable_list out(7);
+    variable_list out(5);
     out[0] = dx;
     out[1] = dw;
     out[2] = dg;
@@ -409,11 +460,10 @@ Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates,
   const Tensor x = flat ? x0.unsqueeze(1) : x0;
   if (T * k * x.size(1) > kInt32Max - 128)
     throw py::value_error(text(T * k * x.size(1), " rows: 2^31 or more are not supported"));
-  const bool grad = needs_grad({&x, &weight, &g});
-  if (grad || !few_rows({T, x.size(1), x.size(2), weight.size(2), E, k}, code)) plan->lists();
-  const Tensor y = grad ? ExpertLinearFn::apply(x, weight, maybe(g), experts, plan->offsets, plan->order, (int64_t)code)
-                        : ExpertLinearFn::run(x, weight.contiguous(), g.defined() ? g.contiguous() : g, experts,
-                                              plan->offsets, plan->order, code);
+  const Tensor y = needs_grad({&x, &weight, &g})
+                       ? ExpertLinearFn::apply(x, weight, maybe(g), plan, (int64_t)code)
+                       : ExpertLinearFn::run(x, weight.contiguous(), g.defined() ? g.contiguous() : g, experts,
+                                             [&]() { return plan->lists(); }, code);
   return flat ? y.squeeze(1) : y;
 }
 }  // namespace
@@ -425,11 +475,11 @@ PYBIND11_MODULE(mm_torch_ops, m) {
   py::class_<Plan, std::shared_ptr<Plan>>(m, "ExpertPlan")
       .def_property_readonly("experts", [](Plan& p) { return p.experts; })
       .def_property_readonly("n_experts", [](Plan& p) { return p.E; })
-      .def_property_readonly("offsets", [](Plan& p) { return p.lists(), p.offsets; })
-      .def_property_readonly("order", [](Plan& p) { return p.lists(), p.order; })
+      .def_property_readonly("offsets", [](Plan& p) { return p.lists().offsets; })
+      .def_property_readonly("order", [](Plan& p) { return p.lists().order; })
       .def_property_readonly("counts", [](Plan& p) {
-        p.lists();
-        return at::sub(p.offsets.narrow(0, 1, p.E), p.offsets.narrow(0, 0, p.E));
+        const Tensor o = p.lists().offsets;
+        return at::sub(o.narrow(0, 1, p.E), o.narrow(0, 0, p.E));
       });
   m.def("plan_experts", &plan_experts);
   m.def("expert_linear", &expert_linear);

@@ -97,6 +97,8 @@ SIGNATURES = {
     "mm_route_bwd": [P, L, I, L, I, I, I, I, F, P, P, P, P, P],
     "mm_expert_plan_scratch": [I, I, P],
     "mm_expert_plan": [P, I, I, P, P, P, P],
+    "mm_expert_plan_pairs": [P, I, I, P, P, P, P],
+    "mm_expert_joined": [P, L, L, I, I, I, I, I, I, P, I, I, P, P, P, P, P, P, L, L, P, P],
     "mm_expert_rows": [P, L, L, I, I, I, I, I, I, P, I, I, P, P, P, P],
     "mm_expert_few": [P, L, L, I, I, I, I, I, I, P, I, P, P, P, P],
     "mm_expert_combine": [P, P, P, I, L, I, I, I, I, P, P],

@@ -240,3 +240,116 @@ def test_graph_replay():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(y, step())
+
+
+# ------------------------------------------------------------------------------------------------ the variants themselves
+def _rows_reference(x, w, experts, k, transposed):
+    """[S, M, N] products of every slot, 64 bits (zeros without an expert), and sums of magnitudes."""
+    T, M, K = x.shape
+    E = w.shape[0]
+    N = w.shape[1] if transposed else w.shape[2]
+    out = torch.zeros(T * k, M, N, dtype=torch.float64)
+    mag = torch.zeros_like(out)
+    flat, xd, wd = experts.reshape(-1), x.double(), w.double()
+    for e in range(E):
+        s = (flat == e).nonzero()[:, 0]
+        b = wd[e].T if transposed else wd[e]
+        out[s] = xd[s // k] @ b
+        mag[s] = xd[s // k].abs() @ b.abs()
+    return out, mag
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("transposed", [0, 1])
+@pytest.mark.parametrize("T,M,K,N,E,k,off", [
+    (1, 1, 1, 1, 1, 1, 0), (3, 2, 31, 33, 2, 2, 0), (130, 1, 64, 128, 2, 1, 0), (70, 3, 72, 136, 3, 2, 0),
+    (257, 1, 129, 257, 2, 1, 0), (200, 1, 200, 40, 70, 3, 0), (90, 1, 64, 64, 5, 2, 1), (2100, 1, 136, 264, 2, 1, 0),
+    (1500, 1, 512, 520, 2, 2, 0)])
+def test_rows_of_slots(T, M, K, N, E, k, off, transposed, dtype):
+    """mm_expert_rows on its own: tiles of both sizes, cut tiles, odd widths, unaligned rows, slots without an expert."""
+    from mace_onegpu._lib import K as L, stream
+    from mace_onegpu.experts import plan_experts
+    g = torch.Generator().manual_seed(T + K + N)
+    x = torch.randn(T, M, K, generator=g).to(dtype)
+    w = torch.randn(*((E, N, K) if transposed else (E, K, N)), generator=g).to(dtype)
+    experts = torch.randint(-1 if T > 1 else 0, E, (T, k), generator=g, dtype=torch.int32)
+    wide = torch.zeros(T, M, K + 3 * off, dtype=dtype, device="cuda")
+    wide[:, :, off:off + K] = x.cuda()
+    xg = wide[:, :, off:off + K]
+    plan = plan_experts(experts.cuda(), E)
+    out = torch.full((T * k, M, N), 7.0, device="cuda")
+    L.mm_expert_rows(xg, xg.stride(0), xg.stride(1), DTYPES.index(dtype), T * k, k, M, K, N, w.cuda(), transposed, E,
+                     plan.offsets, plan.order, out, stream())
+    ref, mag = _rows_reference(x, w, experts, k, transposed)
+    used = (experts.reshape(-1) >= 0)
+    err = (out.cpu().double() - ref).abs()
+    assert bool((err[used] <= ((K + 16) * U * mag + 1e-37)[used]).all())
+    assert bool((out.cpu()[~used] == 7.0).all())                      # rows of no expert are left alone
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("transposed", [0, 1])
+@pytest.mark.parametrize("T,M,K,N,E,k,off", [
+    (1, 1, 3, 5, 1, 1, 0), (300, 1, 64, 128, 3, 1, 0), (300, 3, 72, 136, 3, 2, 0), (77, 5, 33, 201, 2, 2, 0),
+    (1000, 1, 128, 128, 21, 2, 0), (129, 64, 40, 24, 2, 1, 0), (400, 1, 200, 260, 4, 2, 1), (2000, 1, 128, 64, 4, 2, 0)])
+def test_joined_rows(T, M, K, N, E, k, off, transposed, dtype):
+    """mm_expert_joined on its own: pairs of different and equal experts, one or no expert, and dgates of one choice."""
+    import ctypes
+
+    from mace_onegpu._lib import K as L, stream
+    from mace_onegpu.experts import plan_experts
+    g = torch.Generator().manual_seed(T + K + N)
+    x = torch.randn(T, M, K, generator=g).to(dtype)
+    w = torch.randn(*((E, N, K) if transposed else (E, K, N)), generator=g).to(dtype)
+    experts = torch.randint(-1, E + 1, (T, k), generator=g, dtype=torch.int32)
+    gates = torch.randn(T, k, generator=g)
+    wide = torch.zeros(T, M, K + 3 * off, dtype=dtype, device="cuda")
+    wide[:, :, off:off + K] = x.cuda()
+    xg, code = wide[:, :, off:off + K], DTYPES.index(dtype)
+    if k == 1:
+        plan = plan_experts(experts.cuda(), E)
+        offsets, order = plan.offsets, plan.order
+    else:
+        pairs = (E + 1) * (E + 2) // 2
+        n = ctypes.c_long(0)
+        L.mm_expert_plan_scratch(T, pairs - 1, ctypes.byref(n))
+        offsets = torch.empty(pairs, dtype=torch.int32, device="cuda")
+        order = torch.empty(T, dtype=torch.int32, device="cuda")
+        L.mm_expert_plan_pairs(experts.cuda(), T, E, offsets, order, torch.empty(n.value + 1, dtype=torch.int32,
+                                                                                  device="cuda"), stream())
+        clean = torch.where((experts < 0) | (experts >= E), E, experts).sort(1).values.long()
+        ids = [(a, b) for a in range(E + 1) for b in range(a, E + 1)]
+        key = torch.tensor([ids.index(tuple(p)) for p in clean.tolist()])
+        assert torch.equal(order.cpu().long(), torch.sort(key, stable=True).indices)
+        first = torch.bincount(key, minlength=pairs).cumsum(0) - torch.bincount(key, minlength=pairs)
+        assert torch.equal(offsets.cpu().long(), first)
+    z, mag = (t.view(T, k, M, N) for t in _rows_reference(x, w, torch.where(experts >= E, -1, experts), k, transposed))
+    ref, bound = (z * gates.double()[:, :, None, None]).sum(1), (mag * gates.double().abs()[:, :, None, None]).sum(1)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-37
+    out = torch.full((T, M, N), 7.0, device="cuda").to(dtype)
+    with_dg = k == 1 and transposed and N <= 128
+    xs = torch.randn(T, M, N, generator=g).to(dtype)
+    dg = torch.full((T, 1), 7.0, device="cuda") if with_dg else None
+    xsg = xs.cuda()
+    L.mm_expert_joined(xg, xg.stride(0), xg.stride(1), code, T, k, M, K, N, w.cuda(), transposed, E, gates.cuda(),
+                       experts.cuda(), offsets, order, out, xsg, M * N, N, dg, stream())
+    err = (out.cpu().double() - ref).abs()
+    assert bool((err <= (K + 16) * U * bound + HALF_ULP[dtype] * ref.abs() + tiny).all()), float(err.max())
+    if with_dg:
+        want, most = (z[:, 0] * xs.double()).sum((1, 2)), (mag[:, 0] * xs.double().abs()).sum((1, 2))
+        assert bool(((dg[:, 0].cpu().double() - want).abs() <= (K + M * N + 16) * U * most + 1e-37).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,D,F,E,k", [(9000, 128, 128, 6, 2), (30000, 72, 40, 5, 1), (3000, 256, 256, 4, 2)])
+def test_paths_of_many_rows(T, D, F, E, k, dtype):
+    """The products as they are chosen for many rows, inference and training, give the same result as slot by slot."""
+    from mace_onegpu.experts import expert_linear, plan_experts
+    x, w, experts, gates, dy = _make(T, 1, D, F, E, k, dtype, 17, closed=0.05)
+    ref, mag = _reference(x, w, experts, gates, dy)
+    plan = plan_experts(experts.cuda(), E)
+    y = expert_linear(x.cuda(), w.cuda(), plan, gates.cuda())
+    _check(dict(y=y), ref, mag, dict(y=D), dtype)
+    xg = x.cuda().requires_grad_()
+    (dx,) = torch.autograd.grad(expert_linear(xg, w.cuda(), plan, gates.cuda()), xg, dy.cuda())
+    _check(dict(dx=dx), ref, mag, dict(dx=F), dtype)
