@@ -283,24 +283,25 @@ Lists make_pairs(const Tensor& experts, long E) {
   return {buf.narrow(0, 0, buckets), buf.narrow(0, buckets, T)};
 }
 
-// Up to kPlanLater slots the sort waits until something needs it: few rows do without.  Under graph capture nothing waits,
-// so that a captured plan is sorted by every replay; lists that a capture needs of an older plan are its own and are not
-// kept (they hold nothing until a replay).
-constexpr long kPlanLater = 1024;
-
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
+// The sorts wait until a product (or the caller) needs one: few rows need none, and rows of two choices may need the
+// pairs' instead of the slots'.  Under graph capture the slots are sorted at once, so that a captured plan follows every
+// replay; lists that a capture needs of an older plan are its own and are not kept (they hold nothing until a replay).
 struct Plan {
   Tensor experts;
   long T, k, E;
-  Lists kept;
+  Lists slots, rows;
 
-  Lists lists() {
+  template <typename F>
+  Lists keep(Lists& kept, F make) {
     if (kept.offsets.defined()) return kept;
-    const Lists made = make_lists(experts, E);
+    const Lists made = make(experts, E);
     if (!capturing()) kept = made;
     return made;
   }
+  Lists lists() { return keep(slots, make_lists); }
+  Lists pairs() { return keep(rows, make_pairs); }
 };
 
 std::shared_ptr<Plan> plan_experts(const Tensor& experts, int64_t E) {
@@ -321,7 +322,7 @@ std::shared_ptr<Plan> plan_experts(const Tensor& experts, int64_t E) {
   p->T = experts.size(0);
   p->k = experts.size(1);
   p->E = E;
-  if (S > kPlanLater || capturing()) p->kept = make_lists(p->experts, E);
+  if (capturing()) p->slots = make_lists(p->experts, E);
   return p;
 }
 
@@ -339,34 +340,48 @@ bool few_rows(const Sizes& n, int code) {
 
 Tensor inner(const Tensor& t) { return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; }
 
-// Whether the choices of a row are joined in one workgroup (mm_expert_joined) instead of through fp32 rows of the slots.
-// One choice: always (65,536 rows, 8 experts, us, joined / slots: 128 -> 128 float 34 / 46, bfloat16 16 / 29; 16,384 rows
-// 1024 -> 1024 float 259 / 270, bfloat16 59 / 99).  Two choices: 16-bit types where every pair of experts fills tiles of
-// rows and the slots' rows are 32 M values or more, which pays for the pairs' plan of 15 us (65,536 rows 256 -> 256: 52 / 84;
-// 98,304 rows 128 -> 128: 39 / 56; float, where splitting operands bounds the small tiles: 89 / 97, 1024 -> 1024 521 / 484).
-bool join_rows(const Sizes& n, int code) {
+// Whether the choices of a row are joined before they are written (mm_expert_joined) instead of through fp32 rows of the
+// slots; K values a row go in, N come out.  One choice: always (65,536 rows, 8 experts, us, joined / slots: 128 -> 128
+// float 25 / 37, bfloat16 16 / 29; 16,384 rows 1024 -> 1024 float 259 / 270, bfloat16 59 / 99).  Two choices: where every
+// pair of experts fills tiles of rows and enough values are not written and read again to pay for the pairs' plan
+// (15 us): float up to 128 values from 2 M results on (98,304 rows 128 -> 128: 44 / 70), beyond that splitting the operands
+// of the small tiles costs more (256 -> 256, 65,536 rows: 159 / 173, 1024 -> 1024 521 / 484); 16-bit types from 16 M
+// results on (65,536 rows 256 -> 256: 52 / 84; 98,304 rows 128 -> 128: 39 / 56).
+bool join_rows(const Sizes& n, long K, long N, int code) {
   if (n.M > 64) return false;
   if (n.k == 1) return true;
-  const long pairs = (n.E + 1) * (n.E + 2) / 2;
-  return n.k == 2 && code != 0 && n.E <= 21 && n.T * n.M >= 128 * pairs && 2 * n.T * n.M * n.F >= 32000000;
+  const long pairs = (n.E + 1) * (n.E + 2) / 2, results = n.T * n.M * N;
+  if (n.k != 2 || n.E > 21 || n.T * n.M < 128 * pairs) return false;
+  return code == 0 ? K <= 128 && n.M <= 16 && results >= 2000000 : results >= 16000000;
+}
+
+// dx with dgates likewise: all columns in one workgroup, two choices for float only (bfloat16, DG: 57 / 67, but 41 / 36 with 3
+// components)
+bool join_gradients(const Sizes& n, int code, bool dgates) {
+  return join_rows(n, n.F, n.D, code) && (!dgates || (n.D <= 128 && (n.k == 1 || code == 0)));
 }
 
 struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Maybe& gates,
                         const std::shared_ptr<Plan>& plan, int64_t code) {
     const Tensor w = weight.contiguous(), g = gates ? gates->contiguous() : Tensor();
-    const Lists l = plan->lists();   // the backward's
-    ctx->save_for_backward({x, w, g, plan->experts, l.offsets, l.order});
+    const Sizes n = sizes(x, w, plan->experts);
+    const bool dg = g.defined() && g.requires_grad(), dxg = x.requires_grad() || dg;
+    const bool joined = join_gradients(n, (int)code, dg);
+    Lists l, p;   // the backward's
+    if (weight.requires_grad() || (dxg && !(joined && n.k == 2))) l = plan->lists();
+    if (dxg && joined && n.k == 2) p = plan->pairs();
+    ctx->save_for_backward({x, w, g, plan->experts, l.offsets, l.order, p.offsets, p.order});
     ctx->saved_data["code"] = code;
-    return run(x, w, g, plan->experts, [&]() { return l; }, (int)code);
+    return run(x, w, g, *plan, (int)code);
   }
 
   static Sizes sizes(const Tensor& x, const Tensor& w, const Tensor& experts) {
     return Sizes{x.size(0), x.size(1), x.size(2), w.size(2), w.size(0), experts.size(1)};
   }
 
-  template <typename L>
-  static Tensor run(const Tensor& x0, const Tensor& w, const Tensor& gates, const Tensor& experts, L lists, int code) {
+  static Tensor run(const Tensor& x0, const Tensor& w, const Tensor& gates, Plan& plan, int code) {
+    const Tensor& experts = plan.experts;
     const Sizes n = sizes(x0, w, experts);
     const Tensor x = inner(x0);
     Tensor y = at::empty({n.T, n.M, n.F}, x.options());
@@ -376,13 +391,13 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
                          iptr(experts), ptr(y), stream()));
       return y;
     }
-    if (join_rows(n, code)) {
-      const Lists l = k == 2 ? make_pairs(experts, E) : lists();
+    if (join_rows(n, n.D, n.F, code)) {
+      const Lists l = k == 2 ? plan.pairs() : plan.lists();
       done(mm_expert_joined(ptr(x), x.stride(0), x.stride(1), code, T, k, M, D, F, ptr(w), 0, E, fptr(gates),
                             iptr(experts), iptr(l.offsets), iptr(l.order), ptr(y), nullptr, 0, 0, nullptr, stream()));
       return y;
     }
-    const Lists l = lists();
+    const Lists l = plan.lists();
     const Tensor rows = f32({n.T * n.k, n.M, n.F}, x);
     done(mm_expert_rows(ptr(x), x.stride(0), x.stride(1), code, T * k, k, M, D, F, ptr(w), 0, E, iptr(l.offsets),
                         iptr(l.order), fptr(rows), stream()));
@@ -393,7 +408,7 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor x = inner(saved[0]), &w = saved[1], &gates = saved[2], &experts = saved[3], &offsets = saved[4],
-                 &order = saved[5];
+                 &order = saved[5], &pair_offsets = saved[6], &pair_order = saved[7];
     const Tensor dy = inner(grads[0]);
     const int code = (int)ctx->saved_data["code"].toInt();
     const Sizes n = sizes(x, w, experts);
@@ -402,11 +417,12 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
     if (ctx->needs_input_grad(0)) dx = at::empty({n.T, n.M, n.D}, x.options());
     if (ctx->needs_input_grad(1)) dw = at::empty({n.E, n.D, n.F}, x.options());
     if (gates.defined() && ctx->needs_input_grad(2)) dg = f32({n.T, n.k}, x);
-    if ((dx.defined() || dg.defined()) && k == 1 && M <= 64 && (D <= 128 || !dg.defined())) {
-      // one choice: dx and dgates straight from the products (128 -> 128, 65,536 rows, us: bfloat16 21 / 36, float 41 / 55)
-      done(mm_expert_joined(ptr(dy), dy.stride(0), dy.stride(1), code, (int)n.T, 1, M, F, D, ptr(w), 1, E, fptr(gates),
-                            iptr(experts), iptr(offsets), iptr(order), ptr(dx), ptr(x), x.stride(0), x.stride(1),
-                            fptr(dg), stream()));
+    // (joined or not was settled by whether the gates needed a gradient; if it is dropped here, that choice still holds)
+    if ((dx.defined() || dg.defined()) && join_gradients(n, code, gates.defined() && gates.requires_grad())) {
+      const bool pairs = k == 2;
+      done(mm_expert_joined(ptr(dy), dy.stride(0), dy.stride(1), code, (int)n.T, k, M, F, D, ptr(w), 1, E, fptr(gates),
+                            iptr(experts), iptr(pairs ? pair_offsets : offsets), iptr(pairs ? pair_order : order),
+                            ptr(dx), ptr(x), x.stride(0), x.stride(1), fptr(dg), stream()));
     } else if (dx.defined() || dg.defined()) {
       const Tensor rows = f32({S, M, D}, x);
       done(mm_expert_rows(ptr(dy), dy.stride(0), dy.stride(1), code, S, k, M, F, D, ptr(w), 1, E, iptr(offsets),
@@ -462,8 +478,7 @@ Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates,
     throw py::value_error(text(T * k * x.size(1), " rows: 2^31 or more are not supported"));
   const Tensor y = needs_grad({&x, &weight, &g})
                        ? ExpertLinearFn::apply(x, weight, maybe(g), plan, (int64_t)code)
-                       : ExpertLinearFn::run(x, weight.contiguous(), g.defined() ? g.contiguous() : g, experts,
-                                             [&]() { return plan->lists(); }, code);
+                       : ExpertLinearFn::run(x, weight.contiguous(), g.defined() ? g.contiguous() : g, *plan, code);
   return flat ? y.squeeze(1) : y;
 }
 }  // namespace

@@ -39,8 +39,9 @@ def plan_experts(experts, n_experts):
 
     experts int32 [T, k], n_experts
     order int32 [T k], offsets int32 [n_experts + 1]: the slots of expert e are order[offsets[e] : offsets[e + 1]], in
-        ascending order; slots with an expert outside [0, n_experts) come after them, from offsets[n_experts] on.  For up
-        to 1024 slots the sort waits until something needs it (few rows do without), except under graph capture.
+        ascending order; slots with an expert outside [0, n_experts) come after them, from offsets[n_experts] on.  Sorted
+        when first needed (few rows need no order, rows of two choices may be sorted by pair of experts instead), except
+        under graph capture, where it is recorded at once.
     counts int32 [n_experts]: slots of each expert (its load, for a balance bias)"""
     return ops().plan_experts(experts, n_experts)
 

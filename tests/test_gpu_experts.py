@@ -291,7 +291,8 @@ def test_rows_of_slots(T, M, K, N, E, k, off, transposed, dtype):
 @pytest.mark.parametrize("transposed", [0, 1])
 @pytest.mark.parametrize("T,M,K,N,E,k,off", [
     (1, 1, 3, 5, 1, 1, 0), (300, 1, 64, 128, 3, 1, 0), (300, 3, 72, 136, 3, 2, 0), (77, 5, 33, 201, 2, 2, 0),
-    (1000, 1, 128, 128, 21, 2, 0), (129, 64, 40, 24, 2, 1, 0), (400, 1, 200, 260, 4, 2, 1), (2000, 1, 128, 64, 4, 2, 0)])
+    (1000, 1, 128, 128, 21, 2, 0), (3000, 3, 128, 128, 2, 2, 0),
+    (5000, 1, 32, 128, 3, 2, 0), (2500, 2, 100, 60, 2, 2, 1), (129, 64, 40, 24, 2, 1, 0), (400, 1, 200, 260, 4, 2, 1), (2000, 1, 128, 64, 4, 2, 0)])
 def test_joined_rows(T, M, K, N, E, k, off, transposed, dtype):
     """mm_expert_joined on its own: pairs of different and equal experts, one or no expert, and dgates of one choice."""
     import ctypes
@@ -327,17 +328,17 @@ def test_joined_rows(T, M, K, N, E, k, off, transposed, dtype):
     ref, bound = (z * gates.double()[:, :, None, None]).sum(1), (mag * gates.double().abs()[:, :, None, None]).sum(1)
     tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-37
     out = torch.full((T, M, N), 7.0, device="cuda").to(dtype)
-    with_dg = k == 1 and transposed and N <= 128
+    with_dg = transposed and N <= 128 and (k == 1 or (dtype == torch.float32 and K <= 128 and M <= 16))
     xs = torch.randn(T, M, N, generator=g).to(dtype)
-    dg = torch.full((T, 1), 7.0, device="cuda") if with_dg else None
+    dg = torch.full((T, k), 7.0, device="cuda") if with_dg else None
     xsg = xs.cuda()
     L.mm_expert_joined(xg, xg.stride(0), xg.stride(1), code, T, k, M, K, N, w.cuda(), transposed, E, gates.cuda(),
                        experts.cuda(), offsets, order, out, xsg, M * N, N, dg, stream())
     err = (out.cpu().double() - ref).abs()
     assert bool((err <= (K + 16) * U * bound + HALF_ULP[dtype] * ref.abs() + tiny).all()), float(err.max())
     if with_dg:
-        want, most = (z[:, 0] * xs.double()).sum((1, 2)), (mag[:, 0] * xs.double().abs()).sum((1, 2))
-        assert bool(((dg[:, 0].cpu().double() - want).abs() <= (K + M * N + 16) * U * most + 1e-37).all())
+        want, most = (z * xs.double()[:, None]).sum((2, 3)), (mag * xs.double().abs()[:, None]).sum((2, 3))
+        assert bool(((dg.cpu().double() - want).abs() <= (K + M * N + 16) * U * most + 1e-37).all())
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
