@@ -1278,16 +1278,32 @@ __global__ void __launch_bounds__(64 * WD * WF, 2) mm_expert_wgrad_kernel(MMWgra
   uint4 *Xs = mm_lds, *Ys = Xs + 2 * BD * 8;             // [2][BD * 8], [2][BF * 8]
   long *s_x = (long*)(Ys + 2 * BF * 8), *s_y = s_x + MM_WG_ROWS;
   float* s_g = (float*)(s_y + MM_WG_ROWS);
+  const int lane_id = threadIdx.x & 63;
   int df, tile;
   MMTile t;
   if constexpr (SPLIT) {
     t = mm_expert_tile(a.offsets, a.E, a.offsets[a.E], a.M, chunk, tiles_df, blockIdx.x, &df, &tile);
     if (t.e < 0) return;
-  } else {   // an XCD gets every 8th expert: lists of different lengths, each read by one XCD
-    const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
-    tile = i / tiles_df * 8 + x;
+  } else {
+    // Each list is read by one XCD, whose L2 serves all tiles of dW[e].  The longest lists first, dealt out to the XCDs
+    // forth and back, so that they end together (64 experts at most; beyond that every 8th as they come).  Lists of uneven
+    // load (lognormal, 0.7), 64 experts, 1024 x 1024: 338 us in the order of the experts, 279 us so.
+    const int x = blockIdx.x & 7, i = blockIdx.x >> 3, turn = i / tiles_df;
+    tile = 8 * turn + x;
     df = i % tiles_df;
     if (tile >= a.E) return;
+    if (a.E <= 64) {
+      const int own = lane_id < a.E ? a.offsets[lane_id + 1] - a.offsets[lane_id] : -1;
+      int rank = 0;
+      for (int o = 0; o < a.E; ++o) {
+        const int other = __builtin_amdgcn_readlane(own, o);
+        rank += other > own || (other == own && o < lane_id);
+      }
+      const int snake = turn & 1 ? 8 * turn + 7 - x : tile;
+      const int want = snake < a.E ? snake : tile;
+      const unsigned long long is = __ballot(lane_id < a.E && rank == want);
+      tile = __ffsll(is) - 1;
+    }
     t = MMTile{tile, 0, (a.offsets[tile + 1] - a.offsets[tile]) * a.M};
   }
   const int d0 = df / tiles_f * BD, f0 = df % tiles_f * BF;
@@ -1395,19 +1411,13 @@ __global__ void __launch_bounds__(256) mm_expert_wgrad_sum_kernel(MMWgrad a, int
 #pragma unroll
   for (int d = 32; d; d >>= 1) first += __shfl_xor(first, d);
   const int n = ((a.offsets[e + 1] - a.offsets[e]) * a.M + chunk - 1) / chunk;
-  const long size = (long)a.D * a.F, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  const long size = (long)a.D * a.F, i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= size) return;
   const float* __restrict__ p = part + (size_t)first * size + i;
-  const int left = (int)min(size - i, 4L);
-  float t[4] = {};
+  float t = 0.f;
 #pragma unroll 8
-  for (int c = 0; c < n; ++c) {
-    float v[4];
-    mm_load4(p + c * size, 0, left, v);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) t[q] += v[q];
-  }
-  mm_store4((T*)a.dW + (size_t)e * size + i, 0, left, t);
+  for (int c = 0; c < n; ++c) t += p[c * size];
+  ((T*)a.dW)[(size_t)e * size + i] = (T)t;
 }
 
 // ------------------------------------------------------------------------------------------------ entry points
@@ -1784,7 +1794,7 @@ extern "C" int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, 
   if (rc != MM_OK) return rc;
   if (chunk)
     MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_wgrad_sum_kernel<T_>),
-                                          dim3((unsigned)(((long)D * F + 1023) / 1024), E), dim3(256), 0, stream, a, chunk,
+                                          dim3((unsigned)(((long)D * F + 255) / 256), E), dim3(256), 0, stream, a, chunk,
                                           workspace));
   return mm::launch_status("mm_expert_wgrad");
 }
