@@ -97,7 +97,8 @@ def _build_torch_ops():
     obj = os.path.join(OBJ, "torch_ops.o")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I" + os.path.join(root, "include"),
+           "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-I" + os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include"),
            "-I" + sysconfig.get_paths()["include"], "-c", os.path.join(CSRC, "torch", "ops.cpp"), "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -108,8 +109,8 @@ def _build_torch_ops():
 
 def _link_torch_ops(obj, torch_lib):
     tmp = TORCH_OPS + ".tmp"
-    cmd = ["g++", "-shared", "-o", tmp, obj, "-L" + LIB_DIR, "-l:" + os.path.basename(LIB), "-L" + torch_lib, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
-           "-ltorch", "-Wl,-rpath,$ORIGIN"]
+    cmd = ["g++", "-shared", "-o", tmp, obj, "-L" + LIB_DIR, "-l:" + os.path.basename(LIB), "-L" + torch_lib,
+           "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")

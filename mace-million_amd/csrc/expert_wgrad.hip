@@ -1,0 +1,243 @@
+// dW[e] = sum over the slots of expert e and their components of gate x^T dy.
+#include "experts.h"
+
+struct MMWgrad {
+  const void *x, *dy;
+  const float* gates;
+  const int *offsets, *order;
+  void* dW;
+  long xt, xm, yt, ym;
+  int k, M, D, F, E;
+};
+
+// A workgroup: a BD x BF tile of dW[e] over a chunk of the expert's rows (SPLIT: chunks of `chunk` rows, each into its
+// own fp32 partial sums, which mm_expert_wgrad_sum_kernel adds in order; else all rows, straight into dW).  x goes
+// into LDS as it is, dy through registers times its gate: in 16-bit types that rounds gate x dy to the type, an error
+// of the size that dy's own rounding has.  Rows past the end are zeros on both sides.
+#define MM_WG_ROWS 512   // rows whose offsets are kept in LDS at a time
+
+template <typename T, bool SPLIT, bool DMA, int BD, int BF, int WD, int WF>
+__global__ void __launch_bounds__(64 * WD * WF, 2) mm_expert_wgrad_kernel(MMWgrad a, int chunk, int tiles_f,
+                                                                          int tiles_df, float* __restrict__ part) {
+  constexpr int TH = 64 * WD * WF, BK = MM_TILE_K<T>, N = MMVec<T>::N, UD = BD / N, UF = BF / N, KS = BK / 32;
+  constexpr int NX = BD * 8 / TH, NY = BF * 8 / TH, FD = BD / WD / 16, FF = BF / WF / 16;
+  extern __shared__ uint4 mm_lds[];
+  uint4 *Xs = mm_lds, *Ys = Xs + 2 * BD * 8;             // [2][BD * 8], [2][BF * 8]
+  long *s_x = (long*)(Ys + 2 * BF * 8), *s_y = s_x + MM_WG_ROWS;
+  float* s_g = (float*)(s_y + MM_WG_ROWS);
+  const int lane_id = threadIdx.x & 63;
+  int df, tile;
+  MMTile t;
+  if constexpr (SPLIT) {
+    t = mm_expert_tile(a.offsets, a.E, a.offsets[a.E], a.M, chunk, tiles_df, blockIdx.x, &df, &tile);
+    if (t.e < 0) return;
+  } else {
+    // Each list is read by one XCD, whose L2 serves all tiles of dW[e].  The longest lists first, dealt out to the
+    // XCDs forth and back, so that they end together (64 experts at most; beyond that every 8th as they come).  Lists
+    // of uneven load (lognormal, 0.7), 64 experts, 1024 x 1024: 338 us in the order of the experts, 279 us so.
+    const int x = blockIdx.x & 7, i = blockIdx.x >> 3, turn = i / tiles_df;
+    tile = 8 * turn + x;
+    df = i % tiles_df;
+    if (tile >= a.E) return;
+    if (a.E <= 64) {
+      const int own = lane_id < a.E ? a.offsets[lane_id + 1] - a.offsets[lane_id] : -1;
+      int rank = 0;
+      for (int o = 0; o < a.E; ++o) {
+        const int other = __builtin_amdgcn_readlane(own, o);
+        rank += other > own || (other == own && o < lane_id);
+      }
+      const int snake = turn & 1 ? 8 * turn + 7 - x : tile;
+      const int want = snake < a.E ? snake : tile;
+      const unsigned long long is = __ballot(lane_id < a.E && rank == want);
+      tile = __ffsll(is) - 1;
+    }
+    t = MMTile{tile, 0, (a.offsets[tile + 1] - a.offsets[tile]) * a.M};
+  }
+  const int d0 = df / tiles_f * BD, f0 = df % tiles_f * BF;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int* __restrict__ list = a.order + a.offsets[t.e];
+  int qx[NX], left_d[NX], cx[NX], qy[NY], left_f[NY], cy[NY];
+#pragma unroll
+  for (int j = 0; j < NX; ++j) {
+    const int pu = tid + TH * j;
+    qx[j] = pu / UD;
+    cx[j] = ((pu % UD) ^ mm_nc_swizzle<T, UD>(qx[j])) * N;
+    left_d[j] = a.D - d0 - cx[j];
+  }
+#pragma unroll
+  for (int j = 0; j < NY; ++j) {
+    const int pu = tid + TH * j;
+    qy[j] = pu / UF;
+    cy[j] = ((pu % UF) ^ mm_nc_swizzle<T, UF>(qy[j])) * N;
+    left_f[j] = a.F - f0 - cy[j];
+  }
+  MMStage<T, TH, NX, DMA> sx;
+  MMStage<T, TH, NY, false> sy;
+  float gy[NY];
+  auto load = [&](int r0, int buf) {   // rows r0 .. r0 + BK of the chunk, within one block of offsets
+#pragma unroll
+    for (int j = 0; j < NX; ++j) {
+      const bool in = r0 + qx[j] < t.rows;
+      const long at_x = in ? s_x[(r0 + qx[j]) & (MM_WG_ROWS - 1)] : 0;
+      sx.load(Xs + buf * BD * 8, j, (const T*)a.x + at_x + d0 + cx[j], in ? left_d[j] : 0);
+    }
+#pragma unroll
+    for (int j = 0; j < NY; ++j) {
+      const bool in = r0 + qy[j] < t.rows;
+      const int r = (r0 + qy[j]) & (MM_WG_ROWS - 1);
+      sy.load(Ys + buf * BF * 8, j, (const T*)a.dy + (in ? s_y[r] : 0) + f0 + cy[j], in ? left_f[j] : 0);
+      gy[j] = in ? s_g[r] : 0.f;
+    }
+  };
+  auto put = [&](int buf) {
+    sx.put(Xs + buf * BD * 8);
+    if (a.gates) {
+#pragma unroll
+      for (int j = 0; j < NY; ++j) {
+        typename MMVec<T>::type v = __builtin_bit_cast(typename MMVec<T>::type, sy.v[j]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (T)(gy[j] * (float)v[i]);
+        sy.v[j] = __builtin_bit_cast(uint4, v);
+      }
+    }
+    sy.put(Ys + buf * BF * 8);
+  };
+  auto rows_of = [&](int r0) {
+    for (int i = tid; i < MM_WG_ROWS && r0 + i < t.rows; i += TH) {
+      const int r = t.row0 + r0 + i, p = r / a.M, m = r - p * a.M, slot = list[p];
+      const long tok = slot / a.k;
+      s_x[i] = tok * a.xt + m * a.xm;
+      s_y[i] = tok * a.yt + m * a.ym;
+      s_g[i] = a.gates ? a.gates[slot] : 1.f;
+    }
+    __syncthreads();
+  };
+  floatx4 acc[FF][FD] = {};
+  const int wd = (wave % WD) * (BD / WD), wf = (wave / WD) * (BF / WF);
+  if (t.rows > 0) {
+    rows_of(0);
+    load(0, 0);
+    put(0);
+    mm_stage_done();
+  }
+  int buf = 0;
+  for (int r0 = 0; r0 < t.rows; r0 += BK) {
+    const int next = r0 + BK;
+    const bool more = next < t.rows;
+    if (more) {
+      if (next % MM_WG_ROWS == 0) rows_of(next);   // the previous block's offsets are used up (the last barrier)
+      load(next, buf ^ 1);
+    }
+    mm_products<T, FF, FD, KS>(
+        acc, [&](int s, int i) { return mm_read_nc<T, UF>(Ys + buf * BF * 8, wf + 16 * i, s, lane); },
+        [&](int s, int j) { return mm_read_nc<T, UD>(Xs + buf * BD * 8, wd + 16 * j, s, lane); });
+    if (more) put(buf ^ 1);
+    mm_stage_done();
+    buf ^= 1;
+  }
+  const size_t base = SPLIT ? (size_t)tile * a.D * a.F : (size_t)t.e * a.D * a.F;
+#pragma unroll
+  for (int j = 0; j < FD; ++j) {
+    const int d = d0 + wd + 16 * j + (lane & 15);
+    if (d >= a.D) continue;
+#pragma unroll
+    for (int i = 0; i < FF; ++i) {
+      const int f = f0 + wf + 16 * i + 4 * (lane >> 4);
+      if constexpr (SPLIT) mm_store4(part + base + (size_t)d * a.F, f, a.F, (const float*)&acc[i][j]);
+      else mm_store4((T*)a.dW + base + (size_t)d * a.F, f, a.F, (const float*)&acc[i][j]);
+    }
+  }
+}
+
+// dW[e] = the partial sums of the expert's chunks, in order
+template <typename T>
+__global__ void __launch_bounds__(256) mm_expert_wgrad_sum_kernel(MMWgrad a, int chunk,
+                                                                  const float* __restrict__ part) {
+  const int lane = threadIdx.x & 63, e = blockIdx.y;
+  int first = 0;   // chunks of the experts before e
+  for (int o = lane; o < e; o += 64) first += ((a.offsets[o + 1] - a.offsets[o]) * a.M + chunk - 1) / chunk;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) first += __shfl_xor(first, d);
+  const int n = ((a.offsets[e + 1] - a.offsets[e]) * a.M + chunk - 1) / chunk;
+  const long size = (long)a.D * a.F, i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= size) return;
+  const float* __restrict__ p = part + (size_t)first * size + i;
+  float t = 0.f;
+#pragma unroll 8
+  for (int c = 0; c < n; ++c) t += p[c * size];
+  ((T*)a.dW)[(size_t)e * size + i] = (T)t;
+}
+
+// ------------------------------------------------------------------------------------------------ entry points
+namespace {
+// two stages of both operands, then the offsets and gates of a block of rows
+template <int BD, int BF>
+constexpr int wgrad_lds() { return 2 * (BD + BF) * 128 + MM_WG_ROWS * 20; }
+
+template <typename T, bool SPLIT, bool DMA, int BD, int BF, int WD, int WF>
+int launch_wgrad_tile(const MMWgrad& a, int S, int chunk, float* part, hipStream_t stream) {
+  const int tiles_f = (a.F + BF - 1) / BF, tiles_df = (a.D + BD - 1) / BD * tiles_f;
+  const long wg = (SPLIT ? (long)S * a.M / chunk + (a.E < S ? a.E : S) : (a.E + 7L) / 8 * 8) * tiles_df;
+  if (too_many(wg, 64 * WD * WF)) return range_error("mm_expert_wgrad", "output too large for one launch");
+  constexpr auto kernel = mm_expert_wgrad_kernel<T, SPLIT, DMA, BD, BF, WD, WF>;
+  constexpr int lds = wgrad_lds<BD, BF>();
+  if (!lds_granted<kernel>(lds)) return MM_ELAUNCH;
+  if (wg)
+    hipLaunchKernelGGL(kernel, dim3((unsigned)wg), dim3(64 * WD * WF), lds, stream, a, chunk, tiles_f, tiles_df, part);
+  return mm::launch_status("mm_expert_wgrad");
+}
+
+template <typename T, bool SPLIT, bool DMA>
+int launch_wgrad(const MMWgrad& a, int S, int chunk, bool big, float* part, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2 && DMA && !SPLIT)
+    if (big) return launch_wgrad_tile<T, SPLIT, DMA, 256, 256, 2, 4>(a, S, chunk, part, stream);
+  return launch_wgrad_tile<T, SPLIT, DMA, 128, 128, 2, 2>(a, S, chunk, part, stream);
+}
+
+// Rows per chunk of dW's sums; 0: no chunks.  A card of 256 CUs takes 512 workgroups at a time: with at least that
+// many (expert, tile) pairs none are made; else chunks for about 1024 workgroups, of 256 rows or more (a chunk's
+// partial sums are 64 KB per tile to write and read, 256 rows of both operands 128 KB or more).
+int wgrad_chunk(long rows, int D, int F, int E) {
+  const long tiles = (long)((D + 127) / 128) * ((F + 127) / 128);
+  if (E * tiles >= 512 || rows < 512) return 0;
+  const long c = (rows * tiles + 1023) / 1024;
+  return (int)(c < 256 ? 256 : (c + 63) / 64 * 64);
+}
+}  // namespace
+
+extern "C" int mm_expert_wgrad_workspace(int S, int M, int D, int F, int E, size_t* bytes) {
+  MM_CHECK_ARG(S >= 0 && M >= 1 && D >= 1 && F >= 1 && E >= 1 && bytes, "bad sizes");
+  const long rows = (long)S * M, c = wgrad_chunk(rows, D, F, E);
+  *bytes = c ? (size_t)(rows / c + (E < S ? E : S)) * D * F * sizeof(float) : 0;
+  return MM_OK;
+}
+
+extern "C" int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, long yt, long ym, int dtype, int S,
+                               int k, int M, int D, int F, int E, const float* gates, const int* offsets,
+                               const int* order, void* dW, float* workspace, hipStream_t stream) {
+  MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");
+  MM_CHECK_ARG(S >= 0 && k >= 1 && M >= 1 && D >= 1 && F >= 1 && E >= 1, "bad sizes");
+  MM_CHECK_ARG(xt >= 0 && xm >= 0 && yt >= 0 && ym >= 0, "bad strides");
+  if (E > MM_EXPERT_MAX_E) return range_error("mm_expert_wgrad", "more than 1024 experts are not supported");
+  if ((long)S * M > 2147483647L - 128) return range_error("mm_expert_wgrad", "2^31 rows or more are not supported");
+  const MMWgrad a{x, dy, gates, offsets, order, dW, xt, xm, yt, ym, k, M, D, F, E};
+  const int chunk = wgrad_chunk((long)S * M, D, F, E);
+  MM_CHECK_ARG(!chunk || workspace, "workspace is null");
+  const int unit = dtype == MM_F32 ? 4 : 8;
+  const bool dma = aligned(x) && xt % unit == 0 && (M == 1 || xm % unit == 0) && D % unit == 0;
+  int rc = MM_OK;
+#define CALL(split, dma)                                                                              \
+  if (dtype == MM_F32) rc = launch_wgrad<float, split, dma>(a, S, chunk, false, workspace, stream);   \
+  else if (dtype == MM_BF16) rc = launch_wgrad<__bf16, split, dma>(a, S, chunk, big, workspace, stream); \
+  else rc = launch_wgrad<_Float16, split, dma>(a, S, chunk, big, workspace, stream);
+  const bool big = dma && !chunk && D > 128 && F > 128 && E * ((D + 255) / 256) * ((F + 255) / 256) >= 512;
+  if (chunk) { if (dma) { CALL(true, true) } else { CALL(true, false) } }
+  else { if (dma) { CALL(false, true) } else { CALL(false, false) } }
+#undef CALL
+  if (rc != MM_OK) return rc;
+  if (chunk)
+    MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_wgrad_sum_kernel<T_>),
+                                          dim3((unsigned)(((long)D * F + 255) / 256), E), dim3(256), 0, stream, a,
+                                          chunk, workspace));
+  return mm::launch_status("mm_expert_wgrad");
+}

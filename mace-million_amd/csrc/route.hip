@@ -2,15 +2,17 @@
 //     key_e = logit_e + bias_e (fp32, one rounding); a logit or key of -inf closes the expert
 //     groups: the top_groups groups (of E / groups experts each) of largest key stay open
 //     chosen: the k largest keys, ties to the lowest index; expert -1 and gate 0 where no open expert is left
-//     score: softmax over the E logits, or sigmoid of each; gate_j = scale score_j / sum_chosen score, or scale score_j
-// The bias moves the choice only, not the gates.  It is added to the logits, of which both scores are monotone functions:
-// one rounded addition, so the choice does not depend on the order of a sum or the rounding of an exponential, and
-// saturated sigmoids do not tie.  Renormalised gates are a softmax over the chosen of the scores' logarithms (of the
-// logits, or of log sigmoid), so that scores that all underflow still give gates of sum scale.  A NaN logit is chosen
-// first and makes the gates NaN.
-// A row lies in LPR lanes, C consecutive logits each; k rounds of a maximum over the lanes' best keys (as integers of the
-// same order), the lowest lane with it giving its first such logit: no sort, no memory but the logits and the results.
-// Bound by the rounds' vector instructions for large k, by HBM for small k.
+//     score: softmax over the E logits, or sigmoid of each
+//     gate_j = scale score_j / sum_chosen score, or scale score_j
+// The bias moves the choice only, not the gates.  It is added to the logits, of which both scores are monotone
+// functions: one rounded addition, so the choice does not depend on the order of a sum or the rounding of an
+// exponential, and saturated sigmoids do not tie.  Renormalised gates are a softmax over the chosen of the scores'
+// logarithms (of the logits, or of log sigmoid), so that scores that all underflow still give gates of sum scale.  A
+// NaN logit is chosen first and makes the gates NaN.
+// A row lies in LPR lanes, C consecutive logits each; k rounds of a
+// maximum over the lanes' best keys (as integers of the same order), the lowest lane with it giving its first such
+// logit: no sort, no memory but the logits and the results. Bound by the rounds' vector instructions for large k, by
+// HBM for small k.
 #include "rowvec.h"
 
 #define MM_ROUTE_MAX_E 1024
@@ -42,8 +44,8 @@ __device__ __forceinline__ unsigned mm_route_max(unsigned v) {
   return v;
 }
 
-// exp(x) for x <= 0 (NaN stays NaN) to 2 units in the last place: 2^(x log2 e) with the rounding error of the product put
-// back to first order.  A softmax over a whole row takes one per logit, and expf twice the instructions.
+// exp(x) for x <= 0 (NaN stays NaN) to 2 units in the last place: 2^(x log2 e) with the rounding error of the product
+// put back to first order.  A softmax over a whole row takes one per logit, and expf twice the instructions.
 __device__ __forceinline__ float mm_exp_neg(float x) {
   x = x < -150.f ? -150.f : x;   // 0 either way
   const float t = x * 1.44269504088896340736f;
@@ -220,8 +222,8 @@ __global__ void __launch_bounds__(256) mm_route_fwd_kernel(MMRoute a, const T* _
 //   renormalised       d log score_j = gate_j (dgate_j - sum_i w_i dgate_i)
 //   sigmoid, plain     d log score_j = gate_j dgate_j
 //   softmax, plain     dl_e = [e chosen] gate_e dgate_e - p_e sum_j gate_j dgate_j,  p over all E logits
-// and d log score / dl = 1 (softmax, renormalised) or 1 - sigmoid(l).  The E values of a row are put together in LDS and
-// written once; the logits are read where a formula has them.  Bound by HBM.
+// and d log score / dl = 1 (softmax, renormalised) or 1 - sigmoid(l).  The E values of a row are put together in LDS
+// and written once; the logits are read where a formula has them.  Bound by HBM.
 template <typename T, int LPR, int C, int KM>
 __global__ void __launch_bounds__(256) mm_route_bwd_kernel(MMRoute a, const T* __restrict__ logits,
                                                            const float* __restrict__ gates,
@@ -301,6 +303,8 @@ __global__ void __launch_bounds__(256) mm_route_bwd_kernel(MMRoute a, const T* _
 }
 
 namespace {
+unsigned route_wg(long rows, int lanes) { return (unsigned)((rows + 256 / lanes - 1) / (256 / lanes)); }
+
 int route_args(const char* name, int dtype, long T, int E, int k, int scoring, int groups, int top_groups, long ldl,
                float scale, MMRoute* a, int renorm) {
   auto bad = [&](const char* what, int code) {
@@ -340,8 +344,8 @@ extern "C" int mm_route_fwd(const void* logits, long ldl, int dtype, long T, int
   const int rc = route_args("mm_route_fwd", dtype, T, E, k, scoring, groups, top_groups, ldl, scale, &a, renorm);
   if (rc != MM_OK || T == 0) return rc;
 #define X(l, c, km)                                                                                             \
-  hipLaunchKernelGGL((mm_route_fwd_kernel<T_, l, c, km>), dim3((unsigned)((a.T + 256 / l - 1) / (256 / l))), dim3(256), 0, \
-                     stream, a, (const T_*)logits, bias, gates, experts);
+  hipLaunchKernelGGL((mm_route_fwd_kernel<T_, l, c, km>), dim3(route_wg(a.T, l)), dim3(256), 0, stream, a, \
+                     (const T_*)logits, bias, gates, experts);
   if (dtype == MM_F32) { using T_ = float; MM_ROUTE_SHAPES(X) }
   else if (dtype == MM_BF16) { using T_ = __bf16; MM_ROUTE_SHAPES(X) }
   else { using T_ = _Float16; MM_ROUTE_SHAPES(X) }
@@ -356,8 +360,8 @@ extern "C" int mm_route_bwd(const void* logits, long ldl, int dtype, long T, int
   const int rc = route_args("mm_route_bwd", dtype, T, E, k, scoring, 1, 1, ldl, scale, &a, renorm);
   if (rc != MM_OK || T == 0) return rc;
 #define X(l, c, km)                                                                                             \
-  hipLaunchKernelGGL((mm_route_bwd_kernel<T_, l, c, km>), dim3((unsigned)((a.T + 256 / l - 1) / (256 / l))), dim3(256), 0, \
-                     stream, a, (const T_*)logits, gates, experts, dgates, (T_*)dlogits);
+  hipLaunchKernelGGL((mm_route_bwd_kernel<T_, l, c, km>), dim3(route_wg(a.T, l)), dim3(256), 0, stream, a, \
+                     (const T_*)logits, gates, experts, dgates, (T_*)dlogits);
   if (dtype == MM_F32) { using T_ = float; MM_ROUTE_SHAPES(X) }
   else if (dtype == MM_BF16) { using T_ = __bf16; MM_ROUTE_SHAPES(X) }
   else { using T_ = _Float16; MM_ROUTE_SHAPES(X) }

@@ -1,8 +1,9 @@
 // PyTorch functions of the layer norm, routing and expert kernels: argument checks, output and workspace tensors, the
 // calls of the C ABI on torch's current stream, and their place in autograd.
 //
-// In C++ because small calls are bound by the host: with the forward and backward as Python functions, a training call took
-// 130 - 210 us whatever its kernels took, most of it the hand-over of the interpreter to autograd's thread and back.
+// In C++ because small calls are bound by the host: with the forward and backward as Python functions, a training call
+// took 130 - 210 us whatever its kernels took, most of it the hand-over of the interpreter to autograd's thread and
+// back.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
@@ -139,7 +140,8 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     const auto p_type = p_code == 0 ? at::kFloat : x.scalar_type();
     const int at_bias = weight.defined() ? 2 : 1;   // autograd counts the tensors that are there
     if (weight.defined() && ctx->needs_input_grad(1)) dw = at::empty({D}, x.options().dtype(p_type));
-    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(at_bias)) db = at::empty({D}, x.options().dtype(p_type));
+    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(at_bias))
+      db = at::empty({D}, x.options().dtype(p_type));
     if (dw.defined() || db.defined()) {
       size_t bytes = 0;
       done(mm_layernorm_workspace(rows, (int)D, code, &bytes));
@@ -216,7 +218,8 @@ struct RouteFn : torch::autograd::Function<RouteFn> {
     const Tensor dg = grads[0].contiguous();
     Tensor dl = at::empty({T, E}, x.options());
     done(mm_route_bwd(ptr(x), distance(x), (int)args[0], T, (int)E, (int)k, (int)args[1], (int)args[2],
-                      (float)ctx->saved_data["scale"].toDouble(), fptr(gates), iptr(experts), fptr(dg), ptr(dl), stream()));
+                      (float)ctx->saved_data["scale"].toDouble(), fptr(gates), iptr(experts), fptr(dg), ptr(dl),
+                      stream()));
     variable_list out(9);
     out[0] = dl;
     return once(out, "route");
@@ -279,15 +282,17 @@ Lists make_pairs(const Tensor& experts, long E) {
   done(mm_expert_plan_scratch((int)T, (int)buckets - 1, &scratch));
   const Tensor buf = i32({T + buckets + scratch}, experts);
   int* p = iptr(buf);
-  done(mm_expert_plan_pairs(iptr(experts), (int)T, (int)E, p, p + buckets, scratch ? p + buckets + T : nullptr, stream()));
+  done(mm_expert_plan_pairs(iptr(experts), (int)T, (int)E, p, p + buckets, scratch ? p + buckets + T : nullptr,
+                            stream()));
   return {buf.narrow(0, 0, buckets), buf.narrow(0, buckets, T)};
 }
 
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
 // The sorts wait until a product (or the caller) needs one: few rows need none, and rows of two choices may need the
-// pairs' instead of the slots'.  Under graph capture the slots are sorted at once, so that a captured plan follows every
-// replay; lists that a capture needs of an older plan are its own and are not kept (they hold nothing until a replay).
+// pairs' instead of the slots'.  Under graph capture the slots are sorted at once, so that a captured plan follows
+// every replay; lists that a capture needs of an older plan are its own and are not kept (they hold nothing until a
+// replay).
 struct Plan {
   Tensor experts;
   long T, k, E;
@@ -329,10 +334,10 @@ std::shared_ptr<Plan> plan_experts(const Tensor& experts, int64_t E) {
 // ------------------------------------------------------------------------------------------------ products
 struct Sizes { long T, M, D, F, E, k; };
 
-// Whether rows go straight through their blocks (mm_expert_few), without a plan and without joining slots: while the blocks'
-// bytes that they read, mostly from the L2s, stay below 64 MB.  Measured (us, straight against sorted): 128 -> 128 float, 2
-// of 8 experts: 1 row 3.6 / 19, 128 rows (17 MB) 4.4 / 21; 1024 -> 1024 bfloat16, 4 of 64: 1 row 17 / 26, 8 rows (67 MB)
-// 33 / 32, 16 rows 36 / 35, 64 rows 126 / 36; the same in float: 4 rows (67 MB) 26 / 75.
+// Whether rows go straight through their blocks (mm_expert_few), without a plan and without joining slots: while the
+// blocks' bytes that they read, mostly from the L2s, stay below 64 MB.  Measured (us, straight against sorted): 128 ->
+// 128 float, 2 of 8 experts: 1 row 3.6 / 19, 128 rows (17 MB) 4.4 / 21; 1024 -> 1024 bfloat16, 4 of 64: 1 row 17 / 26,
+// 8 rows (67 MB) 33 / 32, 16 rows 36 / 35, 64 rows 126 / 36; the same in float: 4 rows (67 MB) 26 / 75.
 bool few_rows(const Sizes& n, int code) {
   const double bytes = (double)n.T * n.M * n.k * n.D * n.F * (code == 0 ? 4 : 2);
   return bytes <= 64e6 && n.T <= 65535 && n.M <= 65535;
@@ -340,13 +345,13 @@ bool few_rows(const Sizes& n, int code) {
 
 Tensor inner(const Tensor& t) { return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; }
 
-// Whether the choices of a row are joined before they are written (mm_expert_joined) instead of through fp32 rows of the
-// slots; K values a row go in, N come out.  One choice: always (65,536 rows, 8 experts, us, joined / slots: 128 -> 128
-// float 25 / 37, bfloat16 16 / 29; 16,384 rows 1024 -> 1024 float 259 / 270, bfloat16 59 / 99).  Two choices: where every
-// pair of experts fills tiles of rows and enough values are not written and read again to pay for the pairs' plan
-// (15 us): float up to 128 values from 2 M results on (98,304 rows 128 -> 128: 44 / 70), beyond that splitting the operands
-// of the small tiles costs more (256 -> 256, 65,536 rows: 159 / 173, 1024 -> 1024 521 / 484); 16-bit types from 16 M
-// results on (65,536 rows 256 -> 256: 52 / 84; 98,304 rows 128 -> 128: 39 / 56).
+// Whether the choices of a row are joined before they are written (mm_expert_joined) instead of through fp32 rows of
+// the slots; K values a row go in, N come out.  One choice: always (65,536 rows, 8 experts, us, joined / slots: 128 ->
+// 128 float 25 / 37, bfloat16 16 / 29; 16,384 rows 1024 -> 1024 float 259 / 270, bfloat16 59 / 99).  Two choices:
+// where every pair of experts fills tiles of rows and enough values are not written and read again to pay for the
+// pairs' plan (15 us): float up to 128 values from 2 M results on (98,304 rows 128 -> 128: 44 / 70), beyond that
+// splitting the operands of the small tiles costs more (256 -> 256, 65,536 rows: 159 / 173, 1024 -> 1024 521 / 484);
+// 16-bit types from 16 M results on (65,536 rows 256 -> 256: 52 / 84; 98,304 rows 128 -> 128: 39 / 56).
 bool join_rows(const Sizes& n, long K, long N, int code) {
   if (n.M > 64) return false;
   if (n.k == 1) return true;
@@ -355,8 +360,8 @@ bool join_rows(const Sizes& n, long K, long N, int code) {
   return code == 0 ? K <= 128 && n.M <= 16 && results >= 2000000 : results >= 16000000;
 }
 
-// dx with dgates likewise: all columns in one workgroup, two choices for float only (bfloat16, DG: 57 / 67, but 41 / 36 with 3
-// components)
+// dx with dgates likewise: all columns in one workgroup, two choices for float only (bfloat16, DG: 57 / 67, but 41 /
+// 36 with 3 components)
 bool join_gradients(const Sizes& n, int code, bool dgates) {
   return join_rows(n, n.F, n.D, code) && (!dgates || (n.D <= 128 && (n.k == 1 || code == 0)));
 }
@@ -417,7 +422,8 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
     if (ctx->needs_input_grad(0)) dx = at::empty({n.T, n.M, n.D}, x.options());
     if (ctx->needs_input_grad(1)) dw = at::empty({n.E, n.D, n.F}, x.options());
     if (gates.defined() && ctx->needs_input_grad(2)) dg = f32({n.T, n.k}, x);
-    // (joined or not was settled by whether the gates needed a gradient; if it is dropped here, that choice still holds)
+    // (joined or not was settled by whether the gates needed a gradient; if it is dropped here, that choice still
+    // holds)
     if ((dx.defined() || dg.defined()) && join_gradients(n, code, gates.defined() && gates.requires_grad())) {
       const bool pairs = k == 2;
       done(mm_expert_joined(ptr(dy), dy.stride(0), dy.stride(1), code, (int)n.T, k, M, F, D, ptr(w), 1, E, fptr(gates),
@@ -427,16 +433,16 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
       const Tensor rows = f32({S, M, D}, x);
       done(mm_expert_rows(ptr(dy), dy.stride(0), dy.stride(1), code, S, k, M, F, D, ptr(w), 1, E, iptr(offsets),
                           iptr(order), fptr(rows), stream()));
-      done(mm_expert_combine_bwd(fptr(rows), fptr(gates), iptr(experts), ptr(x), x.stride(0), x.stride(1), code, n.T, k, M,
-                                 D, E, ptr(dx), fptr(dg), stream()));
+      done(mm_expert_combine_bwd(fptr(rows), fptr(gates), iptr(experts), ptr(x), x.stride(0), x.stride(1), code, n.T, k,
+                                 M, D, E, ptr(dx), fptr(dg), stream()));
     }
     if (dw.defined()) {
       size_t bytes = 0;
       done(mm_expert_wgrad_workspace(S, M, D, F, E, &bytes));
       Tensor ws;
       if (bytes) ws = f32({(int64_t)(bytes / sizeof(float))}, x);
-      done(mm_expert_wgrad(ptr(x), x.stride(0), x.stride(1), ptr(dy), dy.stride(0), dy.stride(1), code, S, k, M, D, F, E,
-                           fptr(gates), iptr(offsets), iptr(order), ptr(dw), fptr(ws), stream()));
+      done(mm_expert_wgrad(ptr(x), x.stride(0), x.stride(1), ptr(dy), dy.stride(0), dy.stride(1), code, S, k, M, D, F,
+                           E, fptr(gates), iptr(offsets), iptr(order), ptr(dw), fptr(ws), stream()));
     }
     variable_list out(5);
     out[0] = dx;
