@@ -331,10 +331,10 @@ int mm_spline_coeffs(const double* samples, int M, int nW, double eps, double h,
 /* ---------------------------------------------------------------------------------------------- mixtures of experts
  * Layer norm, routing and the experts' products (no counterpart in the reference; its nearest operation is SpeciesSkip,
  * fast_layers.py:41-105).  dtype: 0 float, 1 bfloat16, 2 float16, of x, y, W, logits and their gradients; gates, means
- * and sums are float.  Strides (ld*, st, sm, xt, xm, yt, ym) count elements; rows are contiguous along their last axis and
- * need only the alignment of an element. */
-/* y = (x - mean) rstd w + b over rows of D <= 16384 values (-3 beyond); w, b [D] of p_dtype (dtype or 0), nullable; mean,
- * rstd [rows] nullable together */
+ * and sums are float.  Strides (ld*, st, sm, xt, xm, yt, ym) count elements; rows are contiguous along their last axis
+ * and need only the alignment of an element. */
+/* y = (x - mean) rstd w + b over rows of D <= 16384 values (-3 beyond); w, b [D] of p_dtype (dtype or 0), nullable;
+ * mean, rstd [rows] nullable together */
 int mm_layernorm_fwd(const void* x, long ldx, int dtype, long rows, int D, const void* w, const void* b, int p_dtype,
                      float eps, void* y, long ldy, float* mean, float* rstd, mm_stream_t stream);
 int mm_layernorm_workspace(long rows, int D, int dtype, size_t* bytes /* HOST */);
@@ -342,9 +342,10 @@ int mm_layernorm_workspace(long rows, int D, int dtype, size_t* bytes /* HOST */
 int mm_layernorm_bwd(const void* dy, long lddy, const void* x, long ldx, int dtype, long rows, int D, const void* w,
                      int p_dtype, const float* mean, const float* rstd, void* dx, long lddx, void* dw, void* db,
                      float* workspace, mm_stream_t stream);
-/* gates, experts [T, k]: the k <= 32 of E <= 1024 experts of largest logit + bias (bias [E] nullable), ties to the lowest
- * index, expert -1 and gate 0 where fewer are open (a logit of -inf closes an expert); of `groups` <= 64 equal groups only
- * the top_groups with the largest keys.  scoring 0 softmax, 1 sigmoid; renorm: gates of sum `scale` (not 0). */
+/* gates, experts [T, k]: the k <= 32 of E <= 1024 experts of largest logit + bias (bias [E] nullable), ties to the
+ * lowest index, expert -1 and gate 0 where fewer are open (a logit of -inf closes an expert); of `groups` <= 64 equal
+ * groups only the top_groups with the largest keys.  scoring 0 softmax, 1 sigmoid; renorm: gates of sum `scale` (not
+ * 0). */
 int mm_route_fwd(const void* logits, long ldl, int dtype, long T, int E, int k, int scoring, const float* bias,
                  int groups, int top_groups, int renorm, float scale, float* gates, int* experts, mm_stream_t stream);
 /* dlogits [T, E] (all of it written) of the gates and experts that mm_route_fwd gave */
@@ -354,19 +355,19 @@ int mm_route_bwd(const void* logits, long ldl, int dtype, long T, int E, int k, 
  * expert outside [0, E) order[offsets[E] .. S).  scratch: as many ints as mm_expert_plan_scratch says (0: null) */
 int mm_expert_plan_scratch(int S, int E, long* ints /* HOST */);
 int mm_expert_plan(const int* experts, int S, int E, int* offsets, int* order, int* scratch, mm_stream_t stream);
-/* The rows 0 .. T - 1 of two choices each sorted by the pair of their experts, E <= 21: pair i of (E + 1)(E + 2) / 2 has
- * the rows from order[offsets[i]] on, the last one to T; pairs e1 <= e2 in ascending order of (e1, e2), an expert outside
- * [0, E) counting as E.  scratch: of mm_expert_plan_scratch(T, (E + 1)(E + 2) / 2 - 1, ...) ints */
+/* The rows 0 .. T - 1 of two choices each sorted by the pair of their experts, E <= 21: pair i of (E + 1)(E + 2) / 2
+ * has the rows from order[offsets[i]] on, the last one to T; pairs e1 <= e2 in ascending order of (e1, e2), an expert
+ * outside [0, E) counting as E.  scratch: of mm_expert_plan_scratch(T, (E + 1)(E + 2) / 2 - 1, ...) ints */
 int mm_expert_plan_pairs(const int* experts, int T, int E, int* offsets, int* order, int* scratch, mm_stream_t stream);
-/* out [T, M, N] (of in's type, rows without an expert 0) = sum over the k = 1 or 2 choices of gate in[t, m] @ W[e] (W as in
- * mm_expert_rows), joined before they are written; offsets and order of mm_expert_plan (k = 1) or mm_expert_plan_pairs
- * (k = 2).  dgates [T, k] nullable: with in = dy and W transposed, sum_m <x[t, m], dy[t, m] @ W[e]^T>, N <= 128, and either
- * k = 1 or float, K <= 128 and M <= 16 (out then nullable).  M <= 64 */
+/* out [T, M, N] (of in's type, rows without an expert 0) = sum over the k = 1 or 2 choices of gate in[t, m] @ W[e] (W
+ * as in mm_expert_rows), joined before they are written; offsets and order of mm_expert_plan (k = 1) or
+ * mm_expert_plan_pairs (k = 2).  dgates [T, k] nullable: with in = dy and W transposed, sum_m <x[t, m], dy[t, m] @
+ * W[e]^T>, N <= 128, and either k = 1 or float, K <= 128 and M <= 16 (out then nullable).  M <= 64 */
 int mm_expert_joined(const void* in, long st, long sm, int dtype, int T, int k, int M, int K, int N, const void* W,
                      int transposed, int E, const float* gates, const int* experts, const int* offsets,
                      const int* order, void* out, const void* x, long xt, long xm, float* dgates, mm_stream_t stream);
-/* out [S, M, N] (slots without an expert are not written): out[s, m] = in[s / k, m] @ W[e], W [E, K, N], or [E, N, K] with
- * `transposed`; in at (row, component) offset row st + component sm; S M < 2^31 */
+/* out [S, M, N] (slots without an expert are not written): out[s, m] = in[s / k, m] @ W[e], W [E, K, N], or [E, N, K]
+ * with `transposed`; in at (row, component) offset row st + component sm; S M < 2^31 */
 int mm_expert_rows(const void* in, long st, long sm, int dtype, int S, int k, int M, int K, int N, const void* W,
                    int transposed, int E, const int* offsets, const int* order, float* out, mm_stream_t stream);
 /* y [T, M, F] = sum_j gates[t, j] x[t, m] @ W[experts[t, j]] (W [E, D, F]) in one launch without a plan, for few rows;
@@ -376,8 +377,8 @@ int mm_expert_few(const void* x, long st, long sm, int dtype, int T, int k, int 
 /* y [T, M, N] = sum_j gates[t, j] rows[t k + j] (gates null: ones) over the slots with an expert in [0, E) */
 int mm_expert_combine(const float* rows, const float* gates, const int* experts, int dtype, long T, int k, int M, int N,
                       int E, void* y, mm_stream_t stream);
-/* from rows = dy @ W^T of every slot: dx [T, M, N] as mm_expert_combine, dgates[t, j] = sum_m <x[t, m], rows[t k + j, m]>
- * (0 without an expert); each nullable */
+/* from rows = dy @ W^T of every slot: dx [T, M, N] as mm_expert_combine, dgates[t, j] = sum_m <x[t, m], rows[t k + j,
+ * m]> (0 without an expert); each nullable */
 int mm_expert_combine_bwd(const float* rows, const float* gates, const int* experts, const void* x, long st, long sm,
                           int dtype, long T, int k, int M, int N, int E, void* dx, float* dgates, mm_stream_t stream);
 /* dW [E, D, F] = sum over the slots of e and the components of gate x^T dy; 0 for an expert without slots; workspace of

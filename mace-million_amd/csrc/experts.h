@@ -176,9 +176,9 @@ __device__ __forceinline__ void mm_products(floatx4 (&acc)[FN][FM], A a, B b, co
 // KC (the summed index contiguous in memory): a row of 8 units (128 bytes), unit u of row r at 8 r + (u ^ (r & 7)), so
 // that the 16 rows of an operand read spread over all banks.
 // NC (the other index contiguous): a row per value of the summed index, UPR units; unit u of row q at
-// UPR q + (u ^ s(q)), s(q) chosen so that the rows read together lie in different banks.  16-bit operands come out of it
-// by transposing reads (ds_read_b64_tr_b16: 16 lanes give the addresses of a 4 x 16 block, four lanes a row, and lane i
-// receives its column i), float operands value by value.
+// UPR q + (u ^ s(q)), s(q) chosen so that the rows read together lie in different banks.  16-bit operands come out of
+// it by transposing reads (ds_read_b64_tr_b16: 16 lanes give the addresses of a 4 x 16 block, four lanes a row, and
+// lane i receives its column i), float operands value by value.
 // Staged by loads straight into LDS (16 bytes a lane, the wave's units in order, so the swizzle is in the addresses of
 // the sources) where the units are aligned, else through registers.
 template <typename T>

@@ -11,7 +11,7 @@ Module map (mirrors the reference package mace_onegpu, same module paths for the
   fast_layers       per-chunk layer pipelines on the HIP kernels
   layer_norm        layer_norm, LayerNorm: forward and backward kernels over the last axis
   experts           mixtures of expert weight blocks: route, plan_experts, expert_linear
-  expert_mix        ExpertMix: a mixture of expert linears on node features (norm, route, products), and a command that fits one
+  expert_mix        ExpertMix: a mixture of expert linears on node features, and a command that fits one
   lammps_data       periodic-image ML-IAP data object (one GPU stands in for LAMMPS' ghost exchange)
   model, o3, codegen, systems, _lib, _ops   architecture, couplings, kernel generator, inputs, C-ABI and torch bindings
 """

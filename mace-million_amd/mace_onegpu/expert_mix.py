@@ -1,4 +1,5 @@
-"""ExpertMix: a mixture of expert linears on equivariant node features, and a command that fits one on pass A's features.
+"""ExpertMix: a mixture of expert linears on equivariant node features, and a command that fits one on pass A's
+features.
 
 Where the species-block skip multiplies an atom's features by the block of its species (SpeciesSkip of the reference,
 fast_layers.py:41-105), a mixture gives every atom k of E blocks with learned gates: norm of the scalars, a router,
@@ -23,10 +24,10 @@ from .layer_norm import LayerNorm
 
 
 class ExpertMix(torch.nn.Module):
-    """out[i, l, :] = sum_j gates[i, j] h[i, l, :] @ blocks[l][experts[i, j]] for ir_mul features h [N, components, C] (or
-    [N, components C]) with irreps ls (every one C channels); gates and experts from the layer norm of `by` [N, C] (the
-    scalars of h).  balance [n_experts] is added to the logits for the choice alone; update_balance moves it against
-    the loads of the last call."""
+    """out[i, l, :] = sum_j gates[i, j] h[i, l, :] @ blocks[l][experts[i, j]] for ir_mul features h [N, components, C]
+    (or [N, components C]) with irreps ls (every one C channels); gates and experts from the layer norm of `by` [N, C]
+    (the scalars of h).  balance [n_experts] is added to the logits for the choice alone; update_balance moves it
+    against the loads of the last call."""
 
     def __init__(self, channels=128, ls=(0, 1), n_experts=8, k=2, scoring="softmax", groups=1, top_groups=None,
                  renormalize=True, seed=0, dtype=torch.float32, device="cuda"):

@@ -5,8 +5,8 @@
 x: float32, bfloat16 or float16, [..., D] with D up to 16384; rows may be strided (the scalar component h[:, 0, :] of
 ir_mul features) and are read in place when the last axis is contiguous.  weight and bias: [D], of x's type or float32,
 either may be None.  Means, variances and the gradients' sums are float32.  Backward gives dx, dweight (summed over the
-rows in a fixed order: the same bits in every run) and dbias, once (no second derivative).  Runs on torch's current stream,
-can be captured into a HIP graph, and needs the GPU: there is no CPU path.  The reference has no counterpart.
+rows in a fixed order: the same bits in every run) and dbias, once (no second derivative).  Runs on torch's current
+stream, can be captured into a HIP graph, and needs the GPU: there is no CPU path.  The reference has no counterpart.
 """
 import torch
 

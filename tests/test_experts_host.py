@@ -53,7 +53,8 @@ def test_layernorm_bwd(change, code, match):
 @needs_lib
 @pytest.mark.parametrize("change,code,match", [
     (dict(dtype=5), -1, "dtype"), (dict(T=-1), -1, "sizes"), (dict(E=0), -1, "sizes"), (dict(k=0), -1, "sizes"),
-    (dict(k=9), -1, "sizes"), (dict(ldl=7), -1, "sizes"), (dict(scoring=2), -1, "scoring"), (dict(groups=3), -1, "groups"),
+    (dict(k=9), -1, "sizes"), (dict(ldl=7), -1, "sizes"), (dict(scoring=2), -1, "scoring"),
+    (dict(groups=3), -1, "groups"),
     (dict(groups=4, top_groups=5), -1, "groups"), (dict(groups=4, top_groups=0), -1, "groups"),
     (dict(scale=0.0), -1, "scale"), (dict(E=1025, ldl=1025), -3, "1024"), (dict(E=64, ldl=64, k=33), -3, "32"),
     (dict(E=130, ldl=130, groups=65), -3, "64")])

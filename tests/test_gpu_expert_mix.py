@@ -13,8 +13,8 @@ def _mix(**kw):
 
 
 def test_value_and_gradients_against_plain_operations():
-    """64-bit autograd through the same formula with the module's choice of experts.  Errors of the gates (96 u, and of the
-    logits behind them: 128 products and a norm, 250 u of magnitudes below 40) and products (144 u) stay below
+    """64-bit autograd through the same formula with the module's choice of experts.  Errors of the gates (96 u, and of
+    the logits behind them: 128 products and a norm, 250 u of magnitudes below 40) and products (144 u) stay below
     1e-4 of each result's largest value."""
     m = _mix(n_experts=5, k=2)
     h = torch.randn(300, 4, 128, generator=torch.Generator().manual_seed(1)).cuda().requires_grad_()

@@ -1,9 +1,9 @@
 """plan_experts against a stable sort (exact), and expert_linear with its gradients against plain sums in 64 bits.
 
-Tolerances, element by element: a sum of n products in float32 is off by at most (n + 16) u sum |terms|, u = 2^-24 (16 for
-the gate, the joining of the k slots, and products of split operands, 3 u each); rounding to the output's type adds half a
-unit in its last place, and dW of 16-bit types may round gate x dy to that type before the product: one more half unit of
-the sum of magnitudes."""
+Tolerances, element by element: a sum of n products in float32 is off by at most (n + 16) u sum |terms|, u = 2^-24 (16
+for the gate, the joining of the k slots, and products of split operands, 3 u each); rounding to the output's type adds
+half a unit in its last place, and dW of 16-bit types may round gate x dy to that type before the product: one more
+half unit of the sum of magnitudes."""
 import pytest
 import torch
 
@@ -242,7 +242,7 @@ def test_graph_replay():
             assert torch.equal(y, step())
 
 
-# ------------------------------------------------------------------------------------------------ the variants themselves
+# ------------------------------------------------------------------------------------------------ the variants
 def _rows_reference(x, w, experts, k, transposed):
     """[S, M, N] products of every slot, 64 bits (zeros without an expert), and sums of magnitudes."""
     T, M, K = x.shape
@@ -266,7 +266,8 @@ def _rows_reference(x, w, experts, k, transposed):
     (257, 1, 129, 257, 2, 1, 0), (200, 1, 200, 40, 70, 3, 0), (90, 1, 64, 64, 5, 2, 1), (2100, 1, 136, 264, 2, 1, 0),
     (1500, 1, 512, 520, 2, 2, 0)])
 def test_rows_of_slots(T, M, K, N, E, k, off, transposed, dtype):
-    """mm_expert_rows on its own: tiles of both sizes, cut tiles, odd widths, unaligned rows, slots without an expert."""
+    """mm_expert_rows on its own: tiles of both sizes, cut tiles, odd widths, unaligned rows, slots without an
+    expert."""
     from mace_onegpu._lib import K as L, stream
     from mace_onegpu.experts import plan_experts
     g = torch.Generator().manual_seed(T + K + N)
@@ -292,7 +293,8 @@ def test_rows_of_slots(T, M, K, N, E, k, off, transposed, dtype):
 @pytest.mark.parametrize("T,M,K,N,E,k,off", [
     (1, 1, 3, 5, 1, 1, 0), (300, 1, 64, 128, 3, 1, 0), (300, 3, 72, 136, 3, 2, 0), (77, 5, 33, 201, 2, 2, 0),
     (1000, 1, 128, 128, 21, 2, 0), (3000, 3, 128, 128, 2, 2, 0),
-    (5000, 1, 32, 128, 3, 2, 0), (2500, 2, 100, 60, 2, 2, 1), (129, 64, 40, 24, 2, 1, 0), (400, 1, 200, 260, 4, 2, 1), (2000, 1, 128, 64, 4, 2, 0)])
+    (5000, 1, 32, 128, 3, 2, 0), (2500, 2, 100, 60, 2, 2, 1), (129, 64, 40, 24, 2, 1, 0), (400, 1, 200, 260, 4, 2, 1),
+    (2000, 1, 128, 64, 4, 2, 0)])
 def test_joined_rows(T, M, K, N, E, k, off, transposed, dtype):
     """mm_expert_joined on its own: pairs of different and equal experts, one or no expert, and dgates of one choice."""
     import ctypes

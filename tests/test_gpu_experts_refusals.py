@@ -27,7 +27,8 @@ def test_layer_norm():
 def test_route():
     from mace_onegpu.experts import route
     x = _z(3, 8)
-    for args, kw, err, match in [((x[0], 2), {}, ValueError, r"\[rows, experts\]"), ((x, 0), {}, ValueError, "k must be"),
+    for args, kw, err, match in [((x[0], 2), {}, ValueError, r"\[rows, experts\]"),
+                                 ((x, 0), {}, ValueError, "k must be"),
                                  ((x, 9), {}, ValueError, "k must be"), ((_z(3, 64), 33), {}, ValueError, "k must be"),
                                  ((_z(3, 1025), 2), {}, ValueError, "1024 experts"),
                                  ((x, 2), dict(scoring="relu"), ValueError, "scoring"),
@@ -51,7 +52,8 @@ def test_plan_and_products():
         with pytest.raises(err, match=match):
             plan_experts(*args)
     plan, x, w, g = plan_experts(e, 3), _z(4, 8), _z(3, 8, 5), _z(4, 2)
-    for args, err, match in [((x, w.half(), plan, g), TypeError, "weight must be"), ((x, w, e, g), TypeError, "ExpertPlan"),
+    for args, err, match in [((x, w.half(), plan, g), TypeError, "weight must be"),
+                             ((x, w, e, g), TypeError, "ExpertPlan"),
                              ((x[0], w, plan, g), ValueError, "x must be"), ((x[:3], w, plan, g), ValueError, "3 rows"),
                              ((x, w[:2], plan, g), ValueError, "weight must be"), ((x[:, :7], w, plan, g), ValueError,
                                                                                     "weight must be"),

@@ -1,9 +1,9 @@
 """layer_norm and its gradients against the formula in 64 bits on the same (rounded) inputs.
 
 Tolerances, element by element, u = 2^-24: a sum of n values in lanes and trees has at most C = 32 + 10 roundings on any
-path (32 values a lane, 1024 lanes), so the mean is off by at most C u max|x| and, scaled by rstd and w, so is y; the other
-operations add less than 16 u of their terms.  Rounding to the output's type adds half a unit in its last place.  dw and
-db: the same with sums over rows (a lane's rows, then up to 1024 partial sums in trees and 16 in a row)."""
+path (32 values a lane, 1024 lanes), so the mean is off by at most C u max|x| and, scaled by rstd and w, so is y; the
+other operations add less than 16 u of their terms.  Rounding to the output's type adds half a unit in its last place. 
+dw and db: the same with sums over rows (a lane's rows, then up to 1024 partial sums in trees and 16 in a row)."""
 import pytest
 import torch
 
@@ -144,7 +144,8 @@ def test_no_rows_and_constant_and_non_finite_rows():
 
 @pytest.mark.parametrize("D", [64, 1000])
 def test_gradient_against_differences(D):
-    """<grad, v> against (f(x + h v) - f(x - h v)) / 2 h, f summed in 64 bits: off by O(h^2) and roundings of f over h."""
+    """<grad, v> against (f(x + h v) - f(x - h v)) / 2 h, f summed in 64 bits: off by O(h^2) and roundings of f over
+    h."""
     from mace_onegpu.layer_norm import layer_norm
     x, w, b, dy = (t.cuda() for t in _inputs(11, D, torch.float32, torch.float32, D))
     g = torch.Generator().manual_seed(9)

@@ -1,9 +1,10 @@
 """route and its gradient against a plain row-by-row implementation in 64 bits.
 
 The choice is defined by float32 sums logit + bias and compared exactly.  Gates: u = 2^-24; an exponent's argument is a
-difference rounded once (off by u |x - m|, |x - m| <= 40 here unless the exponential is 0 next to another), expf and log1pf
-are good to 4 u, a sum of up to 1024 scores in lanes of 16 and trees has 26 roundings, and a division one more: 96 u in all,
-relative.  The gradient's terms carry the gates' errors and a sum over k <= 32 of them: 256 u of the sum of magnitudes."""
+difference rounded once (off by u |x - m|, |x - m| <= 40 here unless the exponential is 0 next to another), expf and
+log1pf are good to 4 u, a sum of up to 1024 scores in lanes of 16 and trees has 26 roundings, and a division one more:
+96 u in all, relative.  The gradient's terms carry the gates' errors and a sum over k <= 32 of them: 256 u of the sum
+of magnitudes."""
 import math
 
 import pytest
@@ -94,8 +95,8 @@ def _check(logits, k, dgates=None, **kw):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalize", [True, False])
-@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 8, 2), (67, 5, 5), (130, 16, 2), (65, 17, 3), (33, 64, 6), (70, 89, 3),
-                                   (20, 128, 8), (40, 256, 8), (9, 300, 32), (5, 1024, 17)])
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 8, 2), (67, 5, 5), (130, 16, 2), (65, 17, 3), (33, 64, 6),
+                                   (70, 89, 3), (20, 128, 8), (40, 256, 8), (9, 300, 32), (5, 1024, 17)])
 def test_choice_gates_and_gradient(T, E, k, renormalize, scoring, dtype):
     g = torch.Generator().manual_seed(1000 * T + E + k)
     logits = (1.5 * torch.randn(T, E, generator=g)).to(dtype)
