@@ -38,8 +38,9 @@ __device__ __forceinline__ void mm_held_put(uint4* stage, int row, int k4, const
 
 // KS: steps of 32 values.  FULL: K = 32 KS and whole tiles of columns, so that no load or store stands behind a
 // branch: the compiler then counts them and waits for the loads it needs only, not for the stores before them.  One
-// row's 8 values g of step t, plane p at unit ((tile * 3 + p) * 4 KS + 4 t + g) * 17 + row.
-template <bool TRANS, int KS, bool FULL>
+// row's 8 values g of step t, plane p at unit ((tile * 3 + p) * 4 KS + 4 t + g) * 17 + row.  RG = 2 (64 columns or
+// fewer): the waves share a stage's row tiles as well as the columns, so that none is left without work.
+template <bool TRANS, int KS, bool FULL, int RG>
 __global__ void __launch_bounds__(256, 2) mm_expert_held_kernel(MMHeld h, int tiles_n, int chunk) {
   constexpr int KG = 4 * KS, UNITS = 2 * 3 * KG * MM_HELD_AS, PER = KS;   // float4 a thread and stage: 32 * 8 KS / 256
   __shared__ uint4 Al[2][UNITS];
@@ -55,7 +56,7 @@ __global__ void __launch_bounds__(256, 2) mm_expert_held_kernel(MMHeld h, int ti
              __builtin_amdgcn_readfirstlane(t.rows)};
   part = __builtin_amdgcn_readfirstlane(part);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, i = lane & 15, g = lane >> 4;
-  const int n0 = part * 128 + 32 * wave;
+  const int n0 = part * 128 + 32 * (RG == 1 ? wave : wave & 1), tile0 = RG == 1 ? 0 : wave >> 1;   // columns, row tile
   const int* __restrict__ list = a.order + a.offsets[t.e];
   if (t.e >= a.E) {   // slots without an expert
     for (int r = wave; r < t.rows; r += 4) {
@@ -127,16 +128,16 @@ __global__ void __launch_bounds__(256, 2) mm_expert_held_kernel(MMHeld h, int ti
     for (int b = 0; b < 2; ++b) {   // stage st is in Al[b], stage st + 1 in x[b ^ 1]
       const int st = st0 + b;
       if (st >= nst) break;
-      floatx4 acc[2][2] = {};   // [row tile][column tile]
+      floatx4 acc[2 / RG][2] = {};   // [row tile][column tile]
       load(st + 2, x[b]);
-      MMFrag<float> f[2][2];
+      MMFrag<float> f[2][2 / RG];
       auto operands = [&](int s) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < 2 / RG; ++r)
 #pragma unroll
           for (int p = 0; p < 3; ++p)
             f[s & 1][r].v[p] =
-                __builtin_bit_cast(bf16x8, Al[b][((r * 3 + p) * KG + 4 * s + g) * MM_HELD_AS + i]);
+                __builtin_bit_cast(bf16x8, Al[b][(((tile0 + r) * 3 + p) * KG + 4 * s + g) * MM_HELD_AS + i]);
       };
       operands(0);
 #pragma unroll
@@ -145,13 +146,13 @@ __global__ void __launch_bounds__(256, 2) mm_expert_held_kernel(MMHeld h, int ti
         __builtin_amdgcn_sched_barrier(0);   // the reads of the next step stay ahead of the products of this one
         put(b ^ 1, s, x[b ^ 1]);             // a part of the next stage beside them (PER = KS)
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < 2 / RG; ++r)
 #pragma unroll
           for (int c = 0; c < 2; ++c) mm_mma(acc[r][c], w[s][c], f[s & 1][r]);
       }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = 32 * st + 16 * r + i;   // past the last row: that one again, with the same values
+      for (int r = 0; r < 2 / RG; ++r) {
+        const int row = 32 * st + 16 * (tile0 + r) + i;   // past the last row: that one again, with the same values
         float* __restrict__ o = a.out + (long)s_out[row] * a.N;
         const float gate = s_g[row];
 #pragma unroll
@@ -172,8 +173,8 @@ __global__ void __launch_bounds__(256, 2) mm_expert_held_kernel(MMHeld h, int ti
 // same 96 registers at K = 128), every operand of a row is read once for both, and the two products of a row are
 // joined and written once.  64 rows a stage, one workgroup a CU.  DG: with the rows of dy and W[e]^T also dgates[t, j]
 // = sum over m of <x[t, m], (dy W[e_j]^T)[t, m]>; all columns are then in one workgroup, and a chunk holds whole rows
-// t.
-template <bool TRANS, int KS, bool FULL, bool DG>
+// t.  RG = 2 (64 columns or fewer): 4 waves a half of a stage's rows.
+template <bool TRANS, int KS, bool FULL, bool DG, int RG>
 __global__ void __launch_bounds__(512, 2) mm_expert_held_pairs_kernel(MMPairs a, int tiles_n, int chunk) {
   constexpr int KG = 4 * KS, UNITS = 4 * 3 * KG * MM_HELD_AS, PER = KS;   // float4 a thread and stage: 64 * 8 KS / 512
   __shared__ uint4 Al[2][UNITS];
@@ -187,7 +188,8 @@ __global__ void __launch_bounds__(512, 2) mm_expert_held_pairs_kernel(MMPairs a,
   const int bucket = __builtin_amdgcn_readfirstlane(tile.e);
   part = __builtin_amdgcn_readfirstlane(part);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, i = lane & 15, g = lane >> 4;
-  const int n0 = part * 128 + 16 * wave;
+  const int n0 = part * 128 + 16 * (RG == 1 ? wave : wave & 3);
+  const int tile0 = RG == 1 ? 0 : wave >> 2 << 1;   // first row tile
   const int* __restrict__ list = a.order + a.offsets[bucket];
   int e0 = 0, e1 = bucket;
   while (e1 >= a.E + 1 - e0) e1 -= a.E + 1 - e0++;
@@ -279,37 +281,39 @@ __global__ void __launch_bounds__(512, 2) mm_expert_held_pairs_kernel(MMPairs a,
     for (int b = 0; b < 2; ++b) {   // stage st is in Al[b], stage st + 1 in x[b ^ 1]
       const int st = st0 + b;
       if (st >= nst) break;
-      float xv[DG ? 4 : 1][4];
+      float xv[DG ? 4 / RG : 1][4];
       if constexpr (DG) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) mm_load4(a.x + s_x[64 * st + 16 * r + i], n0 + 4 * g, a.N, xv[r]);
+        for (int r = 0; r < 4 / RG; ++r)
+          mm_load4(a.x + s_x[64 * st + 16 * (tile0 + r) + i], n0 + 4 * g, a.N, xv[r]);
       }
       load(st + 2, x[b]);
-      floatx4 acc[2][4] = {};   // [choice][row tile]
+      constexpr int H = 2 / RG;
+      floatx4 acc[2][2 * H] = {};   // [choice][row tile]
       MMFrag<float> f[2][2];
-      // row tiles 2 h, 2 h + 1 of step s: number 2 s + h
+      // row tiles 2 h, 2 h + 1 of this wave's, step s: number H s + h
       auto operands = [&](int q) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
           for (int p = 0; p < 3; ++p)
             f[q & 1][r].v[p] = __builtin_bit_cast(
-                bf16x8, Al[b][(((2 * (q & 1) + r) * 3 + p) * KG + 4 * (q >> 1) + g) * MM_HELD_AS + i]);
+                bf16x8, Al[b][(((tile0 + 2 * (q % H) + r) * 3 + p) * KG + 4 * (q / H) + g) * MM_HELD_AS + i]);
       };
       operands(0);
 #pragma unroll
-      for (int q = 0; q < 2 * KS; ++q) {
-        if (q + 1 < 2 * KS) operands(q + 1);
-        __builtin_amdgcn_sched_barrier(0);               // the reads of the next step stay ahead of the products
-        if (q & 1) put(b ^ 1, q >> 1, x[b ^ 1]);         // a part of the next stage beside them (PER = KS)
+      for (int q = 0; q < H * KS; ++q) {
+        if (q + 1 < H * KS) operands(q + 1);
+        __builtin_amdgcn_sched_barrier(0);                     // the reads of the next step stay ahead of the products
+        if (q % H == H - 1) put(b ^ 1, q / H, x[b ^ 1]);       // a part of the next stage beside them (PER = KS)
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) mm_mma(acc[c][2 * (q & 1) + r], w[c][q >> 1], f[q & 1][r]);
+          for (int c = 0; c < 2; ++c) mm_mma(acc[c][2 * (q % H) + r], w[c][q / H], f[q & 1][r]);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 64 * st + 16 * r + i;   // past the last row: that one again, with the same values
+      for (int r = 0; r < 2 * H; ++r) {
+        const int row = 64 * st + 16 * (tile0 + r) + i;   // past the last row: that one again, with the same values
         const float g0 = s_g[0][row], g1 = s_g[1][row];
         float v[4], d0 = 0.f, d1 = 0.f;
 #pragma unroll
@@ -331,18 +335,18 @@ __global__ void __launch_bounds__(512, 2) mm_expert_held_pairs_kernel(MMPairs a,
           d0 += __shfl_xor(d0, 32);
           d1 += __shfl_xor(d1, 32);
           if (lane < 16) {
-            s_part[b][wave][0][16 * r + i] = d0;
-            s_part[b][wave][1][16 * r + i] = d1;
+            s_part[b][wave][0][16 * (tile0 + r) + i] = d0;
+            s_part[b][wave][1][16 * (tile0 + r) + i] = d1;
           }
         }
       }
       __syncthreads();
       if constexpr (DG) {   // the columns of a row, wave by wave; the other s_part is written next
         if (tid < 128) {
-          const int c = tid >> 6;
+          const int c = tid >> 6, wave0 = RG == 2 ? lane / 32 * 4 : 0;   // the waves of this row
           float d = 0.f;
 #pragma unroll
-          for (int v = 0; v < 8; ++v) d += s_part[b][v][c][lane];
+          for (int v = 0; v < 8 / RG; ++v) d += s_part[b][wave0 + v][c][lane];
           s_dg[c][64 * st + lane] = d;
         }
       }
@@ -387,12 +391,13 @@ int launch_held(const char* name, const MMRows& a, int S, const float* gates, in
   if (too_many(wg, 256)) return range_error(name, "output too large for one launch");
   const MMHeld h{a, gates, lists, S};
   const bool whole = a.N % 128 == 0;
-#define CALL2(trans, ks, full)                                                                           \
-  hipLaunchKernelGGL((mm_expert_held_kernel<trans, ks, full>), dim3((unsigned)wg), dim3(256), 0, stream, \
+#define CALL2(trans, ks, full, rg)                                                                           \
+  hipLaunchKernelGGL((mm_expert_held_kernel<trans, ks, full, rg>), dim3((unsigned)wg), dim3(256), 0, stream, \
                      h, tiles_n, chunk)
 #define CALL(trans, ks)                                   \
-  if (a.K == 32 * ks && whole) CALL2(trans, ks, true);    \
-  else CALL2(trans, ks, false)
+  if (a.K == 32 * ks && whole) CALL2(trans, ks, true, 1); \
+  else if (a.N <= 64) CALL2(trans, ks, false, 2);         \
+  else CALL2(trans, ks, false, 1)
 #define CALLS(trans)                    \
   if (a.K <= 32) { CALL(trans, 1); }    \
   else if (a.K <= 64) { CALL(trans, 2); } \
@@ -421,12 +426,13 @@ int launch_pairs(const char* name, const MMPairs& a, int transposed, int chunk, 
   const int tiles_n = (a.N + 127) / 128;
   const long wg = (((long)a.T * a.M + chunk - 1) / chunk + (a.buckets < a.T ? a.buckets : a.T)) * tiles_n;
   if (too_many(wg, 512)) return range_error(name, "output too large for one launch");
-#define CALL2(trans, ks, full, dg)                                                                             \
-  hipLaunchKernelGGL((mm_expert_held_pairs_kernel<trans, ks, full, dg>), dim3((unsigned)wg), dim3(512), 0, stream, \
-                     a, tiles_n, chunk)
-#define CALL(trans, ks, dg)                                          \
-  if (a.K == 32 * ks && a.N % 128 == 0) CALL2(trans, ks, true, dg);  \
-  else CALL2(trans, ks, false, dg);
+#define CALL2(trans, ks, full, dg, rg)                                                                             \
+  hipLaunchKernelGGL((mm_expert_held_pairs_kernel<trans, ks, full, dg, rg>), dim3((unsigned)wg), dim3(512), 0, \
+                     stream, a, tiles_n, chunk)
+#define CALL(trans, ks, dg)                                             \
+  if (a.K == 32 * ks && a.N % 128 == 0) CALL2(trans, ks, true, dg, 1);  \
+  else if (a.N <= 64) CALL2(trans, ks, false, dg, 2);                   \
+  else CALL2(trans, ks, false, dg, 1);
 #define CALLS(trans, dg)                              \
   if (a.K <= 32) { CALL(trans, 1, dg) }               \
   else if (a.K <= 64) { CALL(trans, 2, dg) }          \

@@ -444,6 +444,7 @@ template <typename T, bool TRANS, bool DMA>
 int launch_rows(const MMRows& a, int S, bool big, hipStream_t stream) {
   if constexpr (sizeof(T) == 2 && DMA)
     if (big) return launch_rows_tile<T, TRANS, DMA, 256, 256, 2, 4>(a, S, stream);
+  if (a.N <= 64) return launch_rows_tile<T, TRANS, DMA, 128, 64, 2, 2>(a, S, stream);
   return launch_rows_tile<T, TRANS, DMA, 128, 128, 2, 2>(a, S, stream);
 }
 

@@ -191,6 +191,11 @@ template <typename T, bool SPLIT, bool DMA>
 int launch_wgrad(const MMWgrad& a, int S, int chunk, bool big, float* part, hipStream_t stream) {
   if constexpr (sizeof(T) == 2 && DMA && !SPLIT)
     if (big) return launch_wgrad_tile<T, SPLIT, DMA, 256, 256, 2, 4>(a, S, chunk, part, stream);
+  if (a.D <= 64) {
+    if (a.F <= 64) return launch_wgrad_tile<T, SPLIT, DMA, 64, 64, 2, 2>(a, S, chunk, part, stream);
+    return launch_wgrad_tile<T, SPLIT, DMA, 64, 128, 2, 2>(a, S, chunk, part, stream);
+  }
+  if (a.F <= 64) return launch_wgrad_tile<T, SPLIT, DMA, 128, 64, 2, 2>(a, S, chunk, part, stream);
   return launch_wgrad_tile<T, SPLIT, DMA, 128, 128, 2, 2>(a, S, chunk, part, stream);
 }
 

@@ -356,3 +356,12 @@ def test_paths_of_many_rows(T, D, F, E, k, dtype):
     xg = x.cuda().requires_grad_()
     (dx,) = torch.autograd.grad(expert_linear(xg, w.cuda(), plan, gates.cuda()), xg, dy.cuda())
     _check(dict(dx=dx), ref, mag, dict(dx=F), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,M,D,F,E,k", [
+    (11000, 3, 112, 32, 3, 2), (40001, 1, 64, 64, 2, 2), (9000, 1, 64, 64, 5, 1), (5000, 1, 300, 24, 4, 3),
+    (4000, 1, 48, 300, 3, 2), (6000, 2, 16, 16, 5, 4), (3001, 1, 201, 57, 7, 3)])
+def test_narrow_blocks(T, M, D, F, E, k, dtype):
+    """Blocks of up to 64 columns or rows: narrow tiles, and held blocks whose waves share the rows of a stage."""
+    _run_and_check(*_make(T, M, D, F, E, k, dtype, T + D, closed=0.02), dtype)
