@@ -84,20 +84,19 @@ __global__ void __launch_bounds__(256) mm_route_fwd_kernel(MMRoute a, const T* _
                                                            const float* __restrict__ bias, float* __restrict__ gates,
                                                            int* __restrict__ experts) {
   constexpr int RPB = 256 / LPR;   // rows per workgroup
-  __shared__ unsigned s_best[RPB][MM_ROUTE_MAX_G], s_open[RPB][2];
+  constexpr int G = LPR * C < MM_ROUTE_MAX_G ? LPR * C : MM_ROUTE_MAX_G;   // groups, at most
+  __shared__ unsigned s_best[RPB][G], s_open[RPB][2];
   const int lane = threadIdx.x & (LPR - 1), sub = threadIdx.x / LPR, c0 = lane * C;
   const long row = (long)blockIdx.x * RPB + sub;
   const bool ok = row < a.T;
   const long r = ok ? row : a.T - 1;
   const float none = -__builtin_inff();
-  float x[C];
+  float x[C], b[C] = {};
   unsigned key[C];
   mm_route_load<T, C>(logits + r * a.ldl, c0, a.E, none, x);
+  if (bias) mm_route_load<float, C>(bias, c0, a.E, 0.f, b);
 #pragma unroll
-  for (int i = 0; i < C; ++i) {
-    const float b = bias && c0 + i < a.E ? bias[c0 + i] : 0.f;
-    key[i] = x[i] == none ? 0u : mm_route_key(x[i] + b);
-  }
+  for (int i = 0; i < C; ++i) key[i] = x[i] == none ? 0u : mm_route_key(x[i] + b[i]);
   if (a.groups > 1) {
     const int gs = a.E / a.groups, g0 = c0 / gs, rem = c0 - g0 * gs;
     for (int q = lane; q < a.groups; q += LPR) s_best[sub][q] = 0;
@@ -155,34 +154,57 @@ __global__ void __launch_bounds__(256) mm_route_fwd_kernel(MMRoute a, const T* _
     for (int i = 0; i < C; ++i) whole += mm_exp_neg(x[i] - top);   // rows with nothing open have no gate that uses it
     whole = mm_lanes_sum<LPR>(whole);
   }
-  unsigned best = 0;
+  // the rounds; a lane's keys lie in LDS by fours where it has more than four, and in registers only the fours' best:
+  // taking the best one out is then one read, one write and a few maxima, where a pass over C registers was most of a
+  // round (65,536 rows of 256, k = 8 of 4 in 8 groups: 55 us so, 29 us now)
+  constexpr int Q = C / 4;
+  __shared__ uint4 s_key[C > 4 ? RPB : 1][C > 4 ? Q * LPR : 1];
+  __shared__ int s_pick[RPB][KM * LPR];
+  unsigned four[Q], best = 0;
 #pragma unroll
-  for (int i = 0; i < C; ++i) best = max(best, key[i]);
-  int ej[KM];
+  for (int q = 0; q < Q; ++q) {
+    four[q] = max(max(key[4 * q], key[4 * q + 1]), max(key[4 * q + 2], key[4 * q + 3]));
+    best = max(best, four[q]);
+    if constexpr (C > 4)
+      s_key[sub][q * LPR + lane] = make_uint4(key[4 * q], key[4 * q + 1], key[4 * q + 2], key[4 * q + 3]);
+  }
 #pragma unroll
-  for (int q = 0; q < KM; ++q) ej[q] = -1;
+  for (int q = 0; q < KM; ++q) s_pick[sub][q * LPR + lane] = -1;
   const int first_lane = (threadIdx.x & 63) & ~(LPR - 1);
   for (int j = 0; j < a.k; ++j) {
     const unsigned m = mm_route_max<LPR>(best);
     if (__ballot(m != 0) == 0) break;   // no row of the wave has an open expert left
     const unsigned long long have = __ballot(best == m) >> first_lane;
     const int src = __ffsll((unsigned long long)have) - 1;   // the lane of this row with the lowest such index
-    int ib = 0;                                              // every lane's first logit of its best key
+    if (m != 0 && lane == src) {
+      int qi = 0, i = 3;   // its first four with that key, and the first in it
 #pragma unroll
-    for (int i = C - 1; i >= 0; --i) ib = key[i] == best ? i : ib;
-    const int ew = __shfl(c0 + ib, src, LPR);
-#pragma unroll
-    for (int q = 0; q < KM; ++q)
-      if (m != 0 && j == q * LPR + lane) ej[q] = ew;
-    if (lane == src) {
+      for (int q = Q - 1; q >= 0; --q) qi = four[q] == m ? q : qi;
+      uint4 v = make_uint4(key[0], key[1], key[2], key[3]);
+      if constexpr (C > 4) v = s_key[sub][qi * LPR + lane];
+      i = v.z == m ? 2 : i;
+      i = v.y == m ? 1 : i;
+      i = v.x == m ? 0 : i;
+      s_pick[sub][j] = c0 + 4 * qi + i;
+      v = make_uint4(i == 0 ? 0 : v.x, i == 1 ? 0 : v.y, i == 2 ? 0 : v.z, i == 3 ? 0 : v.w);
+      if constexpr (C > 4) {
+        ((unsigned*)&s_key[sub][qi * LPR + lane])[i] = 0;
+      } else {
+        key[0] = v.x, key[1] = v.y, key[2] = v.z, key[3] = v.w;
+      }
+      const unsigned rest = max(max(v.x, v.y), max(v.z, v.w));
       best = 0;
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        key[i] = i == ib ? 0 : key[i];
-        best = max(best, key[i]);
+      for (int q = 0; q < Q; ++q) {
+        four[q] = q == qi ? rest : four[q];
+        best = max(best, four[q]);
       }
     }
   }
+  mm_wave_lds_sync();
+  int ej[KM];
+#pragma unroll
+  for (int q = 0; q < KM; ++q) ej[q] = s_pick[sub][q * LPR + lane];
   float xj[KM];
 #pragma unroll
   for (int q = 0; q < KM; ++q) xj[q] = ej[q] >= 0 ? (float)logits[r * a.ldl + ej[q]] : none;
@@ -230,7 +252,7 @@ __global__ void __launch_bounds__(256) mm_route_bwd_kernel(MMRoute a, const T* _
                                                            const int* __restrict__ experts,
                                                            const float* __restrict__ dgates, T* __restrict__ dlogits) {
   constexpr int RPB = 256 / LPR;
-  __shared__ float s_d[RPB][LPR * C];
+  __shared__ floatx4 s_d[RPB][C / 4 * LPR];   // four q of lane l at q LPR + l: every bank once
   const int lane = threadIdx.x & (LPR - 1), sub = threadIdx.x / LPR, c0 = lane * C;
   const long row = (long)blockIdx.x * RPB + sub;
   const bool ok = row < a.T;
@@ -275,15 +297,23 @@ __global__ void __launch_bounds__(256) mm_route_bwd_kernel(MMRoute a, const T* _
     for (int i = 0; i < C; ++i) v[i] = 0.f;
   }
 #pragma unroll
-  for (int i = 0; i < C; ++i) s_d[sub][c0 + i] = v[i];
+  for (int q = 0; q < C / 4; ++q)
+    s_d[sub][q * LPR + lane] = floatx4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
   mm_wave_lds_sync();
 #pragma unroll
-  for (int q = 0; q < KM; ++q)
-    if (e[q] >= 0) s_d[sub][e[q]] += d[q];   // the chosen of a row are different experts
+  for (int q = 0; q < KM; ++q) {
+    if (e[q] < 0) continue;   // the chosen of a row are different experts
+    float* p = (float*)&s_d[sub][e[q] % C / 4 * LPR + e[q] / C] + e[q] % 4;
+    *p += d[q];
+  }
   mm_wave_lds_sync();
   if (!ok) return;
 #pragma unroll
-  for (int i = 0; i < C; ++i) v[i] = s_d[sub][c0 + i];
+  for (int q = 0; q < C / 4; ++q) {
+    const floatx4 t = s_d[sub][q * LPR + lane];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[4 * q + i] = t[i];
+  }
   T* __restrict__ o = dlogits + row * a.E;
   constexpr int N = C < MMVec<T>::N ? C : MMVec<T>::N;
   typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
