@@ -196,8 +196,17 @@ __global__ void __launch_bounds__(1024) mm_layernorm_sum_kernel(const float* __r
   const int c = blockIdx.x * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
   const float* __restrict__ p = part + (size_t)blockIdx.y * n_part * D;
   float t = 0.f;
-  if (c < D)
-    for (int r = q; r < n_part; r += 64) t += p[(size_t)r * D + c];
+  if (c < D) {
+    int r = q;
+    for (; r + 448 < n_part; r += 512) {   // eight loads on their way
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = p[(size_t)(r + 64 * i) * D + c];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t += v[i];
+    }
+    for (; r < n_part; r += 64) t += p[(size_t)r * D + c];
+  }
   s[q][threadIdx.x & 15] = t;
   __syncthreads();
   if (q || c >= D) return;
@@ -212,29 +221,38 @@ __global__ void __launch_bounds__(1024) mm_layernorm_sum_kernel(const float* __r
 }
 
 namespace {
-// workgroups of the backward: as many as have rows, at most MM_NORM_WG
 long norm_rows_per_wg(int lpr) { return lpr > 256 ? 1 : 256 / lpr; }
 
-// lanes per row and vectors per lane: the least that hold D columns
+// Lanes per row and vectors per lane: the least that hold D columns.  Rows of 1025 .. 2048 16-bit values take a
+// workgroup: 32 values a lane of one wave leave too few waves for the loads (backward, bfloat16, us, a wave / a
+// workgroup: 16,384 x 2048 72 / 54, 60,000 x 2000 224 / 164; forward 32 / 26, 107 / 97).
 struct Shape { int lpr, nv; };
-const Shape kShapes[] = {{4, 1}, {8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2},
-                         {1024, 4}};
+const Shape kShapes[] = {{4, 1}, {8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 1}, {256, 2}, {256, 4},
+                         {1024, 2}, {1024, 4}};
+constexpr int kUnused[] = {7, 6};   // shape that float, that 16-bit types do without
 
 int shape_of(int D, int dtype) {
-  const int n = dtype == MM_F32 ? 4 : 8;
+  const int n = dtype == MM_F32 ? 4 : 8, without = kUnused[dtype != MM_F32];
   int i = 0;
-  while (kShapes[i].lpr * kShapes[i].nv * n < D) ++i;
+  while (kShapes[i].lpr * kShapes[i].nv * n < D || i == without) ++i;
   return i;
 }
 
-int bwd_workgroups(long rows, int lpr) {
-  const long n = (rows + norm_rows_per_wg(lpr) - 1) / norm_rows_per_wg(lpr);
-  return (int)(n < MM_NORM_WG ? n : MM_NORM_WG);
+// Workgroups of the backward: as many as have rows, at most MM_NORM_WG.  Long rows, where the partial sums are a part
+// of the traffic that counts: half of that below 32 rows each (us, 1024 / 512: float 8192 x 4096 92 / 82, 4096 x 8192
+// 106 / 92, but 60,000 x 2000 278 / 307); not for 16-bit rows of up to 4096, whose loads need the waves (8192 x 4096:
+// 58 / 73).
+int bwd_workgroups(long rows, int D, int dtype) {
+  const Shape sh = kShapes[shape_of(D, dtype)];
+  const long rpb = norm_rows_per_wg(sh.lpr), n = (rows + rpb - 1) / rpb;
+  const bool is_long = sh.lpr > 256 || (sh.lpr == 256 && (dtype == MM_F32 || sh.nv == 4));
+  const long most = is_long && rows < 32L * MM_NORM_WG ? MM_NORM_WG / 2 : MM_NORM_WG;
+  return (int)(n < most ? n : most);
 }
 }  // namespace
 
 #define MM_NORM_SHAPES(X) X(0, 4, 1) X(1, 8, 1) X(2, 16, 1) X(3, 32, 1) X(4, 64, 1) X(5, 64, 2) X(6, 64, 4) \
-  X(7, 256, 2) X(8, 256, 4) X(9, 1024, 2) X(10, 1024, 4)
+  X(7, 256, 1) X(8, 256, 2) X(9, 256, 4) X(10, 1024, 2) X(11, 1024, 4)
 
 extern "C" int mm_layernorm_fwd(const void* x, long ldx, int dtype, long rows, int D, const void* w, const void* b,
                                 int p_dtype, float eps, void* y, long ldy, float* mean, float* rstd,
@@ -252,7 +270,7 @@ extern "C" int mm_layernorm_fwd(const void* x, long ldx, int dtype, long rows, i
   const long rpb = norm_rows_per_wg(lpr), n = (rows + rpb - 1) / rpb;
   const dim3 grid((unsigned)(n < 4096 ? n : 4096));
 #define X(i, l, v)                                                                                              \
-  if constexpr (l * v * MMVec<T_>::N <= MM_NORM_MAX_D) if (sh == i)                                              \
+  if constexpr (l * v * MMVec<T_>::N <= MM_NORM_MAX_D && i != kUnused[sizeof(T_) == 2]) if (sh == i) \
     hipLaunchKernelGGL((mm_layernorm_fwd_kernel<T_, l, v>), grid, dim3(l > 256 ? l : 256), 0, stream, (const T_*)x, \
                        ldx, rows, D, w, b, p_dtype == MM_F32, eps, (T_*)y, ldy, mean, rstd);
   MM_DISPATCH(dtype, MM_NORM_SHAPES(X));
@@ -262,7 +280,7 @@ extern "C" int mm_layernorm_fwd(const void* x, long ldx, int dtype, long rows, i
 
 extern "C" int mm_layernorm_workspace(long rows, int D, int dtype, size_t* bytes) {
   MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16 && rows >= 0 && D > 0 && D <= MM_NORM_MAX_D && bytes, "bad sizes");
-  *bytes = (size_t)2 * bwd_workgroups(rows, kShapes[shape_of(D, dtype)].lpr) * D * sizeof(float);
+  *bytes = (size_t)2 * bwd_workgroups(rows, D, dtype) * D * sizeof(float);
   return MM_OK;
 }
 
@@ -277,10 +295,10 @@ extern "C" int mm_layernorm_bwd(const void* dy, long lddy, const void* x, long l
     mm::set_error("mm_layernorm_bwd: rows longer than 16384 are not supported");
     return MM_ERANGE;
   }
-  const int sh = shape_of(D, dtype), n = bwd_workgroups(rows, kShapes[sh].lpr);
+  const int sh = shape_of(D, dtype), n = bwd_workgroups(rows, D, dtype);
   float* part = dw || db ? workspace : nullptr;
 #define X(i, l, v)                                                                                               \
-  if constexpr (l * v * MMVec<T_>::N <= MM_NORM_MAX_D) if (sh == i)                                               \
+  if constexpr (l * v * MMVec<T_>::N <= MM_NORM_MAX_D && i != kUnused[sizeof(T_) == 2]) if (sh == i) \
     hipLaunchKernelGGL((mm_layernorm_bwd_kernel<T_, l, v>), dim3(n), dim3(l > 256 ? l : 256), 0, stream,          \
                        (const T_*)dy, lddy, (const T_*)x, ldx, rows, D, w, p_dtype == MM_F32, mean, rstd, (T_*)dx,  \
                        lddx, part);
