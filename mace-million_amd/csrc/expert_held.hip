@@ -7,7 +7,7 @@
 // once and written to LDS in operand order, one stage ahead of the products and two ahead in registers, so an operand
 // is split once where the tiles of mm_expert_rows split it in every wave, and the block is read once per chunk.  Bound
 // by the products and the rows' traffic.  With gates (one choice a row) the rows are the result itself; list E, the
-// slots without an expert, is then written as zeros.
+// slots without an expert, is then written as zeros.  65,536 rows 128 -> 128, one of 8 experts: 25 us (86 TFLOP/s).
 #define MM_HELD_AS 17       // LDS distance (16 B) of the groups of 8 values of a row tile: every bank once
 
 struct MMHeld {
@@ -173,7 +173,9 @@ __global__ void __launch_bounds__(256, 2) mm_expert_held_kernel(MMHeld h, int ti
 // same 96 registers at K = 128), every operand of a row is read once for both, and the two products of a row are
 // joined and written once.  64 rows a stage, one workgroup a CU.  DG: with the rows of dy and W[e]^T also dgates[t, j]
 // = sum over m of <x[t, m], (dy W[e_j]^T)[t, m]>; all columns are then in one workgroup, and a chunk holds whole rows
-// t.  RG = 2 (64 columns or fewer): 4 waves a half of a stage's rows.
+// t.  RG = 2 (64 columns or fewer): 4 waves a half of a stage's rows (203,760 rows 112 -> 32: 108 us without, 85 so).
+// 98,304 rows 128 -> 128, 2 of 8 experts: 43 us (150 TFLOP/s of 207 that split operands allow); each further 98,304
+// rows add 30 us, the rest is the first loads and the blocks' split.  DG, 49,152 rows: 43 us.
 template <bool TRANS, int KS, bool FULL, bool DG, int RG>
 __global__ void __launch_bounds__(512, 2) mm_expert_held_pairs_kernel(MMPairs a, int tiles_n, int chunk) {
   constexpr int KG = 4 * KS, UNITS = 4 * 3 * KG * MM_HELD_AS, PER = KS;   // float4 a thread and stage: 64 * 8 KS / 512

@@ -5,7 +5,8 @@
 // slots, each in the registers of one workgroup (16 a thread, loaded together).  Up to MM_PLAN_ONE tiles: one launch,
 // whose workgroups count the other tiles' slots as well.  Beyond: the tiles' counts, then the scatter, whose
 // workgroups add up the counts of all tiles themselves as long as that is at most MM_PLAN_SUM loads a thread; else a
-// launch between them takes the prefix sums.
+// launch between them takes the prefix sums.  Bound by latency: 196,608 slots of 8 experts take 4.7 + 5.8 us, 98,304
+// rows by pairs 4.9 + 7.4 us (0.8 MB in, 0.8 MB out: 0.3 us at HBM's rate).
 #define MM_PLAN_TILE 4096
 #define MM_PLAN_ONE 4
 #define MM_PLAN_SUM 128
@@ -88,7 +89,7 @@ __host__ __device__ inline int mm_plan_across(int buckets, int th) {
 // One tile.  Each of the NW waves ranks its share of the slots, 64 consecutive ones at a time: one ballot per bit of
 // the bucket finds the equals, the first of which takes places for all of them from the wave's counters.  Then the
 // counters become places in the order.  Bound by the latency of these rounds, so as many waves as the counters leave
-// room for share them (4 instead of 16: 12.6 us instead of the figure below for 4,000 slots of 89 experts).  MODE 0:
+// room for share them (4 instead of 16: 12.6 us instead of 7.2 for 4,000 slots of 89 experts).  MODE 0:
 // the other tiles are counted here; 1: the counts of all tiles are added up here; 2: counts are prefix sums, with the
 // totals.  BITS: of the largest bucket, or more.
 template <int MODE, int NW, int BITS, bool PAIRS>

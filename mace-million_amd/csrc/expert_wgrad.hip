@@ -13,7 +13,10 @@ struct MMWgrad {
 // A workgroup: a BD x BF tile of dW[e] over a chunk of the expert's rows (SPLIT: chunks of `chunk` rows, each into its
 // own fp32 partial sums, which mm_expert_wgrad_sum_kernel adds in order; else all rows, straight into dW).  x goes
 // into LDS as it is, dy through registers times its gate: in 16-bit types that rounds gate x dy to the type, an error
-// of the size that dy's own rounding has.  Rows past the end are zeros on both sides.
+// of the size that dy's own rounding has.  Rows past the end are zeros on both sides.  Bound by the waits between
+// stages and, for float, by the vector instructions of the split: 65,536 bfloat16 rows, 64 blocks of 1024 x 1024 275
+// us (500 TFLOP/s); 98,304 float rows, 16 blocks of 128 x 128 41 + 7 us.  Tiles of 64 where a side has no more
+// (407,520 float rows 112 x 32: 140 -> 97 us).
 #define MM_WG_ROWS 512   // rows whose offsets are kept in LDS at a time
 
 template <typename T, bool SPLIT, bool DMA, int BD, int BF, int WD, int WF>
@@ -149,23 +152,45 @@ __global__ void __launch_bounds__(64 * WD * WF, 2) mm_expert_wgrad_kernel(MMWgra
   }
 }
 
-// dW[e] = the partial sums of the expert's chunks, in order
-template <typename T>
+// dW[e] = the partial sums of the expert's chunks, in a fixed order.  V values a thread: 4 where that leaves threads
+// for the card, from 2^19 values on (89 x 201 x 137: 11.6 -> 6.6 us; 16 x 128 x 128 would take 19 instead of 8).  G
+// waves share the chunks: 4 where the values alone are too few, below 2^18 (2 x 216 x 72: 8 -> 5 us; 16 x 128 x 128: 8
+// -> 9.7).
+template <typename T, int V, int G>
 __global__ void __launch_bounds__(256) mm_expert_wgrad_sum_kernel(MMWgrad a, int chunk,
                                                                   const float* __restrict__ part) {
-  const int lane = threadIdx.x & 63, e = blockIdx.y;
+  constexpr int COLUMNS = 256 / G * V;
+  __shared__ float s_t[G][G > 1 ? 64 : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.y;
   int first = 0;   // chunks of the experts before e
   for (int o = lane; o < e; o += 64) first += ((a.offsets[o + 1] - a.offsets[o]) * a.M + chunk - 1) / chunk;
 #pragma unroll
   for (int d = 32; d; d >>= 1) first += __shfl_xor(first, d);
   const int n = ((a.offsets[e + 1] - a.offsets[e]) * a.M + chunk - 1) / chunk;
-  const long size = (long)a.D * a.F, i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= size) return;
+  const long size = (long)a.D * a.F, i = (long)blockIdx.x * COLUMNS + (G > 1 ? lane : V * (int)threadIdx.x);
+  const int left = (int)(size - i < V ? size - i : V);
   const float* __restrict__ p = part + (size_t)first * size + i;
-  float t = 0.f;
+  float t[V] = {};
+  if (left > 0) {
 #pragma unroll 8
-  for (int c = 0; c < n; ++c) t += p[c * size];
-  ((T*)a.dW)[(size_t)e * size + i] = (T)t;
+    for (int c = G > 1 ? wave : 0; c < n; c += G) {
+      float v[V];
+      if constexpr (V == 1) v[0] = p[c * size];
+      else mm_load4(p + c * size, 0, left, v);
+#pragma unroll
+      for (int q = 0; q < V; ++q) t[q] += v[q];
+    }
+  }
+  if constexpr (G > 1) {
+    s_t[wave][lane] = t[0];
+    __syncthreads();
+    if (wave) return;
+    t[0] = s_t[0][lane] + s_t[1][lane] + s_t[2][lane] + s_t[3][lane];
+  }
+  if (left <= 0) return;
+  T* __restrict__ o = (T*)a.dW + (size_t)e * size + i;
+  if constexpr (V == 1) *o = (T)t[0];
+  else mm_store4(o, 0, left, t);
 }
 
 // ------------------------------------------------------------------------------------------------ entry points
@@ -243,9 +268,16 @@ extern "C" int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, 
   else { if (dma) { CALL(false, true) } else { CALL(false, false) } }
 #undef CALL
   if (rc != MM_OK) return rc;
-  if (chunk)
-    MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_wgrad_sum_kernel<T_>),
-                                          dim3((unsigned)(((long)D * F + 255) / 256), E), dim3(256), 0, stream, a,
-                                          chunk, workspace));
+  const long size = (long)D * F;
+#define SUM(v, g)                                                                                               \
+  MM_DISPATCH(dtype, hipLaunchKernelGGL((mm_expert_wgrad_sum_kernel<T_, v, g>),                                 \
+                                        dim3((unsigned)((size + 256 / g * v - 1) / (256 / g * v)), E), dim3(256), 0, \
+                                        stream, a, chunk, workspace))
+  if (chunk) {
+    if (E * size < 1 << 18) SUM(1, 4);
+    else if (E * size < 1 << 19) SUM(1, 1);
+    else SUM(4, 1);
+  }
+#undef SUM
   return mm::launch_status("mm_expert_wgrad");
 }

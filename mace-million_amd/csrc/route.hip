@@ -9,10 +9,11 @@
 // exponential, and saturated sigmoids do not tie.  Renormalised gates are a softmax over the chosen of the scores'
 // logarithms (of the logits, or of log sigmoid), so that scores that all underflow still give gates of sum scale.  A
 // NaN logit is chosen first and makes the gates NaN.
-// A row lies in LPR lanes, C consecutive logits each; k rounds of a
-// maximum over the lanes' best keys (as integers of the same order), the lowest lane with it giving its first such
-// logit: no sort, no memory but the logits and the results. Bound by the rounds' vector instructions for large k, by
-// HBM for small k.
+// A row lies in LPR lanes, C consecutive logits each; k rounds of a maximum over the lanes' best keys (as integers of
+// the same order), the lowest lane with it giving its first such logit: no sort, no memory but the logits and the
+// results.  Bound by the rounds' vector instructions for large k, by HBM for small k.  Measured, forward and backward:
+// 500,000 float rows of 16, k = 2: 17.6 and 10.2 us (40 and 44 MB); 65,536 bfloat16 rows of 256, k = 8 of 4 in 8
+// groups: 29 and 13 us (38 MB each); 98,304 float16 rows of 89, k = 3, plain softmax: 18 us; one row: 2.7 us.
 #include "rowvec.h"
 
 #define MM_ROUTE_MAX_E 1024
