@@ -343,7 +343,12 @@ bool few_rows(const Sizes& n, int code) {
   return bytes <= 64e6 && n.T <= 65535 && n.M <= 65535;
 }
 
-Tensor inner(const Tensor& t) { return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; }
+// t [T, D] or [T, M, D] as [T, M, D] with a contiguous last axis.  Taken inside the autograd function, where a view costs
+// no node of its own (two views outside took 6 - 10 us of a training call).
+Tensor inner(const Tensor& t0) {
+  const Tensor t = t0.dim() == 2 ? t0.unsqueeze(1) : t0;
+  return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t;
+}
 
 // Whether the choices of a row are joined before they are written (mm_expert_joined) instead of through fp32 rows of
 // the slots; K values a row go in, N come out.  One choice: always (65,536 rows, 8 experts, us, joined / slots: 128 ->
@@ -382,14 +387,14 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
   }
 
   static Sizes sizes(const Tensor& x, const Tensor& w, const Tensor& experts) {
-    return Sizes{x.size(0), x.size(1), x.size(2), w.size(2), w.size(0), experts.size(1)};
+    return Sizes{x.size(0), x.dim() == 2 ? 1 : x.size(1), x.size(-1), w.size(2), w.size(0), experts.size(1)};
   }
 
   static Tensor run(const Tensor& x0, const Tensor& w, const Tensor& gates, Plan& plan, int code) {
     const Tensor& experts = plan.experts;
     const Sizes n = sizes(x0, w, experts);
     const Tensor x = inner(x0);
-    Tensor y = at::empty({n.T, n.M, n.F}, x.options());
+    Tensor y = x0.dim() == 2 ? at::empty({n.T, n.F}, x.options()) : at::empty({n.T, n.M, n.F}, x.options());
     const int T = (int)n.T, k = (int)n.k, M = (int)n.M, D = (int)n.D, F = (int)n.F, E = (int)n.E;
     if (few_rows(n, code)) {
       done(mm_expert_few(ptr(x), x.stride(0), x.stride(1), code, T, k, M, D, F, ptr(w), E, fptr(gates),
@@ -419,7 +424,7 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
     const Sizes n = sizes(x, w, experts);
     const int S = (int)(n.T * n.k), k = (int)n.k, M = (int)n.M, D = (int)n.D, F = (int)n.F, E = (int)n.E;
     Tensor dx, dw, dg;
-    if (ctx->needs_input_grad(0)) dx = at::empty({n.T, n.M, n.D}, x.options());
+    if (ctx->needs_input_grad(0)) dx = at::empty(saved[0].sizes(), x.options());
     if (ctx->needs_input_grad(1)) dw = at::empty({n.E, n.D, n.F}, x.options());
     if (gates.defined() && ctx->needs_input_grad(2)) dg = f32({n.T, n.k}, x);
     // (joined or not was settled by whether the gates needed a gradient; if it is dropped here, that choice still
@@ -478,14 +483,10 @@ Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates,
   }
   const Tensor& experts = plan->experts;
   if (experts.device() != x0.device()) throw py::value_error("x and the plan must be on one device");
-  const bool flat = x0.dim() == 2;
-  const Tensor x = flat ? x0.unsqueeze(1) : x0;
-  if (T * k * x.size(1) > kInt32Max - 128)
-    throw py::value_error(text(T * k * x.size(1), " rows: 2^31 or more are not supported"));
-  const Tensor y = needs_grad({&x, &weight, &g})
-                       ? ExpertLinearFn::apply(x, weight, maybe(g), plan, (int64_t)code)
-                       : ExpertLinearFn::run(x, weight.contiguous(), g.defined() ? g.contiguous() : g, *plan, code);
-  return flat ? y.squeeze(1) : y;
+  const long slots = T * k * (x0.dim() == 2 ? 1 : x0.size(1));
+  if (slots > kInt32Max - 128) throw py::value_error(text(slots, " rows: 2^31 or more are not supported"));
+  if (needs_grad({&x0, &weight, &g})) return ExpertLinearFn::apply(x0, weight, maybe(g), plan, (int64_t)code);
+  return ExpertLinearFn::run(x0, weight.contiguous(), g.defined() ? g.contiguous() : g, *plan, code);
 }
 }  // namespace
 
