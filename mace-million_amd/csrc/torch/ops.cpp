@@ -343,8 +343,8 @@ bool few_rows(const Sizes& n, int code) {
   return bytes <= 64e6 && n.T <= 65535 && n.M <= 65535;
 }
 
-// t [T, D] or [T, M, D] as [T, M, D] with a contiguous last axis.  Taken inside the autograd function, where a view costs
-// no node of its own (two views outside took 6 - 10 us of a training call).
+// t [T, D] or [T, M, D] as [T, M, D] with a contiguous last axis.  Taken inside the autograd function, where a view
+// costs no node of its own (two views outside took 6 - 10 us of a training call).
 Tensor inner(const Tensor& t0) {
   const Tensor t = t0.dim() == 2 ? t0.unsqueeze(1) : t0;
   return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t;
