@@ -11,23 +11,25 @@ struct MMWgrad {
 };
 
 // A workgroup: a BD x BF tile of dW[e] over a chunk of the expert's rows (SPLIT: chunks of `chunk` rows, each into its
-// own fp32 partial sums, which mm_expert_wgrad_sum_kernel adds in order; else all rows, straight into dW).  x goes
-// into LDS as it is, dy through registers times its gate: in 16-bit types that rounds gate x dy to the type, an error
-// of the size that dy's own rounding has.  Rows past the end are zeros on both sides.  Bound by the waits between
-// stages and, for float, by the vector instructions of the split: 65,536 bfloat16 rows, 64 blocks of 1024 x 1024 275
-// us (500 TFLOP/s); 98,304 float rows, 16 blocks of 128 x 128 41 + 7 us.  Tiles of 64 where a side has no more
-// (407,520 float rows 112 x 32: 140 -> 97 us).
+// own fp32 partial sums, which mm_expert_wgrad_sum_kernel adds in order; else all rows, straight into dW).  x and dy go
+// into LDS as they are, float dy times its gate.  16-bit types with gates (GATED): gate x dy, taken in fp32, would lose
+// bits and, in float16, its range if it were rounded to the type, so it enters the products as two bf16 parts
+// (mm_products_gated).  Rows past the end are zeros on both sides.  Bound by the waits between stages and the vector
+// instructions of the split: 65,536 rows, 64 blocks of 1024 x 1024, 2 of 64: bfloat16 380 us, float16 535 us (without
+// gates 250 us, 550 TFLOP/s: one product instead of two or three); 98,304 float rows, 16 blocks of 128 x 128 41 + 7 us.
+// Tiles of 64 where a side has no more (407,520 float rows 112 x 32: 140 -> 97 us).
 #define MM_WG_ROWS 512   // rows whose offsets are kept in LDS at a time
 
-template <typename T, bool SPLIT, bool DMA, int BD, int BF, int WD, int WF>
+template <typename T, bool SPLIT, bool DMA, bool GATED, int BD, int BF, int WD, int WF>
 __global__ void __launch_bounds__(64 * WD * WF, 2) mm_expert_wgrad_kernel(MMWgrad a, int chunk, int tiles_f,
                                                                           int tiles_df, float* __restrict__ part) {
   constexpr int TH = 64 * WD * WF, BK = MM_TILE_K<T>, N = MMVec<T>::N, UD = BD / N, UF = BF / N, KS = BK / 32;
   constexpr int NX = BD * 8 / TH, NY = BF * 8 / TH, FD = BD / WD / 16, FF = BF / WF / 16;
+  constexpr bool YDMA = BD == 256;   // the 256 x 256 tiles have no registers for dy on its way
   extern __shared__ uint4 mm_lds[];
   uint4 *Xs = mm_lds, *Ys = Xs + 2 * BD * 8;             // [2][BD * 8], [2][BF * 8]
   long *s_x = (long*)(Ys + 2 * BF * 8), *s_y = s_x + MM_WG_ROWS;
-  float* s_g = (float*)(s_y + MM_WG_ROWS);
+  float *s_g = (float*)(s_y + MM_WG_ROWS), *s_gate = s_g + MM_WG_ROWS;   // s_gate [2][BK]: of the stages (GATED)
   const int lane_id = threadIdx.x & 63;
   int df, tile;
   MMTile t;
@@ -75,7 +77,7 @@ __global__ void __launch_bounds__(64 * WD * WF, 2) mm_expert_wgrad_kernel(MMWgra
     left_f[j] = a.F - f0 - cy[j];
   }
   MMStage<T, TH, NX, DMA> sx;
-  MMStage<T, TH, NY, false> sy;
+  MMStage<T, TH, NY, YDMA> sy;
   float gy[NY];
   auto load = [&](int r0, int buf) {   // rows r0 .. r0 + BK of the chunk, within one block of offsets
 #pragma unroll
@@ -91,15 +93,16 @@ __global__ void __launch_bounds__(64 * WD * WF, 2) mm_expert_wgrad_kernel(MMWgra
       sy.load(Ys + buf * BF * 8, j, (const T*)a.dy + (in ? s_y[r] : 0) + f0 + cy[j], in ? left_f[j] : 0);
       gy[j] = in ? s_g[r] : 0.f;
     }
+    if (GATED && tid < BK) s_gate[buf * BK + tid] = r0 + tid < t.rows ? s_g[(r0 + tid) & (MM_WG_ROWS - 1)] : 0.f;
   };
   auto put = [&](int buf) {
     sx.put(Xs + buf * BD * 8);
-    if (a.gates) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int j = 0; j < NY; ++j) {
-        typename MMVec<T>::type v = __builtin_bit_cast(typename MMVec<T>::type, sy.v[j]);
+        floatx4 v = __builtin_bit_cast(floatx4, sy.v[j]);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = (T)(gy[j] * (float)v[i]);
+        for (int i = 0; i < N; ++i) v[i] = gy[j] * v[i];
         sy.v[j] = __builtin_bit_cast(uint4, v);
       }
     }
@@ -131,9 +134,10 @@ __global__ void __launch_bounds__(64 * WD * WF, 2) mm_expert_wgrad_kernel(MMWgra
       if (next % MM_WG_ROWS == 0) rows_of(next);   // the previous block's offsets are used up (the last barrier)
       load(next, buf ^ 1);
     }
-    mm_products<T, FF, FD, KS>(
-        acc, [&](int s, int i) { return mm_read_nc<T, UF>(Ys + buf * BF * 8, wf + 16 * i, s, lane); },
-        [&](int s, int j) { return mm_read_nc<T, UD>(Xs + buf * BD * 8, wd + 16 * j, s, lane); });
+    auto y_of = [&](int s, int i) { return mm_read_nc<T, UF>(Ys + buf * BF * 8, wf + 16 * i, s, lane); };
+    auto x_of = [&](int s, int j) { return mm_read_nc<T, UD>(Xs + buf * BD * 8, wd + 16 * j, s, lane); };
+    if constexpr (GATED) mm_products_gated<T, FF, FD, KS>(acc, y_of, x_of, s_gate + buf * BK, lane);
+    else mm_products<T, FF, FD, KS>(acc, y_of, x_of);
     if (more) put(buf ^ 1);
     mm_stage_done();
     buf ^= 1;
@@ -195,33 +199,40 @@ __global__ void __launch_bounds__(256) mm_expert_wgrad_sum_kernel(MMWgrad a, int
 
 // ------------------------------------------------------------------------------------------------ entry points
 namespace {
-// two stages of both operands, then the offsets and gates of a block of rows
-template <int BD, int BF>
-constexpr int wgrad_lds() { return 2 * (BD + BF) * 128 + MM_WG_ROWS * 20; }
+// two stages of both operands, then the offsets and gates of a block of rows, then the gates of two stages
+template <int BD, int BF, int BK>
+constexpr int wgrad_lds() { return 2 * (BD + BF) * 128 + MM_WG_ROWS * 20 + 2 * BK * 4; }
 
-template <typename T, bool SPLIT, bool DMA, int BD, int BF, int WD, int WF>
+template <typename T, bool SPLIT, bool DMA, bool GATED, int BD, int BF, int WD, int WF>
 int launch_wgrad_tile(const MMWgrad& a, int S, int chunk, float* part, hipStream_t stream) {
   const int tiles_f = (a.F + BF - 1) / BF, tiles_df = (a.D + BD - 1) / BD * tiles_f;
   const long wg = (SPLIT ? (long)S * a.M / chunk + (a.E < S ? a.E : S) : (a.E + 7L) / 8 * 8) * tiles_df;
   if (too_many(wg, 64 * WD * WF)) return range_error("mm_expert_wgrad", "output too large for one launch");
-  constexpr auto kernel = mm_expert_wgrad_kernel<T, SPLIT, DMA, BD, BF, WD, WF>;
-  constexpr int lds = wgrad_lds<BD, BF>();
+  constexpr auto kernel = mm_expert_wgrad_kernel<T, SPLIT, DMA, GATED, BD, BF, WD, WF>;
+  constexpr int lds = wgrad_lds<BD, BF, MM_TILE_K<T>>();
   if (!lds_granted<kernel>(lds)) return MM_ELAUNCH;
   if (wg)
     hipLaunchKernelGGL(kernel, dim3((unsigned)wg), dim3(64 * WD * WF), lds, stream, a, chunk, tiles_f, tiles_df, part);
   return mm::launch_status("mm_expert_wgrad");
 }
 
+template <typename T, bool SPLIT, bool DMA, bool GATED>
+int launch_wgrad_tiles(const MMWgrad& a, int S, int chunk, bool big, float* part, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2 && DMA && !SPLIT)
+    if (big) return launch_wgrad_tile<T, SPLIT, DMA, GATED, 256, 256, 2, 4>(a, S, chunk, part, stream);
+  if (a.D <= 64) {
+    if (a.F <= 64) return launch_wgrad_tile<T, SPLIT, DMA, GATED, 64, 64, 2, 2>(a, S, chunk, part, stream);
+    return launch_wgrad_tile<T, SPLIT, DMA, GATED, 64, 128, 2, 2>(a, S, chunk, part, stream);
+  }
+  if (a.F <= 64) return launch_wgrad_tile<T, SPLIT, DMA, GATED, 128, 64, 2, 2>(a, S, chunk, part, stream);
+  return launch_wgrad_tile<T, SPLIT, DMA, GATED, 128, 128, 2, 2>(a, S, chunk, part, stream);
+}
+
 template <typename T, bool SPLIT, bool DMA>
 int launch_wgrad(const MMWgrad& a, int S, int chunk, bool big, float* part, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2 && DMA && !SPLIT)
-    if (big) return launch_wgrad_tile<T, SPLIT, DMA, 256, 256, 2, 4>(a, S, chunk, part, stream);
-  if (a.D <= 64) {
-    if (a.F <= 64) return launch_wgrad_tile<T, SPLIT, DMA, 64, 64, 2, 2>(a, S, chunk, part, stream);
-    return launch_wgrad_tile<T, SPLIT, DMA, 64, 128, 2, 2>(a, S, chunk, part, stream);
-  }
-  if (a.F <= 64) return launch_wgrad_tile<T, SPLIT, DMA, 128, 64, 2, 2>(a, S, chunk, part, stream);
-  return launch_wgrad_tile<T, SPLIT, DMA, 128, 128, 2, 2>(a, S, chunk, part, stream);
+  if constexpr (sizeof(T) == 2)
+    if (a.gates) return launch_wgrad_tiles<T, SPLIT, DMA, true>(a, S, chunk, big, part, stream);
+  return launch_wgrad_tiles<T, SPLIT, DMA, false>(a, S, chunk, big, part, stream);
 }
 
 // Rows per chunk of dW's sums; 0: no chunks.  A card of 256 CUs takes 512 workgroups at a time: with at least that
@@ -263,7 +274,8 @@ extern "C" int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, 
   if (dtype == MM_F32) rc = launch_wgrad<float, split, dma>(a, S, chunk, false, workspace, stream);   \
   else if (dtype == MM_BF16) rc = launch_wgrad<__bf16, split, dma>(a, S, chunk, big, workspace, stream); \
   else rc = launch_wgrad<_Float16, split, dma>(a, S, chunk, big, workspace, stream);
-  const bool big = dma && !chunk && D > 128 && F > 128 && E * ((D + 255) / 256) * ((F + 255) / 256) >= 512;
+  const bool dma_y = aligned(dy) && yt % unit == 0 && (M == 1 || ym % unit == 0) && F % unit == 0;
+  const bool big = dma && dma_y && !chunk && D > 128 && F > 128 && E * ((D + 255) / 256) * ((F + 255) / 256) >= 512;
   if (chunk) { if (dma) { CALL(true, true) } else { CALL(true, false) } }
   else { if (dma) { CALL(false, true) } else { CALL(false, false) } }
 #undef CALL

@@ -172,6 +172,80 @@ __device__ __forceinline__ void mm_products(floatx4 (&acc)[FN][FM], A a, B b, co
   }
 }
 
+// Two bf16 parts of 8 values, scale x v in fp32: off by 2^-18 of each (float16 values without a scale: exact).
+struct MMParts {
+  bf16x8 v[2];
+};
+
+template <typename T, bool SCALED>
+__device__ __forceinline__ MMParts mm_parts(const MMRaw<T>& r, const float* scale) {
+  MMParts p;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = SCALED ? scale[i] * (float)r.f.v[i] : (float)r.f.v[i];
+    const __bf16 h = (__bf16)x;
+    p.v[0][i] = h;
+    p.v[1][i] = (__bf16)(x - (float)h);
+  }
+  return p;
+}
+
+// acc[i][j] += sum over the values q of a stage of gate[q] a(s, i)[q] b(s, j)[q] for 16-bit types, as mm_products does
+// without gates.  gate x a is taken in fp32 and enters as two bf16 parts: rounded to the type it would lose the bits
+// below its own and, in float16, whatever is below 2^-25 or above 65504.  bfloat16 b: two products; float16 b: two
+// parts as well and three products, the fourth being 2^-18 of the first.
+template <typename T, int FN, int FM, int KS, typename A, typename B>
+__device__ __forceinline__ void mm_products_gated(floatx4 (&acc)[FN][FM], A a, B b, const float* gates, int lane) {
+  constexpr bool HALF = __is_same(T, _Float16);
+  constexpr int Q = KS * FM;
+  auto gates_of = [&](int s, float (&g)[8]) {   // of the values that this lane holds of step s
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const floatx4 v = *(const floatx4*)(gates + 32 * s + 8 * (lane >> 4) + 4 * h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[4 * h + i] = v[i];
+    }
+  };
+  MMParts fa[FN], fb[2];
+  MMRaw<T> ra[FN], rb[3];
+  float g[8];
+  auto second = [&](const MMRaw<T>& r, MMParts& p) {
+    if constexpr (HALF) p = mm_parts<T, false>(r, nullptr);
+    else p.v[0] = r.f.v;
+  };
+  gates_of(0, g);
+#pragma unroll
+  for (int i = 0; i < FN; ++i) ra[i] = a(0, i);
+  rb[0] = b(0, 0);
+  rb[1] = b(1 / FM, 1 % FM);
+#pragma unroll
+  for (int i = 0; i < FN; ++i) fa[i] = mm_parts<T, true>(ra[i], g);
+  second(rb[0], fb[0]);
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    const int s = q / FM, j = q % FM;
+    if (q + 2 < Q) rb[(q + 2) % 3] = b((q + 2) / FM, (q + 2) % FM);
+    if (s + 1 < KS) {   // the next step's operands, over the last products of this one
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+        if ((FN < FM ? i + FM - FN : i * FM / FN) == j) ra[i] = a(s + 1, i);
+      if (j == FM - 1) gates_of(s + 1, g);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (q + 1 < Q) second(rb[(q + 1) % 3], fb[(q + 1) & 1]);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      floatx4& c = acc[i][j];
+      const MMParts& x = fb[q & 1];
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i].v[1], x.v[0], c, 0, 0, 0);
+      if constexpr (HALF) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i].v[0], x.v[1], c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i].v[0], x.v[0], c, 0, 0, 0);
+      if (s + 1 < KS && j == FM - 1) fa[i] = mm_parts<T, true>(ra[i], g);   // beside the products of the others
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // Tiles in LDS, in units of 16 bytes.  MM_TILE_K<T> values of the summed index a stage.
 // KC (the summed index contiguous in memory): a row of 8 units (128 bytes), unit u of row r at 8 r + (u ^ (r & 7)), so
 // that the 16 rows of an operand read spread over all banks.
