@@ -462,6 +462,7 @@ extern "C" int mm_expert_rows(const void* in, long st, long sm, int dtype, int S
   MM_CHECK_ARG(S >= 0 && k >= 1 && M >= 1 && K >= 1 && N >= 1 && E >= 1 && st >= 0 && sm >= 0, "bad sizes");
   if ((long)S * M > 2147483647L - 128) return range_error("mm_expert_rows", "2^31 rows or more are not supported");
   if (S == 0) return MM_OK;
+  MM_CHECK_ARG(in && W && offsets && order && out, "a pointer is null");
   const MMRows a{in, W, offsets, order, out, st, sm, k, M, K, N, E};
   if (dtype == MM_F32 && K <= 128) return mm::launch_held("mm_expert_rows", a, S, nullptr, E, transposed, stream);
   const int unit = dtype == MM_F32 ? 4 : 8;
@@ -487,6 +488,7 @@ extern "C" int mm_expert_few(const void* x, long st, long sm, int dtype, int T, 
   if (T > 65535 || M > 65535)
     return range_error("mm_expert_few", "more than 65535 rows or components are not supported");
   if (T == 0) return MM_OK;
+  MM_CHECK_ARG(x && W && experts && y, "a pointer is null");
   const MMFew a{x, W, gates, experts, st, sm, k, M, D, F, E};
 #define CALL(T_)                                                                                             \
   hipLaunchKernelGGL((mm_expert_few_kernel<T_, 4>), dim3((F + 4 * MMVec<T_>::N - 1) / (4 * MMVec<T_>::N), T, M), \
@@ -515,6 +517,7 @@ extern "C" int mm_expert_joined(const void* in, long st, long sm, int dtype, int
     return range_error("mm_expert_joined", "pairs of more than 21 experts are not supported");
   if ((long)T * M > 2147483647L - 128) return range_error("mm_expert_joined", "2^31 rows or more are not supported");
   if (T == 0) return MM_OK;
+  MM_CHECK_ARG(in && W && experts && offsets && order, "a pointer is null");
   if (dtype == MM_F32 && K <= 128 && k == 1 && !dgates && out) {
     const MMRows r{in, W, offsets, order, (float*)out, st, sm, 1, M, K, N, E};
     return mm::launch_held("mm_expert_joined", r, T, gates, E + 1, transposed, stream);
@@ -555,6 +558,7 @@ extern "C" int mm_expert_combine(const float* rows, const float* gates, const in
   const long wg = (T * M * ((N + 3) / 4) + 255) / 256;
   if (too_many(wg, 256)) return range_error("mm_expert_combine", "output too large for one launch");
   if (wg == 0) return MM_OK;
+  MM_CHECK_ARG(rows && experts && y, "a pointer is null");
   const MMCombine a{rows, gates, experts, T, k, M, N, E};
 #define CALL hipLaunchKernelGGL((mm_expert_combine_kernel<T_>), dim3((unsigned)wg), dim3(256), 0, stream, a, (T_*)y)
   if (dtype == MM_F32) { using T_ = float; CALL; }
@@ -572,6 +576,7 @@ extern "C" int mm_expert_combine_bwd(const float* rows, const float* gates, cons
   const long wg = (T + 3) / 4;
   if (too_many(wg, 256)) return range_error("mm_expert_combine_bwd", "too many rows for one launch");
   if (wg == 0) return MM_OK;
+  MM_CHECK_ARG(rows && experts && (x || !dgates), "a pointer is null");
   const MMCombine a{rows, gates, experts, T, k, M, N, E};
 #define CALL2(KB)                                                                                            \
   hipLaunchKernelGGL((mm_expert_combine_bwd_kernel<T_, KB>), dim3((unsigned)wg), dim3(256), 0, stream, a, \

@@ -264,6 +264,7 @@ extern "C" int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, 
   MM_CHECK_ARG(xt >= 0 && xm >= 0 && yt >= 0 && ym >= 0, "bad strides");
   if (E > MM_EXPERT_MAX_E) return range_error("mm_expert_wgrad", "more than 1024 experts are not supported");
   if ((long)S * M > 2147483647L - 128) return range_error("mm_expert_wgrad", "2^31 rows or more are not supported");
+  MM_CHECK_ARG(offsets && dW && (S == 0 || (x && dy && order)), "a pointer is null");
   const MMWgrad a{x, dy, gates, offsets, order, dW, xt, xm, yt, ym, k, M, D, F, E};
   const int chunk = wgrad_chunk((long)S * M, D, F, E);
   MM_CHECK_ARG(!chunk || workspace, "workspace is null");

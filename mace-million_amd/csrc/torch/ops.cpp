@@ -376,13 +376,16 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
                         const std::shared_ptr<Plan>& plan, int64_t code) {
     const Tensor w = weight.contiguous(), g = gates ? gates->contiguous() : Tensor();
     const Sizes n = sizes(x, w, plan->experts);
-    const bool dg = g.defined() && g.requires_grad(), dxg = x.requires_grad() || dg;
+    // Asked of the caller's tensors: copies made in here have no gradient.  The backward takes its path from what is
+    // saved, as it has only these lists.
+    const bool dg = gates && gates->requires_grad(), dxg = x.requires_grad() || dg;
     const bool joined = join_gradients(n, (int)code, dg);
     Lists l, p;   // the backward's
     if (weight.requires_grad() || (dxg && !(joined && n.k == 2))) l = plan->lists();
     if (dxg && joined && n.k == 2) p = plan->pairs();
     ctx->save_for_backward({x, w, g, plan->experts, l.offsets, l.order, p.offsets, p.order});
     ctx->saved_data["code"] = code;
+    ctx->saved_data["joined"] = joined;
     return run(x, w, g, *plan, (int)code);
   }
 
@@ -427,9 +430,7 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
     if (ctx->needs_input_grad(0)) dx = at::empty(saved[0].sizes(), x.options());
     if (ctx->needs_input_grad(1)) dw = at::empty({n.E, n.D, n.F}, x.options());
     if (gates.defined() && ctx->needs_input_grad(2)) dg = f32({n.T, n.k}, x);
-    // (joined or not was settled by whether the gates needed a gradient; if it is dropped here, that choice still
-    // holds)
-    if ((dx.defined() || dg.defined()) && join_gradients(n, code, gates.defined() && gates.requires_grad())) {
+    if ((dx.defined() || dg.defined()) && ctx->saved_data["joined"].toBool()) {
       const bool pairs = k == 2;
       done(mm_expert_joined(ptr(dy), dy.stride(0), dy.stride(1), code, (int)n.T, k, M, F, D, ptr(w), 1, E, fptr(gates),
                             iptr(experts), iptr(pairs ? pair_offsets : offsets), iptr(pairs ? pair_order : order),
