@@ -100,6 +100,25 @@ std::pair<Tensor, long> as_rows(Tensor t) {
   return {t, t.size(0) > 1 ? t.stride(0) : D};
 }
 
+// A saved tensor as its node gets it back.  Hooks on saved tensors (offloading, compression) may return it with any
+// strides, so its layout is taken from what comes back; sizes and type have to be those that were saved.
+const Tensor& unpacked(const Tensor& t, at::IntArrayRef size, at::ScalarType type, const Tensor& like,
+                       const char* name) {
+  if (t.defined() && (t.sizes() != size || t.scalar_type() != type || t.device() != like.device()))
+    throw std::runtime_error(text(name, " was saved for the backward as ", type_name(type), " ", size, " on ",
+                                  like.device(), " and came back as ", type_name(t.scalar_type()), " ", t.sizes(),
+                                  " on ", t.device()));
+  return t;
+}
+
+Tensor unpacked_dense(const Tensor& t, at::IntArrayRef size, at::ScalarType type, const Tensor& like,
+                      const char* name) {
+  unpacked(t, size, type, like, name);
+  return t.defined() ? t.contiguous() : t;
+}
+
+at::ScalarType type_of(int64_t code) { return code == 0 ? at::kFloat : code == 1 ? at::kBFloat16 : at::kHalf; }
+
 // ------------------------------------------------------------------------------------------------ layer norm
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& w, const Maybe& b, double eps, int64_t code,
@@ -111,7 +130,6 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     ctx->save_for_backward({x2, weight, stats});
     ctx->saved_data["bias"] = bias.defined();
     ctx->saved_data["codes"] = code * 4 + p_code;
-    ctx->saved_data["ldx"] = (int64_t)ldx;
     ctx->saved_data["shape"] = x.sizes().vec();
     return y;
   }
@@ -130,16 +148,18 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
     const int64_t codes = ctx->saved_data["codes"].toInt();
     const int code = (int)(codes / 4), p_code = (int)(codes % 4);
-    const long rows = x.size(0), D = x.size(1), ldx = ctx->saved_data["ldx"].toInt();
     auto [dy, lddy] = as_rows(grads[0]);
+    const long rows = dy.size(0), D = dy.size(1);
+    const auto p_type = type_of(p_code);
+    auto [x, ldx] = as_rows(unpacked(saved[0], {rows, D}, type_of(code), dy, "x"));
+    const Tensor w = unpacked_dense(saved[1], {D}, p_type, dy, "weight");
+    const Tensor stats = unpacked_dense(saved[2], {2, rows}, at::kFloat, dy, "statistics");
     Tensor dx, dw, db, ws;
     if (ctx->needs_input_grad(0)) dx = at::empty(ctx->saved_data["shape"].toIntVector(), x.options());
-    const auto p_type = p_code == 0 ? at::kFloat : x.scalar_type();
-    const int at_bias = weight.defined() ? 2 : 1;   // autograd counts the tensors that are there
-    if (weight.defined() && ctx->needs_input_grad(1)) dw = at::empty({D}, x.options().dtype(p_type));
+    const int at_bias = w.defined() ? 2 : 1;   // autograd counts the tensors that are there
+    if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty({D}, x.options().dtype(p_type));
     if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(at_bias))
       db = at::empty({D}, x.options().dtype(p_type));
     if (dw.defined() || db.defined()) {
@@ -147,7 +167,6 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
       done(mm_layernorm_workspace(rows, (int)D, code, &bytes));
       ws = f32({(int64_t)(bytes / sizeof(float))}, x);
     }
-    const Tensor w = weight.defined() ? weight.contiguous() : weight;
     const float* mean = fptr(stats);
     done(mm_layernorm_bwd(ptr(dy), lddy, ptr(x), ldx, code, rows, (int)D, ptr(w), p_code, mean, mean + rows, ptr(dx), D,
                           ptr(dw), ptr(db), fptr(ws), stream()));
@@ -188,7 +207,7 @@ struct RouteFn : torch::autograd::Function<RouteFn> {
     const Tensor x = rows(logits);
     auto [gates, experts] = run(x, value(bias), code, k, scoring, groups, top_groups, renorm, scale);
     ctx->save_for_backward({x, gates, experts});
-    ctx->saved_data["args"] = std::vector<int64_t>{code, scoring, renorm};
+    ctx->saved_data["args"] = std::vector<int64_t>{code, scoring, renorm, x.size(1), k};
     ctx->saved_data["scale"] = scale;
     ctx->mark_non_differentiable({experts});
     return {gates, experts};
@@ -212,10 +231,12 @@ struct RouteFn : torch::autograd::Function<RouteFn> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &gates = saved[1], &experts = saved[2];
     const auto args = ctx->saved_data["args"].toIntVector();
-    const long T = x.size(0), E = x.size(1), k = gates.size(1);
     const Tensor dg = grads[0].contiguous();
+    const long T = dg.size(0), E = args[3], k = args[4];
+    const Tensor x = rows(unpacked(saved[0], {T, E}, type_of(args[0]), dg, "logits"));
+    const Tensor gates = unpacked_dense(saved[1], {T, k}, at::kFloat, dg, "gates");
+    const Tensor experts = unpacked_dense(saved[2], {T, k}, at::kInt, dg, "experts");
     Tensor dl = at::empty({T, E}, x.options());
     done(mm_route_bwd(ptr(x), distance(x), (int)args[0], T, (int)E, (int)k, (int)args[1], (int)args[2],
                       (float)ctx->saved_data["scale"].toDouble(), fptr(gates), iptr(experts), fptr(dg), ptr(dl),
@@ -384,8 +405,7 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
     if (weight.requires_grad() || (dxg && !(joined && n.k == 2))) l = plan->lists();
     if (dxg && joined && n.k == 2) p = plan->pairs();
     ctx->save_for_backward({x, w, g, plan->experts, l.offsets, l.order, p.offsets, p.order});
-    ctx->saved_data["code"] = code;
-    ctx->saved_data["joined"] = joined;
+    ctx->saved_data["args"] = std::vector<int64_t>{code, joined, n.T, n.M, n.D, n.F, n.E, n.k};
     return run(x, w, g, *plan, (int)code);
   }
 
@@ -420,17 +440,26 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor x = inner(saved[0]), &w = saved[1], &gates = saved[2], &experts = saved[3], &offsets = saved[4],
-                 &order = saved[5], &pair_offsets = saved[6], &pair_order = saved[7];
+    const auto args = ctx->saved_data["args"].toIntVector();
+    const int code = (int)args[0];
+    const Sizes n{args[2], args[3], args[4], args[5], args[6], args[7]};
     const Tensor dy = inner(grads[0]);
-    const int code = (int)ctx->saved_data["code"].toInt();
-    const Sizes n = sizes(x, w, experts);
+    const auto type = type_of(code);
+    const Tensor x = inner(grads[0].dim() == 2 ? unpacked(saved[0], {n.T, n.D}, type, dy, "x")
+                                               : unpacked(saved[0], {n.T, n.M, n.D}, type, dy, "x"));
+    const Tensor w = unpacked_dense(saved[1], {n.E, n.D, n.F}, type, dy, "weight");
+    const Tensor gates = unpacked_dense(saved[2], {n.T, n.k}, at::kFloat, dy, "gates");
+    const Tensor experts = unpacked_dense(saved[3], {n.T, n.k}, at::kInt, dy, "experts");
+    const Tensor offsets = unpacked_dense(saved[4], {n.E + 1}, at::kInt, dy, "offsets");
+    const Tensor order = unpacked_dense(saved[5], {n.T * n.k}, at::kInt, dy, "order");
+    const Tensor pair_offsets = unpacked_dense(saved[6], {(n.E + 1) * (n.E + 2) / 2}, at::kInt, dy, "pairs");
+    const Tensor pair_order = unpacked_dense(saved[7], {n.T}, at::kInt, dy, "pairs' order");
     const int S = (int)(n.T * n.k), k = (int)n.k, M = (int)n.M, D = (int)n.D, F = (int)n.F, E = (int)n.E;
     Tensor dx, dw, dg;
     if (ctx->needs_input_grad(0)) dx = at::empty(saved[0].sizes(), x.options());
     if (ctx->needs_input_grad(1)) dw = at::empty({n.E, n.D, n.F}, x.options());
     if (gates.defined() && ctx->needs_input_grad(2)) dg = f32({n.T, n.k}, x);
-    if ((dx.defined() || dg.defined()) && ctx->saved_data["joined"].toBool()) {
+    if ((dx.defined() || dg.defined()) && args[1]) {
       const bool pairs = k == 2;
       done(mm_expert_joined(ptr(dy), dy.stride(0), dy.stride(1), code, (int)n.T, k, M, F, D, ptr(w), 1, E, fptr(gates),
                             iptr(experts), iptr(pairs ? pair_offsets : offsets), iptr(pairs ? pair_order : order),
