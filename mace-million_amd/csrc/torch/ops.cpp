@@ -10,6 +10,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/sub.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -21,6 +22,7 @@
 #include <sstream>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../../include/mace_million_amd.h"
 
@@ -310,23 +312,52 @@ Lists make_pairs(const Tensor& experts, long E) {
 
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
+c10::Stream current_stream(const Tensor& t) {
+  return c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device());
+}
+
 // The sorts wait until a product (or the caller) needs one: few rows need none, and rows of two choices may need the
-// pairs' instead of the slots'.  Under graph capture the slots are sorted at once, so that a captured plan follows
-// every replay; lists that a capture needs of an older plan are its own and are not kept (they hold nothing until a
-// replay).
+// pairs' instead of the slots'.  The caller cannot see which call sorts and so cannot order another stream behind it:
+// every stream sorts its own lists (an event for each sort costs every training call 5 us of the host, sorting once
+// more only those that use several streams, 5 - 12 us of the GPU).  Under graph capture the slots are sorted at once, so
+// that a captured plan follows every replay.  A capture takes the lists that an older plan has, if they are there;
+// those it has to sort are its own and are not kept (they hold nothing until a replay).
 struct Plan {
+  struct Kept {
+    c10::Stream stream;
+    Lists lists;
+  };
   Tensor experts;
   long T, k, E;
-  Lists slots, rows;
+  Lists captured;   // the slots of a plan made under capture
+  std::vector<Kept> slots, rows;
+  std::vector<c10::Stream> streams;   // that the allocator knows to use experts, which may be the plan's own copy
+
+  void use() {
+    const c10::Stream s = current_stream(experts);
+    if (std::find(streams.begin(), streams.end(), s) != streams.end()) return;
+    experts.record_stream(s);
+    streams.push_back(s);
+  }
 
   template <typename F>
-  Lists keep(Lists& kept, F make) {
-    if (kept.offsets.defined()) return kept;
+  Lists keep(std::vector<Kept>& kept, F make) {
+    const c10::Stream s = current_stream(experts);
+    if (!kept.empty() && capturing()) {
+      const Kept& older = kept.back();
+      if (older.stream == s) return make(experts, E);
+      // a capture cannot wait for work outside it, so the host does
+      const c10::hip::HIPStreamCaptureModeGuard relaxed(hipStreamCaptureModeRelaxed);
+      c10::impl::VirtualGuardImpl(s.device_type()).synchronizeStream(older.stream);
+      return older.lists;
+    }
+    for (const Kept& q : kept)
+      if (q.stream == s) return q.lists;
     const Lists made = make(experts, E);
-    if (!capturing()) kept = made;
+    if (!capturing()) kept.push_back({s, made});
     return made;
   }
-  Lists lists() { return keep(slots, make_lists); }
+  Lists lists() { return captured.offsets.defined() ? captured : keep(slots, make_lists); }
   Lists pairs() { return keep(rows, make_pairs); }
 };
 
@@ -348,7 +379,8 @@ std::shared_ptr<Plan> plan_experts(const Tensor& experts, int64_t E) {
   p->T = experts.size(0);
   p->k = experts.size(1);
   p->E = E;
-  if (capturing()) p->slots = make_lists(p->experts, E);
+  p->streams = {current_stream(p->experts)};
+  if (capturing()) p->captured = make_lists(p->experts, E);
   return p;
 }
 
@@ -415,6 +447,7 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
 
   static Tensor run(const Tensor& x0, const Tensor& w, const Tensor& gates, Plan& plan, int code) {
     const Tensor& experts = plan.experts;
+    plan.use();
     const Sizes n = sizes(x0, w, experts);
     const Tensor x = inner(x0);
     Tensor y = x0.dim() == 2 ? at::empty({n.T, n.F}, x.options()) : at::empty({n.T, n.M, n.F}, x.options());
