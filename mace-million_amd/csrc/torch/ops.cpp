@@ -12,6 +12,7 @@
 #include <ATen/ops/sub.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPException.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
@@ -310,7 +311,14 @@ Lists make_pairs(const Tensor& experts, long E) {
   return {buf.narrow(0, 0, buckets), buf.narrow(0, buckets, T)};
 }
 
-bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+// the graph capture that the current stream is part of
+std::optional<unsigned long long> capture() {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_HIP_CHECK(hipStreamGetCaptureInfo(c10::hip::getCurrentHIPStream().stream(), &status, &id));
+  if (status == hipStreamCaptureStatusNone) return std::nullopt;
+  return id;
+}
 
 c10::Stream current_stream(const Tensor& t) {
   return c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device());
@@ -320,8 +328,9 @@ c10::Stream current_stream(const Tensor& t) {
 // pairs' instead of the slots'.  The caller cannot see which call sorts and so cannot order another stream behind it:
 // every stream sorts its own lists (an event for each sort costs every training call 5 us of the host, sorting once
 // more only those that use several streams, 5 - 12 us of the GPU).  Under graph capture the slots are sorted at once, so
-// that a captured plan follows every replay.  A capture takes the lists that an older plan has, if they are there;
-// those it has to sort are its own and are not kept (they hold nothing until a replay).
+// that a captured plan follows every replay.  Outside that capture such a plan is sorted anew by every call: its experts
+// change with the replays, and what its graph sorted holds nothing before the first.  A capture takes the lists that an
+// older plan has, if they are there; those it has to sort are its own and are not kept.
 struct Plan {
   struct Kept {
     c10::Stream stream;
@@ -329,7 +338,8 @@ struct Plan {
   };
   Tensor experts;
   long T, k, E;
-  Lists captured;   // the slots of a plan made under capture
+  std::optional<unsigned long long> made_in;   // the capture that the plan was made in, and its slots
+  Lists captured;
   std::vector<Kept> slots, rows;
   std::vector<c10::Stream> streams;   // that the allocator knows to use experts, which may be the plan's own copy
 
@@ -343,21 +353,19 @@ struct Plan {
   template <typename F>
   Lists keep(std::vector<Kept>& kept, F make) {
     const c10::Stream s = current_stream(experts);
-    if (!kept.empty() && capturing()) {
-      const Kept& older = kept.back();
-      if (older.stream == s) return make(experts, E);
+    if (made_in || capture()) {
+      if (kept.empty() || kept.back().stream == s) return make(experts, E);
       // a capture cannot wait for work outside it, so the host does
       const c10::hip::HIPStreamCaptureModeGuard relaxed(hipStreamCaptureModeRelaxed);
-      c10::impl::VirtualGuardImpl(s.device_type()).synchronizeStream(older.stream);
-      return older.lists;
+      c10::impl::VirtualGuardImpl(s.device_type()).synchronizeStream(kept.back().stream);
+      return kept.back().lists;
     }
     for (const Kept& q : kept)
       if (q.stream == s) return q.lists;
-    const Lists made = make(experts, E);
-    if (!capturing()) kept.push_back({s, made});
-    return made;
+    kept.push_back({s, make(experts, E)});
+    return kept.back().lists;
   }
-  Lists lists() { return captured.offsets.defined() ? captured : keep(slots, make_lists); }
+  Lists lists() { return made_in && made_in == capture() ? captured : keep(slots, make_lists); }
   Lists pairs() { return keep(rows, make_pairs); }
 };
 
@@ -380,7 +388,8 @@ std::shared_ptr<Plan> plan_experts(const Tensor& experts, int64_t E) {
   p->k = experts.size(1);
   p->E = E;
   p->streams = {current_stream(p->experts)};
-  if (capturing()) p->captured = make_lists(p->experts, E);
+  p->made_in = capture();
+  if (p->made_in) p->captured = make_lists(p->experts, E);
   return p;
 }
 

@@ -42,8 +42,9 @@ def plan_experts(experts, n_experts):
     experts int32 [T, k], n_experts
     order int32 [T k], offsets int32 [n_experts + 1]: the slots of expert e are order[offsets[e] : offsets[e + 1]], in
         ascending order; slots with an expert outside [0, n_experts) come after them, from offsets[n_experts] on.
-        Sorted when first needed (few rows need no order, rows of two choices may be sorted by pair of experts
-        instead), except under graph capture, where it is recorded at once.
+        Sorted when first needed on a stream (few rows need no order, rows of two choices may be sorted by pair of
+        experts instead), except under graph capture, where it is recorded at once.  Outside that capture the plan's
+        fields and products sort its experts as they are by then, after the last replay, at every use.
     counts int32 [n_experts]: slots of each expert (its load, for a balance bias)"""
     return ops().plan_experts(experts, n_experts)
 
