@@ -340,10 +340,21 @@ struct Plan {
   long T, k, E;
   std::optional<unsigned long long> made_in;   // the capture that the plan was made in, and its slots
   Lists captured;
+  long version = 0;   // of experts
   std::vector<Kept> slots, rows;
   std::vector<c10::Stream> streams;   // that the allocator knows to use experts, which may be the plan's own copy
 
+  // The lists and the experts are read together, and experts may be the caller's tensor: one that was written since the
+  // plan was made is refused instead of being read beside older lists.  (A replay changes the experts of a captured plan
+  // with its lists, and elsewhere such a plan is sorted anew; tensors of inference mode have no version.)
+  void check() {
+    if (experts.is_inference() || (made_in && made_in != capture())) return;
+    if ((long)experts._version() != version)
+      throw std::runtime_error("the experts of this plan were changed in place after plan_experts: make a new plan");
+  }
+
   void use() {
+    check();
     const c10::Stream s = current_stream(experts);
     if (std::find(streams.begin(), streams.end(), s) != streams.end()) return;
     experts.record_stream(s);
@@ -365,7 +376,10 @@ struct Plan {
     kept.push_back({s, make(experts, E)});
     return kept.back().lists;
   }
-  Lists lists() { return made_in && made_in == capture() ? captured : keep(slots, make_lists); }
+  Lists lists() {
+    check();
+    return made_in && made_in == capture() ? captured : keep(slots, make_lists);
+  }
   Lists pairs() { return keep(rows, make_pairs); }
 };
 
@@ -387,6 +401,7 @@ std::shared_ptr<Plan> plan_experts(const Tensor& experts, int64_t E) {
   p->T = experts.size(0);
   p->k = experts.size(1);
   p->E = E;
+  if (!p->experts.is_inference()) p->version = (long)p->experts._version();
   p->streams = {current_stream(p->experts)};
   p->made_in = capture();
   if (p->made_in) p->captured = make_lists(p->experts, E);
