@@ -6,6 +6,7 @@
 // back.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ops/empty.h>
@@ -83,6 +84,15 @@ bool needs_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// Forward-mode derivatives and traces go through dispatched operations only, so they would miss these functions without a
+// word: the result would pass for a constant, the trace for memory that nothing writes.
+void refuse_modes(const char* what, std::initializer_list<const Tensor*> ts) {
+  if (torch::jit::tracer::isTracing()) throw std::runtime_error(text(what, " cannot be traced (torch.jit.trace)"));
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined())
+      throw std::runtime_error(text(what, " has no forward-mode derivative: its inputs must not be dual tensors"));
 }
 
 // Gradients that raise when they are differentiated again, instead of passing for constants.
@@ -198,6 +208,7 @@ Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, doubl
   if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
     throw py::type_error(text("weight and bias must have one type, got ", type_name(w.scalar_type()), " and ",
                               type_name(b.scalar_type())));
+  refuse_modes("layer_norm", {&x, &w, &b});
   if (needs_grad({&x, &w, &b})) return LayerNormFn::apply(x, maybe(w), maybe(b), eps, (int64_t)code, (int64_t)p_code);
   auto [x2, ldx] = as_rows(x);
   return LayerNormFn::run(x, x2, ldx, w, b, eps, code, p_code, nullptr);
@@ -277,6 +288,7 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::str
       throw py::value_error(text("bias must be [", E, "], got ", bias->sizes()));
     b = bias->detach().contiguous();
   }
+  refuse_modes("route", {&logits});
   const int64_t s = scoring == "sigmoid", r = renormalize;
   if (needs_grad({&logits})) {
     const variable_list out = RouteFn::apply(logits, maybe(b), (int64_t)code, k, s, groups, top_groups, r, scale);
@@ -393,6 +405,7 @@ std::shared_ptr<Plan> plan_experts(const Tensor& experts, int64_t E) {
   if (experts.dim() != 2 || experts.size(1) == 0)
     throw py::value_error(text("experts must be [rows, k], got ", experts.sizes()));
   if (E < 1 || E > kMaxExperts) throw py::value_error(text("n_experts must be 1 .. ", kMaxExperts, ", got ", E));
+  refuse_modes("plan_experts", {});
   const long S = experts.numel();
   if (S > kInt32Max) throw py::value_error(text("more than 2^31 - 1 slots (", S, ")"));
   auto p = std::make_shared<Plan>();
@@ -572,6 +585,7 @@ Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates,
   if (experts.device() != x0.device()) throw py::value_error("x and the plan must be on one device");
   const long slots = T * k * (x0.dim() == 2 ? 1 : x0.size(1));
   if (slots > kInt32Max - 128) throw py::value_error(text(slots, " rows: 2^31 or more are not supported"));
+  refuse_modes("expert_linear", {&x0, &weight, &g});
   if (needs_grad({&x0, &weight, &g})) return ExpertLinearFn::apply(x0, weight, maybe(g), plan, (int64_t)code);
   return ExpertLinearFn::run(x0, weight.contiguous(), g.defined() ? g.contiguous() : g, *plan, code);
 }
