@@ -50,7 +50,13 @@ void done(int rc) {
 
 mm_stream_t stream() { return (mm_stream_t)c10::hip::getCurrentHIPStream().stream(); }
 
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// Fake, wrapped and zero tensors pass for GPU tensors and have no memory.
+void* ptr(const Tensor& t) {
+  if (!t.defined()) return nullptr;
+  void* p = t.numel() ? t.data_ptr() : nullptr;
+  if (!p && t.numel()) throw py::type_error("a tensor without memory (fake, wrapped or zero tensor) cannot be read");
+  return p;
+}
 float* fptr(const Tensor& t) { return (float*)ptr(t); }
 int* iptr(const Tensor& t) { return (int*)ptr(t); }
 
@@ -73,6 +79,9 @@ int check_gpu(const Tensor& t, const char* name) {
 
 Tensor f32(at::IntArrayRef size, const Tensor& like) { return at::empty(size, like.options().dtype(at::kFloat)); }
 Tensor i32(at::IntArrayRef size, const Tensor& like) { return at::empty(size, like.options().dtype(at::kInt)); }
+
+// The values of a lazily negated view (of a conjugate's imaginary part, say) are not those of its memory.
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 
 // Autograd takes absent tensors as empty optionals.
 using Maybe = std::optional<Tensor>;
@@ -115,19 +124,19 @@ std::pair<Tensor, long> as_rows(Tensor t) {
 
 // A saved tensor as its node gets it back.  Hooks on saved tensors (offloading, compression) may return it with any
 // strides, so its layout is taken from what comes back; sizes and type have to be those that were saved.
-const Tensor& unpacked(const Tensor& t, at::IntArrayRef size, at::ScalarType type, const Tensor& like,
+Tensor unpacked(const Tensor& t, at::IntArrayRef size, at::ScalarType type, const Tensor& like,
                        const char* name) {
   if (t.defined() && (t.sizes() != size || t.scalar_type() != type || t.device() != like.device()))
     throw std::runtime_error(text(name, " was saved for the backward as ", type_name(type), " ", size, " on ",
                                   like.device(), " and came back as ", type_name(t.scalar_type()), " ", t.sizes(),
                                   " on ", t.device()));
-  return t;
+  return plain(t);
 }
 
 Tensor unpacked_dense(const Tensor& t, at::IntArrayRef size, at::ScalarType type, const Tensor& like,
                       const char* name) {
-  unpacked(t, size, type, like, name);
-  return t.defined() ? t.contiguous() : t;
+  const Tensor u = unpacked(t, size, type, like, name);
+  return u.defined() ? u.contiguous() : u;
 }
 
 at::ScalarType type_of(int64_t code) { return code == 0 ? at::kFloat : code == 1 ? at::kBFloat16 : at::kHalf; }
@@ -163,7 +172,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     const auto saved = ctx->get_saved_variables();
     const int64_t codes = ctx->saved_data["codes"].toInt();
     const int code = (int)(codes / 4), p_code = (int)(codes % 4);
-    auto [dy, lddy] = as_rows(grads[0]);
+    auto [dy, lddy] = as_rows(plain(grads[0]));
     const long rows = dy.size(0), D = dy.size(1);
     const auto p_type = type_of(p_code);
     auto [x, ldx] = as_rows(unpacked(saved[0], {rows, D}, type_of(code), dy, "x"));
@@ -187,7 +196,8 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   }
 };
 
-Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, double eps) {
+Tensor layer_norm(const Tensor& x0, const Maybe& weight, const Maybe& bias, double eps) {
+  const Tensor x = plain(x0);
   const int code = check_gpu(x, "x");
   if (x.dim() < 1 || x.size(-1) == 0)
     throw py::value_error(text("x must be [..., D] with D > 0, got ", x.sizes()));
@@ -202,7 +212,7 @@ Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, doubl
       throw py::type_error(text(name, " must be ", type_name(x.scalar_type()), " (as x) or float32, got ",
                                 type_name(p->scalar_type())));
     if (p->dim() != 1 || p->size(0) != D) throw py::value_error(text(name, " must be [", D, "], got ", p->sizes()));
-    return *p;
+    return plain(*p);
   };
   const Tensor w = param(weight, "weight"), b = param(bias, "bias");
   if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
@@ -246,7 +256,7 @@ struct RouteFn : torch::autograd::Function<RouteFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const auto args = ctx->saved_data["args"].toIntVector();
-    const Tensor dg = grads[0].contiguous();
+    const Tensor dg = plain(grads[0]).contiguous();
     const long T = dg.size(0), E = args[3], k = args[4];
     const Tensor x = rows(unpacked(saved[0], {T, E}, type_of(args[0]), dg, "logits"));
     const Tensor gates = unpacked_dense(saved[1], {T, k}, at::kFloat, dg, "gates");
@@ -261,9 +271,10 @@ struct RouteFn : torch::autograd::Function<RouteFn> {
   }
 };
 
-std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::string& scoring,
+std::tuple<Tensor, Tensor> route(const Tensor& logits0, int64_t k, const std::string& scoring,
                                  const Maybe& bias, int64_t groups, std::optional<int64_t> top,
                                  bool renormalize, double scale) {
+  const Tensor logits = plain(logits0);
   const int code = check_gpu(logits, "logits");
   if (logits.dim() != 2 || logits.size(1) == 0)
     throw py::value_error(text("logits must be [rows, experts], got ", logits.sizes()));
@@ -286,7 +297,7 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::str
       throw py::type_error(text("bias must be float32, got ", type_name(bias->scalar_type())));
     if (bias->dim() != 1 || bias->size(0) != E)
       throw py::value_error(text("bias must be [", E, "], got ", bias->sizes()));
-    b = bias->detach().contiguous();
+    b = plain(bias->detach()).contiguous();
   }
   refuse_modes("route", {&logits});
   const int64_t s = scoring == "sigmoid", r = renormalize;
@@ -395,7 +406,8 @@ struct Plan {
   Lists pairs() { return keep(rows, make_pairs); }
 };
 
-std::shared_ptr<Plan> plan_experts(const Tensor& experts, int64_t E) {
+std::shared_ptr<Plan> plan_experts(const Tensor& experts0, int64_t E) {
+  const Tensor experts = plain(experts0);
   if (!experts.is_cuda()) throw py::type_error("experts must be a GPU tensor");
   if (experts.scalar_type() != at::kInt && experts.scalar_type() != at::kLong)
     throw py::type_error(text("experts must be int32 or int64, got ", type_name(experts.scalar_type())));
@@ -513,7 +525,7 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
     const auto args = ctx->saved_data["args"].toIntVector();
     const int code = (int)args[0];
     const Sizes n{args[2], args[3], args[4], args[5], args[6], args[7]};
-    const Tensor dy = inner(grads[0]);
+    const Tensor dy = inner(plain(grads[0]));
     const auto type = type_of(code);
     const Tensor x = inner(grads[0].dim() == 2 ? unpacked(saved[0], {n.T, n.D}, type, dy, "x")
                                                : unpacked(saved[0], {n.T, n.M, n.D}, type, dy, "x"));
@@ -557,7 +569,8 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
   }
 };
 
-Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates, const std::shared_ptr<Plan>& plan) {
+Tensor expert_linear(const Tensor& x1, const Tensor& weight1, const Maybe& gates, const std::shared_ptr<Plan>& plan) {
+  const Tensor x0 = plain(x1), weight = plain(weight1);
   const int code = check_gpu(x0, "x");
   if (check_gpu(weight, "weight") != code)
     throw py::type_error(text("weight must be ", type_name(x0.scalar_type()), " (as x), got ",
@@ -574,7 +587,7 @@ Tensor expert_linear(const Tensor& x0, const Tensor& weight, const Maybe& gates,
   if (weight.size(1) > kInt32Max || weight.size(2) > kInt32Max) throw py::value_error("weight blocks are too large");
   Tensor g;
   if (gates) {
-    g = *gates;
+    g = plain(*gates);
     check_gpu(g, "gates");
     if (g.scalar_type() != at::kFloat)
       throw py::type_error(text("gates must be float32, got ", type_name(g.scalar_type())));
