@@ -192,10 +192,10 @@ __global__ void __launch_bounds__(256, 2) mm_expert_joined_kernel(MMJoined a, in
     sa.put(As + buf * BM * 8);
     sb.put(Bs + buf * BN * 8);
   };
-  // The gates: on the rows' values as they become operands (float without DG: one more rounding of 2^-24), or on each
-  // choice's products, in sums of their own (16 bits, where the operands' rounding would show; DG, which needs the
-  // products without the gates).
-  constexpr bool SCALED = sizeof(T) == 4 && !DG, SUM = !SCALED;
+  // The gates: on each choice's products, in sums of their own, or on the rows' values as they become operands (two
+  // choices of float, whose planes leave no registers for the sums: one more rounding of 2^-24, and gate x value must
+  // stay below what rounds to infinity in bfloat16).
+  constexpr bool SCALED = sizeof(T) == 4 && J == 2, SUM = !SCALED;
   floatx4 acc[FN][FM] = {}, sum[SUM ? FN : 1][SUM ? FM : 1] = {};
   const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
   int buf = 0;
@@ -276,9 +276,11 @@ __global__ void __launch_bounds__(256, 2) mm_expert_joined_kernel(MMJoined a, in
 
 // ------------------------------------------------------------------------------------------------ few rows
 // y[t, m] straight from the choices of row t, without a plan: a workgroup takes LC vectors of columns, its other
-// threads share the sum over d, W is read once per row, coalesced along the columns, fp32 sums.  Bound by latency: the
-// sum over d is split as far as the workgroup goes, and the columns over many workgroups (1 row 128 -> 128, k = 2: 3.6
-// us; 64 rows 64 -> 64: 3.6 us).
+// threads share the sum over d, W is read once per row, coalesced along the columns, fp32 sums.  float operands that
+// round to infinity in bfloat16 give NaN, as they do in the split operands of many rows.  Bound by latency: the sum over
+// d is split as far as the workgroup goes, and the columns over many workgroups, with no branch between the loads (a
+// check for cut vectors among them took 16 us instead of 8 for 1 row 1024 -> 1024 bfloat16, 4 of 64; 1 row 128 -> 128
+// float, k = 2: 3.5 us; 64 rows 64 -> 64: 3.4 us).
 struct MMFew {
   const void *x, *W;
   const float* gates;
@@ -287,12 +289,17 @@ struct MMFew {
   int k, M, D, F, E;
 };
 
+// the least float that rounds to infinity in bfloat16
+#define MM_SPLIT_LIMIT 0x1.ffp127f
+
 template <typename T, int LC>
 __global__ void __launch_bounds__(256) mm_expert_few_kernel(MMFew a, T* __restrict__ y) {
   constexpr int N = MMVec<T>::N, G = 256 / LC;
   __shared__ float red[4][LC * N];
   const long t = blockIdx.y;
-  const int m = blockIdx.z, lc = threadIdx.x % LC, gd = threadIdx.x / LC, f = (blockIdx.x * LC + lc) * N;
+  const int m = blockIdx.z, lc = threadIdx.x % LC, gd = threadIdx.x / LC, f0 = (blockIdx.x * LC + lc) * N;
+  // a vector cut by the last column starts earlier instead: some columns are written twice, with the same bits
+  const int f = a.F >= N ? min(f0, a.F - N) : f0;
   const T* __restrict__ x = (const T*)a.x + t * a.st + m * a.sm;
   float acc[N] = {};
   for (int j = 0; j < a.k; ++j) {
@@ -300,16 +307,39 @@ __global__ void __launch_bounds__(256) mm_expert_few_kernel(MMFew a, T* __restri
     if ((unsigned)e >= (unsigned)a.E) continue;
     const float g = a.gates ? a.gates[t * a.k + j] : 1.f;
     const T* __restrict__ W = (const T*)a.W + (size_t)e * a.D * a.F;
-    float sum[N] = {};
-    if (f < a.F) {
+    float sum[N] = {}, top[N] = {}, top_x = 0.f;   // largest magnitudes (float; a NaN is in the sum anyway)
+    auto add = [&](int d, const float (&w)[N]) {
+      const float xv = (float)x[d];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        sum[i] = fmaf(xv, w[i], sum[i]);
+        if constexpr (sizeof(T) == 4) top[i] = fmaxf(top[i], fabsf(w[i]));
+      }
+      if constexpr (sizeof(T) == 4) top_x = fmaxf(top_x, fabsf(xv));
+    };
+    if (a.F >= N) {
+      if (f0 < a.F) {
 #pragma unroll 8
+        for (int d = gd; d < a.D; d += G) {
+          const typename MMVec<T>::type v = *(const typename MMVec<T>::type*)(W + (size_t)d * a.F + f);
+          float w[N];
+#pragma unroll
+          for (int i = 0; i < N; ++i) w[i] = (float)v[i];
+          add(d, w);
+        }
+      }
+    } else if (f == 0) {
+#pragma unroll 1
       for (int d = gd; d < a.D; d += G) {
         float w[N];
-        mm_load_vec(W + (size_t)d * a.F, f, a.F, w);
-        const float xv = (float)x[d];
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] = fmaf(xv, w[i], sum[i]);
+        mm_load_vec(W + (size_t)d * a.F, 0, a.F, w);
+        add(d, w);
       }
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (fmaxf(top[i], top_x) >= MM_SPLIT_LIMIT) sum[i] = __builtin_nanf("");
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = fmaf(g, sum[i], acc[i]);
@@ -322,7 +352,7 @@ __global__ void __launch_bounds__(256) mm_expert_few_kernel(MMFew a, T* __restri
     if ((threadIdx.x & 63) < LC) red[threadIdx.x >> 6][lc * N + i] = acc[i];
   }
   __syncthreads();
-  if (threadIdx.x >= LC || f >= a.F) return;
+  if (threadIdx.x >= LC || f0 >= a.F) return;
 #pragma unroll
   for (int i = 0; i < N; ++i)
     acc[i] = red[0][lc * N + i] + red[1][lc * N + i] + red[2][lc * N + i] + red[3][lc * N + i];

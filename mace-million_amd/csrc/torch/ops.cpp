@@ -438,8 +438,9 @@ struct Sizes { long T, M, D, F, E, k; };
 
 // Whether rows go straight through their blocks (mm_expert_few), without a plan and without joining slots: while the
 // blocks' bytes that they read, mostly from the L2s, stay below 64 MB.  Measured (us, straight against sorted): 128 ->
-// 128 float, 2 of 8 experts: 1 row 3.6 / 19, 128 rows (17 MB) 4.4 / 21; 1024 -> 1024 bfloat16, 4 of 64: 1 row 17 / 26,
-// 8 rows (67 MB) 33 / 32, 16 rows 36 / 35, 64 rows 126 / 36; the same in float: 4 rows (67 MB) 26 / 75.
+// 128 float, 2 of 8 experts: 1 row 3.5 / 13, 128 rows (17 MB) 4.5 / 15, 512 rows (67 MB) 10 / 15, 1000 rows 18 / 16;
+// 1024 -> 1024 bfloat16, 4 of 64: 1 row 8 / 22, 8 rows (67 MB) 22 / 27, 16 rows 38 / 29, 64 rows 139 / 32; the same in
+// float: 4 rows (67 MB) 21 / 70, 8 rows 39 / 72.
 bool few_rows(const Sizes& n, int code) {
   const double bytes = (double)n.T * n.M * n.k * n.D * n.F * (code == 0 ? 4 : 2);
   return bytes <= 64e6 && n.T <= 65535 && n.M <= 65535;

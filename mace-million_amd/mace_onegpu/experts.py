@@ -57,5 +57,8 @@ def expert_linear(x, weight, plan, gates=None):
     x [T, D], or [T, M, D]: M components of a row that share its experts (the 2 l + 1 components of an irrep; a slice of
     ir_mul features is read in place).  weight [E, D, F], of x's type; gates float32 [T, k] (None: ones).  Returns
     [T, (M,) F] of x's type.  Differentiable in x, weight and gates.  float32 products are taken from three bfloat16
-    parts of each operand at float32 accuracy (as the model's linears do); operands beyond 3.38e38 give NaN."""
+    parts of each operand at float32 accuracy (as the model's linears do).  float32 operands that round to infinity in
+    bfloat16 (from 3.396e38 on, infinity among them) give NaN in the results that they enter, for one row as for many;
+    16-bit operands give infinity or NaN as their sums do.  In the gradient of weight the operand is gate times
+    cotangent, of 16-bit types in two bfloat16 parts, and an infinite value gives infinity or NaN."""
     return ops().expert_linear(x, weight, gates, plan)
