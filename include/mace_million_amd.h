@@ -367,7 +367,8 @@ int mm_expert_joined(const void* in, long st, long sm, int dtype, int T, int k, 
                      int transposed, int E, const float* gates, const int* experts, const int* offsets,
                      const int* order, void* out, const void* x, long xt, long xm, float* dgates, mm_stream_t stream);
 /* out [S, M, N] (slots without an expert are not written): out[s, m] = in[s / k, m] @ W[e], W [E, K, N], or [E, N, K]
- * with `transposed`; in at (row, component) offset row st + component sm; S M < 2^31 */
+ * with `transposed`; in at (row, component) offset row st + component sm; S M <= 2^31 - 2^16 (-3 beyond;
+ * so mm_expert_joined's T M and mm_expert_wgrad's S M) */
 int mm_expert_rows(const void* in, long st, long sm, int dtype, int S, int k, int M, int K, int N, const void* W,
                    int transposed, int E, const int* offsets, const int* order, float* out, mm_stream_t stream);
 /* y [T, M, F] = sum_j gates[t, j] x[t, m] @ W[experts[t, j]] (W [E, D, F]) in one launch without a plan, for few rows;

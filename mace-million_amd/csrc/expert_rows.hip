@@ -490,7 +490,7 @@ extern "C" int mm_expert_rows(const void* in, long st, long sm, int dtype, int S
                               hipStream_t stream) {
   MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");
   MM_CHECK_ARG(S >= 0 && k >= 1 && M >= 1 && K >= 1 && N >= 1 && E >= 1 && st >= 0 && sm >= 0, "bad sizes");
-  if ((long)S * M > 2147483647L - 128) return range_error("mm_expert_rows", "2^31 rows or more are not supported");
+  if ((long)S * M > MM_EXPERT_MAX_ROWS) return range_error("mm_expert_rows", TOO_MANY_ROWS);
   if (S == 0) return MM_OK;
   MM_CHECK_ARG(in && W && offsets && order && out, "a pointer is null");
   const MMRows a{in, W, offsets, order, out, st, sm, k, M, K, N, E};
@@ -518,6 +518,7 @@ extern "C" int mm_expert_few(const void* x, long st, long sm, int dtype, int T, 
   if (T > 65535 || M > 65535)
     return range_error("mm_expert_few", "more than 65535 rows or components are not supported");
   if (T == 0) return MM_OK;
+  if (too_many(F / 16L + 1, 256)) return range_error("mm_expert_few", "output too large for one launch");
   MM_CHECK_ARG(x && W && experts && y, "a pointer is null");
   const MMFew a{x, W, gates, experts, st, sm, k, M, D, F, E};
 #define CALL(T_)                                                                                             \
@@ -545,7 +546,7 @@ extern "C" int mm_expert_joined(const void* in, long st, long sm, int dtype, int
   if (M > 64) return range_error("mm_expert_joined", "more than 64 components are not supported");
   if (k == 2 && E > MM_PAIRS_MAX_E)
     return range_error("mm_expert_joined", "pairs of more than 21 experts are not supported");
-  if ((long)T * M > 2147483647L - 128) return range_error("mm_expert_joined", "2^31 rows or more are not supported");
+  if ((long)T * M > MM_EXPERT_MAX_ROWS) return range_error("mm_expert_joined", TOO_MANY_ROWS);
   if (T == 0) return MM_OK;
   MM_CHECK_ARG(in && W && experts && offsets && order, "a pointer is null");
   if (dtype == MM_F32 && K <= 128 && k == 1 && !dgates && out) {

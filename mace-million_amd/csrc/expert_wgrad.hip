@@ -167,10 +167,10 @@ __global__ void __launch_bounds__(256) mm_expert_wgrad_sum_kernel(MMWgrad a, int
   __shared__ float s_t[G][G > 1 ? 64 : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.y;
   int first = 0;   // chunks of the experts before e
-  for (int o = lane; o < e; o += 64) first += ((a.offsets[o + 1] - a.offsets[o]) * a.M + chunk - 1) / chunk;
+  for (int o = lane; o < e; o += 64) first += mm_pieces((a.offsets[o + 1] - a.offsets[o]) * a.M, chunk);
 #pragma unroll
   for (int d = 32; d; d >>= 1) first += __shfl_xor(first, d);
-  const int n = ((a.offsets[e + 1] - a.offsets[e]) * a.M + chunk - 1) / chunk;
+  const int n = mm_pieces((a.offsets[e + 1] - a.offsets[e]) * a.M, chunk);
   const long size = (long)a.D * a.F, i = (long)blockIdx.x * COLUMNS + (G > 1 ? lane : V * (int)threadIdx.x);
   const int left = (int)(size - i < V ? size - i : V);
   const float* __restrict__ p = part + (size_t)first * size + i;
@@ -245,12 +245,13 @@ int wgrad_chunk(long rows, int D, int F, int E) {
   const long tiles = (long)((D + 127) / 128) * ((F + 127) / 128);
   if (E * tiles >= 512 || rows < 512) return 0;
   const long room = 480 - tiles * E / 2, wg = room < 128 ? 128 : room, c = (rows * tiles + wg - 1) / wg;
-  return (int)(c < 128 ? 128 : (c + 31) / 32 * 32);
+  return (int)(c < 128 ? 128 : ((c < rows ? c : rows) + 31) / 32 * 32);
 }
 }  // namespace
 
 extern "C" int mm_expert_wgrad_workspace(int S, int M, int D, int F, int E, size_t* bytes) {
   MM_CHECK_ARG(S >= 0 && M >= 1 && D >= 1 && F >= 1 && E >= 1 && bytes, "bad sizes");
+  if ((long)S * M > MM_EXPERT_MAX_ROWS) return range_error("mm_expert_wgrad_workspace", TOO_MANY_ROWS);
   const long rows = (long)S * M, c = wgrad_chunk(rows, D, F, E);
   *bytes = c ? (size_t)(rows / c + (E < S ? E : S)) * D * F * sizeof(float) : 0;
   return MM_OK;
@@ -263,7 +264,7 @@ extern "C" int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, 
   MM_CHECK_ARG(S >= 0 && k >= 1 && M >= 1 && D >= 1 && F >= 1 && E >= 1, "bad sizes");
   MM_CHECK_ARG(xt >= 0 && xm >= 0 && yt >= 0 && ym >= 0, "bad strides");
   if (E > MM_EXPERT_MAX_E) return range_error("mm_expert_wgrad", "more than 1024 experts are not supported");
-  if ((long)S * M > 2147483647L - 128) return range_error("mm_expert_wgrad", "2^31 rows or more are not supported");
+  if ((long)S * M > MM_EXPERT_MAX_ROWS) return range_error("mm_expert_wgrad", TOO_MANY_ROWS);
   MM_CHECK_ARG(offsets && dW && (S == 0 || (x && dy && order)), "a pointer is null");
   const MMWgrad a{x, dy, gates, offsets, order, dW, xt, xm, yt, ym, k, M, D, F, E};
   const int chunk = wgrad_chunk((long)S * M, D, F, E);

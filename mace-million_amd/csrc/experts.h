@@ -13,6 +13,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));   // 16 bytes known to be float-aligned only
 
 #define MM_EXPERT_MAX_E 1024
+#define MM_EXPERT_MAX_ROWS (2147483648L - 65536)   // rows (slots x M); indices within a tile or stage past them fit an int
 #define MM_PAIRS_MAX_E 21   // 253 pairs
 #define MM_HELD_ROWS 1024   // rows of a workgroup with its blocks in registers, at most
 
@@ -29,6 +30,11 @@ struct MMTile {
   int e, row0, rows;   // expert, first of its rows (slots x M), rows in the tile; e < 0: no such tile
 };
 
+// pieces of `size` that n >= 0 values make (n + size may pass 2^31)
+__host__ __device__ inline int mm_pieces(int n, int size) {
+  return (int)(((unsigned)n + (unsigned)size - 1u) / (unsigned)size);
+}
+
 // Workgroup b of `per` for each of the tiles of BM rows that the row lists of the buckets have (every list ends in a
 // cut tile); list i: entries offsets[i] .. offsets[i + 1], the last one to `end`, M rows each.  Every wave finds its
 // tile by itself, 64 lists at a time.  Workgroups are dealt out to the 8 XCDs in turn; the work is numbered so that an
@@ -41,9 +47,9 @@ __device__ __forceinline__ MMTile mm_expert_tile(const int* __restrict__ offsets
     return ((i + 1 < lists ? offsets[i + 1] : end) - offsets[i]) * M;
   };
   const int head = rows_of(lane);
-  int all = (head + BM - 1) / BM;
+  int all = mm_pieces(head, BM);
 #pragma unroll 4
-  for (int i = 64 + lane; i - lane < lists; i += 64) all += (rows_of(i) + BM - 1) / BM;
+  for (int i = 64 + lane; i - lane < lists; i += 64) all += mm_pieces(rows_of(i), BM);
 #pragma unroll
   for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
   all *= per;
@@ -54,7 +60,7 @@ __device__ __forceinline__ MMTile mm_expert_tile(const int* __restrict__ offsets
   *part = at - tile * per;
   *number = tile;
   for (int i0 = 0; i0 < lists; i0 += 64) {
-    const int rows = i0 ? rows_of(i0 + lane) : head, n = (rows + BM - 1) / BM;
+    const int rows = i0 ? rows_of(i0 + lane) : head, n = mm_pieces(rows, BM);
     int inc = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -375,6 +381,8 @@ inline int range_error(const char* name, const char* what) {
   mm::set_error(std::string(name) + ": " + what);
   return MM_ERANGE;
 }
+
+constexpr char TOO_MANY_ROWS[] = "more than 2^31 - 2^16 rows are not supported";
 
 // a launch takes fewer than 2^32 threads
 inline bool too_many(long workgroups, long threads) { return workgroups * threads >= 4294967296L; }

@@ -350,7 +350,8 @@ int route_args(const char* name, int dtype, long T, int E, int k, int scoring, i
   if (E > MM_ROUTE_MAX_E) return bad("more than 1024 experts are not supported", MM_ERANGE);
   if (k > MM_ROUTE_MAX_K) return bad("more than 32 experts a row are not supported", MM_ERANGE);
   if (groups > MM_ROUTE_MAX_G) return bad("more than 64 groups are not supported", MM_ERANGE);
-  if (T > 2147483647L * 4) return bad("too many rows", MM_ERANGE);
+  const int lanes = E <= 16 ? 4 : E <= 32 ? 8 : E <= 256 ? 16 : E <= 512 ? 32 : 64;   // of a row (MM_ROUTE_SHAPES)
+  if ((T + 255) * lanes >= 4294967296L) return bad("too many rows for one launch", MM_ERANGE);   // of 2^32 threads
   *a = MMRoute{T, ldl, E, k, scoring, groups, top_groups, renorm != 0, scale};
   return MM_OK;
 }

@@ -34,7 +34,7 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-constexpr long kInt32Max = 2147483647L;
+constexpr long kInt32Max = 2147483647L, kMaxRows = 2147483648L - 65536;
 constexpr int kMaxDim = 16384, kMaxExperts = 1024, kMaxK = 32, kMaxGroups = 64;
 
 template <typename... A>
@@ -598,7 +598,7 @@ Tensor expert_linear(const Tensor& x1, const Tensor& weight1, const Maybe& gates
   const Tensor& experts = plan->experts;
   if (experts.device() != x0.device()) throw py::value_error("x and the plan must be on one device");
   const long slots = T * k * (x0.dim() == 2 ? 1 : x0.size(1));
-  if (slots > kInt32Max - 128) throw py::value_error(text(slots, " rows: 2^31 or more are not supported"));
+  if (slots > kMaxRows) throw py::value_error(text(slots, " rows: more than 2^31 - 2^16 are not supported"));
   refuse_modes("expert_linear", {&x0, &weight, &g});
   if (needs_grad({&x0, &weight, &g})) return ExpertLinearFn::apply(x0, weight, maybe(g), plan, (int64_t)code);
   return ExpertLinearFn::run(x0, weight.contiguous(), g.defined() ? g.contiguous() : g, *plan, code);
