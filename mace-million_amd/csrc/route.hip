@@ -4,14 +4,17 @@
 //     chosen: the k largest keys, ties to the lowest index; expert -1 and gate 0 where no open expert is left
 //     score: softmax over the E logits, or sigmoid of each
 //     gate_j = scale score_j / sum_chosen score, or scale score_j
-// The bias moves the choice only, not the gates.  It is added to the logits, of which both scores are monotone
-// functions: one rounded addition, so the choice does not depend on the order of a sum or the rounding of an
-// exponential, and saturated sigmoids do not tie.  Renormalised gates are a softmax over the chosen of the scores'
-// logarithms (of the logits, or of log sigmoid), so that scores that all underflow still give gates of sum scale.  A
-// NaN logit is chosen first and makes the gates NaN.
+// The bias moves the choice only, not the gates.  It is added to the logits: one rounded addition, so the choice does not
+// depend on the order of a sum or the rounding of an exponential, and saturated sigmoids do not tie.  This is a rule of
+// its own: with a bias that differs between experts, score + bias (or a group's key from the sum of its two best)
+// orders them otherwise, so a router trained with that rule chooses other experts here; without a bias the orders are
+// the same.  Renormalised gates are a softmax over the chosen of the scores' logarithms (of the logits, or of log
+// sigmoid), so that scores that all underflow still give gates of sum scale.  A NaN logit is chosen first and makes the
+// gates of its row NaN (of plain sigmoids: its own gate).
 // A row lies in LPR lanes, C consecutive logits each; k rounds of a maximum over the lanes' best keys (as integers of
 // the same order), the lowest lane with it giving its first such logit: no sort, no memory but the logits and the
-// results.  Bound by the rounds' vector instructions for large k, by HBM for small k.  Measured, forward and backward:
+// results.  Bound by vector instructions where there are many experts (1,000 a wave of 4 rows of 256 with k = 8 and
+// groups, 470 of 89 with k = 3: the SIMDs issue them without a pause), by HBM for few.  Measured, forward and backward:
 // 500,000 float rows of 16, k = 2: 17.6 and 10.2 us (40 and 44 MB); 65,536 bfloat16 rows of 256, k = 8 of 4 in 8
 // groups: 29 and 13 us (38 MB each); 98,304 float16 rows of 89, k = 3, plain softmax: 18 us; one row: 2.7 us.
 #include "rowvec.h"

@@ -22,10 +22,12 @@ def route(logits, k, scoring="softmax", bias=None, groups=1, top_groups=None, re
     descending order of the key, ties to the lowest index.
 
     logits [T, E], E up to 1024, k up to 32: -inf closes an expert to a row; a slot without an open expert gets expert
-        -1 and gate 0 (a row with nothing open: all slots).  A NaN logit is chosen first and makes the row's gates NaN.
+        -1 and gate 0 (a row with nothing open: all slots).  A NaN logit is chosen first and makes the row's gates NaN
+        (plain sigmoids: its own gate).
     scoring: "softmax" (over the row's E logits) or "sigmoid" (of each).
     bias float32 [E]: moves the choice (balance of the experts' load) and not the gates; no gradient.  It is added to
-        the logits, of which both scores are monotone functions.
+        the logits.  That is a rule of its own: a router whose bias was trained on the scores (score + bias, groups by
+        the sum of their two best) chooses other experts here.
     groups, top_groups: the E experts in `groups` equal runs (64 at most), of which only the top_groups with the largest
         keys are open (None: all).
     renormalize: gates = scale * score / sum of the chosen scores, finite also where all scores underflow; else
