@@ -538,12 +538,12 @@ extern "C" int mm_expert_joined(const void* in, long st, long sm, int dtype, int
   MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");
   MM_CHECK_ARG(T >= 0 && M >= 1 && K >= 1 && N >= 1 && E >= 1 && st >= 0 && sm >= 0, "bad sizes");
   MM_CHECK_ARG(k == 1 || k == 2, "k must be 1 or 2");
+  if (M > 64) return range_error("mm_expert_joined", "more than 64 components are not supported");
   const int tiles_n = (N + 127) / 128, buckets = k == 1 ? E + 1 : E <= MM_PAIRS_MAX_E ? mm_pair_buckets(E) : 0;
   const int chunk = dtype == MM_F32 && K <= 128 && k == 2 && T ? mm::pairs_chunk((long)T * M, tiles_n, buckets, M) : 0;
   MM_CHECK_ARG(out || dgates, "nothing to compute");
   MM_CHECK_ARG(!dgates || (transposed && x && xt >= 0 && xm >= 0 && N <= 128 && (k == 1 || chunk || T == 0)),
                "dgates needs the transposed blocks, x, at most 128 columns, and one choice or short float rows");
-  if (M > 64) return range_error("mm_expert_joined", "more than 64 components are not supported");
   if (k == 2 && E > MM_PAIRS_MAX_E)
     return range_error("mm_expert_joined", "pairs of more than 21 experts are not supported");
   if ((long)T * M > MM_EXPERT_MAX_ROWS) return range_error("mm_expert_joined", TOO_MANY_ROWS);
