@@ -491,6 +491,7 @@ extern "C" int mm_expert_rows(const void* in, long st, long sm, int dtype, int S
   MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");
   MM_CHECK_ARG(S >= 0 && k >= 1 && M >= 1 && K >= 1 && N >= 1 && E >= 1 && st >= 0 && sm >= 0, "bad sizes");
   if ((long)S * M > MM_EXPERT_MAX_ROWS) return range_error("mm_expert_rows", TOO_MANY_ROWS);
+  if (too_wide(K, N)) return range_error("mm_expert_rows", TOO_WIDE);
   if (S == 0) return MM_OK;
   MM_CHECK_ARG(in && W && offsets && order && out, "a pointer is null");
   const MMRows a{in, W, offsets, order, out, st, sm, k, M, K, N, E};
@@ -519,6 +520,7 @@ extern "C" int mm_expert_few(const void* x, long st, long sm, int dtype, int T, 
     return range_error("mm_expert_few", "more than 65535 rows or components are not supported");
   if (T == 0) return MM_OK;
   if (too_many(F / 16L + 1, 256)) return range_error("mm_expert_few", "output too large for one launch");
+  if (too_wide(D, F)) return range_error("mm_expert_few", TOO_WIDE);
   MM_CHECK_ARG(x && W && experts && y, "a pointer is null");
   const MMFew a{x, W, gates, experts, st, sm, k, M, D, F, E};
 #define CALL(T_)                                                                                             \
@@ -539,6 +541,7 @@ extern "C" int mm_expert_joined(const void* in, long st, long sm, int dtype, int
   MM_CHECK_ARG(T >= 0 && M >= 1 && K >= 1 && N >= 1 && E >= 1 && st >= 0 && sm >= 0, "bad sizes");
   MM_CHECK_ARG(k == 1 || k == 2, "k must be 1 or 2");
   if (M > 64) return range_error("mm_expert_joined", "more than 64 components are not supported");
+  if (too_wide(K, N)) return range_error("mm_expert_joined", TOO_WIDE);
   const int tiles_n = (N + 127) / 128, buckets = k == 1 ? E + 1 : E <= MM_PAIRS_MAX_E ? mm_pair_buckets(E) : 0;
   const int chunk = dtype == MM_F32 && K <= 128 && k == 2 && T ? mm::pairs_chunk((long)T * M, tiles_n, buckets, M) : 0;
   MM_CHECK_ARG(out || dgates, "nothing to compute");
@@ -586,6 +589,7 @@ extern "C" int mm_expert_combine(const float* rows, const float* gates, const in
                                  int M, int N, int E, void* y, hipStream_t stream) {
   MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");
   MM_CHECK_ARG(T >= 0 && k >= 1 && M >= 1 && N >= 1 && E >= 1, "bad sizes");
+  if (too_wide(N, N)) return range_error("mm_expert_combine", TOO_WIDE);
   const long wg = (T * M * ((N + 3) / 4) + 255) / 256;
   if (too_many(wg, 256)) return range_error("mm_expert_combine", "output too large for one launch");
   if (wg == 0) return MM_OK;
@@ -604,6 +608,7 @@ extern "C" int mm_expert_combine_bwd(const float* rows, const float* gates, cons
                                      hipStream_t stream) {
   MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");
   MM_CHECK_ARG(T >= 0 && k >= 1 && M >= 1 && N >= 1 && E >= 1 && st >= 0 && sm >= 0, "bad sizes");
+  if (too_wide(N, N)) return range_error("mm_expert_combine_bwd", TOO_WIDE);
   const long wg = (T + 3) / 4;
   if (too_many(wg, 256)) return range_error("mm_expert_combine_bwd", "too many rows for one launch");
   if (wg == 0) return MM_OK;

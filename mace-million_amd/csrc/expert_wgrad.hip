@@ -252,6 +252,7 @@ int wgrad_chunk(long rows, int D, int F, int E) {
 extern "C" int mm_expert_wgrad_workspace(int S, int M, int D, int F, int E, size_t* bytes) {
   MM_CHECK_ARG(S >= 0 && M >= 1 && D >= 1 && F >= 1 && E >= 1 && bytes, "bad sizes");
   if ((long)S * M > MM_EXPERT_MAX_ROWS) return range_error("mm_expert_wgrad_workspace", TOO_MANY_ROWS);
+  if (too_wide(D, F)) return range_error("mm_expert_wgrad_workspace", TOO_WIDE);
   const long rows = (long)S * M, c = wgrad_chunk(rows, D, F, E);
   *bytes = c ? (size_t)(rows / c + (E < S ? E : S)) * D * F * sizeof(float) : 0;
   return MM_OK;
@@ -265,6 +266,7 @@ extern "C" int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, 
   MM_CHECK_ARG(xt >= 0 && xm >= 0 && yt >= 0 && ym >= 0, "bad strides");
   if (E > MM_EXPERT_MAX_E) return range_error("mm_expert_wgrad", "more than 1024 experts are not supported");
   if ((long)S * M > MM_EXPERT_MAX_ROWS) return range_error("mm_expert_wgrad", TOO_MANY_ROWS);
+  if (too_wide(D, F)) return range_error("mm_expert_wgrad", TOO_WIDE);
   MM_CHECK_ARG(offsets && dW && (S == 0 || (x && dy && order)), "a pointer is null");
   const MMWgrad a{x, dy, gates, offsets, order, dW, xt, xm, yt, ym, k, M, D, F, E};
   const int chunk = wgrad_chunk((long)S * M, D, F, E);

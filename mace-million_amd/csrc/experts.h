@@ -383,6 +383,8 @@ inline int range_error(const char* name, const char* what) {
 }
 
 constexpr char TOO_MANY_ROWS[] = "more than 2^31 - 2^16 rows are not supported";
+constexpr char TOO_WIDE[] = "blocks of more than 2^31 - 2^16 rows or columns are not supported";
+inline bool too_wide(long a, long b) { return a > MM_EXPERT_MAX_ROWS || b > MM_EXPERT_MAX_ROWS; }
 
 // a launch takes fewer than 2^32 threads
 inline bool too_many(long workgroups, long threads) { return workgroups * threads >= 4294967296L; }

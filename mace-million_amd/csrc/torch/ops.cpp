@@ -585,7 +585,7 @@ Tensor expert_linear(const Tensor& x1, const Tensor& weight1, const Maybe& gates
   if (weight.size(0) != E || weight.size(1) != x0.size(-1) || weight.size(1) == 0 || weight.size(2) == 0)
     throw py::value_error(text("weight must be [", E, ", ", x0.size(-1), ", F], got ", weight.sizes()));
   if (x0.dim() == 3 && x0.size(1) == 0) throw py::value_error("x has no components");
-  if (weight.size(1) > kInt32Max || weight.size(2) > kInt32Max) throw py::value_error("weight blocks are too large");
+  if (weight.size(1) > kMaxRows || weight.size(2) > kMaxRows) throw py::value_error("weight blocks are too large");
   Tensor g;
   if (gates) {
     g = plain(*gates);

@@ -4,7 +4,7 @@ import os
 
 import pytest
 from test_experts_host import ROUTE, ROUTE_BWD
-from test_experts_null_host import FEW, JOINED, ROWS, WGRAD
+from test_experts_null_host import COMBINE, COMBINE_BWD, FEW, JOINED, ROWS, WGRAD
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB = os.path.join(ROOT, "mace-million_amd", "lib", "libmace_million_amd.so")
@@ -48,3 +48,13 @@ def test_partial_sums_of_the_longest_lists(S, M, D, F, E):
     assert _lib.lib().mm_expert_wgrad_workspace(S, M, D, F, E, ctypes.byref(n)) == 0
     assert D * F * 4 <= n.value <= (1024 + E) * D * F * 4
     assert _lib.lib().mm_expert_wgrad_workspace(MOST + 1, 1, D, F, E, ctypes.byref(n)) == -3
+
+
+@pytest.mark.parametrize("name,base,widths", [
+    ("mm_expert_rows", ROWS, "KN"), ("mm_expert_joined", JOINED, "KN"), ("mm_expert_few", FEW, "D"),
+    ("mm_expert_combine", COMBINE, "N"), ("mm_expert_combine_bwd", COMBINE_BWD, "N"), ("mm_expert_wgrad", WGRAD, "DF")])
+def test_widths(name, base, widths):
+    """An index a tile past the last column still fits an int."""
+    for w in widths:
+        for n in (MOST + 1, 2 ** 31 - 1):
+            _refused(name, dict(base, **{w: n}), "2^31 - 2^16 rows or columns")
