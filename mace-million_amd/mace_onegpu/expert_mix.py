@@ -42,6 +42,9 @@ class ExpertMix(torch.nn.Module):
         self.register_buffer("balance", torch.zeros(n_experts, device=device))
         self.plan = None        # of the last call
 
+    def __getstate__(self):     # copies and saved modules go without it
+        return dict(super().__getstate__(), plan=None)
+
     def forward(self, h, by=None):
         n_comp = sum(2 * l + 1 for l in self.ls)
         C = self.blocks[0].shape[1]
