@@ -334,11 +334,13 @@ Lists make_pairs(const Tensor& experts, long E) {
   return {buf.narrow(0, 0, buckets), buf.narrow(0, buckets, T)};
 }
 
-// the graph capture that the current stream is part of
-std::optional<unsigned long long> capture() {
+hipStream_t raw_stream() { return c10::hip::getCurrentHIPStream().stream(); }
+
+// the graph capture that a stream is part of
+std::optional<unsigned long long> capture(hipStream_t s = raw_stream()) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   unsigned long long id = 0;
-  C10_HIP_CHECK(hipStreamGetCaptureInfo(c10::hip::getCurrentHIPStream().stream(), &status, &id));
+  C10_HIP_CHECK(hipStreamGetCaptureInfo(s, &status, &id));
   if (status == hipStreamCaptureStatusNone) return std::nullopt;
   return id;
 }
@@ -353,10 +355,10 @@ c10::Stream current_stream(const Tensor& t) {
 // more only those that use several streams, 5 - 12 us of the GPU).  Under graph capture the slots are sorted at once, so
 // that a captured plan follows every replay.  Outside that capture such a plan is sorted anew by every call: its experts
 // change with the replays, and what its graph sorted holds nothing before the first.  A capture takes the lists that an
-// older plan has, if they are there; those it has to sort are its own and are not kept.
+// older plan has from a stream outside the capture; those it has to sort are its own and are not kept.
 struct Plan {
   struct Kept {
-    c10::Stream stream;
+    hipStream_t stream;
     Lists lists;
   };
   Tensor experts;
@@ -386,13 +388,16 @@ struct Plan {
 
   template <typename F>
   Lists keep(std::vector<Kept>& kept, F make) {
-    const c10::Stream s = current_stream(experts);
-    if (made_in || capture()) {
-      if (kept.empty() || kept.back().stream == s) return make(experts, E);
-      // a capture cannot wait for work outside it, so the host does
+    const hipStream_t s = raw_stream();
+    if (made_in) return make(experts, E);
+    if (capture()) {
       const c10::hip::HIPStreamCaptureModeGuard relaxed(hipStreamCaptureModeRelaxed);
-      c10::impl::VirtualGuardImpl(s.device_type()).synchronizeStream(kept.back().stream);
-      return kept.back().lists;
+      for (const Kept& q : kept) {
+        if (q.stream == s || capture(q.stream)) continue;
+        C10_HIP_CHECK(hipStreamSynchronize(q.stream));   // a capture cannot wait for work outside it: the host does
+        return q.lists;
+      }
+      return make(experts, E);
     }
     for (const Kept& q : kept)
       if (q.stream == s) return q.lists;
