@@ -362,7 +362,8 @@ int mm_expert_plan_pairs(const int* experts, int T, int E, int* offsets, int* or
 /* out [T, M, N] (of in's type, rows without an expert 0) = sum over the k = 1 or 2 choices of gate in[t, m] @ W[e] (W
  * as in mm_expert_rows), joined before they are written; offsets and order of mm_expert_plan (k = 1) or
  * mm_expert_plan_pairs (k = 2).  dgates [T, k] nullable: with in = dy and W transposed, sum_m <x[t, m], dy[t, m] @
- * W[e]^T>, N <= 128, and either k = 1 or float, K <= 128 and M <= 16 (out then nullable).  M <= 64 */
+ * W[e]^T>, N <= 128, and either k = 1 or float, K <= 128 and M <= 16 (out then nullable).  M <= 64.  Two choices of
+ * float with K > 128 or M > 16 multiply in by the gates first, which must stay below 3.396e38 */
 int mm_expert_joined(const void* in, long st, long sm, int dtype, int T, int k, int M, int K, int N, const void* W,
                      int transposed, int E, const float* gates, const int* experts, const int* offsets,
                      const int* order, void* out, const void* x, long xt, long xm, float* dgates, mm_stream_t stream);

@@ -277,10 +277,10 @@ __global__ void __launch_bounds__(256, 2) mm_expert_joined_kernel(MMJoined a, in
 // ------------------------------------------------------------------------------------------------ few rows
 // y[t, m] straight from the choices of row t, without a plan: a workgroup takes LC vectors of columns, its other
 // threads share the sum over d, W is read once per row, coalesced along the columns, fp32 sums.  float operands that
-// round to infinity in bfloat16 give NaN, as they do in the split operands of many rows.  Bound by latency: the sum over
-// d is split as far as the workgroup goes, and the columns over many workgroups, with no branch between the loads (a
-// check for cut vectors among them took 16 us instead of 8 for 1 row 1024 -> 1024 bfloat16, 4 of 64; 1 row 128 -> 128
-// float, k = 2: 3.5 us; 64 rows 64 -> 64: 3.4 us).
+// round to infinity in bfloat16 give NaN, as they do in the split operands of many rows.  Bound by latency: the sum
+// over d is split as far as the workgroup goes, and the columns over many workgroups, with no branch between the loads
+// (a check for cut vectors among them took 16 us instead of 8 for 1 row 1024 -> 1024 bfloat16, 4 of 64; 1 row 128 ->
+// 128 float, k = 2: 3.5 us; 64 rows 64 -> 64: 3.4 us).
 struct MMFew {
   const void *x, *W;
   const float* gates;

@@ -13,7 +13,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));   // 16 bytes known to be float-aligned only
 
 #define MM_EXPERT_MAX_E 1024
-#define MM_EXPERT_MAX_ROWS (2147483648L - 65536)   // rows (slots x M); indices within a tile or stage past them fit an int
+#define MM_EXPERT_MAX_ROWS (2147483648L - 65536)   // rows (slots x M); an index a tile or stage past them fits an int
 #define MM_PAIRS_MAX_E 21   // 253 pairs
 #define MM_HELD_ROWS 1024   // rows of a workgroup with its blocks in registers, at most
 

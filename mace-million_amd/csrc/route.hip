@@ -4,11 +4,11 @@
 //     chosen: the k largest keys, ties to the lowest index; expert -1 and gate 0 where no open expert is left
 //     score: softmax over the E logits, or sigmoid of each
 //     gate_j = scale score_j / sum_chosen score, or scale score_j
-// The bias moves the choice only, not the gates.  It is added to the logits: one rounded addition, so the choice does not
-// depend on the order of a sum or the rounding of an exponential, and saturated sigmoids do not tie.  This is a rule of
-// its own: with a bias that differs between experts, score + bias (or a group's key from the sum of its two best)
-// orders them otherwise, so a router trained with that rule chooses other experts here; without a bias the orders are
-// the same.  Renormalised gates are a softmax over the chosen of the scores' logarithms (of the logits, or of log
+// The bias moves the choice only, not the gates.  It is added to the logits: one rounded addition, so the choice does
+// not depend on the order of a sum or the rounding of an exponential, and saturated sigmoids do not tie.  This is a
+// rule of its own: with a bias that differs between experts, score + bias (or a group's key from the sum of its two
+// best) orders them otherwise, so a router trained with that rule chooses other experts here; without a bias the orders
+// are the same.  Renormalised gates are a softmax over the chosen of the scores' logarithms (of the logits, or of log
 // sigmoid), so that scores that all underflow still give gates of sum scale.  A NaN logit is chosen first and makes the
 // gates of its row NaN (of plain sigmoids: its own gate).
 // A row lies in LPR lanes, C consecutive logits each; k rounds of a maximum over the lanes' best keys (as integers of

@@ -95,8 +95,8 @@ bool needs_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
-// Forward-mode derivatives and traces go through dispatched operations only, so they would miss these functions without a
-// word: the result would pass for a constant, the trace for memory that nothing writes.
+// Forward-mode derivatives and traces go through dispatched operations only, so they would miss these functions without
+// a word: the result would pass for a constant, the trace would hold memory that nothing writes.
 void refuse_modes(const char* what, std::initializer_list<const Tensor*> ts) {
   if (torch::jit::tracer::isTracing()) throw std::runtime_error(text(what, " cannot be traced (torch.jit.trace)"));
   for (const Tensor* t : ts)
@@ -352,10 +352,10 @@ c10::Stream current_stream(const Tensor& t) {
 // The sorts wait until a product (or the caller) needs one: few rows need none, and rows of two choices may need the
 // pairs' instead of the slots'.  The caller cannot see which call sorts and so cannot order another stream behind it:
 // every stream sorts its own lists (an event for each sort costs every training call 5 us of the host, sorting once
-// more only those that use several streams, 5 - 12 us of the GPU).  Under graph capture the slots are sorted at once, so
-// that a captured plan follows every replay.  Outside that capture such a plan is sorted anew by every call: its experts
-// change with the replays, and what its graph sorted holds nothing before the first.  A capture takes the lists that an
-// older plan has from a stream outside the capture; those it has to sort are its own and are not kept.
+// more only those that use several streams, 5 - 12 us of the GPU).  Under graph capture the slots are sorted at once,
+// so that a captured plan follows every replay.  Outside that capture such a plan is sorted anew by every call: its
+// experts change with the replays, and what its graph sorted holds nothing before the first.  A capture takes the lists
+// that an older plan has from a stream outside the capture; those it has to sort are its own and are not kept.
 struct Plan {
   struct Kept {
     hipStream_t stream;
@@ -370,8 +370,8 @@ struct Plan {
   std::vector<c10::Stream> streams;   // that the allocator knows to use experts, which may be the plan's own copy
 
   // The lists and the experts are read together, and experts may be the caller's tensor: one that was written since the
-  // plan was made is refused instead of being read beside older lists.  (A replay changes the experts of a captured plan
-  // with its lists, and elsewhere such a plan is sorted anew; tensors of inference mode have no version.)
+  // plan was made is refused instead of being read beside older lists.  (A replay changes the experts of a captured
+  // plan with its lists, and elsewhere such a plan is sorted anew; tensors of inference mode have no version.)
   void check() {
     if (experts.is_inference() || (made_in && made_in != capture())) return;
     if ((long)experts._version() != version)

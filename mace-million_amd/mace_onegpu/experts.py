@@ -40,8 +40,8 @@ def plan_experts(experts, n_experts):
     """The plan of experts [T, k] (int32 or int64; -1 for none), n_experts up to 1024, for expert_linear: a stable
     counting sort of the slots s = t k + j by expert.  A contiguous int32 tensor is not copied: it is read again by
     every product, and a plan whose experts were changed in place raises RuntimeError (under torch.inference_mode, where
-    tensors carry no version, it cannot: leave them alone there).  Its fields (tensors are not to be changed: the kernels
-    trust them):
+    tensors carry no version, it cannot: leave them alone there).  Its fields (tensors are not to be changed: the
+    kernels trust them):
 
     experts int32 [T, k], n_experts
     order int32 [T k], offsets int32 [n_experts + 1]: the slots of expert e are order[offsets[e] : offsets[e + 1]], in
