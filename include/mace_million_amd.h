@@ -390,6 +390,24 @@ int mm_expert_wgrad(const void* x, long xt, long xm, const void* dy, long yt, lo
                     int D, int F, int E, const float* gates, const int* offsets, const int* order, void* dW,
                     float* workspace, mm_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------- training of heads
+ * Group norm with an activation, linear cross entropy, Newton-Schulz orthogonalisation (no counterpart in the
+ * reference); dtype codes as above. */
+/* y = act((x - mean) rstd w + b), mean and variance over the rows of a structure and the C / groups channels of a group
+ * (at most 16384 bytes, -3 beyond).  rows < 2^31 - 2^16 rows of C channels, in `structs` structures: of equal size, or
+ * (offsets, int [structs + 1], ascending) rows offsets[s] .. offsets[s + 1]; y of rows outside them is 0.  act 0 none, 1
+ * silu, 2 gelu (erf).  stats [structs][groups][2] (mean, rstd): for the backward, nullable where the workspace is empty;
+ * workspace: of mm_groupnorm_workspace bytes (0: null) */
+int mm_groupnorm_workspace(long rows, int structs, int ragged, int C, int groups, int dtype, int backward,
+                           size_t* bytes /* HOST */);
+int mm_groupnorm_fwd(const void* x, long ldx, int dtype, long rows, int structs, const int* offsets, int C, int groups,
+                     const void* w, const void* b, int p_dtype, float eps, int act, void* y, long ldy, float* stats,
+                     float* workspace, mm_stream_t stream);
+/* dx (0 in rows outside the structures), dw, db [C] of p_dtype: each nullable */
+int mm_groupnorm_bwd(const void* dy, long lddy, const void* x, long ldx, int dtype, long rows, int structs,
+                     const int* offsets, int C, int groups, const void* w, const void* b, int p_dtype, int act,
+                     const float* stats, void* dx, long lddx, void* dw, void* db, float* workspace, mm_stream_t stream);
+
 /* ---------------------------------------------------------------------------------------------- utilities */
 int mm_fill_f32(float* p, long n, float v, mm_stream_t stream);
 int mm_fill_f64(double* p, long n, double v, mm_stream_t stream);

@@ -85,31 +85,38 @@ def _count_ops(name):
 
 
 TORCH_OPS = os.path.join(LIB_DIR, "mm_torch_ops.so")
+TORCH_SOURCES = ("ops", "train")
 
 
 def _build_torch_ops():
-    """lib/mm_torch_ops.so: csrc/torch/ops.cpp, host C++ against the installed torch (linked by _link_torch_ops)."""
+    """lib/mm_torch_ops.so: csrc/torch/*.cpp, host C++ against the installed torch (linked by _link_torch_ops)."""
     import sysconfig
 
     import torch
 
     root = os.path.dirname(torch.__file__)
-    obj = os.path.join(OBJ, "torch_ops.o")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+    base = ["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I" + os.path.join(root, "include"),
            "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-I" + os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include"),
-           "-I" + sysconfig.get_paths()["include"], "-c", os.path.join(CSRC, "torch", "ops.cpp"), "-o", obj]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
-    return obj, os.path.join(root, "lib")
+           "-I" + sysconfig.get_paths()["include"]]
+
+    def one(name):
+        obj = os.path.join(OBJ, f"torch__{name}.o")
+        cmd = base + ["-c", os.path.join(CSRC, "torch", name + ".cpp"), "-o", obj]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+        return obj
+
+    with ThreadPoolExecutor(len(TORCH_SOURCES)) as ex:
+        return list(ex.map(one, TORCH_SOURCES)), os.path.join(root, "lib")
 
 
-def _link_torch_ops(obj, torch_lib):
+def _link_torch_ops(objs, torch_lib):
     tmp = TORCH_OPS + ".tmp"
-    cmd = ["g++", "-shared", "-o", tmp, obj, "-L" + LIB_DIR, "-l:" + os.path.basename(LIB), "-L" + torch_lib,
+    cmd = ["g++", "-shared", "-o", tmp] + objs + ["-L" + LIB_DIR, "-l:" + os.path.basename(LIB), "-L" + torch_lib,
            "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

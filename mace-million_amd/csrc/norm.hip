@@ -9,7 +9,7 @@
 // partial sums, and a second launch adds the workgroups' in a fixed order: no atomics, so the gradients are the same
 // in every run.  Measured: 1,474,560 float rows of 64: forward 147 us (5.1 TB/s), backward 225 + 5 us (5.0 TB/s);
 // 8,191 bfloat16 rows of 4096: 32 us (4.2 TB/s) and 44 + 11 us (the partial sums are a sixth of the traffic there).
-#include "rowvec.h"
+#include "norm.h"
 
 #define MM_NORM_MAX_D 16384
 #define MM_NORM_WG 1024   // workgroups of the backward (partial sums of dw and db)
@@ -27,20 +27,6 @@ __device__ __forceinline__ float mm_norm_sum(float v, float* s) {
 #pragma unroll
     for (int w = 0; w < LPR / 64; ++w) t += s[w];
     return t;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void mm_norm_param(const void* p, int pdtype_f32, float none, int c, int D, float* v) {
-  constexpr int N = MMVec<T>::N;
-  if (!p) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = none;
-  } else if (pdtype_f32) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = c + i < D ? ((const float*)p)[c + i] : 0.f;
-  } else {
-    mm_load_vec((const T*)p, c, D, v);
   }
 }
 
@@ -252,6 +238,13 @@ int bwd_workgroups(long rows, int D, int dtype) {
 }
 }  // namespace
 
+namespace mm {
+void sum_partials(const float* part, int n_part, int D, int out_dtype, void* dw, void* db, hipStream_t stream) {
+  hipLaunchKernelGGL(mm_layernorm_sum_kernel, dim3((D + 15) / 16, 2), dim3(1024), 0, stream, part, n_part, D, out_dtype,
+                     dw, db);
+}
+}  // namespace mm
+
 #define MM_NORM_SHAPES(X) X(0, 4, 1) X(1, 8, 1) X(2, 16, 1) X(3, 32, 1) X(4, 64, 1) X(5, 64, 2) X(6, 64, 4) \
   X(7, 256, 1) X(8, 256, 2) X(9, 256, 4) X(10, 1024, 2) X(11, 1024, 4)
 
@@ -305,8 +298,6 @@ extern "C" int mm_layernorm_bwd(const void* dy, long lddy, const void* x, long l
                        lddx, part);
   if (n && (dx || part)) MM_DISPATCH(dtype, MM_NORM_SHAPES(X));
 #undef X
-  if (dw || db)
-    hipLaunchKernelGGL(mm_layernorm_sum_kernel, dim3((D + 15) / 16, 2), dim3(1024), 0, stream, workspace, n, D, p_dtype,
-                       dw, db);
+  if (dw || db) mm::sum_partials(workspace, n, D, p_dtype, dw, db, stream);
   return mm::launch_status("mm_layernorm_bwd");
 }

@@ -105,6 +105,10 @@ SIGNATURES = {
     "mm_expert_combine_bwd": [P, P, P, P, L, L, I, L, I, I, I, I, P, P, P],
     "mm_expert_wgrad_workspace": [I, I, I, I, I, P],
     "mm_expert_wgrad": [P, L, L, P, L, L, I, I, I, I, I, I, I, P, P, P, P, P, P],
+    # training of heads: group norm, linear cross entropy, Newton-Schulz orthogonalisation
+    "mm_groupnorm_workspace": [L, I, I, I, I, I, I, P],
+    "mm_groupnorm_fwd": [P, L, I, L, I, P, I, I, P, P, I, F, I, P, L, P, P, P],
+    "mm_groupnorm_bwd": [P, L, P, L, I, L, I, P, I, I, P, P, I, I, P, P, L, P, P, P, P],
     # tables
     "mm_radial_mlp_f64": [I, P, P, P, P, P, I, I, I, D, I, D, P, P],
     "mm_spline_coeffs": [P, I, I, D, D, I, I, P, P],
