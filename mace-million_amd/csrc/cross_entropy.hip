@@ -1,0 +1,725 @@
+// Cross entropy of linear logits, without keeping them:
+//     l[t, v] = x[t] . W[v],  lse[t] = log sum_v exp(l[t, v]),  loss[t] = lse[t] - l[t, y[t]]
+//     d[t, v] = exp(l[t, v] - lse[t]) - [v = y[t]]:  dx[t] = g[t] d[t] W,  dW = sum_t g[t] d[t]^T x[t]
+// Rows whose target is ignored are taken out at the start: `list` has the asked rows in their order, and everything
+// runs over their number, which stays on the GPU.
+// Forward: tiles of logits in registers, of which every row's maximum, sum of exponentials and target's logit go out.
+// Backward: pieces of the vocabulary; the logits of a piece are taken again and become d, stored in 16 bits by rows
+// and transposed, and two products give the piece's part of dx (kept in fp32 over the pieces) and its rows of dW.
+// Bound by the matrix cores: 2 T D V operations forward, 6 T D V backward.
+//
+// Operands (nt.h): 16-bit types as they are; float as three bfloat16 planes (six products, fp32 accuracy).  d is rounded
+// to the type (relative error 2^-9 in bfloat16, 2^-12 in float16, of each of the many terms of dx and dW, as the
+// operands themselves are); in float16 it is scaled by 2^14 first, so that probabilities down to 2^-28 keep all their
+// bits and none above 2^-39 vanishes.  The incoming gradient g stays out of d in dx (applied in fp32 at the end) and
+// enters the transposed d as g / max|g|.  All sums are fp32 and in a fixed order.
+#include "nt.h"
+
+#define MM_CE_SUM 1
+#define MM_CE_MEAN 2
+
+namespace {
+// int buffer of a call: [0] number of asked rows, then list [T], y [T] (of the asked rows), pos [T] (-1: ignored)
+struct Rows {
+  int *count, *list, *y, *pos;
+};
+Rows rows_of(int* buf, long T) { return Rows{buf, buf + 4, buf + 4 + T, buf + 4 + 2 * T}; }
+}  // namespace
+
+#define MM_CE_SCAN 16   // rows of a thread
+
+template <typename Y>
+__device__ __forceinline__ int mm_ce_asked(const Y* __restrict__ y, long t, long T, long ignore) {
+  return t < T && (long)y[t] != ignore;
+}
+
+// asked rows of every 1024 x 16
+template <typename Y>
+__global__ void __launch_bounds__(1024) mm_ce_count_kernel(const Y* __restrict__ y, long T, long ignore,
+                                                           int* __restrict__ counts) {
+  __shared__ float s[16];
+  const long t0 = ((long)blockIdx.x * 1024 + threadIdx.x) * MM_CE_SCAN;
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < MM_CE_SCAN; ++i) n += mm_ce_asked(y, t0 + i, T, ignore);
+  const float w = mm_lanes_sum<64>((float)n);   // exact: below 2^24
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = w;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = 0.f;
+    for (int i = 0; i < 16; ++i) t += s[i];
+    counts[blockIdx.x] = (int)t;
+  }
+}
+
+// list, y, pos and the count; loss (nullable): 0 for ignored rows.  A target outside [0, V) becomes -1.
+template <typename Y>
+__global__ void __launch_bounds__(1024) mm_ce_list_kernel(const Y* __restrict__ y, long T, int V, long ignore,
+                                                          const int* __restrict__ counts, int* __restrict__ count,
+                                                          int* __restrict__ list, int* __restrict__ yc,
+                                                          int* __restrict__ pos, float* __restrict__ loss) {
+  __shared__ int s[16], s_before[16];
+  const long t0 = ((long)blockIdx.x * 1024 + threadIdx.x) * MM_CE_SCAN;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int n = 0, before = 0;
+#pragma unroll
+  for (int i = 0; i < MM_CE_SCAN; ++i) n += mm_ce_asked(y, t0 + i, T, ignore);
+  for (int b = threadIdx.x; b < (int)blockIdx.x; b += 1024) before += counts[b];
+  int inc = n;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(inc, d);
+    if (lane >= d) inc += u;
+    before += __shfl_xor(before, d);
+  }
+  if (lane == 63) s[wave] = inc;
+  if (lane == 0) s_before[wave] = before;
+  __syncthreads();
+  int at = inc - n, all = 0;
+  for (int w = 0; w < 16; ++w) {
+    at += s_before[w] + (w < wave ? s[w] : 0);
+    all += s_before[w] + s[w];
+  }
+  for (int i = 0; i < MM_CE_SCAN; ++i) {
+    const long t = t0 + i;
+    if (t >= T) break;
+    const long v = (long)y[t];
+    if (v != ignore) {
+      list[at] = (int)t;
+      yc[at] = v >= 0 && v < V ? (int)v : -1;
+      pos[t] = at++;
+    } else {
+      pos[t] = -1;
+      if (loss) loss[t] = 0.f;
+    }
+  }
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *count = all;
+}
+
+// ------------------------------------------------------------------------------------------------ operands
+// Values of T as planes of H: three for float, one otherwise.
+template <typename T>
+struct MMCeType {
+  typedef T H;
+  static constexpr int P = 1, PLANES = 1;
+};
+template <>
+struct MMCeType<float> {
+  typedef __bf16 H;
+  static constexpr int P = 6, PLANES = 3;
+};
+
+template <typename T>
+__device__ __forceinline__ void mm_ce_put4(typename MMCeType<T>::H* __restrict__ p, long plane, const float* v) {
+  typedef typename MMCeType<T>::H H;
+  typedef H vec __attribute__((ext_vector_type(4)));
+  float r[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int q = 0; q < MMCeType<T>::PLANES; ++q) {
+    vec h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[i] = (H)r[i];
+      r[i] -= (float)h[i];
+    }
+    *(vec*)(p + q * plane) = h;
+  }
+}
+
+struct MMPack {
+  const void* src;          // [.., cols], rows ld apart
+  const int *list, *count;  // rows list[0 .. *count) of src, or (null) rows row0 .. row0 + rows
+  void *out, *outT;         // planes [rows, ldo] and [cols, ldt], each nullable; zeros past the last column (row)
+  long ld, row0, ldo, ldt, plane, planeT;
+  int rows, cols;
+};
+
+// 64 x 64 values a workgroup
+template <typename T>
+__global__ void __launch_bounds__(256) mm_ce_pack_kernel(MMPack a) {
+  typedef typename MMCeType<T>::H H;
+  __shared__ float s[64][65];
+  const int rows = a.count ? *a.count : a.rows, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  if (r0 >= mm_up(rows, 64)) return;
+  const int q = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = q + 16 * k;
+    float v[4] = {};
+    if (r0 + r < rows) {
+      const long at = a.list ? a.list[r0 + r] : a.row0 + r0 + r;
+      mm_load4((const T*)a.src + at * a.ld, c0 + c, a.cols, v);
+      if (a.out) mm_ce_put4<T>((H*)a.out + (long)(r0 + r) * a.ldo + c0 + c, a.plane, v);
+    }
+    if (a.outT) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[r][c + i] = v[i];
+    }
+  }
+  if (!a.outT) return;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int col = q + 16 * k;
+    if (c0 + col >= a.cols) continue;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = s[c + i][col];
+    mm_ce_put4<T>((H*)a.outT + (long)(c0 + col) * a.ldt + r0 + c, a.planeT, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ logits
+struct MMCeRow {
+  float top, sum;   // sum of exp(l - top)
+};
+
+__device__ __forceinline__ MMCeRow mm_ce_join(MMCeRow a, MMCeRow b) {
+  const float top = fmaxf(a.top, b.top);
+  if (top == -INFINITY) return MMCeRow{top, a.sum + b.sum};   // nothing yet, or -inf alone
+  return MMCeRow{top, a.sum * __expf(a.top - top) + b.sum * __expf(b.top - top)};
+}
+
+template <typename H>
+struct MMCeLogits {
+  MMNtOperand<H> x, w;
+  const int *count, *y;
+  int V, K;              // K: stages
+  // forward
+  float *part, *picked;  // [tiles of columns][T][2], [T]
+  long T;
+  // backward: columns v0 .. v0 + n
+  const float *lse, *g, *gmax;   // g [asked rows] and max |g|, both null: ones
+  H *d, *dT;                     // [T][ldd], [n][ldt] (planes)
+  long ldd, ldt, plane, planeT;
+  int v0, n;
+  float scale;
+};
+
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2)
+mm_ce_logits_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
+  typedef typename MMCeType<T>::H H;
+  typedef MMNt<H, MMCeType<T>::P, BM, BN, WM, WN> Nt;
+  extern __shared__ uint4 mm_ce_lds[];
+  const int count = *a.count;
+  int e, tm, tn;
+  if (!mm_nt_tile(blockIdx.x, 1, (count + BM - 1) / BM, tiles_n, &e, &tm, &tn)) return;
+  const int m0 = tm * BM, n0 = tn * BN;
+  MMNtOperand<H> x = a.x;
+  x.rows = count;
+  Nt t;
+  t.run(x, m0, a.w, n0, 0, a.K, mm_ce_lds);
+  MMCeRow* s = (MMCeRow*)mm_ce_lds;   // [WN][BM]
+#pragma unroll
+  for (int j = 0; j < Nt::FM; ++j) {
+    const int m = m0 + t.row(j), y = a.y[min(m, count - 1)];
+    MMCeRow r{-INFINITY, 0.f};
+    float hit = 0.f;
+    bool has = false;
+#pragma unroll
+    for (int i = 0; i < Nt::FN; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = n0 + t.col(i) + q;
+        if (n < a.V) r.top = fmaxf(r.top, t.acc[i][j][q]);
+        if (n == y) {
+          hit = t.acc[i][j][q];
+          has = true;
+        }
+      }
+    if (has && m < count) a.picked[m] = hit;
+    const float top = r.top == -INFINITY ? 0.f : r.top;
+#pragma unroll
+    for (int i = 0; i < Nt::FN; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (n0 + t.col(i) + q < a.V) r.sum += __expf(t.acc[i][j][q] - top);
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) r = mm_ce_join(r, MMCeRow{__shfl_xor(r.top, d), __shfl_xor(r.sum, d)});
+    if (t.lane < 16) s[(threadIdx.x >> 6) / WM * BM + t.row(j)] = r;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < BM && m0 + (int)threadIdx.x < count) {
+    MMCeRow r = s[threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < WN; ++w) r = mm_ce_join(r, s[w * BM + threadIdx.x]);
+    float* p = a.part + ((long)tn * a.T + m0 + threadIdx.x) * 2;
+    p[0] = r.top;
+    p[1] = r.sum;
+  }
+}
+
+// 32 rows a workgroup, 8 threads for the tiles of each; lse and the losses; sums [blocks] (nullable): of the losses
+__global__ void __launch_bounds__(256)
+mm_ce_rows_kernel(const float* __restrict__ part, long T, int tiles_n, const int* __restrict__ count,
+                  const int* __restrict__ list, const int* __restrict__ y, const float* __restrict__ picked,
+                  float* __restrict__ lse, float* __restrict__ loss, float* __restrict__ sums) {
+  __shared__ MMCeRow s[8][32];
+  __shared__ float s_loss[32];
+  const int row = threadIdx.x & 31, q = threadIdx.x >> 5, i = blockIdx.x * 32 + row, n = *count;
+  MMCeRow r{-INFINITY, 0.f};
+  if (i < n)
+    for (int t = q; t < tiles_n; t += 8) {
+      const float* p = part + ((long)t * T + i) * 2;
+      r = mm_ce_join(r, MMCeRow{p[0], p[1]});
+    }
+  s[q][row] = r;
+  __syncthreads();
+  if (q) return;
+#pragma unroll
+  for (int t = 1; t < 8; ++t) r = mm_ce_join(r, s[t][row]);
+  float l = 0.f;
+  if (i < n) {
+    const float z = r.top + logf(r.sum);
+    lse[i] = z;
+    l = y[i] < 0 ? __builtin_nanf("") : z - picked[i];
+    if (loss) loss[list[i]] = l;
+  }
+  if (!sums) return;
+  s_loss[row] = l;
+  mm_wave_lds_sync();
+  if (row == 0) {
+    float t = 0.f;
+    for (int k = 0; k < 32; ++k) t += s_loss[k];
+    sums[blockIdx.x] = t;
+  }
+}
+
+// sum (mean) of the blocks' sums
+__global__ void __launch_bounds__(1024) mm_ce_total_kernel(const float* __restrict__ sums, const int* __restrict__ count,
+                                                           int mean, float* __restrict__ loss) {
+  __shared__ double s[16];
+  const int n = *count, blocks = (n + 31) / 32;
+  double t = 0.;
+  for (int i = threadIdx.x; i < blocks; i += 1024) t += (double)sums[i];
+#pragma unroll
+  for (int d = 32; d; d >>= 1) t += __shfl_xor(t, d);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = t;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < 16; ++w) t += s[w];
+  *loss = (float)(mean ? t / (double)max(n, 1) : t);
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// g of the asked rows (none: of every row; else dloss, over the count for the mean) and the largest finite |g|; one
+// workgroup
+__global__ void __launch_bounds__(1024) mm_ce_grad_kernel(const float* __restrict__ dloss, int reduction,
+                                                          const int* __restrict__ count, const int* __restrict__ list,
+                                                          float* __restrict__ g, float* __restrict__ gmax) {
+  __shared__ float s[16];
+  const int n = *count;
+  float top = 0.f;
+  const float all = reduction == 0 ? 0.f : dloss[0] / (reduction == MM_CE_MEAN ? (float)max(n, 1) : 1.f);
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const float v = reduction == 0 ? dloss[list[i]] : all;
+    g[i] = v;
+    if (fabsf(v) < INFINITY) top = fmaxf(top, fabsf(v));
+  }
+  top = mm_lanes_max<64>(top);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < 16; ++w) top = fmaxf(top, s[w]);
+  *gmax = top;
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2)
+mm_ce_d_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
+  typedef typename MMCeType<T>::H H;
+  typedef MMNt<H, MMCeType<T>::P, BM, BN, WM, WN> Nt;
+  extern __shared__ uint4 mm_ce_lds[];
+  const int count = *a.count;
+  int e, tm, tn;
+  if (!mm_nt_tile(blockIdx.x, 1, (count + BM - 1) / BM, tiles_n, &e, &tm, &tn)) return;
+  const int m0 = tm * BM, n0 = tn * BN;
+  MMNtOperand<H> x = a.x;
+  x.rows = count;
+  Nt t;
+  t.run(x, m0, a.w, n0, 0, a.K, mm_ce_lds);
+  const float gmax = *a.gmax;
+  const long rows = mm_up(count, MM_NT_K), cols = mm_up(a.n, MM_NT_K);
+#pragma unroll
+  for (int j = 0; j < Nt::FM; ++j) {
+    const int m = m0 + t.row(j), at = min(m, count - 1), y = a.y[at] - a.v0;
+    const float lse = a.lse[at], r = gmax > 0.f ? a.g[at] / gmax : a.g[at];
+    if (m >= rows) continue;
+#pragma unroll
+    for (int i = 0; i < Nt::FN; ++i) {
+      const int n = n0 + t.col(i);
+      float d[4], dt[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        // a target out of range (loss NaN) makes the row NaN
+        const float p = a.y[at] < 0 ? __builtin_nanf("") : __expf(t.acc[i][j][q] - lse) - (n + q == y ? 1.f : 0.f);
+        d[q] = n + q < a.n && m < count ? p * a.scale : 0.f;
+        dt[q] = n + q < a.n && m < count ? p * a.scale * r : 0.f;
+      }
+      if (m < count && n < cols) mm_ce_put4<T>(a.d + (long)m * a.ldd + n, a.plane, d);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (n + q < a.n) {
+          float v = dt[q];
+#pragma unroll
+          for (int b = 0; b < MMCeType<T>::PLANES; ++b) {
+            const H h = (H)v;
+            a.dT[b * a.planeT + (long)(n + q) * a.ldt + m] = h;
+            v -= (float)h;
+          }
+        }
+    }
+  }
+}
+
+// C = A B^T of a piece.  dx: rows of A are the asked rows (count), fp32 sums part [splits][T][N], added to what is there
+// unless `first`.  dW: the summed index is the asked rows; part [splits][M][N] (written), or with one split the rows of
+// dW themselves, times *gmax / scale.
+template <typename H>
+struct MMCeProduct {
+  MMNtOperand<H> a, b;
+  const int* count;
+  int M, N, K;          // K: stages (dx)
+  int splits, first;
+  float* part;
+  long rows;            // of part
+  void* out;
+  const float* gmax;
+  float inv;
+};
+
+template <typename T, bool DX, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2)
+mm_ce_product_kernel(MMCeProduct<typename MMCeType<T>::H> a, int tiles_n) {
+  typedef typename MMCeType<T>::H H;
+  typedef MMNt<H, MMCeType<T>::P, BM, BN, WM, WN> Nt;
+  extern __shared__ uint4 mm_ce_lds[];
+  const int count = *a.count, M = DX ? count : a.M;
+  const int K = DX ? a.K : (count + MM_NT_K - 1) / MM_NT_K;
+  int e, tm, tn;
+  if (!mm_nt_tile(blockIdx.x, 1, (M + BM - 1) / BM, tiles_n, &e, &tm, &tn)) return;
+  const int m0 = tm * BM, n0 = tn * BN, split = blockIdx.y;
+  MMNtOperand<H> A = a.a;
+  A.rows = M;
+  Nt t;
+  t.run(A, m0, a.b, n0, (int)((long)K * split / a.splits), (int)((long)K * (split + 1) / a.splits), mm_ce_lds);
+  const float f = a.out ? *a.gmax * a.inv : 1.f;
+#pragma unroll
+  for (int j = 0; j < Nt::FM; ++j) {
+    const int m = m0 + t.row(j);
+    if (m >= M) continue;
+#pragma unroll
+    for (int i = 0; i < Nt::FN; ++i) {
+      const int n = n0 + t.col(i);
+      float v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = t.acc[i][j][q];
+      if (!DX && a.out) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] *= f;
+        mm_store4((T*)a.out + (long)m * a.N, n, a.N, v);
+      } else {
+        float* p = a.part + ((long)split * a.rows + m) * a.N;
+        if (DX && !a.first) {
+          float u[4];
+          mm_load4(p, n, a.N, u);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] += u[q];
+        }
+        mm_store4(p, n, a.N, v);
+      }
+    }
+  }
+}
+
+// out = the sum of the splits' sums: dx (pos: row of part, or none: 0; factor g) or dW (factor *gmax)
+template <typename T, bool DX>
+__global__ void __launch_bounds__(256)
+mm_ce_join_kernel(const float* __restrict__ part, int splits, long part_rows, long rows, int N,
+                  const int* __restrict__ pos, const float* __restrict__ g, float inv, T* __restrict__ out) {
+  const int nv = (N + 3) / 4;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < rows * nv; i += (long)gridDim.x * 256) {
+    const long row = i / nv, at = DX ? pos[row] : row;
+    const int c = (int)(i - row * nv) * 4;
+    float v[4] = {};
+    if (at >= 0) {
+      for (int s = 0; s < splits; ++s) {
+        float u[4];
+        mm_load4(part + (s * part_rows + at) * N, c, N, u);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] += u[q];
+      }
+      const float f = (DX ? g[at] : g[0]) * inv;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] *= f;
+    }
+    mm_store4(out + row * N, c, N, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+namespace {
+constexpr long MAX_SIDE = 2147483648L - 65536;
+constexpr int BM = 128, BN = 128;
+constexpr float HALF_SCALE = 16384.f;   // of d in float16
+
+struct Sizes {
+  long T, D, V;
+  int dtype;
+  long Dp, Tp;
+  int planes;
+  bool w_in_place;   // the weights are operands as they are
+  long piece, pieces, piece_p;
+  int dx_splits, dw_splits;
+};
+
+long div_up(long a, long b) { return (a + b - 1) / b; }
+long clamp(long v, long lo, long hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// Workspace regions, 256 bytes apart from each other.
+struct Space {
+  char* base;
+  size_t used = 0;
+  template <typename T>
+  T* take(size_t n) {
+    T* p = base ? (T*)(base + used) : nullptr;
+    used += (n * sizeof(T) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+bool sizes_of(const char* name, long T, long D, long V, int dtype, const void* w, Sizes* s) {
+  if (T > MAX_SIDE || D > MAX_SIDE || V > MAX_SIDE || div_up(T, BM) * div_up(V, BN) * 256 >= 4294967296L ||
+      div_up(T > V ? T : V, 64) * div_up(D, 64) * 256 >= 4294967296L || div_up(D, 64) > 65535) {
+    mm::set_error(std::string(name) + ": sizes beyond the launches' limits");
+    return false;
+  }
+  *s = Sizes{T, D, V, dtype};
+  s->Dp = mm_up(D, MM_NT_K);
+  s->Tp = mm_up(T ? T : 1, MM_NT_K);
+  s->planes = dtype == MM_F32 ? 3 : 1;
+  s->w_in_place = dtype != MM_F32 && D % MM_NT_K == 0 && (size_t)w % 16 == 0;
+  // a piece: d by rows and transposed in 256 MB, but never fewer than 1024 columns
+  const long most = clamp((268435456L / (s->Tp * 4 * s->planes)) / 256 * 256, 1024, 1 << 20);
+  s->pieces = div_up(V, most);
+  s->piece = s->pieces == 1 ? V : mm_up(div_up(V, s->pieces), 256);
+  s->pieces = div_up(V, s->piece);
+  s->piece_p = mm_up(s->piece, MM_NT_K);
+  const long dx_tiles = div_up(T, BM) * div_up(D, BN), dw_tiles = div_up(s->piece, BM) * div_up(D, BN);
+  s->dx_splits = (int)clamp(512 / (dx_tiles ? dx_tiles : 1), 1, clamp(s->piece_p / 512, 1, 64));
+  s->dw_splits = (int)clamp(512 / (dw_tiles ? dw_tiles : 1), 1, clamp(s->Tp / 512, 1, 64));
+  return true;
+}
+
+struct Forward {
+  void *x, *w;
+  float *part, *picked, *sums;
+  int* counts;
+};
+size_t forward_space(const Sizes& s, char* base, Forward* f) {
+  Space p{base};
+  f->x = p.take<short>((size_t)s.planes * s.T * s.Dp);
+  f->w = s.w_in_place ? nullptr : p.take<short>((size_t)s.planes * s.V * s.Dp);
+  f->part = p.take<float>((size_t)div_up(s.V, BN) * s.T * 2);
+  f->picked = p.take<float>(s.T);
+  f->sums = p.take<float>(div_up(s.T, 32));
+  f->counts = p.take<int>(div_up(s.T, 1024 * MM_CE_SCAN));
+  return p.used;
+}
+
+struct Backward {
+  void *x, *xT, *w, *wT, *d, *dT;
+  float *g, *gmax, *dx, *dw;
+};
+size_t backward_space(const Sizes& s, bool dx, bool dw, char* base, Backward* b) {
+  Space p{base};
+  b->x = p.take<short>((size_t)s.planes * s.T * s.Dp);
+  b->xT = dw ? p.take<short>((size_t)s.planes * s.D * s.Tp) : nullptr;
+  b->w = s.w_in_place ? nullptr : p.take<short>((size_t)s.planes * s.piece * s.Dp);
+  b->wT = dx ? p.take<short>((size_t)s.planes * s.D * s.piece_p) : nullptr;
+  b->d = p.take<short>((size_t)s.planes * s.T * s.piece_p);
+  b->dT = p.take<short>((size_t)s.planes * s.piece * s.Tp);
+  b->g = p.take<float>(s.T);
+  b->gmax = p.take<float>(1);
+  b->dx = dx ? p.take<float>((size_t)s.dx_splits * s.T * s.D) : nullptr;
+  b->dw = dw && s.dw_splits > 1 ? p.take<float>((size_t)s.dw_splits * s.piece * s.D) : nullptr;
+  return p.used;
+}
+
+template <typename T>
+void pack(const MMPack& a, long rows, hipStream_t stream) {
+  hipLaunchKernelGGL(mm_ce_pack_kernel<T>, dim3((unsigned)div_up(rows, 64), (unsigned)div_up(a.cols, 64)), dim3(256), 0,
+                     stream, a);
+}
+
+template <typename T>
+int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, float* loss, float* lse,
+            const Forward& f, hipStream_t stream) {
+  typedef typename MMCeType<T>::H H;
+  typedef MMNt<H, MMCeType<T>::P, BM, BN, 2, 2> Nt;
+  if (s.T) {
+    MMPack px{x, r.list, r.count, f.x, nullptr, ldx, 0, s.Dp, 0, s.T * s.Dp, 0, (int)s.T, (int)s.D};
+    pack<T>(px, s.T, stream);
+    if (!s.w_in_place) {
+      MMPack pw{w, nullptr, nullptr, f.w, nullptr, s.D, 0, s.Dp, 0, s.V * s.Dp, 0, (int)s.V, (int)s.D};
+      pack<T>(pw, s.V, stream);
+    }
+    MMCeLogits<H> a{};
+    a.x = MMNtOperand<H>{(const H*)f.x, s.Dp, s.T * s.Dp, 0};
+    a.w = s.w_in_place ? MMNtOperand<H>{(const H*)w, s.D, 0, (int)s.V}
+                       : MMNtOperand<H>{(const H*)f.w, s.Dp, s.V * s.Dp, (int)s.V};
+    a.count = r.count;
+    a.y = r.y;
+    a.V = (int)s.V;
+    a.K = (int)(s.Dp / MM_NT_K);
+    a.part = f.part;
+    a.picked = f.picked;
+    a.T = s.T;
+    const int tiles_n = (int)div_up(s.V, BN);
+    hipLaunchKernelGGL((mm_ce_logits_kernel<T, BM, BN, 2, 2>), dim3((unsigned)(div_up(s.T, BM) * tiles_n)), dim3(256),
+                       Nt::LDS, stream, a, tiles_n);
+    hipLaunchKernelGGL(mm_ce_rows_kernel, dim3((unsigned)div_up(s.T, 32)), dim3(256), 0, stream, f.part, s.T, tiles_n,
+                       r.count, r.list, r.y, f.picked, lse, reduction == 0 ? loss : nullptr,
+                       reduction ? f.sums : nullptr);
+  }
+  if (reduction)
+    hipLaunchKernelGGL(mm_ce_total_kernel, dim3(1), dim3(1024), 0, stream, f.sums, r.count, reduction == MM_CE_MEAN,
+                       loss);
+  return mm::launch_status("mm_ce_fwd");
+}
+
+template <typename T>
+int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, const float* lse,
+             const float* dloss, T* dx, T* dw, const Backward& b, hipStream_t stream) {
+  typedef typename MMCeType<T>::H H;
+  typedef MMNt<H, MMCeType<T>::P, BM, BN, 2, 2> Nt;
+  const float scale = s.dtype == MM_F16 ? HALF_SCALE : 1.f;
+  hipLaunchKernelGGL(mm_ce_grad_kernel, dim3(1), dim3(1024), 0, stream, dloss, reduction, r.count, r.list, b.g, b.gmax);
+  MMPack px{x, r.list, r.count, b.x, b.xT, ldx, 0, s.Dp, s.Tp, s.T * s.Dp, s.D * s.Tp, (int)s.T, (int)s.D};
+  pack<T>(px, s.T, stream);
+  for (long p = 0; p < s.pieces; ++p) {
+    const long v0 = p * s.piece, n = s.V - v0 < s.piece ? s.V - v0 : s.piece, np = mm_up(n, MM_NT_K);
+    MMPack pw{w, nullptr, nullptr, b.w, b.wT, s.D, v0, s.Dp, s.piece_p, s.piece * s.Dp, s.D * s.piece_p, (int)n, (int)s.D};
+    if (b.w || b.wT) pack<T>(pw, n, stream);
+    MMCeLogits<H> a{};
+    a.x = MMNtOperand<H>{(const H*)b.x, s.Dp, s.T * s.Dp, 0};
+    a.w = s.w_in_place ? MMNtOperand<H>{(const H*)w + v0 * s.D, s.D, 0, (int)n}
+                       : MMNtOperand<H>{(const H*)b.w, s.Dp, s.piece * s.Dp, (int)n};
+    a.count = r.count;
+    a.y = r.y;
+    a.K = (int)(s.Dp / MM_NT_K);
+    a.T = s.T;
+    a.lse = lse;
+    a.g = b.g;
+    a.gmax = b.gmax;
+    a.d = (H*)b.d;
+    a.dT = (H*)b.dT;
+    a.ldd = s.piece_p;
+    a.ldt = s.Tp;
+    a.plane = s.T * s.piece_p;
+    a.planeT = s.piece * s.Tp;
+    a.v0 = (int)v0;
+    a.n = (int)n;
+    a.scale = scale;
+    const int tiles_n = (int)div_up(n, BN);
+    hipLaunchKernelGGL((mm_ce_d_kernel<T, BM, BN, 2, 2>), dim3((unsigned)(div_up(s.T, BM) * tiles_n)), dim3(256), Nt::LDS,
+                       stream, a, tiles_n);
+    const int tiles_d = (int)div_up(s.D, BN);
+    if (dx) {
+      MMCeProduct<H> q{};
+      q.a = MMNtOperand<H>{(const H*)b.d, s.piece_p, s.T * s.piece_p, 0};
+      q.b = MMNtOperand<H>{(const H*)b.wT, s.piece_p, s.D * s.piece_p, (int)s.D};
+      q.count = r.count;
+      q.N = (int)s.D;
+      q.K = (int)(np / MM_NT_K);
+      q.splits = s.dx_splits;
+      q.first = p == 0;
+      q.part = b.dx;
+      q.rows = s.T;
+      hipLaunchKernelGGL((mm_ce_product_kernel<T, true, BM, BN, 2, 2>),
+                         dim3((unsigned)(div_up(s.T, BM) * tiles_d), q.splits), dim3(256), Nt::LDS, stream, q, tiles_d);
+    }
+    if (dw) {
+      MMCeProduct<H> q{};
+      q.a = MMNtOperand<H>{(const H*)b.dT, s.Tp, s.piece * s.Tp, 0};
+      q.b = MMNtOperand<H>{(const H*)b.xT, s.Tp, s.D * s.Tp, (int)s.D};
+      q.count = r.count;
+      q.M = (int)n;
+      q.N = (int)s.D;
+      q.splits = s.dw_splits;
+      q.part = b.dw;
+      q.rows = n;
+      q.out = s.dw_splits == 1 ? dw + v0 * s.D : nullptr;
+      q.gmax = b.gmax;
+      q.inv = 1.f / scale;
+      hipLaunchKernelGGL((mm_ce_product_kernel<T, false, BM, BN, 2, 2>),
+                         dim3((unsigned)(div_up(n, BM) * tiles_d), q.splits), dim3(256), Nt::LDS, stream, q, tiles_d);
+      if (s.dw_splits > 1)
+        hipLaunchKernelGGL((mm_ce_join_kernel<T, false>), dim3((unsigned)clamp(div_up(n * div_up(s.D, 4), 256), 1, 4096)),
+                           dim3(256), 0, stream, b.dw, s.dw_splits, n, n, (int)s.D, nullptr, b.gmax, 1.f / scale,
+                           dw + v0 * s.D);
+    }
+  }
+  if (dx)
+    hipLaunchKernelGGL((mm_ce_join_kernel<T, true>), dim3((unsigned)clamp(div_up(s.T * div_up(s.D, 4), 256), 1, 4096)),
+                       dim3(256), 0, stream, b.dx, s.dx_splits, s.T, s.T, (int)s.D, r.pos, b.g, 1.f / scale, dx);
+  return mm::launch_status("mm_ce_bwd");
+}
+}  // namespace
+
+#define MM_CE_CHECK(name)                                                                                    \
+  MM_CHECK_ARG(dtype >= MM_F32 && dtype <= MM_F16, "bad dtype");                                             \
+  MM_CHECK_ARG(T >= 0 && D > 0 && V > 0, "bad sizes");                                                       \
+  Sizes s;                                                                                                   \
+  if (!sizes_of(name, T, D, V, dtype, w, &s)) return MM_ERANGE
+
+extern "C" int mm_ce_workspace(long T, long D, long V, int dtype, const void* w, int dx, int dw, size_t* bytes) {
+  MM_CHECK_ARG(bytes, "no result");
+  MM_CE_CHECK("mm_ce_workspace");
+  Forward f;
+  Backward b;
+  *bytes = dx || dw ? backward_space(s, dx, dw, nullptr, &b) : forward_space(s, nullptr, &f);
+  return MM_OK;
+}
+
+extern "C" int mm_ce_fwd(const void* x, long ldx, int dtype, long T, long D, const void* w, long V, const void* targets,
+                         int targets64, long ignore, int reduction, float* loss, float* lse, int* rows, void* workspace,
+                         hipStream_t stream) {
+  MM_CE_CHECK("mm_ce_fwd");
+  MM_CHECK_ARG(ldx >= 0 && reduction >= 0 && reduction <= 2, "bad reduction");
+  MM_CHECK_ARG(loss && rows && (T == 0 || (x && w && targets && lse && workspace)), "null pointer");
+  Forward f;
+  forward_space(s, (char*)workspace, &f);
+  const Rows r = rows_of(rows, T);
+  const unsigned blocks = T ? (unsigned)div_up(T, 1024 * MM_CE_SCAN) : 1;
+  auto scan = [&](auto y) {
+    if (blocks > 1)
+      hipLaunchKernelGGL((mm_ce_count_kernel<std::remove_const_t<std::remove_pointer_t<decltype(y)>>>), dim3(blocks),
+                         dim3(1024), 0, stream, y, T, ignore, f.counts);
+    hipLaunchKernelGGL((mm_ce_list_kernel<std::remove_const_t<std::remove_pointer_t<decltype(y)>>>), dim3(blocks),
+                       dim3(1024), 0, stream, y, T, (int)V, ignore, f.counts, r.count, r.list, r.y, r.pos,
+                       reduction == 0 ? loss : nullptr);
+  };
+  if (targets64) scan((const long*)targets);
+  else scan((const int*)targets);
+  int rc = MM_OK;
+  MM_DISPATCH(dtype, rc = forward<T_>(s, (const T_*)x, ldx, (const T_*)w, r, reduction, loss, lse, f, stream));
+  return rc;
+}
+
+extern "C" int mm_ce_bwd(const void* x, long ldx, int dtype, long T, long D, const void* w, long V, int reduction,
+                         const float* lse, const int* rows, const float* dloss, void* dx, void* dw, void* workspace,
+                         hipStream_t stream) {
+  MM_CE_CHECK("mm_ce_bwd");
+  MM_CHECK_ARG(ldx >= 0 && reduction >= 0 && reduction <= 2, "bad reduction");
+  MM_CHECK_ARG(T > 0 && x && w && lse && rows && dloss && workspace, "null pointer");
+  if (!dx && !dw) return MM_OK;
+  Backward b;
+  backward_space(s, dx, dw, (char*)workspace, &b);
+  const Rows r = rows_of((int*)rows, T);
+  int rc = MM_OK;
+  MM_DISPATCH(dtype, rc = backward<T_>(s, (const T_*)x, ldx, (const T_*)w, r, reduction, lse, dloss, (T_*)dx, (T_*)dw, b,
+                                       stream));
+  return rc;
+}

@@ -1,0 +1,337 @@
+// Newton-Schulz orthogonalisation of a batch of matrices:
+//     X = M / (|M| + eps),  steps times:  A = X X^T,  X <- a X + (b A + c A A) X     (on the shorter side of M)
+// Each step drives the singular values of X towards 1 by the odd polynomial a s + b s^3 + c s^5.  Bound by the matrix
+// cores: with m <= n the sides, 2 m^2 n + 2 m^3 + 2 m^2 n operations a step.
+//
+// X is carried in fp32 and a X is added in fp32: small singular values, which grow by a in every step, keep its bits.
+// The products take float16 operands, scaled by powers of two (X and A by 2^12, B = b A + c A A by 2^10) into the middle
+// of its range: one plane for bfloat16 matrices (2^-12 of an operand, against 2^-9 of the result's own rounding), two
+// planes and three products (2^-22) for float and float16.  |X| and |A| have to stay below 16, |B| below 64: the norm of
+// M bounds them by 1 and the usual coefficients keep them below 3; what passes them becomes infinite or NaN.
+// Norms are summed in 64 bits, so that neither large nor tiny values leave the range.
+#include "nt.h"
+
+#include <utility>
+
+#define MM_ORTHO_PARTS 64     // partial sums of a matrix's norm, at most
+#define MM_ORTHO_X 4096.f     // scales of the operands
+#define MM_ORTHO_A 4096.f
+#define MM_ORTHO_B 1024.f
+
+template <typename T>
+struct MMOrthoType {
+  static constexpr int P = sizeof(T) == 2 && !__is_same(T, _Float16) ? 1 : 3, PLANES = P == 1 ? 1 : 2;
+};
+
+typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
+
+template <int PLANES>
+__device__ __forceinline__ void mm_ortho_put4(_Float16* __restrict__ p, long plane, const float* v) {
+  halfx4 h[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[0][i] = (_Float16)v[i];
+    h[1][i] = (_Float16)(v[i] - (float)h[0][i]);
+  }
+#pragma unroll
+  for (int q = 0; q < PLANES; ++q) *(halfx4*)(p + q * plane) = h[q];
+}
+
+template <int PLANES>
+__device__ __forceinline__ void mm_ortho_put(_Float16* __restrict__ p, long plane, float v) {
+  const _Float16 h = (_Float16)v;
+  p[0] = h;
+  if constexpr (PLANES == 2) p[plane] = (_Float16)(v - (float)h);
+}
+
+// sums of squares of parts of matrix blockIdx.y
+template <typename T>
+__global__ void __launch_bounds__(256) mm_ortho_norm_kernel(const T* __restrict__ m, long size, double* __restrict__ part) {
+  constexpr int N = MMVec<T>::N;
+  __shared__ double s[4];
+  const T* __restrict__ p = m + (long)blockIdx.y * size;
+  const long nv = (size + N - 1) / N;
+  double t = 0.;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < nv; i += (long)gridDim.x * 256) {
+    const long at = i * N;
+    float v[N];
+    mm_load_vec(p + at, 0, (int)min((long)N, size - at), v);
+#pragma unroll
+    for (int j = 0; j < N; ++j) t = fma((double)v[j], (double)v[j], t);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) t += __shfl_xor(t, d);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) part[(long)blockIdx.y * gridDim.x + blockIdx.x] = s[0] + s[1] + s[2] + s[3];
+}
+
+struct MMOrtho {
+  const void* m;
+  void* out;
+  double* part;
+  float* x;                       // [batch][rows][cols]
+  // planes of [batch]: X [rows][ldu], X^T [cols][ldv], A and B [side][lda]; the one that a step multiplies (X^T if rows
+  // <= cols, else X) is written to `next` meanwhile
+  _Float16 *u, *v, *a, *b, *next;
+  long ldu, ldv, lda, pu, pv, pa;   // pu, pv, pa: distance of planes
+  int batch, rows, cols, side, parts;
+  float ca, cb, cc, eps;
+};
+
+// 64 x 64 values a workgroup: X = M / (|M| + eps) and its planes; out (no steps): X itself
+template <typename T>
+__global__ void __launch_bounds__(256) mm_ortho_start_kernel(MMOrtho a, int steps) {
+  constexpr int PLANES = MMOrthoType<T>::PLANES;
+  __shared__ float s[64][65];
+  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, e = blockIdx.z;
+  const int q = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4;
+  double norm = 0.;
+  for (int i = 0; i < a.parts; ++i) norm += a.part[(long)e * a.parts + i];
+  const double by = 1. / (sqrt(norm) + (double)a.eps);
+  const long size = (long)a.rows * a.cols;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = r0 + q + 16 * k;
+    float v[4] = {};
+    if (r < a.rows) {
+      mm_load4((const T*)a.m + e * size + (long)r * a.cols, c0 + c, a.cols, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = v[i] == 0.f ? v[i] : (float)((double)v[i] * by);   // no norm: zeros stay
+      if (!steps) {
+        mm_store4((T*)a.out + e * size + (long)r * a.cols, c0 + c, a.cols, v);
+      } else {
+        mm_store4(a.x + e * size + (long)r * a.cols, c0 + c, a.cols, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] *= MM_ORTHO_X;
+        mm_ortho_put4<PLANES>(a.u + ((long)e * a.rows + r) * a.ldu + c0 + c, a.pu, v);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[q + 16 * k][c + i] = v[i];
+  }
+  if (!steps) return;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int col = c0 + q + 16 * k;
+    if (col >= a.cols) continue;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = s[c + i][q + 16 * k];
+    mm_ortho_put4<PLANES>(a.v + ((long)e * a.cols + col) * a.ldv + r0 + c, a.pv, v);
+  }
+}
+
+// A = X X^T (WHAT 0) or B = b A + c A A (1): planes [side][lda], zeros past the last column
+template <int P, int WHAT, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2) mm_ortho_square_kernel(MMOrtho a, int tiles) {
+  typedef MMNt<_Float16, P, BM, BN, WM, WN> Nt;
+  constexpr int PLANES = P == 1 ? 1 : 2;
+  extern __shared__ uint4 mm_ortho_lds[];
+  int e, tm, tn;
+  if (!mm_nt_tile(blockIdx.x, a.batch, tiles, tiles, &e, &tm, &tn)) return;
+  MMNtOperand<_Float16> x;
+  int k;
+  if constexpr (WHAT == 1) {
+    x = {a.a + (long)e * a.side * a.lda, a.lda, a.pa, a.side};
+    k = (int)(a.lda / MM_NT_K);
+  } else if (a.rows <= a.cols) {
+    x = {a.u + (long)e * a.rows * a.ldu, a.ldu, a.pu, a.side};
+    k = (int)(a.ldu / MM_NT_K);
+  } else {
+    x = {a.v + (long)e * a.cols * a.ldv, a.ldv, a.pv, a.side};
+    k = (int)(a.ldv / MM_NT_K);
+  }
+  Nt t;
+  t.run(x, tm * BM, x, tn * BN, 0, k, mm_ortho_lds);
+  _Float16* out = (WHAT ? a.b : a.a) + (long)e * a.side * a.lda;
+  const _Float16* in = a.a + (long)e * a.side * a.lda;
+#pragma unroll
+  for (int j = 0; j < Nt::FM; ++j) {
+    const int m = tm * BM + t.row(j);
+    if (m >= a.side) continue;
+#pragma unroll
+    for (int i = 0; i < Nt::FN; ++i) {
+      const int n = tn * BN + t.col(i);
+      if (n >= a.lda) continue;
+      float v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (WHAT == 0) {
+          v[q] = t.acc[i][j][q] * (MM_ORTHO_A / (MM_ORTHO_X * MM_ORTHO_X));
+        } else {
+          const long at = (long)m * a.lda + n + q;
+          const float old = (float)in[at] + (PLANES == 2 ? (float)in[at + a.pa] : 0.f);
+          v[q] = a.cb * (MM_ORTHO_B / MM_ORTHO_A) * old
+               + a.cc * (MM_ORTHO_B / (MM_ORTHO_A * MM_ORTHO_A)) * t.acc[i][j][q];
+        }
+        if (n + q >= a.side) v[q] = 0.f;
+      }
+      mm_ortho_put4<PLANES>(out + (long)m * a.lda + n, a.pa, v);
+    }
+  }
+}
+
+// X <- a X + B X (rows <= cols) or a X + X B; the last step writes out alone.  Other workgroups still read the operand
+// of X's planes: its new values go to a.next.
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2)
+mm_ortho_step_kernel(MMOrtho a, int tiles_m, int tiles_n, int last) {
+  constexpr int P = MMOrthoType<T>::P, PLANES = MMOrthoType<T>::PLANES;
+  typedef MMNt<_Float16, P, BM, BN, WM, WN> Nt;
+  extern __shared__ uint4 mm_ortho_lds[];
+  int e, tm, tn;
+  if (!mm_nt_tile(blockIdx.x, a.batch, tiles_m, tiles_n, &e, &tm, &tn)) return;
+  const MMNtOperand<_Float16> b{a.b + (long)e * a.side * a.lda, a.lda, a.pa, a.side};
+  const bool wide = a.rows <= a.cols;
+  _Float16 *u = wide ? a.u : a.next, *vt = wide ? a.next : a.v;
+  Nt t;
+  if (wide) {
+    const MMNtOperand<_Float16> x{a.v + (long)e * a.cols * a.ldv, a.ldv, a.pv, a.cols};
+    t.run(b, tm * BM, x, tn * BN, 0, (int)(a.lda / MM_NT_K), mm_ortho_lds);
+  } else {
+    const MMNtOperand<_Float16> x{a.u + (long)e * a.rows * a.ldu, a.ldu, a.pu, a.rows};
+    t.run(x, tm * BM, b, tn * BN, 0, (int)(a.lda / MM_NT_K), mm_ortho_lds);
+  }
+#pragma unroll
+  for (int j = 0; j < Nt::FM; ++j) {
+    const int m = tm * BM + t.row(j);
+    if (m >= a.ldv) continue;
+    const long row = ((long)e * a.rows + m) * a.cols;
+#pragma unroll
+    for (int i = 0; i < Nt::FN; ++i) {
+      const int n = tn * BN + t.col(i);
+      if (n >= a.ldu) continue;
+      float v[4] = {};   // zeros past the last row and column
+      if (m < a.rows) {
+        mm_load4(a.x + row, n, a.cols, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          v[q] = n + q < a.cols ? fmaf(t.acc[i][j][q], 1.f / (MM_ORTHO_B * MM_ORTHO_X), a.ca * v[q]) : 0.f;
+        if (last) {
+          mm_store4((T*)a.out + row, n, a.cols, v);
+          continue;
+        }
+        mm_store4(a.x + row, n, a.cols, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] *= MM_ORTHO_X;
+        mm_ortho_put4<PLANES>(u + ((long)e * a.rows + m) * a.ldu + n, a.pu, v);
+      } else if (last) {
+        continue;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (n + q < a.cols) mm_ortho_put<PLANES>(vt + ((long)e * a.cols + n + q) * a.ldv + m, a.pv, v[q]);
+    }
+  }
+}
+
+namespace {
+constexpr int BM = 128, BN = 128;
+constexpr long MAX_SIDE = 65536;
+
+long divtup(long a, long b) { return (a + b - 1) / b; }
+
+struct Space {
+  char* base;
+  size_t used = 0;
+  template <typename T>
+  T* take(size_t n) {
+    T* p = base ? (T*)(base + used) : nullptr;
+    used += (n * sizeof(T) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+size_t space(MMOrtho* a, int dtype, char* base) {
+  Space p{base};
+  const int planes = dtype == MM_BF16 ? 1 : 2;
+  a->side = a->rows < a->cols ? a->rows : a->cols;
+  a->ldu = mm_up(a->cols, MM_NT_K);
+  a->ldv = mm_up(a->rows, MM_NT_K);
+  a->lda = mm_up(a->side, MM_NT_K);
+  a->pu = (long)a->batch * a->rows * a->ldu;
+  a->pv = (long)a->batch * a->cols * a->ldv;
+  a->pa = (long)a->batch * a->side * a->lda;
+  const long parts = divtup((long)a->rows * a->cols, 256 * 32);
+  a->parts = (int)(parts < MM_ORTHO_PARTS ? parts : MM_ORTHO_PARTS);
+  a->part = p.take<double>((size_t)a->batch * a->parts);
+  a->x = p.take<float>((size_t)a->batch * a->rows * a->cols);
+  a->u = p.take<_Float16>(planes * a->pu);
+  a->v = p.take<_Float16>(planes * a->pv);
+  a->a = p.take<_Float16>(planes * a->pa);
+  a->b = p.take<_Float16>(planes * a->pa);
+  a->next = p.take<_Float16>(planes * (a->rows <= a->cols ? a->pv : a->pu));
+  return p.used;
+}
+
+template <typename T>
+int orthogonalize(MMOrtho a, int steps, const float* c, hipStream_t stream) {
+  constexpr int P = MMOrthoType<T>::P;
+  typedef MMNt<_Float16, P, BM, BN, 2, 2> Nt;
+  hipLaunchKernelGGL(mm_ortho_norm_kernel<T>, dim3(a.parts, a.batch), dim3(256), 0, stream, (const T*)a.m,
+                     (long)a.rows * a.cols, a.part);
+  hipLaunchKernelGGL(mm_ortho_start_kernel<T>, dim3((unsigned)divtup(a.rows, 64), (unsigned)divtup(a.cols, 64), a.batch),
+                     dim3(256), 0, stream, a, steps);
+  const int sq = (int)divtup(a.side, BM), tm = (int)divtup(a.rows, BM), tn = (int)divtup(a.cols, BN);
+  for (int i = 0; i < steps; ++i, c += 3) {
+    a.ca = c[0];
+    a.cb = c[1];
+    a.cc = c[2];
+    hipLaunchKernelGGL((mm_ortho_square_kernel<P, 0, BM, BN, 2, 2>), dim3(a.batch * sq * sq), dim3(256), Nt::LDS, stream, a,
+                       sq);
+    hipLaunchKernelGGL((mm_ortho_square_kernel<P, 1, BM, BN, 2, 2>), dim3(a.batch * sq * sq), dim3(256), Nt::LDS, stream, a,
+                       sq);
+    hipLaunchKernelGGL((mm_ortho_step_kernel<T, BM, BN, 2, 2>), dim3(a.batch * tm * tn), dim3(256), Nt::LDS, stream, a, tm,
+                       tn, i + 1 == steps);
+    std::swap(a.next, a.rows <= a.cols ? a.v : a.u);
+  }
+  return mm::launch_status("mm_orthogonalize");
+}
+
+int check(const char* name, long batch, long rows, long cols, int dtype) {
+  if (dtype < MM_F32 || dtype > MM_F16 || batch < 0 || rows <= 0 || cols <= 0) {
+    mm::set_error(std::string(name) + ": bad sizes or dtype");
+    return MM_EINVAL;
+  }
+  if (rows > MAX_SIDE || cols > MAX_SIDE || batch > 65535 ||
+      batch * divtup(rows, 64) * divtup(cols, 64) * 256 >= 4294967296L) {
+    mm::set_error(std::string(name) + ": sizes beyond the launches' limits");
+    return MM_ERANGE;
+  }
+  return MM_OK;
+}
+}  // namespace
+
+extern "C" int mm_orthogonalize_workspace(long batch, long rows, long cols, int dtype, size_t* bytes) {
+  const int rc = check("mm_orthogonalize_workspace", batch, rows, cols, dtype);
+  if (rc != MM_OK) return rc;
+  MM_CHECK_ARG(bytes, "no result");
+  MMOrtho a{};
+  a.batch = (int)batch;
+  a.rows = (int)rows;
+  a.cols = (int)cols;
+  *bytes = space(&a, dtype, nullptr);
+  return MM_OK;
+}
+
+extern "C" int mm_orthogonalize(const void* m, int dtype, long batch, long rows, long cols, int steps,
+                                const float* coefficients, float eps, void* out, void* workspace, hipStream_t stream) {
+  const int rc = check("mm_orthogonalize", batch, rows, cols, dtype);
+  if (rc != MM_OK) return rc;
+  MM_CHECK_ARG(steps >= 0 && (steps == 0 || coefficients) && eps >= 0.f, "bad steps, coefficients or eps");
+  if (batch == 0) return MM_OK;
+  MM_CHECK_ARG(m && out && workspace, "null pointer");
+  MMOrtho a{};
+  a.m = m;
+  a.out = out;
+  a.eps = eps;
+  a.batch = (int)batch;
+  a.rows = (int)rows;
+  a.cols = (int)cols;
+  space(&a, dtype, (char*)workspace);
+  int done = MM_OK;
+  MM_DISPATCH(dtype, done = orthogonalize<T_>(a, steps, coefficients, stream));
+  return done;
+}

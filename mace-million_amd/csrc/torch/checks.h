@@ -7,6 +7,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/sub.h>
+#include <ATen/ops/zeros.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPException.h>

@@ -125,8 +125,136 @@ Tensor group_norm(const Tensor& x0, int64_t groups, const Maybe& weight, const M
   return GroupNormFn::run(x, x2, ldx, w, b, offsets, GroupSizes{rows, structs, C, groups}, eps, (int)act, code, p_code,
                           Tensor());
 }
+
+// ------------------------------------------------------------------------------------------------ cross entropy
+Tensor bytes_like(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
+
+struct LossSizes { long T, D, V; };
+
+struct CrossEntropyFn : torch::autograd::Function<CrossEntropyFn> {
+  struct Result { Tensor loss, lse, rows; };
+
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& targets,
+                        int64_t ignore, int64_t reduction, int64_t code) {
+    auto [x2, ldx] = as_rows(x);
+    const Tensor w = weight.contiguous();
+    Result r = run(x2, ldx, w, targets, ignore, (int)reduction, (int)code);
+    ctx->save_for_backward({x2, w, r.lse, r.rows});
+    ctx->saved_data["args"] = std::vector<int64_t>{reduction, code, x2.size(0), x2.size(1), w.size(0)};
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return r.loss;
+  }
+
+  static Result run(const Tensor& x2, long ldx, const Tensor& w, const Tensor& targets, int64_t ignore, int reduction,
+                    int code) {
+    const LossSizes n{x2.size(0), x2.size(1), w.size(0)};
+    const Tensor y = targets.contiguous();
+    Result r{reduction ? f32({}, x2) : f32(targets.sizes(), x2), f32({n.T}, x2), i32({4 + 3 * n.T}, x2)};
+    size_t bytes = 0;
+    done(mm_ce_workspace(n.T, n.D, n.V, code, ptr(w), 0, 0, &bytes));
+    const Tensor ws = bytes_like(bytes, x2);
+    if (n.T || reduction)
+      done(mm_ce_fwd(ptr(x2), ldx, code, n.T, n.D, ptr(w), n.V, ptr(y), y.scalar_type() == at::kLong, ignore, reduction,
+                     fptr(r.loss), fptr(r.lse), iptr(r.rows), ptr(ws), stream()));
+    return r;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto args = ctx->saved_data["args"].toIntVector();
+    const int reduction = (int)args[0], code = (int)args[1];
+    const LossSizes n{args[2], args[3], args[4]};
+    const Tensor dloss = plain(grads[0]).contiguous();
+    const auto type = type_of(code);
+    auto [x, ldx] = as_rows(unpacked(saved[0], {n.T, n.D}, type, dloss, "x"));
+    const Tensor w = unpacked_dense(saved[1], {n.V, n.D}, type, dloss, "weight");
+    const Tensor lse = unpacked_dense(saved[2], {n.T}, at::kFloat, dloss, "log sums");
+    const Tensor rows = unpacked_dense(saved[3], {4 + 3 * n.T}, at::kInt, dloss, "rows");
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = at::empty(ctx->saved_data["shape"].toIntVector(), x.options());
+    if (ctx->needs_input_grad(1)) dw = n.T ? at::empty({n.V, n.D}, x.options()) : at::zeros({n.V, n.D}, x.options());
+    if (n.T && (dx.defined() || dw.defined())) {
+      size_t bytes = 0;
+      done(mm_ce_workspace(n.T, n.D, n.V, code, ptr(w), dx.defined(), dw.defined(), &bytes));
+      const Tensor ws = bytes_like(bytes, x);
+      done(mm_ce_bwd(ptr(x), ldx, code, n.T, n.D, ptr(w), n.V, reduction, fptr(lse), iptr(rows), fptr(dloss), ptr(dx),
+                     ptr(dw), ptr(ws), stream()));
+    }
+    variable_list out(6);
+    out[0] = dx;
+    out[1] = dw;
+    return once(out, "linear_cross_entropy");
+  }
+};
+
+Tensor linear_cross_entropy(const Tensor& x0, const Tensor& weight0, const Tensor& targets0, int64_t ignore,
+                            const std::string& reduction) {
+  const Tensor x = plain(x0), weight = plain(weight0), targets = plain(targets0);
+  const int code = check_gpu(x, "x");
+  if (check_gpu(weight, "weight") != code)
+    throw py::type_error(text("weight must be ", type_name(x.scalar_type()), " (as x), got ",
+                              type_name(weight.scalar_type())));
+  if (x.dim() < 1 || x.size(-1) == 0) throw py::value_error(text("x must be [..., D] with D > 0, got ", x.sizes()));
+  const long D = x.size(-1), T = x.numel() / D;
+  if (weight.dim() != 2 || weight.size(1) != D || weight.size(0) == 0)
+    throw py::value_error(text("weight must be [classes, ", D, "], got ", weight.sizes()));
+  if (!targets.is_cuda()) throw py::type_error("targets must be a GPU tensor");
+  if (targets.scalar_type() != at::kInt && targets.scalar_type() != at::kLong)
+    throw py::type_error(text("targets must be int32 or int64, got ", type_name(targets.scalar_type())));
+  if (targets.device() != x.device()) throw py::value_error("x and targets must be on one device");
+  if (targets.sizes() != x.sizes().slice(0, x.dim() - 1))
+    throw py::value_error(text("targets must be ", x.sizes().slice(0, x.dim() - 1), ", got ", targets.sizes()));
+  const long V = weight.size(0);
+  if (T >= kMaxRows || V >= kMaxRows || D >= kMaxRows)
+    throw py::value_error(text("sizes of 2^31 - 2^16 or more are not supported, got ", x.sizes(), " and ",
+                               weight.sizes()));
+  int64_t how = 0;
+  if (reduction == "sum") how = 1;
+  else if (reduction == "mean") how = 2;
+  else if (reduction != "none")
+    throw py::value_error(text("reduction must be 'mean', 'sum' or 'none', got '", reduction, "'"));
+  refuse_modes("linear_cross_entropy", {&x, &weight});
+  if (needs_grad({&x, &weight})) return CrossEntropyFn::apply(x, weight, targets, ignore, how, (int64_t)code);
+  auto [x2, ldx] = as_rows(x);
+  return CrossEntropyFn::run(x2, ldx, weight.contiguous(), targets, ignore, (int)how, code).loss;
+}
+
+// ------------------------------------------------------------------------------------------------ orthogonalisation
+// Workspace of a batch taken at once, at most (a larger batch goes in parts).
+constexpr size_t kOrthoBytes = 4294967296UL;
+
+Tensor orthogonalize(const Tensor& m0, const std::vector<float>& coefficients, double eps) {
+  const Tensor m1 = plain(m0);
+  const int code = check_gpu(m1, "m");
+  if (m1.dim() < 2 || m1.size(-1) == 0 || m1.size(-2) == 0)
+    throw py::value_error(text("m must be [..., rows, columns], got ", m1.sizes()));
+  if (coefficients.size() % 3) throw py::value_error("coefficients must be triples (a, b, c)");
+  if (!(eps >= 0.) || !std::isfinite((float)eps)) throw py::value_error(text("eps must be finite and >= 0, got ", eps));
+  const long rows = m1.size(-2), cols = m1.size(-1), batch = m1.numel() / (rows * cols);
+  if (rows > 65536 || cols > 65536)
+    throw py::value_error(text("matrices of more than 65536 rows or columns are not supported, got ", m1.sizes()));
+  refuse_modes("orthogonalize", {&m1});
+  if (needs_grad({&m1}))
+    throw std::runtime_error("orthogonalize has no derivative: call it under torch.no_grad() or on a detached tensor");
+  const Tensor m = m1.contiguous();
+  Tensor out = at::empty(m.sizes(), m.options());
+  if (batch == 0) return out;
+  size_t one = 0, bytes = 0;
+  done(mm_orthogonalize_workspace(1, rows, cols, code, &one));
+  const long part = std::max(1L, std::min({batch, (long)(kOrthoBytes / one), 65535L}));
+  done(mm_orthogonalize_workspace(part, rows, cols, code, &bytes));
+  const Tensor ws = bytes_like(bytes, m);
+  const long step = rows * cols * (long)m.element_size();
+  for (long i = 0; i < batch; i += part)
+    done(mm_orthogonalize((const char*)ptr(m) + i * step, code, std::min(part, batch - i), rows, cols,
+                          (int)(coefficients.size() / 3), coefficients.data(), (float)eps, (char*)ptr(out) + i * step,
+                          ptr(ws), stream()));
+  return out;
+}
 }  // namespace
 
 void bind_train(py::module_& m) {
   m.def("group_norm", &group_norm);
+  m.def("linear_cross_entropy", &linear_cross_entropy);
+  m.def("orthogonalize", &orthogonalize);
 }

@@ -11,6 +11,8 @@ Module map (mirrors the reference package mace_onegpu, same module paths for the
   fast_layers       per-chunk layer pipelines on the HIP kernels
   layer_norm        layer_norm, LayerNorm: forward and backward kernels over the last axis
   group_norm        group_norm, GroupNorm: norm over structures and groups of channels with an activation
+  cross_entropy     linear_cross_entropy: the loss of a linear head over many classes, with its gradient
+  muon              orthogonalize by Newton-Schulz products, and Muon, the optimizer that updates weight blocks with it
   experts           mixtures of expert weight blocks: route, plan_experts, expert_linear
   expert_mix        ExpertMix: a mixture of expert linears on node features, and a command that fits one
   lammps_data       periodic-image ML-IAP data object (one GPU stands in for LAMMPS' ghost exchange)

@@ -109,6 +109,11 @@ SIGNATURES = {
     "mm_groupnorm_workspace": [L, I, I, I, I, I, I, P],
     "mm_groupnorm_fwd": [P, L, I, L, I, P, I, I, P, P, I, F, I, P, L, P, P, P],
     "mm_groupnorm_bwd": [P, L, P, L, I, L, I, P, I, I, P, P, I, I, P, P, L, P, P, P, P],
+    "mm_ce_workspace": [L, L, L, I, P, I, I, P],
+    "mm_ce_fwd": [P, L, I, L, L, P, L, P, I, L, I, P, P, P, P, P],
+    "mm_ce_bwd": [P, L, I, L, L, P, L, I, P, P, P, P, P, P, P],
+    "mm_orthogonalize_workspace": [L, L, L, I, P],
+    "mm_orthogonalize": [P, I, L, L, L, I, P, F, P, P, P],
     # tables
     "mm_radial_mlp_f64": [I, P, P, P, P, P, I, I, I, D, I, D, P, P],
     "mm_spline_coeffs": [P, I, I, D, D, I, I, P, P],
