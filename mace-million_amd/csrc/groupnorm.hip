@@ -54,10 +54,21 @@ __device__ __forceinline__ int mm_group_find(const MMGroup& a, long r) {
   return lo;
 }
 
+// Distribution function of the normal distribution, given e = exp(-z^2 / 2): Hastings' approximation of erf (Abramowitz
+// and Stegun 7.1.26), off by 0.75e-7 at most.  With it the activation shares its one exponential with the derivative; erff
+// and expf bound the backward by their instructions.
+__device__ __forceinline__ float mm_normal(float z, float e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
+                           0.254829592f);
+  const float half = 0.5f * p * e;   // of the tail beyond |z|
+  return z > 0.f ? 1.f - half : half;
+}
+
 template <int ACT>
 __device__ __forceinline__ float mm_act(float z) {
-  if constexpr (ACT == MM_GROUP_ACT_SILU) return z / (1.f + expf(-z));
-  if constexpr (ACT == MM_GROUP_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  if constexpr (ACT == MM_GROUP_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+  if constexpr (ACT == MM_GROUP_ACT_GELU) return z * mm_normal(z, __expf(-0.5f * z * z));
   return z;
 }
 
@@ -65,11 +76,13 @@ __device__ __forceinline__ float mm_act(float z) {
 template <int ACT>
 __device__ __forceinline__ float mm_act_slope(float z) {
   if constexpr (ACT == MM_GROUP_ACT_SILU) {
-    const float q = 1.f / (1.f + expf(-z));
+    const float q = __builtin_amdgcn_rcpf(1.f + __expf(-z));
     return fmaf(z * q, 1.f - q, q);
   }
-  if constexpr (ACT == MM_GROUP_ACT_GELU)
-    return fmaf(z * 0.39894228f, expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678f)));
+  if constexpr (ACT == MM_GROUP_ACT_GELU) {
+    const float e = __expf(-0.5f * z * z);
+    return fmaf(z * 0.39894228f, e, mm_normal(z, e));
+  }
   return 1.f;
 }
 
@@ -129,13 +142,15 @@ struct MMGroupLane {
   }
 };
 
-// v = the rows first + sub + j nsub < first + n of this thread's channels, zeros elsewhere
+// v = the rows first + sub + j nsub < first + n of this thread's channels, zeros elsewhere (from the j on that no thread
+// has, v is left alone: loops over j end there)
 template <typename T, int TPB>
 __device__ __forceinline__ void mm_group_load(const MMGroupLane<T, TPB>& l, const T* __restrict__ x, long ldx,
                                               long first, int n, float (&v)[MMGroupLane<T, TPB>::NR][MMVec<T>::N]) {
   constexpr int N = MMVec<T>::N, NR = MMGroupLane<T, TPB>::NR;
 #pragma unroll
   for (int j = 0; j < NR; ++j) {
+    if (j * l.nsub >= n) break;
     const int r = l.sub + j * l.nsub;
     if (r < n && l.c < l.cw) {
       mm_load_vec(x + (first + r) * ldx + l.c0, l.c, l.cw, v[j]);
@@ -154,9 +169,11 @@ __device__ __forceinline__ void mm_group_moments(const MMGroup& a, MMGroupLane<T
   constexpr int N = MMVec<T>::N, NR = MMGroupLane<T, TPB>::NR;
   float t[1][N] = {};
 #pragma unroll
-  for (int j = 0; j < NR; ++j)
+  for (int j = 0; j < NR; ++j) {
+    if (j * l.nsub >= n) break;
 #pragma unroll
     for (int i = 0; i < N; ++i) t[0][i] += v[j][i];
+  }
   l.totals(a, t, mu);
   const float count = (float)n * (float)a.cg;
 #pragma unroll
@@ -165,12 +182,15 @@ __device__ __forceinline__ void mm_group_moments(const MMGroup& a, MMGroupLane<T
     t[0][i] = 0.f;
   }
 #pragma unroll
-  for (int j = 0; j < NR; ++j)
+  for (int j = 0; j < NR; ++j) {
+    if (j * l.nsub >= n) break;
+    const bool on = l.sub + j * l.nsub < n;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      v[j][i] = l.sub + j * l.nsub < n && l.c + i < l.cw ? v[j][i] - mu[0][i] : 0.f;
+      v[j][i] = on && l.c + i < l.cw ? v[j][i] - mu[0][i] : 0.f;
       t[0][i] = fmaf(v[j][i], v[j][i], t[0][i]);
     }
+  }
   l.totals(a, t, m2);
 }
 
@@ -213,6 +233,7 @@ mm_groupnorm_whole_fwd_kernel(MMGroup a, const T* __restrict__ x, long ldx, cons
     for (int i = 0; i < N; ++i) m2[0][i] = 1.f / sqrtf(m2[0][i] / count + eps);
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
+      if (j * l.nsub >= q.n) break;
       const int r = l.sub + j * l.nsub;
       if (r < q.n && l.c < l.cw) {
 #pragma unroll
@@ -272,13 +293,13 @@ mm_groupnorm_tile_stats_kernel(MMGroup a, const T* __restrict__ x, long ldx, lon
     });
 }
 
-// One workgroup per structure of more than `small` rows and group.  FWD: (mean, rstd) of the tiles' (mean, M2); else
+// One workgroup per structure of more than `small` rows, or per group of it where structures are few.  FWD: (mean, rstd) of the tiles' (mean, M2); else
 // the sums of both numbers.
 template <bool FWD>
 __global__ void __launch_bounds__(256)
 mm_groupnorm_join_kernel(MMGroup a, const float* __restrict__ part, float eps, float* __restrict__ out) {
   __shared__ float s0[4], s1[4];
-  const int g = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   auto all = [&](float v, float* lds) {
     v = mm_lanes_sum<64>(v);
     if (lane == 0) lds[wave] = v;
@@ -292,31 +313,33 @@ mm_groupnorm_join_kernel(MMGroup a, const float* __restrict__ part, float eps, f
     if (q.n <= a.small) continue;
     const long t0 = q.first / a.small, t1 = (q.first + q.n - 1) / a.small;
     const long end = q.first + q.n;
-    auto at = [&](long t) { return part + ((t * 2 + (t == t0 && q.first > t * a.small)) * a.G + g) * 2; };
     auto rows = [&](long t) {
       return (float)(int)(min((t + 1) * a.small, end) - max(t * (long)a.small, q.first));
     };
-    float u = 0.f, v = 0.f;
-    for (long t = t0 + threadIdx.x; t <= t1; t += 256) {
-      const float* p = at(t);
-      u = FWD ? fmaf(p[0], rows(t), u) : u + p[0];
-      v += p[1];
-    }
-    u = all(u, s0);
-    v = all(v, s1);
-    if constexpr (FWD) {
-      const float mu = u / (float)q.n;
-      u = mu;
-      float d2 = 0.f;
+    for (int g = blockIdx.y; g < a.G; g += gridDim.y) {
+      auto at = [&](long t) { return part + ((t * 2 + (t == t0 && q.first > t * a.small)) * a.G + g) * 2; };
+      float u = 0.f, v = 0.f;
       for (long t = t0 + threadIdx.x; t <= t1; t += 256) {
-        const float d = at(t)[0] - mu;
-        d2 = fmaf(d * d, rows(t), d2);
+        const float* p = at(t);
+        u = FWD ? fmaf(p[0], rows(t), u) : u + p[0];
+        v += p[1];
       }
-      v = 1.f / sqrtf((v + all(d2, s0) * (float)a.cg) / ((float)q.n * (float)a.cg) + eps);
-    }
-    if (threadIdx.x == 0) {
-      out[(s * a.G + g) * 2] = u;
-      out[(s * a.G + g) * 2 + 1] = v;
+      u = all(u, s0);
+      v = all(v, s1);
+      if constexpr (FWD) {
+        const float mu = u / (float)q.n;
+        u = mu;
+        float d2 = 0.f;
+        for (long t = t0 + threadIdx.x; t <= t1; t += 256) {
+          const float d = at(t)[0] - mu;
+          d2 = fmaf(d * d, rows(t), d2);
+        }
+        v = 1.f / sqrtf((v + all(d2, s0) * (float)a.cg) / ((float)q.n * (float)a.cg) + eps);
+      }
+      if (threadIdx.x == 0) {
+        out[(s * a.G + g) * 2] = u;
+        out[(s * a.G + g) * 2 + 1] = v;
+      }
     }
   }
 }
@@ -395,6 +418,7 @@ __device__ __forceinline__ void mm_group_slopes(const MMGroupLane<T, TPB>& l, in
   for (int i = 0; i < N; ++i) sum[0][i] = sum[1][i] = 0.f;
 #pragma unroll
   for (int j = 0; j < NR; ++j) {
+    if (j * l.nsub >= n) break;
     if (l.sub + j * l.nsub >= n) continue;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -445,6 +469,7 @@ mm_groupnorm_whole_bwd_kernel(MMGroup a, const T* __restrict__ dy, long lddy, co
     }
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
+      if (j * l.nsub >= q.n) break;
       const int r = l.sub + j * l.nsub;
       if (r < q.n && l.c < l.cw) {
 #pragma unroll
@@ -566,16 +591,19 @@ bool make_plan(const char* name, long rows, int structs, const int* offsets, int
   int gb = 1;
   while (gb < G && gb < 256 && gb * 2 * cg <= 1024 * N) gb *= 2;
   if (gb > G) gb = G;
-  int tpb, lpr;
-  for (;; gb = (gb + 1) / 2) {
-    lpr = 1;
-    while (lpr * N < gb * cg) lpr *= 2;
-    tpb = lpr > 256 ? 1024 : 256;
-    const int held = (tpb == 256 ? 64 : 32) / N * (tpb / lpr);
-    if (gb == 1 || held >= want || (gb + 1) / 2 * cg * es < 64) break;
-  }
+  auto lanes = [&](int g) {
+    int l = 1;
+    while (l * N < g * cg) l *= 2;
+    return l;
+  };
+  auto threads = [](int l) { return l > 256 ? 1024 : 256; };
+  auto held = [&](int l) { return (threads(l) == 256 ? 64 : 32) / N * (threads(l) / l); };
+  int least = gb;
+  while (least > 1 && held(lanes(least)) < want && (least + 1) / 2 * cg * es >= 64) least = (least + 1) / 2;
+  if (offsets || held(lanes(least)) >= want) gb = least;   // else tiles: whole rows
+  const int lpr = lanes(gb), tpb = threads(lpr);
   MMGroup& a = p->a;
-  a = MMGroup{offsets, rows, each, structs, C, G, cg, gb, lpr, (tpb == 256 ? 64 : 32) / N * (tpb / lpr)};
+  a = MMGroup{offsets, rows, each, structs, C, G, cg, gb, lpr, held(lpr)};
   p->tpb = tpb;
   p->blocks = (G + gb - 1) / gb;
   p->whole = offsets || each <= a.small;
@@ -585,6 +613,10 @@ bool make_plan(const char* name, long rows, int structs, const int* offsets, int
   p->wg_tiles = (int)(p->n_tiles < MM_GROUP_WG ? p->n_tiles : MM_GROUP_WG);
   p->lds = ((size_t)2 * (tpb / (lpr > 64 ? lpr : 64)) * lpr * N + 2 * gb) * sizeof(float);
   return true;
+}
+
+dim3 join_grid(int structs, int groups) {
+  return structs < 256 ? dim3(structs, groups) : dim3(structs < 4096 ? structs : 4096);
 }
 
 bool bad_sizes(long rows, int structs, const int* offsets, int C, int G) {
@@ -645,7 +677,7 @@ extern "C" int mm_groupnorm_fwd(const void* x, long ldx, int dtype, long rows, i
       if (p.tpb == 256) go(mm_groupnorm_tile_stats_kernel<T_, 256>);
       else go(mm_groupnorm_tile_stats_kernel<T_, 1024>);
     });
-    hipLaunchKernelGGL(mm_groupnorm_join_kernel<true>, dim3(structs < 4096 ? structs : 4096, groups), dim3(256), 0, stream,
+    hipLaunchKernelGGL(mm_groupnorm_join_kernel<true>, join_grid(structs, groups), dim3(256), 0, stream,
                        p.a, workspace, eps, stats);
     MM_GROUP_DISPATCH(mm_groupnorm_tile_fwd_kernel, grid, 0, p.a, (const T_*)x, ldx, w, b, p_dtype == MM_F32, (T_*)y,
                       ldy, p.n_tiles, stats);
@@ -678,7 +710,7 @@ extern "C" int mm_groupnorm_bwd(const void* dy, long lddy, const void* x, long l
       MM_GROUP_DISPATCH(mm_groupnorm_tile_sums_kernel, grid, p.lds, p.a, (const T_*)dy, lddy, (const T_*)x, ldx, w, b,
                         p_dtype == MM_F32, stats, p.n_tiles, dx ? part : nullptr, wpart, (long)p.wg_whole, part_rows);
       if (dx) {
-        hipLaunchKernelGGL(mm_groupnorm_join_kernel<false>, dim3(structs < 4096 ? structs : 4096, groups), dim3(256), 0,
+        hipLaunchKernelGGL(mm_groupnorm_join_kernel<false>, join_grid(structs, groups), dim3(256), 0,
                            stream, p.a, part, 0.f, sums);
         MM_GROUP_DISPATCH(mm_groupnorm_tile_bwd_kernel, grid, 0, p.a, (const T_*)dy, lddy, (const T_*)x, ldx, w, b,
                           p_dtype == MM_F32, stats, sums, (T_*)dx, lddx, p.n_tiles);
