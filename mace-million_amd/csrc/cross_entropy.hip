@@ -213,11 +213,11 @@ struct MMCeLogits {
   float scale;
 };
 
-template <typename T, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2)
+template <typename T, typename Nt>
+__global__ void __launch_bounds__(Nt::TH, Nt::PER_CU)
 mm_ce_logits_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
   typedef typename MMCeType<T>::H H;
-  typedef MMNt<H, MMCeType<T>::P, BM, BN, WM, WN> Nt;
+  constexpr int BM = Nt::BM, BN = Nt::BN;
   extern __shared__ uint4 mm_ce_lds[];
   const int count = *a.count;
   int e, tm, tn;
@@ -254,13 +254,13 @@ mm_ce_logits_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
         if (n0 + t.col(i) + q < a.V) r.sum += __expf(t.acc[i][j][q] - top);
 #pragma unroll
     for (int d = 16; d < 64; d <<= 1) r = mm_ce_join(r, MMCeRow{__shfl_xor(r.top, d), __shfl_xor(r.sum, d)});
-    if (t.lane < 16) s[(threadIdx.x >> 6) / WM * BM + t.row(j)] = r;
+    if (t.lane < 16) s[(threadIdx.x >> 6) / Nt::WM * BM + t.row(j)] = r;
   }
   __syncthreads();
   if ((int)threadIdx.x < BM && m0 + (int)threadIdx.x < count) {
     MMCeRow r = s[threadIdx.x];
 #pragma unroll
-    for (int w = 1; w < WN; ++w) r = mm_ce_join(r, s[w * BM + threadIdx.x]);
+    for (int w = 1; w < Nt::WN; ++w) r = mm_ce_join(r, s[w * BM + threadIdx.x]);
     float* p = a.part + ((long)tn * a.T + m0 + threadIdx.x) * 2;
     p[0] = r.top;
     p[1] = r.sum;
@@ -278,7 +278,7 @@ mm_ce_rows_kernel(const float* __restrict__ part, long T, int tiles_n, const int
   if ((int)blockIdx.x * 32 >= n) return;
   MMCeRow r{-INFINITY, 0.f};
   if (i < n)
-#pragma unroll 4
+#pragma unroll 8
     for (int t = q; t < tiles_n; t += 32) {
       const float2 p = *(const float2*)(part + ((long)t * T + i) * 2);
       r = mm_ce_join(r, MMCeRow{p.x, p.y});
@@ -324,6 +324,123 @@ __global__ void __launch_bounds__(1024) mm_ce_total_kernel(const float* __restri
   *loss = (float)(mean ? t / (double)max(n, 1) : t);
 }
 
+// ------------------------------------------------------------------------------------------------ few rows
+// The forward of few rows, in one launch or two: rows of W go by in vectors, one class a wave, and meet all rows of x
+// (fp32 in LDS); every workgroup lists the rows by itself.  Bound by reading W: one row, 100,003 classes of 4096
+// bfloat16 values.  One workgroup finishes the losses (small heads), more leave partial sums to the rows' kernel.
+#define MM_CE_FEW 16     // rows, at most
+#define MM_CE_FEW_LDS 16384   // floats of x in LDS
+#define MM_CE_CLASSES 4  // of a wave at once
+
+struct MMCeFew {
+  const void *x, *w, *targets;
+  long ldx, ignore;
+  int T, D, V, targets64, reduction;
+  int *count, *list, *y, *pos;
+  float *part, *picked, *lse, *loss;
+};
+
+template <typename T, int ROWS, int TH>
+__global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a) {
+  constexpr int N = MMVec<T>::N, W = TH / 64, C = MM_CE_CLASSES;
+  extern __shared__ float mm_ce_x[];   // [T][D rounded up to whole vectors of a wave]
+  __shared__ MMCeRow s_row[W][ROWS];
+  __shared__ float s_hit[W][ROWS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, Dp = (a.D + 64 * N - 1) / (64 * N) * (64 * N);
+  // lane t of every wave: row t (rows that are left out are computed like the others and go nowhere)
+  const bool has = lane < a.T;
+  const long target = !has ? a.ignore : a.targets64 ? ((const long*)a.targets)[lane] : (long)((const int*)a.targets)[lane];
+#pragma unroll
+  for (int t = 0; t < ROWS; ++t) {
+    if (t >= a.T) break;
+    for (int c = threadIdx.x; c < Dp; c += TH) mm_ce_x[t * Dp + c] = c < a.D ? (float)((const T*)a.x)[t * a.ldx + c] : 0.f;
+  }
+  const unsigned long long asked = __ballot(target != a.ignore);
+  const int at = __popcll(asked & ((1ull << lane) - 1)), n = __popcll(asked);
+  const int y = target >= 0 && target < a.V ? (int)target : -1;
+  if (blockIdx.x == 0 && wave == 0) {
+    if (target != a.ignore) {
+      a.list[at] = lane;
+      a.y[at] = y;
+    }
+    if (has) a.pos[lane] = target != a.ignore ? at : -1;
+    if (has && target == a.ignore && a.reduction == 0) a.loss[lane] = 0.f;
+    if (lane == 0) *a.count = n;
+  }
+  __syncthreads();
+  MMCeRow r{-INFINITY, 0.f};
+  float hit = 0.f;
+  for (int v0 = (blockIdx.x * W + wave) * C; v0 < a.V; v0 += (int)gridDim.x * W * C) {
+    float acc[ROWS][C] = {};
+    const T* __restrict__ p[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k) p[k] = (const T*)a.w + (size_t)min(v0 + k, a.V - 1) * a.D;
+    auto add = [&](int c, int end) {
+      float w[C][N];
+#pragma unroll
+      for (int k = 0; k < C; ++k) mm_load_vec(p[k], c, end, w[k]);
+#pragma unroll
+      for (int t = 0; t < ROWS; ++t) {
+        if (ROWS > 1 && t >= a.T) break;
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          const floatx4 x = *(const floatx4*)(mm_ce_x + t * Dp + c + i);
+#pragma unroll
+          for (int k = 0; k < C; ++k)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[t][k] = fmaf(x[q], w[k][i + q], acc[t][k]);
+        }
+      }
+    };
+    int c = lane * N;
+    const int whole = a.D / (64 * N) * (64 * N);
+#pragma unroll 4
+    for (; c < whole; c += 64 * N) add(c, c + N);
+    if (whole < a.D && c < Dp) add(c, a.D);
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) {
+      if (ROWS > 1 && t >= a.T) break;
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        const float l = mm_lanes_sum<64>(acc[t][k]);
+        if (lane == t && v0 + k < a.V) {
+          r = mm_ce_join(r, MMCeRow{l, 1.f});
+          if (v0 + k == y) hit = l;
+        }
+      }
+    }
+  }
+  if (gridDim.x > 1 && target != a.ignore && y >= 0 && y / C % (int)(gridDim.x * W) == (int)blockIdx.x * W + wave)
+    a.picked[at] = hit;   // by the wave that has the target's class
+  if (lane < ROWS) {
+    s_row[wave][lane] = r;
+    s_hit[wave][lane] = hit;
+  }
+  __syncthreads();
+  if (wave) return;
+  float l = 0.f;
+  if (target != a.ignore) {
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      r = mm_ce_join(r, s_row[w][lane]);
+      hit += s_hit[w][lane];   // 0 but for one wave
+    }
+    if (gridDim.x > 1) {
+      float* p = a.part + ((long)blockIdx.x * a.T + at) * 2;
+      p[0] = r.top;
+      p[1] = r.sum;
+      return;
+    }
+    const float z = r.top + logf(r.sum);
+    a.lse[at] = z;
+    l = y < 0 ? __builtin_nanf("") : z - hit;
+    if (a.reduction == 0) a.loss[lane] = l;
+  }
+  if (gridDim.x > 1 || a.reduction == 0) return;
+  l = mm_lanes_sum<64>(l);
+  if (lane == 0) *a.loss = a.reduction == MM_CE_MEAN ? l / (float)max(n, 1) : l;
+}
+
 // ------------------------------------------------------------------------------------------------ backward
 // g of the asked rows (none: of every row; else dloss, over the count for the mean) and the largest finite |g|; one
 // workgroup
@@ -347,11 +464,11 @@ __global__ void __launch_bounds__(1024) mm_ce_grad_kernel(const float* __restric
   *gmax = top;
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2)
+template <typename T, typename Nt>
+__global__ void __launch_bounds__(Nt::TH, Nt::PER_CU)
 mm_ce_d_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
   typedef typename MMCeType<T>::H H;
-  typedef MMNt<H, MMCeType<T>::P, BM, BN, WM, WN> Nt;
+  constexpr int BM = Nt::BM, BN = Nt::BN;
   extern __shared__ uint4 mm_ce_lds[];
   const int count = *a.count;
   int e, tm, tn;
@@ -362,36 +479,86 @@ mm_ce_d_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
   Nt t;
   t.run(x, m0, a.w, n0, 0, a.K, mm_ce_lds);
   const float gmax = *a.gmax;
-  const long rows = mm_up(count, MM_NT_K), cols = mm_up(a.n, MM_NT_K);
+  const int rows = (int)mm_up(count, MM_NT_K), cols = (int)mm_up(a.n, MM_NT_K);
+  float share[Nt::FM];
 #pragma unroll
   for (int j = 0; j < Nt::FM; ++j) {
-    const int m = m0 + t.row(j), at = min(m, count - 1), y = a.y[at] - a.v0;
-    const float lse = a.lse[at], r = gmax > 0.f ? a.g[at] / gmax : a.g[at];
-    if (m >= rows) continue;
+    const int m = m0 + t.row(j), at = min(m, count - 1), y = a.y[at];
+    const float lse = a.lse[at];
+    share[j] = gmax > 0.f ? a.g[at] / gmax : a.g[at];
 #pragma unroll
-    for (int i = 0; i < Nt::FN; ++i) {
-      const int n = n0 + t.col(i);
-      float d[4], dt[4];
+    for (int i = 0; i < Nt::FN; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
+        const int n = n0 + t.col(i) + q;
+        const float p = __expf(t.acc[i][j][q] - lse) - (n + a.v0 == y ? 1.f : 0.f);
         // a target out of range (loss NaN) makes the row NaN
-        const float p = a.y[at] < 0 ? __builtin_nanf("") : __expf(t.acc[i][j][q] - lse) - (n + q == y ? 1.f : 0.f);
-        d[q] = n + q < a.n && m < count ? p * a.scale : 0.f;
-        dt[q] = n + q < a.n && m < count ? p * a.scale * r : 0.f;
+        t.acc[i][j][q] = n < a.n && m < count ? (y < 0 ? __builtin_nanf("") : p * a.scale) : 0.f;
       }
-      if (m < count && n < cols) mm_ce_put4<T>(a.d + (long)m * a.ldd + n, a.plane, d);
+  }
+  if constexpr (MMCeType<T>::PLANES > 1) {   // three planes: straight from the registers (27 us against 43 through LDS
+                                             // for 14,700 rows, 89 classes)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (n + q < a.n) {
-          float v = dt[q];
+    for (int j = 0; j < Nt::FM; ++j)
 #pragma unroll
-          for (int b = 0; b < MMCeType<T>::PLANES; ++b) {
-            const H h = (H)v;
-            a.dT[b * a.planeT + (long)(n + q) * a.ldt + m] = h;
-            v -= (float)h;
+      for (int i = 0; i < Nt::FN; ++i) {
+        const int m = m0 + t.row(j), n = n0 + t.col(i), mt = m & ~3, nt = n + (t.lane & 3);
+        const floatx4 v = t.acc[i][j];
+        if (m < count && n < cols) mm_ce_put4<T>(a.d + (long)m * a.ldd + n, a.plane, (const float*)&v);
+        floatx4 r = v * share[j];
+#pragma unroll
+        for (int b = 0; b < MMCeType<T>::PLANES; ++b) {
+          typedef H vec __attribute__((ext_vector_type(4)));
+          H h[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            h[q] = (H)r[q];
+            r[q] -= (float)h[q];
           }
+          mm_quad_transpose(h);
+          if (nt < a.n && mt < rows) *(vec*)(a.dT + b * a.planeT + (long)nt * a.ldt + mt) = vec{h[0], h[1], h[2], h[3]};
         }
+      }
+    return;
+  }
+  // Through LDS, so that whole lines go out: rows [BM][BN] of d, then columns [BN][BM] with the rows' shares; 16-byte
+  // units of a row are turned by its number, against bank conflicts.
+  typedef H vec __attribute__((ext_vector_type(4)));
+  H* const tile = (H*)mm_ce_lds;
+#pragma unroll
+  for (int j = 0; j < Nt::FM; ++j)
+#pragma unroll
+    for (int i = 0; i < Nt::FN; ++i) {
+      const int m = t.row(j), n = t.col(i);
+      const floatx4& v = t.acc[i][j];
+      *(vec*)(tile + m * BN + ((n >> 3 ^ (m & 15)) << 3) + (n & 4)) = vec{(H)v[0], (H)v[1], (H)v[2], (H)v[3]};
     }
+  __syncthreads();
+#pragma unroll 4
+  for (int q = threadIdx.x; q < BM * BN / 8; q += Nt::TH) {
+    const int m = q / (BN / 8), u = q % (BN / 8);
+    if (m0 + m < count && n0 + 8 * u < cols)
+      *(uint4*)(a.d + (long)(m0 + m) * a.ldd + n0 + 8 * u) = *(const uint4*)(tile + m * BN + ((u ^ (m & 15)) << 3));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < Nt::FM; ++j)
+#pragma unroll
+    for (int i = 0; i < Nt::FN; ++i) {
+      // this lane's column n + (lane & 3), rows of its quad of lanes
+      H h[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) h[q] = (H)(t.acc[i][j][q] * share[j]);
+      mm_quad_transpose(h);
+      const int m = t.row(j) & ~3, n = t.col(i) + (t.lane & 3);
+      *(vec*)(tile + n * BM + ((m >> 3 ^ (n & 15)) << 3) + (m & 4)) = vec{h[0], h[1], h[2], h[3]};
+    }
+  __syncthreads();
+#pragma unroll 4
+  for (int q = threadIdx.x; q < BM * BN / 8; q += Nt::TH) {
+    const int n = q / (BM / 8), u = q % (BM / 8);
+    if (n0 + n < a.n && m0 + 8 * u < rows)
+      *(uint4*)(a.dT + (long)(n0 + n) * a.ldt + m0 + 8 * u) = *(const uint4*)(tile + n * BM + ((u ^ (n & 15)) << 3));
   }
 }
 
@@ -411,11 +578,11 @@ struct MMCeProduct {
   float inv;
 };
 
-template <typename T, bool DX, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2)
+template <typename T, bool DX, typename Nt>
+__global__ void __launch_bounds__(Nt::TH, Nt::PER_CU)
 mm_ce_product_kernel(MMCeProduct<typename MMCeType<T>::H> a, int tiles_n) {
   typedef typename MMCeType<T>::H H;
-  typedef MMNt<H, MMCeType<T>::P, BM, BN, WM, WN> Nt;
+  constexpr int BM = Nt::BM, BN = Nt::BN;
   extern __shared__ uint4 mm_ce_lds[];
   const int count = *a.count, M = DX ? count : a.M;
   const int K = DX ? a.K : (count + MM_NT_K - 1) / MM_NT_K;
@@ -455,29 +622,41 @@ mm_ce_product_kernel(MMCeProduct<typename MMCeType<T>::H> a, int tiles_n) {
   }
 }
 
-// out = the sum of the splits' sums: dx (pos: row of part, or none: 0; factor g) or dW (factor *gmax)
-template <typename T, bool DX>
+// out = the sum of the splits' sums: dx (pos: row of part, or none: 0; factor g) or dW (factor *gmax).  A vector is
+// summed by WAVES waves.
+template <typename T, bool DX, int WAVES>
 __global__ void __launch_bounds__(256)
 mm_ce_join_kernel(const float* __restrict__ part, int splits, long part_rows, long rows, int N,
                   const int* __restrict__ pos, const float* __restrict__ g, float inv, T* __restrict__ out) {
-  const int nv = (N + 3) / 4;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < rows * nv; i += (long)gridDim.x * 256) {
-    const long row = i / nv, at = DX ? pos[row] : row;
+  constexpr int EACH = 256 / WAVES;
+  __shared__ floatx4 s[WAVES][EACH];
+  const int nv = (N + 3) / 4, lane = threadIdx.x % EACH, wave = threadIdx.x / EACH;
+  for (long i0 = (long)blockIdx.x * EACH; i0 < rows * nv; i0 += (long)gridDim.x * EACH) {
+    const long i = i0 + lane, row = i / nv, at = i >= rows * nv ? -1 : DX ? pos[row] : row;
     const int c = (int)(i - row * nv) * 4;
-    float v[4] = {};
+    floatx4 v = {};
     if (at >= 0) {
-#pragma unroll 8
-      for (int s = 0; s < splits; ++s) {
+#pragma unroll 4
+      for (int k = wave; k < splits; k += WAVES) {
         float u[4];
-        mm_load4(part + (s * part_rows + at) * N, c, N, u);
+        mm_load4(part + (k * part_rows + at) * N, c, N, u);
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[q] += u[q];
       }
-      const float f = (DX ? g[at] : g[0]) * inv;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] *= f;
     }
-    mm_store4(out + row * N, c, N, v);
+    if constexpr (WAVES > 1) {
+      s[wave][lane] = v;
+      __syncthreads();
+    }
+    if (wave == 0 && i < rows * nv) {
+      const float f = at < 0 ? 0.f : (DX ? g[at] : g[0]) * inv;   // 0 rows stay 0 whatever the factor
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) v += s[w][lane];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = at < 0 ? 0.f : v[q] * f;
+      mm_store4(out + row * N, c, N, (const float*)&v);
+    }
+    if constexpr (WAVES > 1) __syncthreads();
   }
 }
 
@@ -495,6 +674,7 @@ struct Sizes {
   bool w_in_place;   // the weights are operands as they are
   long piece, pieces, piece_p;
   int dx_splits, dw_splits;
+  bool dx_big, dw_big;
 };
 
 long div_up(long a, long b) { return (a + b - 1) / b; }
@@ -511,6 +691,20 @@ struct Space {
     return p;
   }
 };
+
+// Large tiles where they are enough for three quarters of the CUs and lie outside the product by less than a fifth more
+// than small ones do.
+bool big_fits(long m, long n) { return 5 * mm_up(m, 256) * mm_up(n, 256) <= 6 * mm_up(m, BM) * mm_up(n, BN); }
+bool big_tiles(long m, long n, int splits) {
+  return big_fits(m, n) && div_up(m, 256) * div_up(n, 256) * splits >= 192;
+}
+
+// Parts of the summed index K of an m x n product, so that there are workgroups for every CU; no part below 512.
+int splits_of(long m, long n, long K, bool* big) {
+  const long most = clamp(K / 512, 1, 64), tiles = div_up(m, 256) * div_up(n, 256), few = div_up(m, BM) * div_up(n, BN);
+  *big = big_fits(m, n) && (tiles >= 192 || (tiles >= 64 && tiles * most >= 192));
+  return (int)clamp(*big ? div_up(192, tiles) : 512 / (few ? few : 1), 1, most);
+}
 
 bool sizes_of(const char* name, long T, long D, long V, int dtype, const void* w, Sizes* s) {
   if (T > MAX_SIDE || D > MAX_SIDE || V > MAX_SIDE || div_up(T, BM) * div_up(V, BN) * 256 >= 4294967296L ||
@@ -529,10 +723,20 @@ bool sizes_of(const char* name, long T, long D, long V, int dtype, const void* w
   s->piece = s->pieces == 1 ? V : mm_up(div_up(V, s->pieces), 256);
   s->pieces = div_up(V, s->piece);
   s->piece_p = mm_up(s->piece, MM_NT_K);
-  const long dx_tiles = div_up(T, BM) * div_up(D, BN), dw_tiles = div_up(s->piece, BM) * div_up(D, BN);
-  s->dx_splits = (int)clamp(512 / (dx_tiles ? dx_tiles : 1), 1, clamp(s->piece_p / 512, 1, 64));
-  s->dw_splits = (int)clamp(512 / (dw_tiles ? dw_tiles : 1), 1, clamp(s->Tp / 512, 1, 64));
+  s->dx_splits = splits_of(T, D, s->piece_p, &s->dx_big);
+  s->dw_splits = splits_of(s->piece, D, s->Tp, &s->dw_big);
   return true;
+}
+
+// Few rows of a head: vectors of W without the matrix cores.
+bool few_rows(const Sizes& s) {
+  const long Dp = mm_up(s.D, s.dtype == MM_F32 ? 256 : 512);
+  return s.T > 0 && s.T <= MM_CE_FEW && s.T * Dp <= MM_CE_FEW_LDS;
+}
+// one workgroup where W has up to 128 KB
+int few_workgroups(const Sizes& s) {
+  if (s.V * s.D * (s.dtype == MM_F32 ? 4 : 2) <= 131072) return 1;
+  return (int)clamp(div_up(s.V, 8 * MM_CE_CLASSES), 2, 512);
 }
 
 struct Forward {
@@ -542,6 +746,12 @@ struct Forward {
 };
 size_t forward_space(const Sizes& s, char* base, Forward* f) {
   Space p{base};
+  if (few_rows(s)) {
+    f->part = p.take<float>((size_t)few_workgroups(s) * s.T * 2);
+    f->picked = p.take<float>(s.T);
+    f->sums = p.take<float>(1);
+    return p.used;
+  }
   f->x = p.take<short>((size_t)s.planes * s.T * s.Dp);
   f->w = s.w_in_place ? nullptr : p.take<short>((size_t)s.planes * s.V * s.Dp);
   f->part = p.take<float>((size_t)div_up(s.V, BN) * s.T * 2);
@@ -576,11 +786,46 @@ void pack(const MMPack& a, long rows, hipStream_t stream) {
                      stream, a);
 }
 
+template <auto KERNEL, typename Nt, typename A>
+bool launch(const A& a, long m, long n, int splits, hipStream_t stream) {
+  if (!lds_granted<KERNEL>(Nt::LDS)) return false;
+  const int tiles_n = (int)div_up(n, Nt::BN);
+  hipLaunchKernelGGL(KERNEL, dim3((unsigned)(div_up(m, Nt::BM) * tiles_n), splits), dim3(Nt::TH), Nt::LDS, stream, a,
+                     tiles_n);
+  return true;
+}
+
+template <typename T, int ROWS, int TH>
+bool launch_few(const MMCeFew& a, int wg, size_t lds, hipStream_t stream) {
+  if (!lds_granted<mm_ce_few_kernel<T, ROWS, TH>>((int)lds)) return false;
+  hipLaunchKernelGGL((mm_ce_few_kernel<T, ROWS, TH>), dim3(wg), dim3(TH), lds, stream, a);
+  return true;
+}
+
+template <typename T>
+int forward_few(const Sizes& s, const MMCeFew& a, float* sums, hipStream_t stream) {
+  const int wg = few_workgroups(s), N = MMVec<T>::N;
+  const size_t lds = (size_t)s.T * mm_up(s.D, 64 * N) * sizeof(float);
+  bool ok;
+  if (wg == 1) ok = s.T == 1 ? launch_few<T, 1, 1024>(a, wg, lds, stream) : launch_few<T, MM_CE_FEW, 1024>(a, wg, lds, stream);
+  else ok = s.T == 1 ? launch_few<T, 1, 512>(a, wg, lds, stream) : launch_few<T, MM_CE_FEW, 512>(a, wg, lds, stream);
+  if (!ok) return MM_ELAUNCH;
+  if (wg > 1) {
+    hipLaunchKernelGGL(mm_ce_rows_kernel, dim3(1), dim3(1024), 0, stream, a.part, s.T, wg, a.count, a.list, a.y,
+                       a.picked, a.lse, a.reduction == 0 ? a.loss : nullptr, a.reduction ? sums : nullptr);
+    if (a.reduction)
+      hipLaunchKernelGGL(mm_ce_total_kernel, dim3(1), dim3(1024), 0, stream, sums, a.count, a.reduction == MM_CE_MEAN,
+                         a.loss);
+  }
+  return mm::launch_status("mm_ce_fwd");
+}
+
 template <typename T>
 int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, float* loss, float* lse,
             const Forward& f, hipStream_t stream) {
   typedef typename MMCeType<T>::H H;
   typedef MMNt<H, MMCeType<T>::P, BM, BN, 2, 2> Nt;
+  typedef MMNtBig<H, MMCeType<T>::P> Big;
   if (s.T) {
     MMPack px{x, r.list, r.count, f.x, nullptr, ldx, 0, s.Dp, 0, s.T * s.Dp, 0, (int)s.T, (int)s.D};
     pack<T>(px, s.T, stream);
@@ -599,9 +844,11 @@ int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int
     a.part = f.part;
     a.picked = f.picked;
     a.T = s.T;
-    const int tiles_n = (int)div_up(s.V, BN);
-    hipLaunchKernelGGL((mm_ce_logits_kernel<T, BM, BN, 2, 2>), dim3((unsigned)(div_up(s.T, BM) * tiles_n)), dim3(256),
-                       Nt::LDS, stream, a, tiles_n);
+    const bool big = big_tiles(s.T, s.V, 1);
+    const int tiles_n = (int)div_up(s.V, big ? Big::BN : BN);
+    if (!(big ? launch<mm_ce_logits_kernel<T, Big>, Big>(a, s.T, s.V, 1, stream)
+              : launch<mm_ce_logits_kernel<T, Nt>, Nt>(a, s.T, s.V, 1, stream)))
+      return MM_ELAUNCH;
     hipLaunchKernelGGL(mm_ce_rows_kernel, dim3((unsigned)div_up(s.T, 32)), dim3(1024), 0, stream, f.part, s.T, tiles_n,
                        r.count, r.list, r.y, f.picked, lse, reduction == 0 ? loss : nullptr,
                        reduction ? f.sums : nullptr);
@@ -612,11 +859,24 @@ int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int
   return mm::launch_status("mm_ce_fwd");
 }
 
+template <typename T, bool DX>
+void join(const float* part, int splits, long part_rows, long rows, int N, const int* pos, const float* g, float inv,
+          T* out, hipStream_t stream) {
+  const long vectors = rows * div_up(N, 4);
+  if (splits < 4)
+    hipLaunchKernelGGL((mm_ce_join_kernel<T, DX, 1>), dim3((unsigned)clamp(div_up(vectors, 256), 1, 4096)), dim3(256), 0,
+                       stream, part, splits, part_rows, rows, N, pos, g, inv, out);
+  else
+    hipLaunchKernelGGL((mm_ce_join_kernel<T, DX, 4>), dim3((unsigned)clamp(div_up(vectors, 64), 1, 4096)), dim3(256), 0,
+                       stream, part, splits, part_rows, rows, N, pos, g, inv, out);
+}
+
 template <typename T>
 int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, const float* lse,
              const float* dloss, T* dx, T* dw, const Backward& b, hipStream_t stream) {
   typedef typename MMCeType<T>::H H;
   typedef MMNt<H, MMCeType<T>::P, BM, BN, 2, 2> Nt;
+  typedef MMNtBig<H, MMCeType<T>::P> Big;
   const float scale = s.dtype == MM_F16 ? HALF_SCALE : 1.f;
   hipLaunchKernelGGL(mm_ce_grad_kernel, dim3(1), dim3(1024), 0, stream, dloss, reduction, r.count, r.list, b.g, b.gmax);
   MMPack px{x, r.list, r.count, b.x, b.xT, ldx, 0, s.Dp, s.Tp, s.T * s.Dp, s.D * s.Tp, (int)s.T, (int)s.D};
@@ -645,10 +905,8 @@ int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, in
     a.v0 = (int)v0;
     a.n = (int)n;
     a.scale = scale;
-    const int tiles_n = (int)div_up(n, BN);
-    hipLaunchKernelGGL((mm_ce_d_kernel<T, BM, BN, 2, 2>), dim3((unsigned)(div_up(s.T, BM) * tiles_n)), dim3(256), Nt::LDS,
-                       stream, a, tiles_n);
-    const int tiles_d = (int)div_up(s.D, BN);
+    bool ok = big_tiles(s.T, n, 1) ? launch<mm_ce_d_kernel<T, Big>, Big>(a, s.T, n, 1, stream)
+                                   : launch<mm_ce_d_kernel<T, Nt>, Nt>(a, s.T, n, 1, stream);
     if (dx) {
       MMCeProduct<H> q{};
       q.a = MMNtOperand<H>{(const H*)b.d, s.piece_p, s.T * s.piece_p, 0};
@@ -660,8 +918,8 @@ int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, in
       q.first = p == 0;
       q.part = b.dx;
       q.rows = s.T;
-      hipLaunchKernelGGL((mm_ce_product_kernel<T, true, BM, BN, 2, 2>),
-                         dim3((unsigned)(div_up(s.T, BM) * tiles_d), q.splits), dim3(256), Nt::LDS, stream, q, tiles_d);
+      ok = ok && (s.dx_big ? launch<mm_ce_product_kernel<T, true, Big>, Big>(q, s.T, s.D, q.splits, stream)
+                           : launch<mm_ce_product_kernel<T, true, Nt>, Nt>(q, s.T, s.D, q.splits, stream));
     }
     if (dw) {
       MMCeProduct<H> q{};
@@ -676,17 +934,14 @@ int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, in
       q.out = s.dw_splits == 1 ? dw + v0 * s.D : nullptr;
       q.gmax = b.gmax;
       q.inv = 1.f / scale;
-      hipLaunchKernelGGL((mm_ce_product_kernel<T, false, BM, BN, 2, 2>),
-                         dim3((unsigned)(div_up(n, BM) * tiles_d), q.splits), dim3(256), Nt::LDS, stream, q, tiles_d);
+      ok = ok && (s.dw_big ? launch<mm_ce_product_kernel<T, false, Big>, Big>(q, n, s.D, q.splits, stream)
+                           : launch<mm_ce_product_kernel<T, false, Nt>, Nt>(q, n, s.D, q.splits, stream));
       if (s.dw_splits > 1)
-        hipLaunchKernelGGL((mm_ce_join_kernel<T, false>), dim3((unsigned)clamp(div_up(n * div_up(s.D, 4), 256), 1, 4096)),
-                           dim3(256), 0, stream, b.dw, s.dw_splits, n, n, (int)s.D, nullptr, b.gmax, 1.f / scale,
-                           dw + v0 * s.D);
+        join<T, false>(b.dw, s.dw_splits, n, n, (int)s.D, nullptr, b.gmax, 1.f / scale, dw + v0 * s.D, stream);
     }
+    if (!ok) return MM_ELAUNCH;
   }
-  if (dx)
-    hipLaunchKernelGGL((mm_ce_join_kernel<T, true>), dim3((unsigned)clamp(div_up(s.T * div_up(s.D, 4), 256), 1, 4096)),
-                       dim3(256), 0, stream, b.dx, s.dx_splits, s.T, s.T, (int)s.D, r.pos, b.g, 1.f / scale, dx);
+  if (dx) join<T, true>(b.dx, s.dx_splits, s.T, s.T, (int)s.D, r.pos, b.g, 1.f / scale, dx, stream);
   return mm::launch_status("mm_ce_bwd");
 }
 }  // namespace
@@ -715,6 +970,13 @@ extern "C" int mm_ce_fwd(const void* x, long ldx, int dtype, long T, long D, con
   Forward f;
   forward_space(s, (char*)workspace, &f);
   const Rows r = rows_of(rows, T);
+  int rc = MM_OK;
+  if (few_rows(s)) {
+    const MMCeFew a{x, w, targets, ldx, ignore, (int)T, (int)D, (int)V, targets64, reduction, r.count, r.list, r.y, r.pos,
+                    f.part, f.picked, lse, loss};
+    MM_DISPATCH(dtype, rc = forward_few<T_>(s, a, f.sums, stream));
+    return rc;
+  }
   const unsigned blocks = T ? (unsigned)div_up(T, 1024 * MM_CE_SCAN) : 1;
   auto scan = [&](auto y) {
     if (blocks > 1)
@@ -726,7 +988,6 @@ extern "C" int mm_ce_fwd(const void* x, long ldx, int dtype, long T, long D, con
   };
   if (targets64) scan((const long*)targets);
   else scan((const int*)targets);
-  int rc = MM_OK;
   MM_DISPATCH(dtype, rc = forward<T_>(s, (const T_*)x, ldx, (const T_*)w, r, reduction, loss, lse, f, stream));
   return rc;
 }

@@ -7,7 +7,6 @@
 #pragma once
 #include "tile.h"
 
-#include <atomic>
 
 typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));   // 16 bytes known to be float-aligned only
 
@@ -109,23 +108,6 @@ inline bool too_many(long workgroups, long threads) { return workgroups * thread
 
 // base of a matrix whose 16-byte units can be loaded straight into LDS
 inline bool aligned(const void* p) { return (size_t)p % 16 == 0; }
-
-// more than 64 KB of LDS has to be asked for, once per kernel and device
-template <auto KERNEL>
-bool lds_granted(int bytes) {
-  static std::atomic<unsigned long long> granted{0};   // a bit per device
-  int dev = 0;
-  if (bytes <= 65536) return true;
-  if (hipGetDevice(&dev) != hipSuccess) dev = 0;
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (granted.load(std::memory_order_relaxed) & bit) return true;
-  if (hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) {
-    mm::set_error("the kernel's LDS was not granted");
-    return false;
-  }
-  granted.fetch_or(bit, std::memory_order_relaxed);
-  return true;
-}
 
 }  // namespace
 

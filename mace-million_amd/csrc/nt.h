@@ -7,6 +7,8 @@
 #pragma once
 #include "tile.h"
 
+#include <type_traits>
+
 #define MM_NT_K 64   // values of the summed index of a stage
 
 template <typename H>
@@ -28,8 +30,9 @@ __device__ __forceinline__ int mm_nt_second(int q) {
 
 // A workgroup's tile of BM rows of A by BN rows of B, WM x WN waves; lane's results acc[i][j][q]: row m = wm + 16 j +
 // (lane & 15) of the tile, column n = wn + 16 i + 4 (lane >> 4) + q.
-template <typename H, int P, int BM, int BN, int WM, int WN>
+template <typename H, int P, int BM_, int BN_, int WM_, int WN_>
 struct MMNt {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, PER_CU = 2;
   static constexpr int TH = 64 * WM * WN, UA = BM * 8 / TH, UB = BN * 8 / TH;
   static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   static constexpr int LDS = 2 * (BM + BN) * 8 * 16;   // bytes
@@ -88,6 +91,133 @@ struct MMNt {
     }
   }
 };
+
+// The same for tiles of 256 x 256 by 8 waves (2 x 4, 128 x 64 each) where there are enough of them for every CU.  128 KB
+// of LDS hold a ring of four stages of 32 values: the loads of a stage have two stages' products (2048 cycles) to
+// arrive, and a wave waits for its own part of the next stage only, once a stage.  Operands are read two products' rows
+// ahead across the stages' borders, so that the matrix cores do not wait at the barrier either.
+// A row of a stage is 4 units of 16 bytes, unit u of row r at 4 r + (u ^ f(r)), so that any 8 or 16 consecutive rows of
+// an operand read lie in different banks.
+template <typename H, int P>
+struct MMNtBig {
+  static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, TH = 512, FM = 8, FN = 4, PER_CU = 1;
+  static constexpr int LDS = 4 * (BM + BN) * 4 * 16;   // bytes
+  floatx4 acc[FN][FM];
+  int wm, wn, lane;
+
+  __device__ __forceinline__ MMNtBig() {
+    const int wave = threadIdx.x >> 6;
+    lane = threadIdx.x & 63;
+    wm = (wave % WM) * (BM / WM);
+    wn = (wave / WM) * (BN / WN);
+  }
+  __device__ __forceinline__ int row(int j) const { return wm + 16 * j + (lane & 15); }
+  __device__ __forceinline__ int col(int i) const { return wn + 16 * i + 4 * (lane >> 4); }
+  static __device__ __forceinline__ int twist(int r) { return (r >> 1 & 3) ^ (r >> 3 & 1); }
+
+  __device__ __forceinline__ void run(const MMNtOperand<H>& a, int m0, const MMNtOperand<H>& b, int n0, int k0, int k1,
+                                      uint4* lds) {
+    typedef typename MMFrag<H>::vec vec;
+    constexpr int STAGE = (BM + BN) * 4;   // units
+    const int tid = threadIdx.x;
+    const H *pa[2], *pb[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = (tid >> 2) + 128 * j, u = ((tid & 3) ^ twist(r)) * 8;
+      pa[j] = a.p + (long)min(m0 + r, a.rows - 1) * a.ld + u;
+      pb[j] = b.p + (long)min(n0 + r, b.rows - 1) * b.ld + u;
+    }
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const int stages = (k1 - k0) * 2 * P;
+    if (stages <= 0) return;
+    long at = (long)k0 * MM_NT_K;   // of the next stage to load, and its pass
+    int pass = 0;
+    auto load = [&](int slot) {
+      const long oa = mm_nt_first<P>(pass) * a.plane + at, ob = mm_nt_second<P>(pass) * b.plane + at;
+      uint4* to = lds + slot * STAGE + (tid & ~63);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        __builtin_amdgcn_global_load_lds((mm_global_ptr)(pa[j] + oa), (mm_lds_ptr)(to + 512 * j), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((mm_global_ptr)(pb[j] + ob), (mm_lds_ptr)(to + BM * 4 + 512 * j), 16, 0, 0);
+      }
+      if (P == 1) {
+        at += 32;
+      } else if (++pass == P) {
+        pass = 0;
+        at += 32;
+      }
+    };
+    const int i16 = lane & 15, unit = 4 * i16 + ((lane >> 4) ^ twist(i16));
+    const int ua = 4 * wm + unit, ub = 4 * (BM + wn) + unit;
+    auto read_a = [&](int slot, int j) { return __builtin_bit_cast(vec, lds[slot * STAGE + ua + 64 * j]); };
+    auto read_b = [&](int slot, int i) { return __builtin_bit_cast(vec, lds[slot * STAGE + ub + 64 * i]); };
+    load(0);
+    if (stages > 1) load(1);
+    if (stages > 2) load(2);
+    if (stages > 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    else if (stages > 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    vec fa[4], fb[2][FN];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) fb[0][i] = read_b(0, i);
+    fa[0] = read_a(0, 0);
+    fa[1] = read_a(0, 1);
+    auto step = [&](int s, auto odd) {
+      constexpr int O = decltype(odd)::value;
+      // this wave's part of stage s + 1 has arrived; after the barrier every wave's has, and nobody reads stage s - 1
+      if (s + 2 < stages) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (s + 3 < stages) load((s + 3) & 3);
+      const int now = s & 3, next = (s + 1) & 3;
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        fa[(j + 2) & 3] = j + 2 < FM ? read_a(now, j + 2) : read_a(next, j + 2 - FM);
+        if (j >= 2 && j < 2 + FN) fb[O ^ 1][j - 2] = read_b(next, j - 2);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+          MMFrag<H> x{fb[O][i]}, y{fa[j & 3]};
+          mm_mma(acc[i][j], x, y);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    for (int s = 0; s < stages; s += 2) {   // stages come in pairs: 64 values
+      step(s, std::integral_constant<int, 0>{});
+      step(s + 1, std::integral_constant<int, 1>{});
+    }
+    __syncthreads();   // the last stage's reads (and those past it, of old values) are done
+  }
+};
+
+// Four 16-bit values of every lane, lane l holding row l & 3 of a 4 x 4 block by its quad of lanes: transposed, so that
+// lane l holds the block's column l & 3.  By lane moves inside the quad: pairs with the lane two further, then halves of
+// pairs with the next one.
+template <typename H>
+__device__ __forceinline__ void mm_quad_transpose(H (&v)[4]) {
+  typedef H pair __attribute__((ext_vector_type(2)));
+  const int r = threadIdx.x & 3;
+  const int w0 = __builtin_bit_cast(int, pair{v[0], v[1]}), w1 = __builtin_bit_cast(int, pair{v[2], v[3]});
+  const int got = __builtin_amdgcn_mov_dpp(r < 2 ? w1 : w0, 0x4E, 0xF, 0xF, true);   // quad_perm [2, 3, 0, 1]
+  const int lo = r < 2 ? w0 : got, hi = r < 2 ? got : w1;
+  const int lo1 = __builtin_amdgcn_mov_dpp(lo, 0xB1, 0xF, 0xF, true);                // quad_perm [1, 0, 3, 2]
+  const int hi1 = __builtin_amdgcn_mov_dpp(hi, 0xB1, 0xF, 0xF, true);
+  // even lanes: the low halves of their own and the other's; odd lanes: the high halves of the other's and their own
+  const unsigned pick = r & 1 ? 0x03020706 : 0x05040100;
+  const pair a = __builtin_bit_cast(pair, __builtin_amdgcn_perm(lo1, lo, pick));
+  const pair b = __builtin_bit_cast(pair, __builtin_amdgcn_perm(hi1, hi, pick));
+  v[0] = a[0];
+  v[1] = a[1];
+  v[2] = b[0];
+  v[3] = b[1];
+}
 
 // Tile of workgroup b among `batch` times tiles_m x tiles_n: consecutive numbers on one XCD (workgroups are dealt out to
 // the 8 XCDs in turn), in bands of 8 tiles of rows, so that neighbours share operands in that XCD's L2.  False: none.

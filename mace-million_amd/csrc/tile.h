@@ -2,6 +2,8 @@
 #pragma once
 #include "rowvec.h"
 
+#include <atomic>
+
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // ------------------------------------------------------------------------------------------------ matrix products
@@ -284,3 +286,22 @@ __device__ __forceinline__ void mm_stage_done() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 }
+
+namespace {
+// more than 64 KB of LDS has to be asked for, once per kernel and device
+template <auto KERNEL>
+bool lds_granted(int bytes) {
+  static std::atomic<unsigned long long> granted{0};   // a bit per device
+  int dev = 0;
+  if (bytes <= 65536) return true;
+  if (hipGetDevice(&dev) != hipSuccess) dev = 0;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (granted.load(std::memory_order_relaxed) & bit) return true;
+  if (hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) {
+    mm::set_error("the kernel's LDS was not granted");
+    return false;
+  }
+  granted.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+}  // namespace

@@ -85,13 +85,15 @@ def _run(x, w, y, dloss, reduction, **kw):
 
 SIZES = [(1, 1, 1), (1, 128, 89), (2, 3, 2), (17, 24, 19), (64, 64, 64), (130, 200, 300), (129, 128, 128),
          (300, 65, 1000), (1000, 32, 130), (5, 777, 2003), (257, 1000, 515), (2000, 16, 7), (9, 40, 70001),
-         (3, 2500, 33), (513, 256, 769)]
+         (3, 2500, 33), (513, 256, 769), (2047, 200, 6201), (2048, 2112, 6144)]
 
 
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,D,V", SIZES)
 def test_loss_and_gradients(T, D, V, dtype, reduction):
+    if T * V * D > 1e9 and reduction != "none":
+        pytest.skip("large tiles: once a type")
     x, w, y, dloss = (t.cuda() for t in _inputs(T, D, V, dtype, T + D + V))
     ref, bound = _reference(x, w, y, dloss, reduction, dtype)
     _check(_run(x, w, y, dloss, reduction), ref, bound)
