@@ -521,45 +521,10 @@ mm_ce_d_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
       }
     return;
   }
-  // Through LDS, so that whole lines go out: rows [BM][BN] of d, then columns [BN][BM] with the rows' shares; 16-byte
-  // units of a row are turned by its number, against bank conflicts.
-  typedef H vec __attribute__((ext_vector_type(4)));
   H* const tile = (H*)mm_ce_lds;
-#pragma unroll
-  for (int j = 0; j < Nt::FM; ++j)
-#pragma unroll
-    for (int i = 0; i < Nt::FN; ++i) {
-      const int m = t.row(j), n = t.col(i);
-      const floatx4& v = t.acc[i][j];
-      *(vec*)(tile + m * BN + ((n >> 3 ^ (m & 15)) << 3) + (n & 4)) = vec{(H)v[0], (H)v[1], (H)v[2], (H)v[3]};
-    }
-  __syncthreads();
-#pragma unroll 4
-  for (int q = threadIdx.x; q < BM * BN / 8; q += Nt::TH) {
-    const int m = q / (BN / 8), u = q % (BN / 8);
-    if (m0 + m < count && n0 + 8 * u < cols)
-      *(uint4*)(a.d + (long)(m0 + m) * a.ldd + n0 + 8 * u) = *(const uint4*)(tile + m * BN + ((u ^ (m & 15)) << 3));
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < Nt::FM; ++j)
-#pragma unroll
-    for (int i = 0; i < Nt::FN; ++i) {
-      // this lane's column n + (lane & 3), rows of its quad of lanes
-      H h[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) h[q] = (H)(t.acc[i][j][q] * share[j]);
-      mm_quad_transpose(h);
-      const int m = t.row(j) & ~3, n = t.col(i) + (t.lane & 3);
-      *(vec*)(tile + n * BM + ((m >> 3 ^ (n & 15)) << 3) + (m & 4)) = vec{h[0], h[1], h[2], h[3]};
-    }
-  __syncthreads();
-#pragma unroll 4
-  for (int q = threadIdx.x; q < BM * BN / 8; q += Nt::TH) {
-    const int n = q / (BM / 8), u = q % (BM / 8);
-    if (n0 + n < a.n && m0 + 8 * u < rows)
-      *(uint4*)(a.dT + (long)(n0 + n) * a.ldt + m0 + 8 * u) = *(const uint4*)(tile + n * BM + ((u ^ (n & 15)) << 3));
-  }
+  mm_nt_store(t, tile, a.d + (long)m0 * a.ldd + n0, a.ldd, count - m0, cols - n0, [&](int i, int j) { return t.acc[i][j]; });
+  mm_nt_store_transposed(t, tile, a.dT + (long)n0 * a.ldt + m0, a.ldt, rows - m0, a.n - n0,
+                         [&](int i, int j) { return t.acc[i][j] * share[j]; });
 }
 
 // C = A B^T of a piece.  dx: rows of A are the asked rows (count), fp32 sums part [splits][T][N], added to what is there

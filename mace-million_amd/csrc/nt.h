@@ -219,6 +219,52 @@ __device__ __forceinline__ void mm_quad_transpose(H (&v)[4]) {
   v[3] = b[1];
 }
 
+// A workgroup's results as rows of 16-bit values, through LDS (`tile`, BM x BN values, free before and after) so that
+// whole lines go out: out[m][n] for m < rows, n < cols, cols a multiple of 8 and rows of out 16-byte aligned.
+// value(i, j): the four values of acc[i][j].  Units of 16 bytes are turned by their row's number, against bank conflicts.
+template <typename H, typename Nt, typename F>
+__device__ __forceinline__ void mm_nt_store(const Nt& t, H* tile, H* out, long ld, int rows, int cols, F value) {
+  typedef H vec __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int j = 0; j < Nt::FM; ++j)
+#pragma unroll
+    for (int i = 0; i < Nt::FN; ++i) {
+      const int m = t.row(j), n = t.col(i);
+      const floatx4 v = value(i, j);
+      *(vec*)(tile + m * Nt::BN + ((n >> 3 ^ (m & 7)) << 3) + (n & 4)) = vec{(H)v[0], (H)v[1], (H)v[2], (H)v[3]};
+    }
+  __syncthreads();
+#pragma unroll 4
+  for (int q = threadIdx.x; q < Nt::BM * Nt::BN / 8; q += Nt::TH) {
+    const int m = q / (Nt::BN / 8), u = q % (Nt::BN / 8);
+    if (m < rows && 8 * u < cols) *(uint4*)(out + (long)m * ld + 8 * u) = *(const uint4*)(tile + m * Nt::BN + ((u ^ (m & 7)) << 3));
+  }
+  __syncthreads();
+}
+
+// The same transposed: out[n][m] for n < cols, m < rows, rows a multiple of 8.
+template <typename H, typename Nt, typename F>
+__device__ __forceinline__ void mm_nt_store_transposed(const Nt& t, H* tile, H* out, long ld, int rows, int cols, F value) {
+  typedef H vec __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int j = 0; j < Nt::FM; ++j)
+#pragma unroll
+    for (int i = 0; i < Nt::FN; ++i) {
+      const floatx4 v = value(i, j);
+      H h[4] = {(H)v[0], (H)v[1], (H)v[2], (H)v[3]};
+      mm_quad_transpose(h);   // this lane's column n + (lane & 3), rows of its quad of lanes
+      const int m = t.row(j) & ~3, n = t.col(i) + (t.lane & 3);
+      *(vec*)(tile + n * Nt::BM + ((m >> 3 ^ (n & 7)) << 3) + (m & 4)) = vec{h[0], h[1], h[2], h[3]};
+    }
+  __syncthreads();
+#pragma unroll 4
+  for (int q = threadIdx.x; q < Nt::BM * Nt::BN / 8; q += Nt::TH) {
+    const int n = q / (Nt::BM / 8), u = q % (Nt::BM / 8);
+    if (n < cols && 8 * u < rows) *(uint4*)(out + (long)n * ld + 8 * u) = *(const uint4*)(tile + n * Nt::BM + ((u ^ (n & 7)) << 3));
+  }
+  __syncthreads();
+}
+
 // Tile of workgroup b among `batch` times tiles_m x tiles_n: consecutive numbers on one XCD (workgroups are dealt out to
 // the 8 XCDs in turn), in bands of 8 tiles of rows, so that neighbours share operands in that XCD's L2.  False: none.
 __device__ __forceinline__ bool mm_nt_tile(int b, int batch, int tiles_m, int tiles_n, int* e, int* tm, int* tn) {
@@ -231,6 +277,20 @@ __device__ __forceinline__ bool mm_nt_tile(int b, int batch, int tiles_m, int ti
   const int band = at / (8 * tiles_n), high = min(8, tiles_m - 8 * band), r = at - band * 8 * tiles_n;
   *tm = 8 * band + r % high;
   *tn = r / high;
+  return true;
+}
+
+// The same for the tiles on and below the diagonal of `batch` square products of `tiles` x `tiles`.
+__device__ __forceinline__ bool mm_nt_lower(int b, int batch, int tiles, int* e, int* tm, int* tn) {
+  const int one = tiles * (tiles + 1) / 2, all = batch * one;
+  if (b >= all) return false;
+  const int share = all / 8, rest = all % 8, x = b % 8;
+  int at = x * share + min(x, rest) + b / 8, m = 0;
+  *e = at / one;
+  at -= *e * one;
+  while (at > m) at -= ++m;   // row m has m + 1 tiles
+  *tm = m;
+  *tn = at;
   return true;
 }
 

@@ -37,13 +37,6 @@ __device__ __forceinline__ void mm_ortho_put4(_Float16* __restrict__ p, long pla
   for (int q = 0; q < PLANES; ++q) *(halfx4*)(p + q * plane) = h[q];
 }
 
-template <int PLANES>
-__device__ __forceinline__ void mm_ortho_put(_Float16* __restrict__ p, long plane, float v) {
-  const _Float16 h = (_Float16)v;
-  p[0] = h;
-  if constexpr (PLANES == 2) p[plane] = (_Float16)(v - (float)h);
-}
-
 // sums of squares of parts of matrix blockIdx.y
 template <typename T>
 __global__ void __launch_bounds__(256) mm_ortho_norm_kernel(const T* __restrict__ m, long size, double* __restrict__ part) {
@@ -123,14 +116,44 @@ __global__ void __launch_bounds__(256) mm_ortho_start_kernel(MMOrtho a, int step
   }
 }
 
-// A = X X^T (WHAT 0) or B = b A + c A A (1): planes [side][lda], zeros past the last column
-template <int P, int WHAT, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2) mm_ortho_square_kernel(MMOrtho a, int tiles) {
-  typedef MMNt<_Float16, P, BM, BN, WM, WN> Nt;
+// plane q of the values f v
+template <int Q>
+__device__ __forceinline__ floatx4 mm_ortho_plane(floatx4 v, float f) {
+  v *= f;
+  if constexpr (Q == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] -= (float)(_Float16)v[i];
+  }
+  return v;
+}
+
+template <int PLANES, typename Nt>
+__device__ __forceinline__ void mm_ortho_tiles(const Nt& t, uint4* lds, _Float16* out, long ld, long plane, int rows,
+                                               int cols, float f) {
+  mm_nt_store(t, (_Float16*)lds, out, ld, rows, cols, [&](int i, int j) { return mm_ortho_plane<0>(t.acc[i][j], f); });
+  if constexpr (PLANES == 2)
+    mm_nt_store(t, (_Float16*)lds, out + plane, ld, rows, cols,
+                [&](int i, int j) { return mm_ortho_plane<1>(t.acc[i][j], f); });
+}
+
+template <int PLANES, typename Nt>
+__device__ __forceinline__ void mm_ortho_tiles_transposed(const Nt& t, uint4* lds, _Float16* out, long ld, long plane,
+                                                          int rows, int cols, float f) {
+  mm_nt_store_transposed(t, (_Float16*)lds, out, ld, rows, cols,
+                         [&](int i, int j) { return mm_ortho_plane<0>(t.acc[i][j], f); });
+  if constexpr (PLANES == 2)
+    mm_nt_store_transposed(t, (_Float16*)lds, out + plane, ld, rows, cols,
+                           [&](int i, int j) { return mm_ortho_plane<1>(t.acc[i][j], f); });
+}
+
+// A = X X^T (WHAT 0) or B = b A + c A A (1): planes [side][lda], zeros past the last column.  Both are symmetric: tiles
+// below the diagonal are written twice, those above are not computed.
+template <int P, int WHAT, typename Nt>
+__global__ void __launch_bounds__(Nt::TH, Nt::PER_CU) mm_ortho_square_kernel(MMOrtho a, int tiles) {
   constexpr int PLANES = P == 1 ? 1 : 2;
   extern __shared__ uint4 mm_ortho_lds[];
   int e, tm, tn;
-  if (!mm_nt_tile(blockIdx.x, a.batch, tiles, tiles, &e, &tm, &tn)) return;
+  if (!mm_nt_lower(blockIdx.x, a.batch, tiles, &e, &tm, &tn)) return;
   MMNtOperand<_Float16> x;
   int k;
   if constexpr (WHAT == 1) {
@@ -143,95 +166,94 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mm_ortho_square_kernel(MMOrth
     x = {a.v + (long)e * a.cols * a.ldv, a.ldv, a.pv, a.side};
     k = (int)(a.ldv / MM_NT_K);
   }
+  const int m0 = tm * Nt::BM, n0 = tn * Nt::BN;
   Nt t;
-  t.run(x, tm * BM, x, tn * BN, 0, k, mm_ortho_lds);
+  t.run(x, m0, x, n0, 0, k, mm_ortho_lds);
   _Float16* out = (WHAT ? a.b : a.a) + (long)e * a.side * a.lda;
   const _Float16* in = a.a + (long)e * a.side * a.lda;
 #pragma unroll
   for (int j = 0; j < Nt::FM; ++j) {
-    const int m = tm * BM + t.row(j);
-    if (m >= a.side) continue;
+    const int m = m0 + t.row(j);
 #pragma unroll
     for (int i = 0; i < Nt::FN; ++i) {
-      const int n = tn * BN + t.col(i);
-      if (n >= a.lda) continue;
-      float v[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (WHAT == 0) {
-          v[q] = t.acc[i][j][q] * (MM_ORTHO_A / (MM_ORTHO_X * MM_ORTHO_X));
+      const int n = n0 + t.col(i);
+      floatx4 v = {};
+      if (m < a.side && n < a.side) {
+        if constexpr (WHAT == 0) {
+          v = t.acc[i][j] * (MM_ORTHO_A / (MM_ORTHO_X * MM_ORTHO_X));
         } else {
-          const long at = (long)m * a.lda + n + q;
-          const float old = (float)in[at] + (PLANES == 2 ? (float)in[at + a.pa] : 0.f);
-          v[q] = a.cb * (MM_ORTHO_B / MM_ORTHO_A) * old
-               + a.cc * (MM_ORTHO_B / (MM_ORTHO_A * MM_ORTHO_A)) * t.acc[i][j][q];
+          const halfx4 h = *(const halfx4*)(in + (long)m * a.lda + n);
+          const halfx4 l = *(const halfx4*)(in + (PLANES == 2 ? a.pa : 0) + (long)m * a.lda + n);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float old = (float)h[q] + (PLANES == 2 ? (float)l[q] : 0.f);
+            v[q] = a.cb * (MM_ORTHO_B / MM_ORTHO_A) * old
+                 + a.cc * (MM_ORTHO_B / (MM_ORTHO_A * MM_ORTHO_A)) * t.acc[i][j][q];
+          }
         }
-        if (n + q >= a.side) v[q] = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = n + q < a.side ? v[q] : 0.f;
       }
-      mm_ortho_put4<PLANES>(out + (long)m * a.lda + n, a.pa, v);
+      t.acc[i][j] = v;
     }
   }
+  const int left = (int)a.lda - n0, low = (int)a.lda - m0;   // columns with their zeros
+  mm_ortho_tiles<PLANES>(t, mm_ortho_lds, out + (long)m0 * a.lda + n0, a.lda, a.pa, a.side - m0, left, 1.f);
+  if (tm != tn)
+    mm_ortho_tiles_transposed<PLANES>(t, mm_ortho_lds, out + (long)n0 * a.lda + m0, a.lda, a.pa, low, a.side - n0, 1.f);
 }
 
 // X <- a X + B X (rows <= cols) or a X + X B; the last step writes out alone.  Other workgroups still read the operand
 // of X's planes: its new values go to a.next.
-template <typename T, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2)
+template <typename T, typename Nt>
+__global__ void __launch_bounds__(Nt::TH, Nt::PER_CU)
 mm_ortho_step_kernel(MMOrtho a, int tiles_m, int tiles_n, int last) {
-  constexpr int P = MMOrthoType<T>::P, PLANES = MMOrthoType<T>::PLANES;
-  typedef MMNt<_Float16, P, BM, BN, WM, WN> Nt;
+  constexpr int PLANES = MMOrthoType<T>::PLANES;
   extern __shared__ uint4 mm_ortho_lds[];
   int e, tm, tn;
   if (!mm_nt_tile(blockIdx.x, a.batch, tiles_m, tiles_n, &e, &tm, &tn)) return;
   const MMNtOperand<_Float16> b{a.b + (long)e * a.side * a.lda, a.lda, a.pa, a.side};
   const bool wide = a.rows <= a.cols;
   _Float16 *u = wide ? a.u : a.next, *vt = wide ? a.next : a.v;
+  const int m0 = tm * Nt::BM, n0 = tn * Nt::BN;
   Nt t;
   if (wide) {
     const MMNtOperand<_Float16> x{a.v + (long)e * a.cols * a.ldv, a.ldv, a.pv, a.cols};
-    t.run(b, tm * BM, x, tn * BN, 0, (int)(a.lda / MM_NT_K), mm_ortho_lds);
+    t.run(b, m0, x, n0, 0, (int)(a.lda / MM_NT_K), mm_ortho_lds);
   } else {
     const MMNtOperand<_Float16> x{a.u + (long)e * a.rows * a.ldu, a.ldu, a.pu, a.rows};
-    t.run(x, tm * BM, b, tn * BN, 0, (int)(a.lda / MM_NT_K), mm_ortho_lds);
+    t.run(x, m0, b, n0, 0, (int)(a.lda / MM_NT_K), mm_ortho_lds);
   }
 #pragma unroll
   for (int j = 0; j < Nt::FM; ++j) {
-    const int m = tm * BM + t.row(j);
-    if (m >= a.ldv) continue;
+    const int m = m0 + t.row(j);
     const long row = ((long)e * a.rows + m) * a.cols;
 #pragma unroll
     for (int i = 0; i < Nt::FN; ++i) {
-      const int n = tn * BN + t.col(i);
-      if (n >= a.ldu) continue;
-      float v[4] = {};   // zeros past the last row and column
-      if (m < a.rows) {
-        mm_load4(a.x + row, n, a.cols, v);
+      const int n = n0 + t.col(i);
+      floatx4 v = {};   // zeros past the last row and column
+      if (m < a.rows && n < a.cols) {
+        mm_load4(a.x + row, n, a.cols, (float*)&v);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           v[q] = n + q < a.cols ? fmaf(t.acc[i][j][q], 1.f / (MM_ORTHO_B * MM_ORTHO_X), a.ca * v[q]) : 0.f;
-        if (last) {
-          mm_store4((T*)a.out + row, n, a.cols, v);
-          continue;
-        }
-        mm_store4(a.x + row, n, a.cols, v);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] *= MM_ORTHO_X;
-        mm_ortho_put4<PLANES>(u + ((long)e * a.rows + m) * a.ldu + n, a.pu, v);
-      } else if (last) {
-        continue;
+        if (last) mm_store4((T*)a.out + row, n, a.cols, (const float*)&v);
+        else mm_store4(a.x + row, n, a.cols, (const float*)&v);
       }
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (n + q < a.cols) mm_ortho_put<PLANES>(vt + ((long)e * a.cols + n + q) * a.ldv + m, a.pv, v[q]);
+      t.acc[i][j] = v;
     }
   }
+  if (last) return;
+  mm_ortho_tiles<PLANES>(t, mm_ortho_lds, u + ((long)e * a.rows + m0) * a.ldu + n0, a.ldu, a.pu, a.rows - m0,
+                         (int)a.ldu - n0, MM_ORTHO_X);
+  mm_ortho_tiles_transposed<PLANES>(t, mm_ortho_lds, vt + ((long)e * a.cols + n0) * a.ldv + m0, a.ldv, a.pv,
+                                    (int)a.ldv - m0, a.cols - n0, MM_ORTHO_X);
 }
 
 namespace {
-constexpr int BM = 128, BN = 128;
 constexpr long MAX_SIDE = 65536;
 
-long divtup(long a, long b) { return (a + b - 1) / b; }
+long div_up(long a, long b) { return (a + b - 1) / b; }
 
 struct Space {
   char* base;
@@ -254,7 +276,7 @@ size_t space(MMOrtho* a, int dtype, char* base) {
   a->pu = (long)a->batch * a->rows * a->ldu;
   a->pv = (long)a->batch * a->cols * a->ldv;
   a->pa = (long)a->batch * a->side * a->lda;
-  const long parts = divtup((long)a->rows * a->cols, 256 * 32);
+  const long parts = div_up((long)a->rows * a->cols, 256 * 32);
   a->parts = (int)(parts < MM_ORTHO_PARTS ? parts : MM_ORTHO_PARTS);
   a->part = p.take<double>((size_t)a->batch * a->parts);
   a->x = p.take<float>((size_t)a->batch * a->rows * a->cols);
@@ -266,28 +288,61 @@ size_t space(MMOrtho* a, int dtype, char* base) {
   return p.used;
 }
 
+// Side of the tiles of `tiles` (at 256, 128, 64) workgroups: the least time by whole rounds of the 256 CUs, a tile of 256
+// taking 1 alone on its CU, tiles of 128 (two on a CU) 0.59 a round, tiles of 64 (four) 0.5: the rates that products of
+// 1024 and more reach with each.
+int tile_side(long t256, long t128, long t64) {
+  const double big = (double)div_up(t256, 256), mid = 0.59 * (double)div_up(t128, 512), low = 0.5 * (double)div_up(t64, 1024);
+  return big <= mid && big <= low ? 256 : mid <= low ? 128 : 64;
+}
+
+template <auto KERNEL, typename Nt, typename... A>
+bool launch(const MMOrtho& a, long workgroups, hipStream_t stream, A... rest) {
+  if (!lds_granted<KERNEL>(Nt::LDS)) return false;
+  hipLaunchKernelGGL(KERNEL, dim3((unsigned)workgroups), dim3(Nt::TH), Nt::LDS, stream, a, rest...);
+  return true;
+}
+
+template <int P, int WHAT, typename Nt>
+bool square(const MMOrtho& a, hipStream_t stream) {
+  const int t = (int)div_up(a.side, Nt::BM);
+  return launch<mm_ortho_square_kernel<P, WHAT, Nt>, Nt>(a, (long)a.batch * t * (t + 1) / 2, stream, t);
+}
+
+template <typename T, typename Nt>
+bool step(const MMOrtho& a, int last, hipStream_t stream) {
+  const int tm = (int)div_up(a.rows, Nt::BM), tn = (int)div_up(a.cols, Nt::BN);
+  return launch<mm_ortho_step_kernel<T, Nt>, Nt>(a, (long)a.batch * tm * tn, stream, tm, tn, last);
+}
+
 template <typename T>
 int orthogonalize(MMOrtho a, int steps, const float* c, hipStream_t stream) {
   constexpr int P = MMOrthoType<T>::P;
-  typedef MMNt<_Float16, P, BM, BN, 2, 2> Nt;
+  typedef MMNtBig<_Float16, P> Big;
+  typedef MMNt<_Float16, P, 128, 128, 2, 2> Mid;
+  typedef MMNt<_Float16, P, 64, 64, 2, 2> Low;
   hipLaunchKernelGGL(mm_ortho_norm_kernel<T>, dim3(a.parts, a.batch), dim3(256), 0, stream, (const T*)a.m,
                      (long)a.rows * a.cols, a.part);
-  hipLaunchKernelGGL(mm_ortho_start_kernel<T>, dim3((unsigned)divtup(a.rows, 64), (unsigned)divtup(a.cols, 64), a.batch),
+  hipLaunchKernelGGL(mm_ortho_start_kernel<T>, dim3((unsigned)div_up(a.rows, 64), (unsigned)div_up(a.cols, 64), a.batch),
                      dim3(256), 0, stream, a, steps);
-  const int sq = (int)divtup(a.side, BM), tm = (int)divtup(a.rows, BM), tn = (int)divtup(a.cols, BN);
-  for (int i = 0; i < steps; ++i, c += 3) {
+  auto lower = [&](long n) { return a.batch * div_up(a.side, n) * (div_up(a.side, n) + 1) / 2; };
+  auto all = [&](long n) { return a.batch * div_up(a.rows, n) * div_up(a.cols, n); };
+  const int sq = tile_side(lower(256), lower(128), lower(64)), st = tile_side(all(256), all(128), all(64));
+  bool ok = true;
+  for (int i = 0; i < steps && ok; ++i, c += 3) {
     a.ca = c[0];
     a.cb = c[1];
     a.cc = c[2];
-    hipLaunchKernelGGL((mm_ortho_square_kernel<P, 0, BM, BN, 2, 2>), dim3(a.batch * sq * sq), dim3(256), Nt::LDS, stream, a,
-                       sq);
-    hipLaunchKernelGGL((mm_ortho_square_kernel<P, 1, BM, BN, 2, 2>), dim3(a.batch * sq * sq), dim3(256), Nt::LDS, stream, a,
-                       sq);
-    hipLaunchKernelGGL((mm_ortho_step_kernel<T, BM, BN, 2, 2>), dim3(a.batch * tm * tn), dim3(256), Nt::LDS, stream, a, tm,
-                       tn, i + 1 == steps);
+    if (sq == 256) ok = square<P, 0, Big>(a, stream) && square<P, 1, Big>(a, stream);
+    else if (sq == 128) ok = square<P, 0, Mid>(a, stream) && square<P, 1, Mid>(a, stream);
+    else ok = square<P, 0, Low>(a, stream) && square<P, 1, Low>(a, stream);
+    const int last = i + 1 == steps;
+    if (st == 256) ok = ok && step<T, Big>(a, last, stream);
+    else if (st == 128) ok = ok && step<T, Mid>(a, last, stream);
+    else ok = ok && step<T, Low>(a, last, stream);
     std::swap(a.next, a.rows <= a.cols ? a.v : a.u);
   }
-  return mm::launch_status("mm_orthogonalize");
+  return ok ? mm::launch_status("mm_orthogonalize") : MM_ELAUNCH;
 }
 
 int check(const char* name, long batch, long rows, long cols, int dtype) {
@@ -296,7 +351,7 @@ int check(const char* name, long batch, long rows, long cols, int dtype) {
     return MM_EINVAL;
   }
   if (rows > MAX_SIDE || cols > MAX_SIDE || batch > 65535 ||
-      batch * divtup(rows, 64) * divtup(cols, 64) * 256 >= 4294967296L) {
+      batch * div_up(rows, 64) * div_up(cols, 64) * 256 >= 4294967296L) {
     mm::set_error(std::string(name) + ": sizes beyond the launches' limits");
     return MM_ERANGE;
   }
