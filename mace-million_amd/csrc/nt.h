@@ -20,18 +20,18 @@ struct MMNtOperand {
 
 // planes of pass q
 template <int P>
-__device__ __forceinline__ int mm_nt_first(int q) {
+__device__ __forceinline__ constexpr int mm_nt_first(int q) {
   return P == 1 ? 0 : P == 3 ? (q == 0 ? 1 : 0) : (q == 0 ? 2 : q == 1 || q == 3 ? 1 : 0);
 }
 template <int P>
-__device__ __forceinline__ int mm_nt_second(int q) {
+__device__ __forceinline__ constexpr int mm_nt_second(int q) {
   return P == 1 ? 0 : P == 3 ? (q == 1 ? 1 : 0) : (q == 2 ? 2 : q == 1 || q == 4 ? 1 : 0);
 }
 
 // A workgroup's tile of BM rows of A by BN rows of B, WM x WN waves; lane's results acc[i][j][q]: row m = wm + 16 j +
 // (lane & 15) of the tile, column n = wn + 16 i + 4 (lane >> 4) + q.
 template <typename H, int P, int BM_, int BN_, int WM_, int WN_>
-struct MMNt {
+struct MMNtOne {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, PER_CU = 2;
   static constexpr int TH = 64 * WM * WN, UA = BM * 8 / TH, UB = BN * 8 / TH;
   static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
@@ -39,7 +39,7 @@ struct MMNt {
   floatx4 acc[FN][FM];
   int wm, wn, lane;
 
-  __device__ __forceinline__ MMNt() {
+  __device__ __forceinline__ MMNtOne() {
     const int wave = threadIdx.x >> 6;
     lane = threadIdx.x & 63;
     wm = (wave % WM) * (BM / WM);
@@ -91,6 +91,108 @@ struct MMNt {
     }
   }
 };
+
+// The same for operands of several planes (P > 1): a stage holds all planes of 32 values, so that a plane is loaded once
+// for the products that it enters.  A ring of SLOTS stages, loads SLOTS - 1 stages ahead; units lie as in MMNtBig.
+template <typename H, int P, int BM_, int BN_, int WM_, int WN_>
+struct MMNtPlanes {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, TH = 64 * WM * WN, PL = P == 3 ? 2 : 3;
+  static constexpr int FM = BM / WM / 16, FN = BN / WN / 16, STAGE = PL * (BM + BN) * 4;   // units
+  static constexpr int SLOTS = STAGE <= 1024 ? 4 : STAGE == 2048 ? 2 : 3, LDS = SLOTS * STAGE * 16;
+  static constexpr int PER_CU = LDS <= 81920 ? 2 : 1, LOADS = STAGE / TH;
+  floatx4 acc[FN][FM];
+  int wm, wn, lane;
+
+  __device__ __forceinline__ MMNtPlanes() {
+    const int wave = threadIdx.x >> 6;
+    lane = threadIdx.x & 63;
+    wm = (wave % WM) * (BM / WM);
+    wn = (wave / WM) * (BN / WN);
+  }
+  __device__ __forceinline__ int row(int j) const { return wm + 16 * j + (lane & 15); }
+  __device__ __forceinline__ int col(int i) const { return wn + 16 * i + 4 * (lane >> 4); }
+  static __device__ __forceinline__ int twist(int r) { return (r >> 1 & 3) ^ (r >> 3 & 1); }
+
+  __device__ __forceinline__ void run(const MMNtOperand<H>& a, int m0, const MMNtOperand<H>& b, int n0, int k0, int k1,
+                                      uint4* lds) {
+    typedef typename MMFrag<H>::vec vec;
+    constexpr int UA = BM * 4 / TH, UB = BN * 4 / TH;   // units of a thread and plane
+    const int tid = threadIdx.x;
+    const H *pa[UA], *pb[UB];
+#pragma unroll
+    for (int j = 0; j < UA; ++j) {
+      const int r = (tid + TH * j) >> 2;
+      pa[j] = a.p + (long)min(m0 + r, a.rows - 1) * a.ld + ((tid & 3) ^ twist(r)) * 8;
+    }
+#pragma unroll
+    for (int j = 0; j < UB; ++j) {
+      const int r = (tid + TH * j) >> 2;
+      pb[j] = b.p + (long)min(n0 + r, b.rows - 1) * b.ld + ((tid & 3) ^ twist(r)) * 8;
+    }
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const int stages = (k1 - k0) * 2;
+    if (stages <= 0) return;
+    auto load = [&](int s) {
+      const long at = (long)k0 * MM_NT_K + 32 * s;
+      uint4* to = lds + s % SLOTS * STAGE + (tid & ~63);
+#pragma unroll
+      for (int p = 0; p < PL; ++p) {
+#pragma unroll
+        for (int j = 0; j < UA; ++j)
+          __builtin_amdgcn_global_load_lds((mm_global_ptr)(pa[j] + p * a.plane + at),
+                                           (mm_lds_ptr)(to + p * BM * 4 + TH * j), 16, 0, 0);
+#pragma unroll
+        for (int j = 0; j < UB; ++j)
+          __builtin_amdgcn_global_load_lds((mm_global_ptr)(pb[j] + p * b.plane + at),
+                                           (mm_lds_ptr)(to + (PL * BM + p * BN) * 4 + TH * j), 16, 0, 0);
+      }
+    };
+    const int i16 = lane & 15, unit = 4 * i16 + ((lane >> 4) ^ twist(i16));
+#pragma unroll
+    for (int s = 0; s < SLOTS - 1; ++s)
+      if (s < stages) load(s);
+    for (int s = 0; s < stages; ++s) {
+      // this wave's part of stage s has arrived; after the barrier every wave's has, and nobody reads stage s - 1
+      if (s + SLOTS - 2 < stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((SLOTS - 2) * LOADS) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (s + SLOTS - 1 < stages) load(s + SLOTS - 1);
+      const uint4* A = lds + s % SLOTS * STAGE + 4 * wm + unit;
+      const uint4* B = lds + s % SLOTS * STAGE + 4 * (PL * BM + wn) + unit;
+      vec fb[PL][FN], fa[2][PL];
+#pragma unroll
+      for (int p = 0; p < PL; ++p) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i) fb[p][i] = __builtin_bit_cast(vec, B[4 * BN * p + 64 * i]);
+        fa[0][p] = __builtin_bit_cast(vec, A[4 * BM * p]);
+      }
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        if (j + 1 < FM) {
+#pragma unroll
+          for (int p = 0; p < PL; ++p) fa[(j + 1) & 1][p] = __builtin_bit_cast(vec, A[4 * BM * p + 64 * (j + 1)]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+#pragma unroll
+          for (int i = 0; i < FN; ++i) {
+            MMFrag<H> x{fb[mm_nt_second<P>(q)][i]}, y{fa[j & 1][mm_nt_first<P>(q)]};
+            mm_mma(acc[i][j], x, y);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __syncthreads();
+  }
+};
+
+template <typename H, int P, int BM, int BN, int WM, int WN>
+using MMNt = std::conditional_t<P == 1, MMNtOne<H, P, BM, BN, WM, WN>, MMNtPlanes<H, P, BM, BN, WM, WN>>;
 
 // The same for tiles of 256 x 256 by 8 waves (2 x 4, 128 x 64 each) where there are enough of them for every CU.  128 KB
 // of LDS hold a ring of four stages of 32 values: the loads of a stage have two stages' products (2048 cycles) to

@@ -116,34 +116,51 @@ __global__ void __launch_bounds__(256) mm_ortho_start_kernel(MMOrtho a, int step
   }
 }
 
-// plane q of the values f v
-template <int Q>
-__device__ __forceinline__ floatx4 mm_ortho_plane(floatx4 v, float f) {
-  v *= f;
-  if constexpr (Q == 1) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] -= (float)(_Float16)v[i];
-  }
-  return v;
-}
-
+// out = f acc as planes, rows (or, transposed, columns) of it: one plane through LDS in whole lines, two from the
+// registers (their tiles are small, and LDS would take two barriers for each plane)
 template <int PLANES, typename Nt>
 __device__ __forceinline__ void mm_ortho_tiles(const Nt& t, uint4* lds, _Float16* out, long ld, long plane, int rows,
                                                int cols, float f) {
-  mm_nt_store(t, (_Float16*)lds, out, ld, rows, cols, [&](int i, int j) { return mm_ortho_plane<0>(t.acc[i][j], f); });
-  if constexpr (PLANES == 2)
-    mm_nt_store(t, (_Float16*)lds, out + plane, ld, rows, cols,
-                [&](int i, int j) { return mm_ortho_plane<1>(t.acc[i][j], f); });
+  if constexpr (PLANES == 1) {
+    mm_nt_store(t, (_Float16*)lds, out, ld, rows, cols, [&](int i, int j) { return t.acc[i][j] * f; });
+  } else {
+#pragma unroll
+    for (int j = 0; j < Nt::FM; ++j)
+#pragma unroll
+      for (int i = 0; i < Nt::FN; ++i) {
+        const floatx4 v = t.acc[i][j] * f;
+        if (t.row(j) < rows && t.col(i) < cols)
+          mm_ortho_put4<2>(out + (long)t.row(j) * ld + t.col(i), plane, (const float*)&v);
+      }
+  }
 }
 
 template <int PLANES, typename Nt>
 __device__ __forceinline__ void mm_ortho_tiles_transposed(const Nt& t, uint4* lds, _Float16* out, long ld, long plane,
                                                           int rows, int cols, float f) {
-  mm_nt_store_transposed(t, (_Float16*)lds, out, ld, rows, cols,
-                         [&](int i, int j) { return mm_ortho_plane<0>(t.acc[i][j], f); });
-  if constexpr (PLANES == 2)
-    mm_nt_store_transposed(t, (_Float16*)lds, out + plane, ld, rows, cols,
-                           [&](int i, int j) { return mm_ortho_plane<1>(t.acc[i][j], f); });
+  if constexpr (PLANES == 1) {
+    mm_nt_store_transposed(t, (_Float16*)lds, out, ld, rows, cols, [&](int i, int j) { return t.acc[i][j] * f; });
+  } else {
+#pragma unroll
+    for (int j = 0; j < Nt::FM; ++j)
+#pragma unroll
+      for (int i = 0; i < Nt::FN; ++i) {
+        const int m = t.row(j) & ~3, n = t.col(i) + (t.lane & 3);
+        const floatx4 v = t.acc[i][j] * f;
+        _Float16 h[4], l[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          h[q] = (_Float16)v[q];
+          l[q] = (_Float16)(v[q] - (float)h[q]);
+        }
+        mm_quad_transpose(h);
+        mm_quad_transpose(l);
+        if (m < rows && n < cols) {
+          *(halfx4*)(out + (long)n * ld + m) = halfx4{h[0], h[1], h[2], h[3]};
+          *(halfx4*)(out + plane + (long)n * ld + m) = halfx4{l[0], l[1], l[2], l[3]};
+        }
+      }
+  }
 }
 
 // A = X X^T (WHAT 0) or B = b A + c A A (1): planes [side][lda], zeros past the last column.  Both are symmetric: tiles
@@ -250,6 +267,203 @@ mm_ortho_step_kernel(MMOrtho a, int tiles_m, int tiles_n, int last) {
                                     (int)a.ldv - m0, a.cols - n0, MM_ORTHO_X);
 }
 
+// ------------------------------------------------------------------------------------------------ small matrices
+// All steps of a small matrix in one workgroup and one launch: wave w holds the rows 16 w .. 16 w + 15 of X (its shorter
+// side) in fp32 registers, and LDS the planes of X, then those of W.  A step:
+//     A = X X^T: a wave's rows of A, which as they come out of the matrix cores are operands of the next two products
+//     W = b X + c (A X), which takes X's place in LDS;  X <- a X + A W, which takes it back
+// so that neither A nor B is stored (B X = A (b X + c A X)).  The order of an operand along the summed index is free as
+// long as both operands agree: 32 values are taken as k = 16 (e / 4) + 4 g + e % 4, the order in which a lane has its
+// results.  |W| stays below 16 where |X| does.  Bound by LDS (an operand read from it meets 16 rows only) and barriers.
+struct MMOrthoSmall {
+  const void* m;
+  void* out;
+  int rows, cols, side, other, steps;   // side <= other: of X
+  float eps, c[3 * 16];                 // a, b, c of at most 16 steps
+};
+
+template <typename T, int WAVES, int NT>
+__global__ void __launch_bounds__(64 * WAVES) mm_ortho_small_kernel(MMOrthoSmall a) {
+  // units of 16 bytes of a row: an odd number, so that any 8 consecutive rows lie in different banks
+  constexpr int PLANES = MMOrthoType<T>::PLANES, P = MMOrthoType<T>::P, MS = WAVES / 2, UNITS = 2 * NT + 1;
+  typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  extern __shared__ uint4 mm_ortho_lds[];
+  __shared__ double s_norm[WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g = lane >> 4;
+  const int mt = (a.side + 15) / 16, ms = (a.side + 31) / 32, plane = ms * 32 * UNITS;   // units of a plane
+  const int row = 16 * wave + i16;
+  const bool wide = a.rows <= a.cols, live = row < a.side, here = wave < 2 * ms, work = wave < mt;
+  const size_t size = (size_t)a.rows * a.cols, base = blockIdx.x * size;
+  floatx4 x[NT], acc[NT > WAVES ? NT : WAVES];
+  double norm = 0.;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int n = 16 * i + 4 * g;
+    x[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (live && wide) {
+      mm_load4((const T*)a.m + base + (size_t)row * a.cols, n, a.cols, (float*)&x[i]);
+    } else if (live) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (n + q < a.other) x[i][q] = (float)((const T*)a.m)[base + (size_t)(n + q) * a.cols + row];
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) norm = fma((double)x[i][q], (double)x[i][q], norm);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) norm += __shfl_xor(norm, d);
+  if (lane == 0) s_norm[wave] = norm;
+  __syncthreads();
+  norm = 0.;
+  for (int w = 0; w < WAVES; ++w) norm += s_norm[w];
+  const double by = 1. / (sqrt(norm) + (double)a.eps);
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[i][q] = x[i][q] == 0.f ? x[i][q] : (float)((double)x[i][q] * by);   // no norm: zeros
+
+  _Float16* const tile = (_Float16*)mm_ortho_lds;
+  auto put = [&](floatx4 r, int i) {   // 4 values of tile i of this lane's row
+    r *= MM_ORTHO_X;
+    _Float16* const at = tile + 8 * (row * UNITS + 2 * i) + 4 * g;
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) {
+      halfx4 h;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        h[q] = (_Float16)r[q];
+        r[q] -= (float)h[q];
+      }
+      *(halfx4*)(at + 8 * p * plane) = h;
+    }
+  };
+  // operand of 16 rows r0 .., values 32 s + 8 g ..
+  const _Float16* const at_row = tile + 8 * (i16 * UNITS + g);
+  auto read_rows = [&](half8 (&v)[PLANES], int r0, int s) {
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) v[p] = *(const half8*)(at_row + 8 * (p * plane + r0 * UNITS + 4 * s));
+  };
+  // operand of 16 columns 16 i .., rows 32 s + 16 (e / 4) + 4 g + e % 4: transposing reads
+  const _Float16* const at_col = tile + 8 * ((4 * g + (i16 >> 2)) * UNITS + (i16 >> 1 & 1)) + 4 * (i16 & 1);
+  auto read_cols = [&](half8 (&v)[PLANES], int i, int s) {
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) {
+      s4 h[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        h[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s4*)(at_col + 8 * (p * plane + (32 * s + 16 * b) * UNITS + 2 * i)));
+      v[p] = __builtin_bit_cast(half8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
+  auto mma = [&](floatx4& c, const half8 (&u)[PLANES], const half8 (&v)[PLANES]) {
+    if constexpr (P == 3) {
+      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[1], v[0], c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[0], v[1], c, 0, 0, 0);
+    }
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[0], v[0], c, 0, 0, 0);
+  };
+
+  if (here) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) put(x[i], i);
+  }
+  __syncthreads();
+  for (int step = 0; step < a.steps; ++step) {
+    const float ca = a.c[3 * step], cb = a.c[3 * step + 1], cc = a.c[3 * step + 2];
+    half8 fa[MS][PLANES];
+    if (work) {   // A: this wave's rows
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int s = 0; s < NT / 2; ++s) {
+        half8 v[PLANES], u[2][PLANES];
+        read_rows(v, 16 * wave, s);
+        read_rows(u[0], 0, s);
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+          if (i + 1 < WAVES && i + 1 < mt) read_rows(u[(i + 1) & 1], 16 * (i + 1), s);
+          __builtin_amdgcn_sched_barrier(0);
+          if (i < mt) mma(acc[i], u[i & 1], v);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < MS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = acc[2 * s + e / 4][e % 4] * (MM_ORTHO_A / (MM_ORTHO_X * MM_ORTHO_X));
+#pragma unroll
+          for (int p = 0; p < PLANES; ++p) {
+            const _Float16 h = (_Float16)v;
+            fa[s][p][e] = h;
+            v -= (float)h;
+          }
+        }
+    }
+    auto product = [&]() {   // acc = this wave's rows of A times what is in LDS, in units of both scales
+      half8 u[2][PLANES];
+      read_cols(u[0], 0, 0);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < MS; ++s) {
+          const int now = (i * MS + s) & 1;   // operands in turn, over the tiles too
+          if (s + 1 < MS) {
+            if (s + 1 < ms) read_cols(u[now ^ 1], i, s + 1);
+          } else if (i + 1 < NT) {
+            read_cols(u[now ^ 1], i + 1, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if (s < ms) mma(acc[i], u[now], fa[s]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    };
+    constexpr float UNIT = 1.f / (MM_ORTHO_A * MM_ORTHO_X);
+    if (work) {
+      product();
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        acc[i] = cb * x[i] + cc * UNIT * acc[i];
+        x[i] *= ca;
+      }
+    }
+    __syncthreads();   // everyone is done with X
+    if (work) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) put(acc[i], i);
+    }
+    __syncthreads();
+    if (work) {
+      product();
+#pragma unroll
+      for (int i = 0; i < NT; ++i) x[i] += UNIT * acc[i];
+    }
+    if (step + 1 == a.steps) break;
+    __syncthreads();
+    if (work) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) put(x[i], i);
+    }
+    __syncthreads();
+  }
+  if (!live) return;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int n = 16 * i + 4 * g;
+    if (wide) {
+      mm_store4((T*)a.out + base + (size_t)row * a.cols, n, a.cols, (const float*)&x[i]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (n + q < a.other) ((T*)a.out)[base + (size_t)(n + q) * a.cols + row] = (T)x[i][q];
+    }
+  }
+}
+
 namespace {
 constexpr long MAX_SIDE = 65536;
 
@@ -313,6 +527,39 @@ template <typename T, typename Nt>
 bool step(const MMOrtho& a, int last, hipStream_t stream) {
   const int tm = (int)div_up(a.rows, Nt::BM), tn = (int)div_up(a.cols, Nt::BN);
   return launch<mm_ortho_step_kernel<T, Nt>, Nt>(a, (long)a.batch * tm * tn, stream, tm, tn, last);
+}
+
+template <typename T, int WAVES, int NT>
+bool small(const MMOrthoSmall& a, int batch, int lds, hipStream_t stream) {
+  if (!lds_granted<mm_ortho_small_kernel<T, WAVES, NT>>(lds)) return false;
+  hipLaunchKernelGGL((mm_ortho_small_kernel<T, WAVES, NT>), dim3(batch), dim3(64 * WAVES), lds, stream, a);
+  return true;
+}
+
+// waves, tiles of columns and LDS of a matrix that a workgroup holds (waves 0: it does not)
+struct Held { int waves, nt, lds; };
+Held held(long rows, long cols, int dtype, int steps) {
+  const long side = rows < cols ? rows : cols, other = rows < cols ? cols : rows;
+  Held h{0, 0, 0};
+  if (steps > 16) return h;
+  if (side <= 64 && other <= 64) h = Held{4, 4, 0};
+  else if (side <= 128 && other <= 128) h = Held{8, 8, 0};
+  else if (side <= 128 && other <= 256) h = Held{8, 16, 0};
+  else if (side <= 160 && other <= 224) h = Held{10, 14, 0};
+  h.lds = (int)(mm_up(side, 32) * (2 * h.nt + 1) * 16 * (dtype == MM_BF16 ? 1 : 2));
+  return h;
+}
+
+template <typename T>
+int orthogonalize_small(const MMOrtho& o, int steps, const float* c, const Held& h, hipStream_t stream) {
+  MMOrthoSmall a{o.m, o.out, o.rows, o.cols, o.side, o.rows < o.cols ? o.cols : o.rows, steps, o.eps, {}};
+  for (int i = 0; i < 3 * steps; ++i) a.c[i] = c[i];
+  bool ok;
+  if (h.waves == 4) ok = small<T, 4, 4>(a, o.batch, h.lds, stream);
+  else if (h.nt == 8) ok = small<T, 8, 8>(a, o.batch, h.lds, stream);
+  else if (h.nt == 16) ok = small<T, 8, 16>(a, o.batch, h.lds, stream);
+  else ok = small<T, 10, 14>(a, o.batch, h.lds, stream);
+  return ok ? mm::launch_status("mm_orthogonalize") : MM_ELAUNCH;
 }
 
 template <typename T>
@@ -387,6 +634,8 @@ extern "C" int mm_orthogonalize(const void* m, int dtype, long batch, long rows,
   a.cols = (int)cols;
   space(&a, dtype, (char*)workspace);
   int done = MM_OK;
-  MM_DISPATCH(dtype, done = orthogonalize<T_>(a, steps, coefficients, stream));
+  const Held h = held(rows, cols, dtype, steps);
+  if (h.waves) MM_DISPATCH(dtype, done = orthogonalize_small<T_>(a, steps, coefficients, h, stream));
+  else MM_DISPATCH(dtype, done = orthogonalize<T_>(a, steps, coefficients, stream));
   return done;
 }

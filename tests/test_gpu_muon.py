@@ -122,6 +122,13 @@ def test_steps_and_coefficients():
         A = x @ x.mT.contiguous()
         x = a * x + (b * A + c * A @ A) @ x
     assert float((got.double().cpu() - x).abs().max()) < 1e-5 * float(x.abs().max())
+    # more steps than one launch takes: the cubic iteration, whose errors only shrink (its slope stays below 1.5)
+    for steps in (16, 17, 25):
+        got = orthogonalize(M.cuda(), steps=steps, coefficients=(1.5, -0.5, 0.0))
+        x = want
+        for _ in range(steps):
+            x = 1.5 * x - 0.5 * (x @ x.mT.contiguous()) @ x
+        assert float((got.double().cpu() - x).abs().max()) < 2e-4 * float(x.abs().max())
 
 
 def test_batches_strides_and_odd_matrices():
