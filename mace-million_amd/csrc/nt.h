@@ -197,12 +197,16 @@ using MMNt = std::conditional_t<P == 1, MMNtOne<H, P, BM, BN, WM, WN>, MMNtPlane
 // The same for tiles of 256 x 256 by 8 waves (2 x 4, 128 x 64 each) where there are enough of them for every CU.  128 KB
 // of LDS hold a ring of four stages of 32 values: the loads of a stage have two stages' products (2048 cycles) to
 // arrive, and a wave waits for its own part of the next stage only, once a stage.  Operands are read two products' rows
-// ahead across the stages' borders, so that the matrix cores do not wait at the barrier either.
+// ahead across the stages' borders, so that the matrix cores do not wait at the barrier either; the loads are issued
+// between the products (all at the start of a stage they hold up its reads: 5 % slower).  Bound by LDS (96 KB read and 32
+// written a stage, 1000 cycles at 128 bytes a cycle) and the matrix cores (1024 cycles) alike.  Four waves of 128 x 128
+// would read a third less, but have nothing to run beside an epilogue (logits of 8192 x 131072, 2048 values: 6.1 ms
+// against 4.1).  bfloat16, 8192 x 2048 results a piece, 8192 products each: 228 us, 1210 TFLOP/s.
 // A row of a stage is 4 units of 16 bytes, unit u of row r at 4 r + (u ^ f(r)), so that any 8 or 16 consecutive rows of
 // an operand read lie in different banks.
 template <typename H, int P>
 struct MMNtBig {
-  static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, TH = 512, FM = 8, FN = 4, PER_CU = 1;
+  static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, TH = 512, FM = 8, FN = 4, PER_CU = 1, LOADS = 1024 / TH;
   static constexpr int LDS = 4 * (BM + BN) * 4 * 16;   // bytes
   floatx4 acc[FN][FM];
   int wm, wn, lane;
@@ -222,10 +226,10 @@ struct MMNtBig {
     typedef typename MMFrag<H>::vec vec;
     constexpr int STAGE = (BM + BN) * 4;   // units
     const int tid = threadIdx.x;
-    const H *pa[2], *pb[2];
+    const H *pa[LOADS], *pb[LOADS];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = (tid >> 2) + 128 * j, u = ((tid & 3) ^ twist(r)) * 8;
+    for (int j = 0; j < LOADS; ++j) {
+      const int r = (tid + TH * j) >> 2, u = ((tid & 3) ^ twist(r)) * 8;
       pa[j] = a.p + (long)min(m0 + r, a.rows - 1) * a.ld + u;
       pb[j] = b.p + (long)min(n0 + r, b.rows - 1) * b.ld + u;
     }
@@ -237,14 +241,12 @@ struct MMNtBig {
     if (stages <= 0) return;
     long at = (long)k0 * MM_NT_K;   // of the next stage to load, and its pass
     int pass = 0;
-    auto load = [&](int slot) {
+    auto load = [&](int slot, int j) {   // part j of a stage, the last one moves on
       const long oa = mm_nt_first<P>(pass) * a.plane + at, ob = mm_nt_second<P>(pass) * b.plane + at;
-      uint4* to = lds + slot * STAGE + (tid & ~63);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        __builtin_amdgcn_global_load_lds((mm_global_ptr)(pa[j] + oa), (mm_lds_ptr)(to + 512 * j), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((mm_global_ptr)(pb[j] + ob), (mm_lds_ptr)(to + BM * 4 + 512 * j), 16, 0, 0);
-      }
+      uint4* to = lds + slot * STAGE + (tid & ~63) + TH * j;
+      __builtin_amdgcn_global_load_lds((mm_global_ptr)(pa[j] + oa), (mm_lds_ptr)to, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((mm_global_ptr)(pb[j] + ob), (mm_lds_ptr)(to + BM * 4), 16, 0, 0);
+      if (j + 1 < LOADS) return;
       if (P == 1) {
         at += 32;
       } else if (++pass == P) {
@@ -252,15 +254,19 @@ struct MMNtBig {
         at += 32;
       }
     };
+    auto load_all = [&](int slot) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) load(slot, j);
+    };
     const int i16 = lane & 15, unit = 4 * i16 + ((lane >> 4) ^ twist(i16));
     const int ua = 4 * wm + unit, ub = 4 * (BM + wn) + unit;
     auto read_a = [&](int slot, int j) { return __builtin_bit_cast(vec, lds[slot * STAGE + ua + 64 * j]); };
     auto read_b = [&](int slot, int i) { return __builtin_bit_cast(vec, lds[slot * STAGE + ub + 64 * i]); };
-    load(0);
-    if (stages > 1) load(1);
-    if (stages > 2) load(2);
-    if (stages > 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    else if (stages > 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    load_all(0);
+    if (stages > 1) load_all(1);
+    if (stages > 2) load_all(2);
+    if (stages > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * LOADS) : "memory");
+    else if (stages > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -272,14 +278,14 @@ struct MMNtBig {
     auto step = [&](int s, auto odd) {
       constexpr int O = decltype(odd)::value;
       // this wave's part of stage s + 1 has arrived; after the barrier every wave's has, and nobody reads stage s - 1
-      if (s + 2 < stages) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      if (s + 2 < stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (s + 3 < stages) load((s + 3) & 3);
       const int now = s & 3, next = (s + 1) & 3;
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
+        if ((j == 1 || j == 4) && s + 3 < stages) load((s + 3) & 3, j / 4);   // apart: together they hold up the reads
         fa[(j + 2) & 3] = j + 2 < FM ? read_a(now, j + 2) : read_a(next, j + 2 - FM);
         if (j >= 2 && j < 2 + FN) fb[O ^ 1][j - 2] = read_b(next, j - 2);
         __builtin_amdgcn_sched_barrier(0);

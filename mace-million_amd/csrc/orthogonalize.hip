@@ -13,7 +13,7 @@
 
 #include <utility>
 
-#define MM_ORTHO_PARTS 64     // partial sums of a matrix's norm, at most
+#define MM_ORTHO_PARTS 1024   // partial sums of a matrix's norm, at most
 #define MM_ORTHO_X 4096.f     // scales of the operands
 #define MM_ORTHO_A 4096.f
 #define MM_ORTHO_B 1024.f
@@ -79,8 +79,14 @@ __global__ void __launch_bounds__(256) mm_ortho_start_kernel(MMOrtho a, int step
   __shared__ float s[64][65];
   const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, e = blockIdx.z;
   const int q = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4;
+  __shared__ double s_norm[4];
   double norm = 0.;
-  for (int i = 0; i < a.parts; ++i) norm += a.part[(long)e * a.parts + i];
+  for (int i = threadIdx.x; i < a.parts; i += 256) norm += a.part[(long)e * a.parts + i];
+#pragma unroll
+  for (int d = 32; d; d >>= 1) norm += __shfl_xor(norm, d);
+  if ((threadIdx.x & 63) == 0) s_norm[threadIdx.x >> 6] = norm;
+  __syncthreads();
+  norm = s_norm[0] + s_norm[1] + s_norm[2] + s_norm[3];
   const double by = 1. / (sqrt(norm) + (double)a.eps);
   const long size = (long)a.rows * a.cols;
 #pragma unroll
@@ -490,7 +496,7 @@ size_t space(MMOrtho* a, int dtype, char* base) {
   a->pu = (long)a->batch * a->rows * a->ldu;
   a->pv = (long)a->batch * a->cols * a->ldv;
   a->pa = (long)a->batch * a->side * a->lda;
-  const long parts = div_up((long)a->rows * a->cols, 256 * 32);
+  const long parts = div_up((long)a->rows * a->cols, 256 * 32);   // the same whatever the batch: so are its sums' bits
   a->parts = (int)(parts < MM_ORTHO_PARTS ? parts : MM_ORTHO_PARTS);
   a->part = p.take<double>((size_t)a->batch * a->parts);
   a->x = p.take<float>((size_t)a->batch * a->rows * a->cols);
