@@ -148,15 +148,37 @@ struct MMPack {
   const int *list, *count;  // rows list[0 .. *count) of src, or (null) rows row0 .. row0 + rows
   void *out, *outT;         // planes [rows, ldo] and [cols, ldt], each nullable; zeros past the last column (row)
   long ld, row0, ldo, ldt, plane, planeT;
-  int rows, cols;
+  int rows, cols, blocks_r, blocks_c;   // blocks of 64 x 64
 };
 
-// 64 x 64 values a workgroup
+// rows of out [rows][N] that belong to no asked row: zeros
+struct MMZero {
+  const int* pos;
+  void* out;
+  long rows;
+  int N, blocks;
+};
+
+// Two operands and the zeros in one launch, 64 x 64 values a workgroup.
 template <typename T>
-__global__ void __launch_bounds__(256) mm_ce_pack_kernel(MMPack a) {
+__global__ void __launch_bounds__(256) mm_ce_pack_kernel(MMPack first, MMPack second, MMZero z) {
   typedef typename MMCeType<T>::H H;
   __shared__ float s[64][65];
-  const int rows = a.count ? *a.count : a.rows, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  const int one = first.blocks_r * first.blocks_c, two = second.blocks_r * second.blocks_c;
+  int b = blockIdx.x;
+  if (b >= one + two) {
+    const int nv = (z.N + 3) / 4;
+    const float none[4] = {};
+    for (long i = (long)(b - one - two) * 256 + threadIdx.x; i < z.rows * nv; i += (long)z.blocks * 256) {
+      const long row = i / nv;
+      if (z.pos[row] < 0) mm_store4((T*)z.out + row * z.N, (int)(i - row * nv) * 4, z.N, none);
+    }
+    return;
+  }
+  const bool is_first = b < one;
+  const MMPack& a = is_first ? first : second;
+  if (!is_first) b -= one;
+  const int rows = a.count ? *a.count : a.rows, r0 = b % a.blocks_r * 64, c0 = b / a.blocks_r * 64;
   if (r0 >= mm_up(rows, 64)) return;
   const int q = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4;
 #pragma unroll
@@ -197,6 +219,19 @@ __device__ __forceinline__ MMCeRow mm_ce_join(MMCeRow a, MMCeRow b) {
   return MMCeRow{top, a.sum * __expf(a.top - top) + b.sum * __expf(b.top - top)};
 }
 
+// The incoming gradient: of every row's loss (g of the asked rows and the largest finite |g|), or (g null) of their sum
+// or mean, dloss [1].
+struct MMCeScale {
+  const float *g, *gmax, *dloss;
+  int mean;
+  // what dW is multiplied by, a row's share of it, and a row's own
+  __device__ __forceinline__ float whole(int count) const {
+    return g ? *gmax : dloss[0] / (mean ? (float)max(count, 1) : 1.f);
+  }
+  __device__ __forceinline__ float share(int at) const { return !g ? 1.f : *gmax > 0.f ? g[at] / *gmax : g[at]; }
+  __device__ __forceinline__ float row(int at, int count) const { return g ? g[at] : whole(count); }
+};
+
 template <typename H>
 struct MMCeLogits {
   MMNtOperand<H> x, w;
@@ -206,7 +241,8 @@ struct MMCeLogits {
   float *part, *picked;  // [tiles of columns][T][2], [T]
   long T;
   // backward: columns v0 .. v0 + n
-  const float *lse, *g, *gmax;   // g [asked rows] and max |g|, both null: ones
+  const float* lse;
+  MMCeScale by;
   H *d, *dT;                     // [T][ldd], [n][ldt] (planes)
   long ldd, ldt, plane, planeT;
   int v0, n;
@@ -442,17 +478,16 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// g of the asked rows (none: of every row; else dloss, over the count for the mean) and the largest finite |g|; one
-// workgroup
-__global__ void __launch_bounds__(1024) mm_ce_grad_kernel(const float* __restrict__ dloss, int reduction,
+// g of the asked rows and the largest finite |g|; one workgroup
+__global__ void __launch_bounds__(1024) mm_ce_grad_kernel(const float* __restrict__ dloss,
                                                           const int* __restrict__ count, const int* __restrict__ list,
                                                           float* __restrict__ g, float* __restrict__ gmax) {
   __shared__ float s[16];
   const int n = *count;
   float top = 0.f;
-  const float all = reduction == 0 ? 0.f : dloss[0] / (reduction == MM_CE_MEAN ? (float)max(n, 1) : 1.f);
+#pragma unroll 4
   for (int i = threadIdx.x; i < n; i += 1024) {
-    const float v = reduction == 0 ? dloss[list[i]] : all;
+    const float v = dloss[list[i]];
     g[i] = v;
     if (fabsf(v) < INFINITY) top = fmaxf(top, fabsf(v));
   }
@@ -478,14 +513,13 @@ mm_ce_d_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
   x.rows = count;
   Nt t;
   t.run(x, m0, a.w, n0, 0, a.K, mm_ce_lds);
-  const float gmax = *a.gmax;
   const int rows = (int)mm_up(count, MM_NT_K), cols = (int)mm_up(a.n, MM_NT_K);
   float share[Nt::FM];
 #pragma unroll
   for (int j = 0; j < Nt::FM; ++j) {
     const int m = m0 + t.row(j), at = min(m, count - 1), y = a.y[at];
     const float lse = a.lse[at];
-    share[j] = gmax > 0.f ? a.g[at] / gmax : a.g[at];
+    share[j] = a.by.share(at);
 #pragma unroll
     for (int i = 0; i < Nt::FN; ++i)
 #pragma unroll
@@ -528,74 +562,79 @@ mm_ce_d_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
 }
 
 // C = A B^T of a piece.  dx: rows of A are the asked rows (count), fp32 sums part [splits][T][N], added to what is there
-// unless `first`.  dW: the summed index is the asked rows; part [splits][M][N] (written), or with one split the rows of
-// dW themselves, times *gmax / scale.
+// unless `first`, or (one piece, one split) the rows list[m] of dx themselves, times the row's g.  dW: the summed index
+// is the asked rows; part [splits][M][N] (written), or with one split the rows of dW, times the whole gradient.
 template <typename H>
 struct MMCeProduct {
   MMNtOperand<H> a, b;
-  const int* count;
-  int M, N, K;          // K: stages (dx)
-  int splits, first;
+  const int *count, *list;
+  int dx, M, N, K;      // K: stages (dx)
+  int splits, first, tiles_n, blocks;
   float* part;
   long rows;            // of part
   void* out;
-  const float* gmax;
+  MMCeScale by;
   float inv;
 };
 
-template <typename T, bool DX, typename Nt>
+// both in one launch, as neither fills the card by itself where rows and classes are few
+template <typename T, typename Nt>
 __global__ void __launch_bounds__(Nt::TH, Nt::PER_CU)
-mm_ce_product_kernel(MMCeProduct<typename MMCeType<T>::H> a, int tiles_n) {
+mm_ce_product_kernel(MMCeProduct<typename MMCeType<T>::H> one, MMCeProduct<typename MMCeType<T>::H> two) {
   typedef typename MMCeType<T>::H H;
   constexpr int BM = Nt::BM, BN = Nt::BN;
   extern __shared__ uint4 mm_ce_lds[];
-  const int count = *a.count, M = DX ? count : a.M;
-  const int K = DX ? a.K : (count + MM_NT_K - 1) / MM_NT_K;
-  int e, tm, tn;
-  if (!mm_nt_tile(blockIdx.x, 1, (M + BM - 1) / BM, tiles_n, &e, &tm, &tn)) return;
-  const int m0 = tm * BM, n0 = tn * BN, split = blockIdx.y;
+  const bool is_one = (int)blockIdx.x < one.blocks;
+  const MMCeProduct<H>& a = is_one ? one : two;
+  const int block = (int)blockIdx.x - (is_one ? 0 : one.blocks), count = *a.count, M = a.dx ? count : a.M;
+  const int K = a.dx ? a.K : (count + MM_NT_K - 1) / MM_NT_K, tiles_m = (M + BM - 1) / BM;
+  int split, tm, tn;
+  if (!mm_nt_tile(block, a.splits, tiles_m, a.tiles_n, &split, &tm, &tn)) return;
+  const int m0 = tm * BM, n0 = tn * BN;
   MMNtOperand<H> A = a.a;
   A.rows = M;
   Nt t;
   t.run(A, m0, a.b, n0, (int)((long)K * split / a.splits), (int)((long)K * (split + 1) / a.splits), mm_ce_lds);
-  const float f = a.out ? *a.gmax * a.inv : 1.f;
 #pragma unroll
   for (int j = 0; j < Nt::FM; ++j) {
     const int m = m0 + t.row(j);
     if (m >= M) continue;
+    float f = 1.f;
+    T* out = nullptr;
+    if (a.out) {
+      f = (a.dx ? a.by.row(m, count) : a.by.whole(count)) * a.inv;
+      out = (T*)a.out + (long)(a.dx ? a.list[m] : m) * a.N;
+    }
 #pragma unroll
     for (int i = 0; i < Nt::FN; ++i) {
       const int n = n0 + t.col(i);
-      float v[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = t.acc[i][j][q];
-      if (!DX && a.out) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] *= f;
-        mm_store4((T*)a.out + (long)m * a.N, n, a.N, v);
+      floatx4 v = t.acc[i][j];
+      if (out) {
+        v *= f;
+        mm_store4(out, n, a.N, (const float*)&v);
       } else {
         float* p = a.part + ((long)split * a.rows + m) * a.N;
-        if (DX && !a.first) {
-          float u[4];
-          mm_load4(p, n, a.N, u);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] += u[q];
+        if (a.dx && !a.first) {
+          floatx4 u;
+          mm_load4(p, n, a.N, (float*)&u);
+          v += u;
         }
-        mm_store4(p, n, a.N, v);
+        mm_store4(p, n, a.N, (const float*)&v);
       }
     }
   }
 }
 
-// out = the sum of the splits' sums: dx (pos: row of part, or none: 0; factor g) or dW (factor *gmax).  A vector is
-// summed by WAVES waves.
+// out = the sum of the splits' sums: dx (pos: row of part, or none: 0; factor of the row) or dW (the whole factor).  A
+// vector is summed by WAVES waves.
 template <typename T, bool DX, int WAVES>
 __global__ void __launch_bounds__(256)
 mm_ce_join_kernel(const float* __restrict__ part, int splits, long part_rows, long rows, int N,
-                  const int* __restrict__ pos, const float* __restrict__ g, float inv, T* __restrict__ out) {
+                  const int* __restrict__ pos, const int* __restrict__ count, MMCeScale by, float inv,
+                  T* __restrict__ out) {
   constexpr int EACH = 256 / WAVES;
   __shared__ floatx4 s[WAVES][EACH];
-  const int nv = (N + 3) / 4, lane = threadIdx.x % EACH, wave = threadIdx.x / EACH;
+  const int nv = (N + 3) / 4, lane = threadIdx.x % EACH, wave = threadIdx.x / EACH, asked = *count;
   for (long i0 = (long)blockIdx.x * EACH; i0 < rows * nv; i0 += (long)gridDim.x * EACH) {
     const long i = i0 + lane, row = i / nv, at = i >= rows * nv ? -1 : DX ? pos[row] : row;
     const int c = (int)(i - row * nv) * 4;
@@ -603,10 +642,9 @@ mm_ce_join_kernel(const float* __restrict__ part, int splits, long part_rows, lo
     if (at >= 0) {
 #pragma unroll 4
       for (int k = wave; k < splits; k += WAVES) {
-        float u[4];
-        mm_load4(part + (k * part_rows + at) * N, c, N, u);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] += u[q];
+        floatx4 u;
+        mm_load4(part + (k * part_rows + at) * N, c, N, (float*)&u);
+        v += u;
       }
     }
     if constexpr (WAVES > 1) {
@@ -614,11 +652,9 @@ mm_ce_join_kernel(const float* __restrict__ part, int splits, long part_rows, lo
       __syncthreads();
     }
     if (wave == 0 && i < rows * nv) {
-      const float f = at < 0 ? 0.f : (DX ? g[at] : g[0]) * inv;   // 0 rows stay 0 whatever the factor
 #pragma unroll
       for (int w = 1; w < WAVES; ++w) v += s[w][lane];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = at < 0 ? 0.f : v[q] * f;
+      if (at >= 0) v *= (DX ? by.row((int)at, asked) : by.whole(asked)) * inv;   // 0 rows stay 0 whatever the factor
       mm_store4(out + row * N, c, N, (const float*)&v);
     }
     if constexpr (WAVES > 1) __syncthreads();
@@ -628,7 +664,7 @@ mm_ce_join_kernel(const float* __restrict__ part, int splits, long part_rows, lo
 // ------------------------------------------------------------------------------------------------ host
 namespace {
 constexpr long MAX_SIDE = 2147483648L - 65536;
-constexpr int BM = 128, BN = 128;
+constexpr int BM = 64, BN = 64;   // the smallest tiles
 constexpr float HALF_SCALE = 16384.f;   // of d in float16
 
 struct Sizes {
@@ -639,7 +675,7 @@ struct Sizes {
   bool w_in_place;   // the weights are operands as they are
   long piece, pieces, piece_p;
   int dx_splits, dw_splits;
-  bool dx_big, dw_big;
+  int dx_side, dw_side;
 };
 
 long div_up(long a, long b) { return (a + b - 1) / b; }
@@ -657,23 +693,32 @@ struct Space {
   }
 };
 
-// Large tiles where they are enough for three quarters of the CUs and lie outside the product by less than a fifth more
-// than small ones do.
-bool big_fits(long m, long n) { return 5 * mm_up(m, 256) * mm_up(n, 256) <= 6 * mm_up(m, BM) * mm_up(n, BN); }
-bool big_tiles(long m, long n, int splits) {
-  return big_fits(m, n) && div_up(m, 256) * div_up(n, 256) * splits >= 192;
-}
+int tiles(long m, long n, int side) { return (int)(div_up(m, side) * div_up(n, side)); }
+int side_of(long m, long n) { return mm_tile_side(tiles(m, n, 256), tiles(m, n, 128), tiles(m, n, 64)); }
 
-// Parts of the summed index K of an m x n product, so that there are workgroups for every CU; no part below 512.
-int splits_of(long m, long n, long K, bool* big) {
-  const long most = clamp(K / 512, 1, 64), tiles = div_up(m, 256) * div_up(n, 256), few = div_up(m, BM) * div_up(n, BN);
-  *big = big_fits(m, n) && (tiles >= 192 || (tiles >= 64 && tiles * most >= 192));
-  return (int)clamp(*big ? div_up(192, tiles) : 512 / (few ? few : 1), 1, most);
+// Tile and parts of the summed index K of an m x n product by the same rule, no part below 512 values; a part costs its
+// sums' way through memory.
+int splits_of(long m, long n, long K, int* side) {
+  const long most = clamp(K / 512, 1, 64);
+  const int sides[] = {256, 128, 64}, slots[] = {256, 512, 1024};
+  const double rate[] = {1., MM_TILE_MID, MM_TILE_LOW};
+  double best = 1e30;
+  int splits = 1;
+  for (int i = 0; i < 3; ++i) {
+    const long t = tiles(m, n, sides[i]) < 1 ? 1 : tiles(m, n, sides[i]), p = clamp(slots[i] / t, 1, most);
+    const double cost = rate[i] * (double)div_up(t * p, slots[i]) / (double)p + 0.002 * (double)p;
+    if (cost < best) {
+      best = cost;
+      splits = (int)p;
+      *side = sides[i];
+    }
+  }
+  return splits;
 }
 
 bool sizes_of(const char* name, long T, long D, long V, int dtype, const void* w, Sizes* s) {
   if (T > MAX_SIDE || D > MAX_SIDE || V > MAX_SIDE || div_up(T, BM) * div_up(V, BN) * 256 >= 4294967296L ||
-      div_up(T > V ? T : V, 64) * div_up(D, 64) * 256 >= 4294967296L || div_up(D, 64) > 65535) {
+      (div_up(T, 64) + div_up(V, 64) + 64) * (div_up(D, 64) + 16) * 256 >= 4294967296L) {
     mm::set_error(std::string(name) + ": sizes beyond the launches' limits");
     return false;
   }
@@ -688,8 +733,8 @@ bool sizes_of(const char* name, long T, long D, long V, int dtype, const void* w
   s->piece = s->pieces == 1 ? V : mm_up(div_up(V, s->pieces), 256);
   s->pieces = div_up(V, s->piece);
   s->piece_p = mm_up(s->piece, MM_NT_K);
-  s->dx_splits = splits_of(T, D, s->piece_p, &s->dx_big);
-  s->dw_splits = splits_of(s->piece, D, s->Tp, &s->dw_big);
+  s->dx_splits = splits_of(T, D, s->piece_p, &s->dx_side);
+  s->dw_splits = splits_of(s->piece, D, s->Tp, &s->dw_side);
   return true;
 }
 
@@ -740,25 +785,64 @@ size_t backward_space(const Sizes& s, bool dx, bool dw, char* base, Backward* b)
   b->dT = p.take<short>((size_t)s.planes * s.piece * s.Tp);
   b->g = p.take<float>(s.T);
   b->gmax = p.take<float>(1);
-  b->dx = dx ? p.take<float>((size_t)s.dx_splits * s.T * s.D) : nullptr;
+  b->dx = dx && (s.pieces > 1 || s.dx_splits > 1) ? p.take<float>((size_t)s.dx_splits * s.T * s.D) : nullptr;
   b->dw = dw && s.dw_splits > 1 ? p.take<float>((size_t)s.dw_splits * s.piece * s.D) : nullptr;
   return p.used;
 }
 
 template <typename T>
-void pack(const MMPack& a, long rows, hipStream_t stream) {
-  hipLaunchKernelGGL(mm_ce_pack_kernel<T>, dim3((unsigned)div_up(rows, 64), (unsigned)div_up(a.cols, 64)), dim3(256), 0,
-                     stream, a);
+void pack(MMPack a, MMPack b, MMZero z, hipStream_t stream) {
+  for (MMPack* p : {&a, &b}) {
+    const bool any = p->out || p->outT;
+    p->blocks_r = any ? (int)div_up(p->rows, 64) : 0;
+    p->blocks_c = any ? (int)div_up(p->cols, 64) : 0;
+  }
+  z.blocks = z.out ? (int)clamp(div_up(z.rows * div_up(z.N, 4), 1024), 1, 4096) : 0;
+  const long blocks = (long)a.blocks_r * a.blocks_c + (long)b.blocks_r * b.blocks_c + z.blocks;
+  if (blocks) hipLaunchKernelGGL(mm_ce_pack_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream, a, b, z);
 }
 
-template <auto KERNEL, typename Nt, typename A>
-bool launch(const A& a, long m, long n, int splits, hipStream_t stream) {
+template <auto KERNEL, typename Nt, typename... A>
+bool launch(long blocks, hipStream_t stream, const A&... a) {
   if (!lds_granted<KERNEL>(Nt::LDS)) return false;
-  const int tiles_n = (int)div_up(n, Nt::BN);
-  hipLaunchKernelGGL(KERNEL, dim3((unsigned)(div_up(m, Nt::BM) * tiles_n), splits), dim3(Nt::TH), Nt::LDS, stream, a,
-                     tiles_n);
+  hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks), dim3(Nt::TH), Nt::LDS, stream, a...);
   return true;
 }
+
+template <typename T>
+struct Tiles {
+  typedef typename MMCeType<T>::H H;
+  static constexpr int P = MMCeType<T>::P;
+  typedef MMNtBig<H, P> Big;
+  typedef MMNt<H, P, 128, 128, 2, 2> Mid;
+  typedef MMNt<H, P, 64, 64, 2, 2> Low;
+
+  // the logits' statistics, or (D) d
+  template <bool D>
+  static bool logits(const MMCeLogits<H>& a, long rows, long n, int side, hipStream_t stream) {
+    const int tn = (int)div_up(n, side), blocks = tiles(rows, n, side);
+    if constexpr (D) {
+      return side == 256   ? launch<mm_ce_d_kernel<T, Big>, Big>(blocks, stream, a, tn)
+             : side == 128 ? launch<mm_ce_d_kernel<T, Mid>, Mid>(blocks, stream, a, tn)
+                           : launch<mm_ce_d_kernel<T, Low>, Low>(blocks, stream, a, tn);
+    } else {
+      return side == 256   ? launch<mm_ce_logits_kernel<T, Big>, Big>(blocks, stream, a, tn)
+             : side == 128 ? launch<mm_ce_logits_kernel<T, Mid>, Mid>(blocks, stream, a, tn)
+                           : launch<mm_ce_logits_kernel<T, Low>, Low>(blocks, stream, a, tn);
+    }
+  }
+
+  static bool products(MMCeProduct<H> a, MMCeProduct<H> b, int side, hipStream_t stream) {
+    for (MMCeProduct<H>* p : {&a, &b}) {
+      p->tiles_n = (int)div_up(p->N, side);
+      p->blocks = p->blocks ? (int)mm_up((long)tiles(p->M, p->N, side) * p->splits, 8) : 0;   // the second one's XCDs
+    }
+    const long blocks = (long)a.blocks + b.blocks;
+    return side == 256   ? launch<mm_ce_product_kernel<T, Big>, Big>(blocks, stream, a, b)
+           : side == 128 ? launch<mm_ce_product_kernel<T, Mid>, Mid>(blocks, stream, a, b)
+                         : launch<mm_ce_product_kernel<T, Low>, Low>(blocks, stream, a, b);
+  }
+};
 
 template <typename T, int ROWS, int TH>
 bool launch_few(const MMCeFew& a, int wg, size_t lds, hipStream_t stream) {
@@ -789,15 +873,10 @@ template <typename T>
 int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, float* loss, float* lse,
             const Forward& f, hipStream_t stream) {
   typedef typename MMCeType<T>::H H;
-  typedef MMNt<H, MMCeType<T>::P, BM, BN, 2, 2> Nt;
-  typedef MMNtBig<H, MMCeType<T>::P> Big;
   if (s.T) {
-    MMPack px{x, r.list, r.count, f.x, nullptr, ldx, 0, s.Dp, 0, s.T * s.Dp, 0, (int)s.T, (int)s.D};
-    pack<T>(px, s.T, stream);
-    if (!s.w_in_place) {
-      MMPack pw{w, nullptr, nullptr, f.w, nullptr, s.D, 0, s.Dp, 0, s.V * s.Dp, 0, (int)s.V, (int)s.D};
-      pack<T>(pw, s.V, stream);
-    }
+    const MMPack px{x, r.list, r.count, f.x, nullptr, ldx, 0, s.Dp, 0, s.T * s.Dp, 0, (int)s.T, (int)s.D};
+    const MMPack pw{w, nullptr, nullptr, f.w, nullptr, s.D, 0, s.Dp, 0, s.V * s.Dp, 0, (int)s.V, (int)s.D};
+    pack<T>(px, pw, MMZero{}, stream);
     MMCeLogits<H> a{};
     a.x = MMNtOperand<H>{(const H*)f.x, s.Dp, s.T * s.Dp, 0};
     a.w = s.w_in_place ? MMNtOperand<H>{(const H*)w, s.D, 0, (int)s.V}
@@ -809,11 +888,8 @@ int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int
     a.part = f.part;
     a.picked = f.picked;
     a.T = s.T;
-    const bool big = big_tiles(s.T, s.V, 1);
-    const int tiles_n = (int)div_up(s.V, big ? Big::BN : BN);
-    if (!(big ? launch<mm_ce_logits_kernel<T, Big>, Big>(a, s.T, s.V, 1, stream)
-              : launch<mm_ce_logits_kernel<T, Nt>, Nt>(a, s.T, s.V, 1, stream)))
-      return MM_ELAUNCH;
+    const int side = side_of(s.T, s.V), tiles_n = (int)div_up(s.V, side);
+    if (!Tiles<T>::template logits<false>(a, s.T, s.V, side, stream)) return MM_ELAUNCH;
     hipLaunchKernelGGL(mm_ce_rows_kernel, dim3((unsigned)div_up(s.T, 32)), dim3(1024), 0, stream, f.part, s.T, tiles_n,
                        r.count, r.list, r.y, f.picked, lse, reduction == 0 ? loss : nullptr,
                        reduction ? f.sums : nullptr);
@@ -825,31 +901,33 @@ int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int
 }
 
 template <typename T, bool DX>
-void join(const float* part, int splits, long part_rows, long rows, int N, const int* pos, const float* g, float inv,
-          T* out, hipStream_t stream) {
+void join(const float* part, int splits, long part_rows, long rows, int N, const int* pos, const int* count,
+          const MMCeScale& by, float inv, T* out, hipStream_t stream) {
   const long vectors = rows * div_up(N, 4);
   if (splits < 4)
     hipLaunchKernelGGL((mm_ce_join_kernel<T, DX, 1>), dim3((unsigned)clamp(div_up(vectors, 256), 1, 4096)), dim3(256), 0,
-                       stream, part, splits, part_rows, rows, N, pos, g, inv, out);
+                       stream, part, splits, part_rows, rows, N, pos, count, by, inv, out);
   else
     hipLaunchKernelGGL((mm_ce_join_kernel<T, DX, 4>), dim3((unsigned)clamp(div_up(vectors, 64), 1, 4096)), dim3(256), 0,
-                       stream, part, splits, part_rows, rows, N, pos, g, inv, out);
+                       stream, part, splits, part_rows, rows, N, pos, count, by, inv, out);
 }
 
 template <typename T>
 int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, const float* lse,
              const float* dloss, T* dx, T* dw, const Backward& b, hipStream_t stream) {
   typedef typename MMCeType<T>::H H;
-  typedef MMNt<H, MMCeType<T>::P, BM, BN, 2, 2> Nt;
-  typedef MMNtBig<H, MMCeType<T>::P> Big;
   const float scale = s.dtype == MM_F16 ? HALF_SCALE : 1.f;
-  hipLaunchKernelGGL(mm_ce_grad_kernel, dim3(1), dim3(1024), 0, stream, dloss, reduction, r.count, r.list, b.g, b.gmax);
-  MMPack px{x, r.list, r.count, b.x, b.xT, ldx, 0, s.Dp, s.Tp, s.T * s.Dp, s.D * s.Tp, (int)s.T, (int)s.D};
-  pack<T>(px, s.T, stream);
+  const MMCeScale by{reduction ? nullptr : b.g, b.gmax, dloss, reduction == MM_CE_MEAN};
+  if (!reduction)
+    hipLaunchKernelGGL(mm_ce_grad_kernel, dim3(1), dim3(1024), 0, stream, dloss, r.count, r.list, b.g, b.gmax);
+  const bool direct = s.pieces == 1 && s.dx_splits == 1;   // dx without sums in memory
   for (long p = 0; p < s.pieces; ++p) {
     const long v0 = p * s.piece, n = s.V - v0 < s.piece ? s.V - v0 : s.piece, np = mm_up(n, MM_NT_K);
-    MMPack pw{w, nullptr, nullptr, b.w, b.wT, s.D, v0, s.Dp, s.piece_p, s.piece * s.Dp, s.D * s.piece_p, (int)n, (int)s.D};
-    if (b.w || b.wT) pack<T>(pw, n, stream);
+    MMPack px{x, r.list, r.count, b.x, b.xT, ldx, 0, s.Dp, s.Tp, s.T * s.Dp, s.D * s.Tp, (int)s.T, (int)s.D};
+    if (p) px.out = px.outT = nullptr;   // once
+    const MMPack pw{w, nullptr, nullptr, b.w, b.wT, s.D, v0, s.Dp, s.piece_p, s.piece * s.Dp, s.D * s.piece_p, (int)n,
+                    (int)s.D};
+    pack<T>(px, pw, MMZero{r.pos, direct ? dx : nullptr, s.T, (int)s.D}, stream);
     MMCeLogits<H> a{};
     a.x = MMNtOperand<H>{(const H*)b.x, s.Dp, s.T * s.Dp, 0};
     a.w = s.w_in_place ? MMNtOperand<H>{(const H*)w + v0 * s.D, s.D, 0, (int)n}
@@ -859,8 +937,7 @@ int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, in
     a.K = (int)(s.Dp / MM_NT_K);
     a.T = s.T;
     a.lse = lse;
-    a.g = b.g;
-    a.gmax = b.gmax;
+    a.by = by;
     a.d = (H*)b.d;
     a.dT = (H*)b.dT;
     a.ldd = s.piece_p;
@@ -870,43 +947,51 @@ int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, in
     a.v0 = (int)v0;
     a.n = (int)n;
     a.scale = scale;
-    bool ok = big_tiles(s.T, n, 1) ? launch<mm_ce_d_kernel<T, Big>, Big>(a, s.T, n, 1, stream)
-                                   : launch<mm_ce_d_kernel<T, Nt>, Nt>(a, s.T, n, 1, stream);
+    bool ok = Tiles<T>::template logits<true>(a, s.T, n, side_of(s.T, n), stream);
+    MMCeProduct<H> q{}, u{};
     if (dx) {
-      MMCeProduct<H> q{};
       q.a = MMNtOperand<H>{(const H*)b.d, s.piece_p, s.T * s.piece_p, 0};
       q.b = MMNtOperand<H>{(const H*)b.wT, s.piece_p, s.D * s.piece_p, (int)s.D};
       q.count = r.count;
+      q.list = r.list;
+      q.dx = q.blocks = 1;
+      q.M = (int)s.T;
       q.N = (int)s.D;
       q.K = (int)(np / MM_NT_K);
       q.splits = s.dx_splits;
       q.first = p == 0;
       q.part = b.dx;
       q.rows = s.T;
-      ok = ok && (s.dx_big ? launch<mm_ce_product_kernel<T, true, Big>, Big>(q, s.T, s.D, q.splits, stream)
-                           : launch<mm_ce_product_kernel<T, true, Nt>, Nt>(q, s.T, s.D, q.splits, stream));
+      q.out = direct ? dx : nullptr;
+      q.by = by;
+      q.inv = 1.f / scale;
     }
     if (dw) {
-      MMCeProduct<H> q{};
-      q.a = MMNtOperand<H>{(const H*)b.dT, s.Tp, s.piece * s.Tp, 0};
-      q.b = MMNtOperand<H>{(const H*)b.xT, s.Tp, s.D * s.Tp, (int)s.D};
-      q.count = r.count;
-      q.M = (int)n;
-      q.N = (int)s.D;
-      q.splits = s.dw_splits;
-      q.part = b.dw;
-      q.rows = n;
-      q.out = s.dw_splits == 1 ? dw + v0 * s.D : nullptr;
-      q.gmax = b.gmax;
-      q.inv = 1.f / scale;
-      ok = ok && (s.dw_big ? launch<mm_ce_product_kernel<T, false, Big>, Big>(q, n, s.D, q.splits, stream)
-                           : launch<mm_ce_product_kernel<T, false, Nt>, Nt>(q, n, s.D, q.splits, stream));
-      if (s.dw_splits > 1)
-        join<T, false>(b.dw, s.dw_splits, n, n, (int)s.D, nullptr, b.gmax, 1.f / scale, dw + v0 * s.D, stream);
+      u.a = MMNtOperand<H>{(const H*)b.dT, s.Tp, s.piece * s.Tp, 0};
+      u.b = MMNtOperand<H>{(const H*)b.xT, s.Tp, s.D * s.Tp, (int)s.D};
+      u.count = r.count;
+      u.blocks = 1;
+      u.M = (int)n;
+      u.N = (int)s.D;
+      u.splits = s.dw_splits;
+      u.part = b.dw;
+      u.rows = n;
+      u.out = s.dw_splits == 1 ? dw + v0 * s.D : nullptr;
+      u.by = by;
+      u.inv = 1.f / scale;
+    }
+    if (dx && dw && s.dx_side == s.dw_side) {
+      ok = ok && Tiles<T>::products(q, u, s.dx_side, stream);
+    } else {
+      if (dx) ok = ok && Tiles<T>::products(q, MMCeProduct<H>{}, s.dx_side, stream);
+      if (dw) ok = ok && Tiles<T>::products(u, MMCeProduct<H>{}, s.dw_side, stream);
     }
     if (!ok) return MM_ELAUNCH;
+    if (dw && s.dw_splits > 1)
+      join<T, false>(b.dw, s.dw_splits, n, n, (int)s.D, nullptr, r.count, by, 1.f / scale, dw + v0 * s.D, stream);
   }
-  if (dx) join<T, true>(b.dx, s.dx_splits, s.T, s.T, (int)s.D, r.pos, b.g, 1.f / scale, dx, stream);
+  if (dx && !direct)
+    join<T, true>(b.dx, s.dx_splits, s.T, s.T, (int)s.D, r.pos, r.count, by, 1.f / scale, dx, stream);
   return mm::launch_status("mm_ce_bwd");
 }
 }  // namespace

@@ -403,3 +403,15 @@ __device__ __forceinline__ bool mm_nt_lower(int b, int batch, int tiles, int* e,
 }
 
 __host__ __device__ inline long mm_up(long n, long size) { return (n + size - 1) / size * size; }
+
+// Time of a whole round of tiles of 128 (two on each of the 256 CUs) and of 64 (four), where one of 256, alone on its CU,
+// takes 1: by the rates that products of 1024 and more reach with each.
+#define MM_TILE_MID 0.59
+#define MM_TILE_LOW 0.5
+
+// Side of the tiles of a launch that would have t256, t128 or t64 of them.
+inline int mm_tile_side(long t256, long t128, long t64) {
+  const double big = (double)((t256 + 255) / 256), mid = MM_TILE_MID * (double)((t128 + 511) / 512);
+  const double low = MM_TILE_LOW * (double)((t64 + 1023) / 1024);
+  return big <= mid && big <= low ? 256 : mid <= low ? 128 : 64;
+}

@@ -508,14 +508,6 @@ size_t space(MMOrtho* a, int dtype, char* base) {
   return p.used;
 }
 
-// Side of the tiles of `tiles` (at 256, 128, 64) workgroups: the least time by whole rounds of the 256 CUs, a tile of 256
-// taking 1 alone on its CU, tiles of 128 (two on a CU) 0.59 a round, tiles of 64 (four) 0.5: the rates that products of
-// 1024 and more reach with each.
-int tile_side(long t256, long t128, long t64) {
-  const double big = (double)div_up(t256, 256), mid = 0.59 * (double)div_up(t128, 512), low = 0.5 * (double)div_up(t64, 1024);
-  return big <= mid && big <= low ? 256 : mid <= low ? 128 : 64;
-}
-
 template <auto KERNEL, typename Nt, typename... A>
 bool launch(const MMOrtho& a, long workgroups, hipStream_t stream, A... rest) {
   if (!lds_granted<KERNEL>(Nt::LDS)) return false;
@@ -580,7 +572,7 @@ int orthogonalize(MMOrtho a, int steps, const float* c, hipStream_t stream) {
                      dim3(256), 0, stream, a, steps);
   auto lower = [&](long n) { return a.batch * div_up(a.side, n) * (div_up(a.side, n) + 1) / 2; };
   auto all = [&](long n) { return a.batch * div_up(a.rows, n) * div_up(a.cols, n); };
-  const int sq = tile_side(lower(256), lower(128), lower(64)), st = tile_side(all(256), all(128), all(64));
+  const int sq = mm_tile_side(lower(256), lower(128), lower(64)), st = mm_tile_side(all(256), all(128), all(64));
   bool ok = true;
   for (int i = 0; i < steps && ok; ++i, c += 3) {
     a.ca = c[0];
