@@ -14,7 +14,8 @@ Module map (mirrors the reference package mace_onegpu, same module paths for the
   cross_entropy     linear_cross_entropy: the loss of a linear head over many classes, with its gradient
   muon              orthogonalize by Newton-Schulz products, and Muon, the optimizer that updates weight blocks with it
   experts           mixtures of expert weight blocks: route, plan_experts, expert_linear
-  expert_mix        ExpertMix: a mixture of expert linears on node features, and a command that fits one
+  expert_mix        ExpertMix, ClassHead: a mixture of expert linears on node features, a head for classes of atoms,
+                    and a command that fits them
   lammps_data       periodic-image ML-IAP data object (one GPU stands in for LAMMPS' ghost exchange)
   model, o3, codegen, systems, _lib, _ops   architecture, couplings, kernel generator, inputs, C-ABI and torch bindings
 """
