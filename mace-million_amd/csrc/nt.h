@@ -404,14 +404,30 @@ __device__ __forceinline__ bool mm_nt_lower(int b, int batch, int tiles, int* e,
 
 __host__ __device__ inline long mm_up(long n, long size) { return (n + size - 1) / size * size; }
 
-// Time of a whole round of tiles of 128 (two on each of the 256 CUs) and of 64 (four), where one of 256, alone on its CU,
-// takes 1: by the rates that products of 1024 and more reach with each.
-#define MM_TILE_MID 0.59
-#define MM_TILE_LOW 0.5
+// Tiles of 256, 128 and 64 for P products: how many run at once, and the time of such a round where one tile of 256 on
+// every CU takes 1, by the rates that products of 1024 and more reach (planes leave room for fewer workgroups on a CU).
+struct MMTileRates {
+  int side[3] = {256, 128, 64}, slots[3];
+  double round[3];
+};
+inline MMTileRates mm_tile_rates(int P) {
+  if (P == 1) return MMTileRates{{256, 128, 64}, {256, 512, 1024}, {1., 0.59, 0.5}};
+  if (P == 3) return MMTileRates{{256, 128, 64}, {256, 512, 512}, {1., 0.59, 0.28}};
+  return MMTileRates{{256, 128, 64}, {256, 256, 512}, {1., 0.31, 0.28}};
+}
 
-// Side of the tiles of a launch that would have t256, t128 or t64 of them.
-inline int mm_tile_side(long t256, long t128, long t64) {
-  const double big = (double)((t256 + 255) / 256), mid = MM_TILE_MID * (double)((t128 + 511) / 512);
-  const double low = MM_TILE_LOW * (double)((t64 + 1023) / 1024);
-  return big <= mid && big <= low ? 256 : mid <= low ? 128 : 64;
+// Side of the tiles of a launch that would have t256, t128 or t64 of them: the least time.
+inline int mm_tile_side(int P, long t256, long t128, long t64) {
+  const MMTileRates r = mm_tile_rates(P);
+  const long t[] = {t256, t128, t64};
+  int best = 0;
+  double least = 1e30;
+  for (int i = 0; i < 3; ++i) {
+    const double time = r.round[i] * (double)((t[i] + r.slots[i] - 1) / r.slots[i]);
+    if (time < least) {
+      least = time;
+      best = r.side[i];
+    }
+  }
+  return best;
 }

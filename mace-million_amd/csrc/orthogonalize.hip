@@ -67,6 +67,8 @@ struct MMOrtho {
   // planes of [batch]: X [rows][ldu], X^T [cols][ldv], A and B [side][lda]; the one that a step multiplies (X^T if rows
   // <= cols, else X) is written to `next` meanwhile
   _Float16 *u, *v, *a, *b, *next;
+  float* sums;                    // [splits][batch][side][lda] of A's parts, where the longer side is split
+  int splits;
   long ldu, ldv, lda, pu, pv, pa;   // pu, pv, pa: distance of planes
   int batch, rows, cols, side, parts;
   float ca, cb, cc, eps;
@@ -175,8 +177,12 @@ template <int P, int WHAT, typename Nt>
 __global__ void __launch_bounds__(Nt::TH, Nt::PER_CU) mm_ortho_square_kernel(MMOrtho a, int tiles) {
   constexpr int PLANES = P == 1 ? 1 : 2;
   extern __shared__ uint4 mm_ortho_lds[];
-  int e, tm, tn;
-  if (!mm_nt_lower(blockIdx.x, a.batch, tiles, &e, &tm, &tn)) return;
+  int e, tm, tn, split = 0;
+  if (!mm_nt_lower(blockIdx.x, WHAT ? a.batch : a.batch * a.splits, tiles, &e, &tm, &tn)) return;
+  if (WHAT == 0) {
+    split = e / a.batch;
+    e -= split * a.batch;
+  }
   MMNtOperand<_Float16> x;
   int k;
   if constexpr (WHAT == 1) {
@@ -191,6 +197,18 @@ __global__ void __launch_bounds__(Nt::TH, Nt::PER_CU) mm_ortho_square_kernel(MMO
   }
   const int m0 = tm * Nt::BM, n0 = tn * Nt::BN;
   Nt t;
+  if (WHAT == 0 && a.splits > 1) {   // a part of the sums, of the lower tiles alone
+    t.run(x, m0, x, n0, (int)((long)k * split / a.splits), (int)((long)k * (split + 1) / a.splits), mm_ortho_lds);
+    float* sums = a.sums + ((long)split * a.batch + e) * a.side * a.lda;
+#pragma unroll
+    for (int j = 0; j < Nt::FM; ++j)
+#pragma unroll
+      for (int i = 0; i < Nt::FN; ++i) {
+        const int m = m0 + t.row(j), n = n0 + t.col(i);
+        if (m < a.side && n < a.lda) *(floatx4*)(sums + (long)m * a.lda + n) = t.acc[i][j];
+      }
+    return;
+  }
   t.run(x, m0, x, n0, 0, k, mm_ortho_lds);
   _Float16* out = (WHAT ? a.b : a.a) + (long)e * a.side * a.lda;
   const _Float16* in = a.a + (long)e * a.side * a.lda;
@@ -224,6 +242,30 @@ __global__ void __launch_bounds__(Nt::TH, Nt::PER_CU) mm_ortho_square_kernel(MMO
   mm_ortho_tiles<PLANES>(t, mm_ortho_lds, out + (long)m0 * a.lda + n0, a.lda, a.pa, a.side - m0, left, 1.f);
   if (tm != tn)
     mm_ortho_tiles_transposed<PLANES>(t, mm_ortho_lds, out + (long)n0 * a.lda + m0, a.lda, a.pa, low, a.side - n0, 1.f);
+}
+
+// A from its parts: the values on and below the diagonal summed and written twice, zeros past the last column; one
+// thread for 4 columns of a row.
+template <int PLANES>
+__global__ void __launch_bounds__(256) mm_ortho_join_kernel(MMOrtho a) {
+  const int nv = (int)(a.lda / 4);
+  const int one = a.side * nv, e = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;   // one: at most 192 x 48
+  if (i >= one) return;
+  const int m = i / nv, n = (i - m * nv) * 4;
+  floatx4 v = {};
+  const float* p = a.sums + (long)e * a.side * a.lda;
+#pragma unroll 8
+  for (int s = 0; s < a.splits; ++s) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = n + q < a.side ? n + q : 0;
+      const float u = c <= m ? p[(long)m * a.lda + c] : p[(long)c * a.lda + m];
+      v[q] += n + q < a.side ? u : 0.f;
+    }
+    p += (long)a.batch * a.side * a.lda;
+  }
+  v *= MM_ORTHO_A / (MM_ORTHO_X * MM_ORTHO_X);
+  mm_ortho_put4<PLANES>(a.a + ((long)e * a.side + m) * a.lda + n, a.pa, (const float*)&v);
 }
 
 // X <- a X + B X (rows <= cols) or a X + X B; the last step writes out alone.  Other workgroups still read the operand
@@ -505,6 +547,11 @@ size_t space(MMOrtho* a, int dtype, char* base) {
   a->a = p.take<_Float16>(planes * a->pa);
   a->b = p.take<_Float16>(planes * a->pa);
   a->next = p.take<_Float16>(planes * (a->rows <= a->cols ? a->pv : a->pu));
+  // A long side is summed in parts of 512 values or more where A has few tiles.  The rule looks at the matrix alone, so
+  // that its result does not depend on how many stand beside it.
+  const long other = a->rows < a->cols ? a->cols : a->rows;
+  a->splits = a->side <= 192 && other >= 1024 ? (int)(other / 512 < 8 ? other / 512 : 8) : 1;
+  a->sums = a->splits > 1 ? p.take<float>(a->splits * a->pa) : nullptr;
   return p.used;
 }
 
@@ -518,7 +565,12 @@ bool launch(const MMOrtho& a, long workgroups, hipStream_t stream, A... rest) {
 template <int P, int WHAT, typename Nt>
 bool square(const MMOrtho& a, hipStream_t stream) {
   const int t = (int)div_up(a.side, Nt::BM);
-  return launch<mm_ortho_square_kernel<P, WHAT, Nt>, Nt>(a, (long)a.batch * t * (t + 1) / 2, stream, t);
+  const long batch = WHAT ? a.batch : (long)a.batch * a.splits;
+  if (!launch<mm_ortho_square_kernel<P, WHAT, Nt>, Nt>(a, batch * t * (t + 1) / 2, stream, t)) return false;
+  if (WHAT == 0 && a.splits > 1)
+    hipLaunchKernelGGL((mm_ortho_join_kernel<P == 1 ? 1 : 2>), dim3((unsigned)div_up(a.side * a.lda / 4, 256), a.batch),
+                       dim3(256), 0, stream, a);
+  return true;
 }
 
 template <typename T, typename Nt>
@@ -572,7 +624,8 @@ int orthogonalize(MMOrtho a, int steps, const float* c, hipStream_t stream) {
                      dim3(256), 0, stream, a, steps);
   auto lower = [&](long n) { return a.batch * div_up(a.side, n) * (div_up(a.side, n) + 1) / 2; };
   auto all = [&](long n) { return a.batch * div_up(a.rows, n) * div_up(a.cols, n); };
-  const int sq = mm_tile_side(lower(256), lower(128), lower(64)), st = mm_tile_side(all(256), all(128), all(64));
+  const int sq = mm_tile_side(P, lower(256) * a.splits, lower(128) * a.splits, lower(64) * a.splits);
+  const int st = mm_tile_side(P, all(256), all(128), all(64));
   bool ok = true;
   for (int i = 0; i < steps && ok; ++i, c += 3) {
     a.ca = c[0];
