@@ -316,8 +316,8 @@ mm_ortho_step_kernel(MMOrtho a, int tiles_m, int tiles_n, int last) {
 }
 
 // ------------------------------------------------------------------------------------------------ small matrices
-// All steps of a small matrix in one workgroup and one launch: wave w holds the rows 16 w .. 16 w + 15 of X (its shorter
-// side) in fp32 registers, and LDS the planes of X, then those of W.  A step:
+// All steps of a small matrix in one workgroup and one launch: a wave holds RT times 16 rows of X (its shorter side) in
+// fp32 registers, and LDS the planes of X, then those of W.  A step:
 //     A = X X^T: a wave's rows of A, which as they come out of the matrix cores are operands of the next two products
 //     W = b X + c (A X), which takes X's place in LDS;  X <- a X + A W, which takes it back
 // so that neither A nor B is stored (B X = A (b X + c A X)).  The order of an operand along the summed index is free as
@@ -330,35 +330,45 @@ struct MMOrthoSmall {
   float eps, c[3 * 16];                 // a, b, c of at most 16 steps
 };
 
-template <typename T, int WAVES, int NT>
+template <typename T, int WAVES, int RT, int NT, int AHEAD>
 __global__ void __launch_bounds__(64 * WAVES) mm_ortho_small_kernel(MMOrthoSmall a) {
   // units of 16 bytes of a row: an odd number, so that any 8 consecutive rows lie in different banks
-  constexpr int PLANES = MMOrthoType<T>::PLANES, P = MMOrthoType<T>::P, MS = WAVES / 2, UNITS = 2 * NT + 1;
+  constexpr int PLANES = MMOrthoType<T>::PLANES, P = MMOrthoType<T>::P, MT = WAVES * RT, MS = MT / 2;
+  constexpr int KS = (NT + 1) / 2, UNITS = 4 * KS + 1;   // stages of 32 columns
   typedef _Float16 half8 __attribute__((ext_vector_type(8)));
   typedef short s4 __attribute__((ext_vector_type(4)));
   extern __shared__ uint4 mm_ortho_lds[];
   __shared__ double s_norm[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g = lane >> 4;
-  const int mt = (a.side + 15) / 16, ms = (a.side + 31) / 32, plane = ms * 32 * UNITS;   // units of a plane
-  const int row = 16 * wave + i16;
-  const bool wide = a.rows <= a.cols, live = row < a.side, here = wave < 2 * ms, work = wave < mt;
+  // All tiles take part (rows past the last one are zeros), so that no branch stands between the reads and the products
+  // (128 x 128 float: 9.4 -> 7.9 us a step) - but for ten waves and two planes, whose 168 registers a branch relieves
+  // (89 of 201 x 137: 305 -> 137 us).
+  constexpr bool GUARD = NT == 13 && PLANES == 2;
+  const int mt = GUARD ? (a.side + 15) / 16 : MT, ms = GUARD ? (a.side + 31) / 32 : MS;
+  const int plane = ms * 32 * UNITS;   // units of a plane
+  const bool work = !GUARD || wave * RT < mt;
+  const bool wide = a.rows <= a.cols;
+  auto row = [&](int t) { return 16 * (wave * RT + t) + i16; };
   const size_t size = (size_t)a.rows * a.cols, base = blockIdx.x * size;
-  floatx4 x[NT], acc[NT > WAVES ? NT : WAVES];
+  floatx4 x[RT][NT], acc[RT][NT > MT ? NT : MT];
   double norm = 0.;
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int n = 16 * i + 4 * g;
-    x[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-    if (live && wide) {
-      mm_load4((const T*)a.m + base + (size_t)row * a.cols, n, a.cols, (float*)&x[i]);
-    } else if (live) {
+  for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (n + q < a.other) x[i][q] = (float)((const T*)a.m)[base + (size_t)(n + q) * a.cols + row];
+    for (int i = 0; i < NT; ++i) {
+      const int n = 16 * i + 4 * g, r = row(t);
+      floatx4 v = {};
+      if (r < a.side && wide) {
+        mm_load4((const T*)a.m + base + (size_t)r * a.cols, n, a.cols, (float*)&v);
+      } else if (r < a.side) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (n + q < a.other) v[q] = (float)((const T*)a.m)[base + (size_t)(n + q) * a.cols + r];
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) norm = fma((double)v[q], (double)v[q], norm);
+      x[t][i] = v;
     }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) norm = fma((double)x[i][q], (double)x[i][q], norm);
-  }
 #pragma unroll
   for (int d = 32; d; d >>= 1) norm += __shfl_xor(norm, d);
   if (lane == 0) s_norm[wave] = norm;
@@ -367,14 +377,19 @@ __global__ void __launch_bounds__(64 * WAVES) mm_ortho_small_kernel(MMOrthoSmall
   for (int w = 0; w < WAVES; ++w) norm += s_norm[w];
   const double by = 1. / (sqrt(norm) + (double)a.eps);
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int t = 0; t < RT; ++t)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) x[i][q] = x[i][q] == 0.f ? x[i][q] : (float)((double)x[i][q] * by);   // no norm: zeros
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float v = x[t][i][q];
+        x[t][i][q] = v == 0.f ? v : (float)((double)v * by);   // no norm: zeros
+      }
 
   _Float16* const tile = (_Float16*)mm_ortho_lds;
-  auto put = [&](floatx4 r, int i) {   // 4 values of tile i of this lane's row
+  auto put = [&](floatx4 r, int t, int i) {   // 4 values of tile i of this lane's row of t
     r *= MM_ORTHO_X;
-    _Float16* const at = tile + 8 * (row * UNITS + 2 * i) + 4 * g;
+    _Float16* const at = tile + 8 * (row(t) * UNITS + 2 * i) + 4 * g;
 #pragma unroll
     for (int p = 0; p < PLANES; ++p) {
       halfx4 h;
@@ -405,67 +420,95 @@ __global__ void __launch_bounds__(64 * WAVES) mm_ortho_small_kernel(MMOrthoSmall
       v[p] = __builtin_bit_cast(half8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
     }
   };
-  auto mma = [&](floatx4& c, const half8 (&u)[PLANES], const half8 (&v)[PLANES]) {
-    if constexpr (P == 3) {
-      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[1], v[0], c, 0, 0, 0);
-      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[0], v[1], c, 0, 0, 0);
-    }
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[0], v[0], c, 0, 0, 0);
+  // c[t][i] += the products of operand u with the rows' operands v[t], by passes, so that no product waits for another
+  auto mma = [&](auto& c, int i, const half8 (&u)[PLANES], const half8 (&v)[RT][PLANES]) {
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        c[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[mm_nt_first<P>(q)], v[t][mm_nt_second<P>(q)], c[t][i], 0, 0, 0);
   };
 
-  if (here) {
+  auto put_all = [&](const auto& v) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) put(x[i], i);
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) put(v[t][i], t, i);
+  };
+
+  if constexpr (NT % 2 == 1) {   // the rest of the last stage, never written again
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int p = 0; p < PLANES; ++p)
+        if (g < 2) mm_ortho_lds[p * plane + row(t) * UNITS + 2 * NT + g] = uint4{0, 0, 0, 0};
   }
+  put_all(x);
   __syncthreads();
   for (int step = 0; step < a.steps; ++step) {
     const float ca = a.c[3 * step], cb = a.c[3 * step + 1], cc = a.c[3 * step + 2];
-    half8 fa[MS][PLANES];
+    half8 fa[RT][MS][PLANES];
     if (work) {   // A: this wave's rows
 #pragma unroll
-      for (int i = 0; i < WAVES; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (int s = 0; s < NT / 2; ++s) {
-        half8 v[PLANES], u[2][PLANES];
-        read_rows(v, 16 * wave, s);
-        read_rows(u[0], 0, s);
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-          if (i + 1 < WAVES && i + 1 < mt) read_rows(u[(i + 1) & 1], 16 * (i + 1), s);
+        for (int i = 0; i < MT; ++i) acc[t][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int s = 0; s < KS; ++s) {
+        half8 v[RT][PLANES], u[AHEAD + 1][PLANES];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) read_rows(v[t], 16 * (wave * RT + t), s);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) read_rows(u[i], 16 * i, s);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if (i + AHEAD < MT && (!GUARD || i + AHEAD < mt)) read_rows(u[(i + AHEAD) % (AHEAD + 1)], 16 * (i + AHEAD), s);
           __builtin_amdgcn_sched_barrier(0);
-          if (i < mt) mma(acc[i], u[i & 1], v);
+          if (!GUARD || i < mt) mma(acc, i, u[i % (AHEAD + 1)], v);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
 #pragma unroll
-      for (int s = 0; s < MS; ++s)
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float v = acc[2 * s + e / 4][e % 4] * (MM_ORTHO_A / (MM_ORTHO_X * MM_ORTHO_X));
+        for (int s = 0; s < MS; ++s)
 #pragma unroll
-          for (int p = 0; p < PLANES; ++p) {
-            const _Float16 h = (_Float16)v;
-            fa[s][p][e] = h;
-            v -= (float)h;
+          for (int e = 0; e < 8; ++e) {
+            float v = acc[t][2 * s + e / 4][e % 4] * (MM_ORTHO_A / (MM_ORTHO_X * MM_ORTHO_X));
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) {
+              const _Float16 h = (_Float16)v;
+              fa[t][s][p][e] = h;
+              v -= (float)h;
+            }
           }
-        }
     }
     auto product = [&]() {   // acc = this wave's rows of A times what is in LDS, in units of both scales
-      half8 u[2][PLANES];
-      read_cols(u[0], 0, 0);
+      half8 u[AHEAD + 1][PLANES];
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s) read_cols(u[s], 0, s);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t][i] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < MS; ++s) {
-          const int now = (i * MS + s) & 1;   // operands in turn, over the tiles too
-          if (s + 1 < MS) {
-            if (s + 1 < ms) read_cols(u[now ^ 1], i, s + 1);
+          constexpr int SEQ = AHEAD + 1;
+          const int q = i * MS + s;   // of the sequence of operands, read AHEAD before their products
+          if (s + AHEAD < MS) {
+            if (!GUARD || s + AHEAD < ms) read_cols(u[(q + AHEAD) % SEQ], i, s + AHEAD);
           } else if (i + 1 < NT) {
-            read_cols(u[now ^ 1], i + 1, 0);
+            read_cols(u[(q + AHEAD) % SEQ], i + 1, s + AHEAD - MS);
           }
           __builtin_amdgcn_sched_barrier(0);
-          if (s < ms) mma(acc[i], u[now], fa[s]);
+          if (!GUARD || s < ms) {
+            half8 v[RT][PLANES];
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+              for (int p = 0; p < PLANES; ++p) v[t][p] = fa[t][s][p];
+            mma(acc, i, u[q % SEQ], v);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -474,40 +517,42 @@ __global__ void __launch_bounds__(64 * WAVES) mm_ortho_small_kernel(MMOrthoSmall
     if (work) {
       product();
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        acc[i] = cb * x[i] + cc * UNIT * acc[i];
-        x[i] *= ca;
-      }
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          acc[t][i] = cb * x[t][i] + cc * UNIT * acc[t][i];
+          x[t][i] *= ca;
+        }
     }
     __syncthreads();   // everyone is done with X
-    if (work) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i) put(acc[i], i);
-    }
+    if (work) put_all(acc);
     __syncthreads();
     if (work) {
       product();
 #pragma unroll
-      for (int i = 0; i < NT; ++i) x[i] += UNIT * acc[i];
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) x[t][i] += UNIT * acc[t][i];
     }
     if (step + 1 == a.steps) break;
     __syncthreads();
-    if (work) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i) put(x[i], i);
-    }
+    if (work) put_all(x);
     __syncthreads();
   }
-  if (!live) return;
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int n = 16 * i + 4 * g;
-    if (wide) {
-      mm_store4((T*)a.out + base + (size_t)row * a.cols, n, a.cols, (const float*)&x[i]);
-    } else {
+  for (int t = 0; t < RT; ++t) {
+    const int r = row(t);
+    if (r >= a.side) break;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (n + q < a.other) ((T*)a.out)[base + (size_t)(n + q) * a.cols + row] = (T)x[i][q];
+    for (int i = 0; i < NT; ++i) {
+      const int n = 16 * i + 4 * g;
+      if (wide) {
+        mm_store4((T*)a.out + base + (size_t)r * a.cols, n, a.cols, (const float*)&x[t][i]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (n + q < a.other) ((T*)a.out)[base + (size_t)(n + q) * a.cols + r] = (T)x[t][i][q];
+      }
     }
   }
 }
@@ -579,24 +624,25 @@ bool step(const MMOrtho& a, int last, hipStream_t stream) {
   return launch<mm_ortho_step_kernel<T, Nt>, Nt>(a, (long)a.batch * tm * tn, stream, tm, tn, last);
 }
 
-template <typename T, int WAVES, int NT>
+template <typename T, int WAVES, int RT, int NT, int AHEAD>
 bool small(const MMOrthoSmall& a, int batch, int lds, hipStream_t stream) {
-  if (!lds_granted<mm_ortho_small_kernel<T, WAVES, NT>>(lds)) return false;
-  hipLaunchKernelGGL((mm_ortho_small_kernel<T, WAVES, NT>), dim3(batch), dim3(64 * WAVES), lds, stream, a);
+  if (!lds_granted<mm_ortho_small_kernel<T, WAVES, RT, NT, AHEAD>>(lds)) return false;
+  hipLaunchKernelGGL((mm_ortho_small_kernel<T, WAVES, RT, NT, AHEAD>), dim3(batch), dim3(64 * WAVES), lds, stream, a);
   return true;
 }
 
-// waves, tiles of columns and LDS of a matrix that a workgroup holds (waves 0: it does not)
-struct Held { int waves, nt, lds; };
+// rows, tiles of columns and LDS of the workgroup that holds a matrix (rows 0: none does)
+struct Held { int rows, nt, lds; };
 Held held(long rows, long cols, int dtype, int steps) {
   const long side = rows < cols ? rows : cols, other = rows < cols ? cols : rows;
   Held h{0, 0, 0};
   if (steps > 16) return h;
-  if (side <= 64 && other <= 64) h = Held{4, 4, 0};
-  else if (side <= 128 && other <= 128) h = Held{8, 8, 0};
-  else if (side <= 128 && other <= 256) h = Held{8, 16, 0};
-  else if (side <= 160 && other <= 224) h = Held{10, 14, 0};
-  h.lds = (int)(mm_up(side, 32) * (2 * h.nt + 1) * 16 * (dtype == MM_BF16 ? 1 : 2));
+  if (side <= 64 && other <= 64) h = Held{64, 4, 0};
+  else if (side <= 64 && other <= 256) h = Held{64, 16, 0};
+  else if (side <= 128 && other <= 128) h = Held{128, 8, 0};
+  else if (side <= 128 && other <= 256) h = Held{128, 16, 0};
+  else if (side <= 160 && other <= 208) h = Held{160, 13, 0};
+  h.lds = h.rows * ((h.nt + 1) / 2 * 4 + 1) * 16 * (dtype == MM_BF16 ? 1 : 2);
   return h;
 }
 
@@ -605,10 +651,11 @@ int orthogonalize_small(const MMOrtho& o, int steps, const float* c, const Held&
   MMOrthoSmall a{o.m, o.out, o.rows, o.cols, o.side, o.rows < o.cols ? o.cols : o.rows, steps, o.eps, {}};
   for (int i = 0; i < 3 * steps; ++i) a.c[i] = c[i];
   bool ok;
-  if (h.waves == 4) ok = small<T, 4, 4>(a, o.batch, h.lds, stream);
-  else if (h.nt == 8) ok = small<T, 8, 8>(a, o.batch, h.lds, stream);
-  else if (h.nt == 16) ok = small<T, 8, 16>(a, o.batch, h.lds, stream);
-  else ok = small<T, 10, 14>(a, o.batch, h.lds, stream);
+  if (h.nt == 4) ok = small<T, 4, 1, 4, 2>(a, o.batch, h.lds, stream);
+  else if (h.rows == 64) ok = small<T, 4, 1, 16, 2>(a, o.batch, h.lds, stream);
+  else if (h.nt == 8) ok = small<T, 8, 1, 8, 2>(a, o.batch, h.lds, stream);
+  else if (h.nt == 16) ok = small<T, 8, 1, 16, 2>(a, o.batch, h.lds, stream);
+  else ok = small<T, 10, 1, 13, 1>(a, o.batch, h.lds, stream);
   return ok ? mm::launch_status("mm_orthogonalize") : MM_ELAUNCH;
 }
 
@@ -686,7 +733,7 @@ extern "C" int mm_orthogonalize(const void* m, int dtype, long batch, long rows,
   space(&a, dtype, (char*)workspace);
   int done = MM_OK;
   const Held h = held(rows, cols, dtype, steps);
-  if (h.waves) MM_DISPATCH(dtype, done = orthogonalize_small<T_>(a, steps, coefficients, h, stream));
+  if (h.rows) MM_DISPATCH(dtype, done = orthogonalize_small<T_>(a, steps, coefficients, h, stream));
   else MM_DISPATCH(dtype, done = orthogonalize<T_>(a, steps, coefficients, stream));
   return done;
 }
