@@ -302,23 +302,26 @@ __device__ __forceinline__ void mm_group_tile(const MMGroup& a, long tile, F f) 
 // WAVES waves per structure of more than `small` rows (and group, where blockIdx.y counts them).  FWD: (mean, rstd) of
 // the tiles' (mean, M2); else the sums of both numbers.
 template <bool FWD, int WAVES>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
 mm_groupnorm_join_kernel(MMGroup a, const float* __restrict__ part, float eps, float* __restrict__ out) {
-  __shared__ float s0[4], s1[4];
+  constexpr int PER = WAVES == 1 ? 4 : 1;   // structures of a workgroup
+  __shared__ float s0[WAVES], s1[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   auto all = [&](float v, float* lds) {
     v = mm_lanes_sum<64>(v);
-    if constexpr (WAVES == 4) {
+    if constexpr (WAVES > 1) {
       if (lane == 0) lds[wave] = v;
       __syncthreads();
-      v = lds[0] + lds[1] + lds[2] + lds[3];
+      v = lds[0];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) v += lds[w];
       __syncthreads();
     }
     return v;
   };
-  const int first = WAVES == 4 ? threadIdx.x : lane;
-  const long step = (long)gridDim.x * (4 / WAVES);
-  for (long s = (long)blockIdx.x * (4 / WAVES) + (WAVES == 4 ? 0 : wave); s < a.structs; s += step) {
+  const int first = WAVES > 1 ? threadIdx.x : lane;
+  const long step = (long)gridDim.x * PER;
+  for (long s = (long)blockIdx.x * PER + (PER > 1 ? wave : 0); s < a.structs; s += step) {
     const MMRange q = mm_group_range(a, s);
     if (q.n <= a.small) continue;
     const long t0 = q.first / a.small, t1 = (q.first + q.n - 1) / a.small;
@@ -437,7 +440,7 @@ bool make_plan(const char* name, long rows, int structs, const int* offsets, int
 template <bool FWD>
 void join_tiles(const MMGroup& a, const float* part, float eps, float* out, hipStream_t stream) {
   if (a.structs < 256) {
-    hipLaunchKernelGGL((mm_groupnorm_join_kernel<FWD, 4>), dim3(a.structs, a.G), dim3(256), 0, stream, a, part, eps, out);
+    hipLaunchKernelGGL((mm_groupnorm_join_kernel<FWD, 16>), dim3(a.structs, a.G), dim3(1024), 0, stream, a, part, eps, out);
   } else {
     const int n = a.structs / 4 + 1;
     hipLaunchKernelGGL((mm_groupnorm_join_kernel<FWD, 1>), dim3(n < 4096 ? n : 4096), dim3(256), 0, stream, a, part, eps,

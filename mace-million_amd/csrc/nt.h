@@ -416,18 +416,23 @@ inline MMTileRates mm_tile_rates(int P) {
   return MMTileRates{{256, 128, 64}, {256, 256, 512}, {1., 0.31, 0.28}};
 }
 
-// Side of the tiles of a launch that would have t256, t128 or t64 of them: the least time.
-inline int mm_tile_side(int P, long t256, long t128, long t64) {
+// Time of a launch that would have t256, t128 or t64 tiles of those sides, with the best of them.
+inline double mm_tile_time(int P, long t256, long t128, long t64, int* side = nullptr) {
   const MMTileRates r = mm_tile_rates(P);
   const long t[] = {t256, t128, t64};
-  int best = 0;
   double least = 1e30;
   for (int i = 0; i < 3; ++i) {
     const double time = r.round[i] * (double)((t[i] + r.slots[i] - 1) / r.slots[i]);
     if (time < least) {
       least = time;
-      best = r.side[i];
+      if (side) *side = r.side[i];
     }
   }
-  return best;
+  return least;
+}
+
+inline int mm_tile_side(int P, long t256, long t128, long t64) {
+  int side = 64;
+  mm_tile_time(P, t256, t128, t64, &side);
+  return side;
 }

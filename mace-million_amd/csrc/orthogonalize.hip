@@ -704,15 +704,40 @@ int check(const char* name, long batch, long rows, long cols, int dtype) {
 }
 }  // namespace
 
+namespace {
+// Matrices taken at once.  Up to 240 MB of workspace, so that their planes stay in the last cache (256 MB) between the
+// products, and a number whose tiles fill their rounds (64 bfloat16 matrices of 1024 x 1024: 64 at once 2900 us, 16 2800,
+// 14 2700).
+int part_of(MMOrtho a, long batch, int dtype) {
+  a.batch = 1;
+  const long fits = 251658240L / (long)space(&a, dtype, nullptr), most = fits < 1 ? 1 : fits < batch ? fits : batch;
+  const int P = dtype == MM_BF16 ? 1 : 3;
+  auto lower = [&](long p, long n) { return p * div_up(a.side, n) * (div_up(a.side, n) + 1) / 2; };
+  auto all = [&](long p, long n) { return p * div_up(a.rows, n) * div_up(a.cols, n); };
+  long best = most;
+  double least = 1e300;
+  for (long p = most; p >= 1 && 2 * p >= most; --p) {
+    double time = 2. * mm_tile_time(P, lower(p, 256), lower(p, 128), lower(p, 64))
+                + mm_tile_time(P, all(p, 256), all(p, 128), all(p, 64));
+    time *= (double)div_up(batch, p);
+    if (time < least) {
+      least = time;
+      best = p;
+    }
+  }
+  return (int)best;
+}
+}  // namespace
+
 extern "C" int mm_orthogonalize_workspace(long batch, long rows, long cols, int dtype, size_t* bytes) {
   const int rc = check("mm_orthogonalize_workspace", batch, rows, cols, dtype);
   if (rc != MM_OK) return rc;
   MM_CHECK_ARG(bytes, "no result");
   MMOrtho a{};
-  a.batch = (int)batch;
   a.rows = (int)rows;
   a.cols = (int)cols;
-  *bytes = space(&a, dtype, nullptr);
+  a.batch = batch ? part_of(a, batch, dtype) : 0;
+  *bytes = batch ? space(&a, dtype, nullptr) : 0;
   return MM_OK;
 }
 
@@ -724,16 +749,24 @@ extern "C" int mm_orthogonalize(const void* m, int dtype, long batch, long rows,
   if (batch == 0) return MM_OK;
   MM_CHECK_ARG(m && out && workspace, "null pointer");
   MMOrtho a{};
-  a.m = m;
-  a.out = out;
   a.eps = eps;
-  a.batch = (int)batch;
   a.rows = (int)rows;
   a.cols = (int)cols;
-  space(&a, dtype, (char*)workspace);
-  int done = MM_OK;
+  a.side = (int)(rows < cols ? rows : cols);
   const Held h = held(rows, cols, dtype, steps);
-  if (h.rows) MM_DISPATCH(dtype, done = orthogonalize_small<T_>(a, steps, coefficients, h, stream));
-  else MM_DISPATCH(dtype, done = orthogonalize<T_>(a, steps, coefficients, stream));
-  return done;
+  const long part = h.rows ? batch : part_of(a, batch, dtype), size = rows * cols * (dtype == MM_F32 ? 4 : 2);
+  for (long i = 0; i < batch; i += part) {
+    a.m = (const char*)m + i * size;
+    a.out = (char*)out + i * size;
+    a.batch = (int)(batch - i < part ? batch - i : part);
+    int done = MM_OK;
+    if (h.rows) {
+      MM_DISPATCH(dtype, done = orthogonalize_small<T_>(a, steps, coefficients, h, stream));
+    } else {
+      space(&a, dtype, (char*)workspace);
+      MM_DISPATCH(dtype, done = orthogonalize<T_>(a, steps, coefficients, stream));
+    }
+    if (done != MM_OK) return done;
+  }
+  return MM_OK;
 }

@@ -220,10 +220,6 @@ Tensor linear_cross_entropy(const Tensor& x0, const Tensor& weight0, const Tenso
 }
 
 // ------------------------------------------------------------------------------------------------ orthogonalisation
-// Workspace of the matrices taken at once: a larger batch goes in equal parts, whose planes then stay in the last cache
-// (256 MB) between the products (64 bfloat16 matrices of 1024 x 1024, 14 MB each: 2900 us at once, 2700 in parts of 14).
-constexpr size_t kOrthoBytes = 251658240UL;
-
 Tensor orthogonalize(const Tensor& m0, const std::vector<float>& coefficients, double eps) {
   const Tensor m1 = plain(m0);
   const int code = check_gpu(m1, "m");
@@ -240,17 +236,16 @@ Tensor orthogonalize(const Tensor& m0, const std::vector<float>& coefficients, d
   const Tensor m = m1.contiguous();
   Tensor out = at::empty(m.sizes(), m.options());
   if (batch == 0) return out;
-  size_t one = 0, bytes = 0;
-  done(mm_orthogonalize_workspace(1, rows, cols, code, &one));
-  const long most = std::max(1L, std::min({batch, (long)(kOrthoBytes / one), 65535L}));
-  const long parts = (batch + most - 1) / most, part = (batch + parts - 1) / parts;
-  done(mm_orthogonalize_workspace(part, rows, cols, code, &bytes));
-  const Tensor ws = bytes_like(bytes, m);
   const long step = rows * cols * (long)m.element_size();
-  for (long i = 0; i < batch; i += part)
-    done(mm_orthogonalize((const char*)ptr(m) + i * step, code, std::min(part, batch - i), rows, cols,
-                          (int)(coefficients.size() / 3), coefficients.data(), (float)eps, (char*)ptr(out) + i * step,
-                          ptr(ws), stream()));
+  Tensor ws;
+  for (long i = 0; i < batch; i += 65535) {   // of a launch's grid
+    const long n = std::min(batch - i, 65535L);
+    size_t bytes = 0;
+    done(mm_orthogonalize_workspace(n, rows, cols, code, &bytes));
+    if (!ws.defined() || bytes > (size_t)ws.numel()) ws = bytes_like(bytes, m);
+    done(mm_orthogonalize((const char*)ptr(m) + i * step, code, n, rows, cols, (int)(coefficients.size() / 3),
+                          coefficients.data(), (float)eps, (char*)ptr(out) + i * step, ptr(ws), stream()));
+  }
   return out;
 }
 }  // namespace
