@@ -409,15 +409,15 @@ int mm_groupnorm_bwd(const void* dy, long lddy, const void* x, long ldx, int dty
                      const float* stats, void* dx, long lddx, void* dw, void* db, float* workspace, mm_stream_t stream);
 /* Cross entropy of the logits x w^T, x [T, D] (rows ldx apart), w [V, D] dense, both of dtype; targets [T] int (int64
  * with targets64), `ignore` leaves a row out, others outside [0, V) make its loss NaN.  reduction 0 none (loss [T], 0 for
- * rows left out), 1 sum, 2 mean over the rows asked (0 if there are none).  lse [T] and rows [4 + 3 T] are what mm_ce_bwd
+ * rows left out), 1 sum, 2 mean over the rows asked (0 if there are none).  stats [2][T] and rows [4 + 3 T] are what mm_ce_bwd
  * needs.  workspace: of mm_ce_workspace bytes (dx = dw = 0: of mm_ce_fwd; it depends on w's alignment) */
 int mm_ce_workspace(long T, long D, long V, int dtype, const void* w, int dx, int dw, size_t* bytes /* HOST */);
 int mm_ce_fwd(const void* x, long ldx, int dtype, long T, long D, const void* w, long V, const void* targets,
-              int targets64, long ignore, int reduction, float* loss, float* lse, int* rows, void* workspace,
+              int targets64, long ignore, int reduction, float* loss, float* stats, int* rows, void* workspace,
               mm_stream_t stream);
 /* dx [T, D] (0 in rows left out), dw [V, D], each nullable; dloss [T] (reduction 0) or [1] */
 int mm_ce_bwd(const void* x, long ldx, int dtype, long T, long D, const void* w, long V, int reduction,
-              const float* lse, const int* rows, const float* dloss, void* dx, void* dw, void* workspace,
+              const float* stats, const int* rows, const float* dloss, void* dx, void* dw, void* workspace,
               mm_stream_t stream);
 /* out = X after `steps` of A = X X^T, X <- a X + (b A + c A A) X (on the shorter side) from X = m / (|m| + eps), for every
  * matrix of m [batch, rows, cols]; coefficients HOST [steps][3]; at most 65535 matrices of 65536 rows and columns */

@@ -1,8 +1,14 @@
 // Cross entropy of linear logits, without keeping them:
-//     l[t, v] = x[t] . W[v],  lse[t] = log sum_v exp(l[t, v]),  loss[t] = lse[t] - l[t, y[t]]
-//     d[t, v] = exp(l[t, v] - lse[t]) - [v = y[t]]:  dx[t] = g[t] d[t] W,  dW = sum_t g[t] d[t]^T x[t]
+//     l[t, v] = x[t] . W[v],  top[t] = max_v l[t, v],  s[t] = sum_v exp(l[t, v] - top[t])
+//     loss[t] = top[t] - l[t, y[t]] + log s[t]
+//     d[t, v] = exp(l[t, v] - top[t]) / s[t] - [v = y[t]]:  dx[t] = g[t] d[t] W,  dW = sum_t g[t] d[t]^T x[t]
+// top and s are kept, not log sum exp: its rounding (2^-24 of it) would be a relative error of a whole row of
+// probabilities, and d of a row that is certain of its class is their difference from 1.  For the same reason backward
+// takes the logits again in the forward's order of sums: few rows by the kernel for few rows, more by tiles.
 // Rows whose target is ignored are taken out at the start: `list` has the asked rows in their order, and everything
-// runs over their number, which stays on the GPU.
+// runs over their number, which stays on the GPU.  (8192 rows, 131,072 classes of 2048 bfloat16 values, both gradients:
+// 16.3 ms, 807 TFLOP/s of the 13.2 T operations.  14,700 rows, 89 classes of 128 float values: 104 us, launches and
+// the six products of small tiles.)
 // Forward: tiles of logits in registers, of which every row's maximum, sum of exponentials and target's logit go out.
 // Backward: pieces of the vocabulary; the logits of a piece are taken again and become d, stored in 16 bits by rows
 // and transposed, and two products give the piece's part of dx (kept in fp32 over the pieces) and its rows of dW.
@@ -241,7 +247,7 @@ struct MMCeLogits {
   float *part, *picked;  // [tiles of columns][T][2], [T]
   long T;
   // backward: columns v0 .. v0 + n
-  const float* lse;
+  const float* stats;            // [2][T]: top, s
   MMCeScale by;
   H *d, *dT;                     // [T][ldd], [n][ldt] (planes)
   long ldd, ldt, plane, planeT;
@@ -303,11 +309,12 @@ mm_ce_logits_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
   }
 }
 
-// 32 rows a workgroup, 32 threads for the tiles of each; lse and the losses; sums [blocks] (nullable): of the losses
+// 32 rows a workgroup, 32 threads for the tiles of each (one thread a row walks the tiles alone, far from filling the
+// card); statistics and losses; sums [blocks] (nullable): of the losses
 __global__ void __launch_bounds__(1024)
 mm_ce_rows_kernel(const float* __restrict__ part, long T, int tiles_n, const int* __restrict__ count,
                   const int* __restrict__ list, const int* __restrict__ y, const float* __restrict__ picked,
-                  float* __restrict__ lse, float* __restrict__ loss, float* __restrict__ sums) {
+                  float* __restrict__ stats, float* __restrict__ loss, float* __restrict__ sums) {
   __shared__ MMCeRow s[32][33];
   const int row = threadIdx.x & 31, q = threadIdx.x >> 5, n = *count;
   int i = blockIdx.x * 32 + row;
@@ -329,9 +336,9 @@ mm_ce_rows_kernel(const float* __restrict__ part, long T, int tiles_n, const int
   i = blockIdx.x * 32 + k;
   float l = 0.f;
   if (i < n && (threadIdx.x & 31) == 0) {
-    const float z = r.top + logf(r.sum);
-    lse[i] = z;
-    l = y[i] < 0 ? __builtin_nanf("") : z - picked[i];
+    stats[i] = r.top;
+    stats[T + i] = r.sum;
+    l = y[i] < 0 ? __builtin_nanf("") : r.top - picked[i] + logf(r.sum);
     if (loss) loss[list[i]] = l;
   }
   if (!sums) return;
@@ -345,8 +352,8 @@ mm_ce_rows_kernel(const float* __restrict__ part, long T, int tiles_n, const int
 }
 
 // sum (mean) of the blocks' sums
-__global__ void __launch_bounds__(1024) mm_ce_total_kernel(const float* __restrict__ sums, const int* __restrict__ count,
-                                                           int mean, float* __restrict__ loss) {
+__global__ void __launch_bounds__(1024)
+mm_ce_total_kernel(const float* __restrict__ sums, const int* __restrict__ count, int mean, float* __restrict__ loss) {
   __shared__ double s[16];
   const int n = *count, blocks = (n + 31) / 32;
   double t = 0.;
@@ -361,9 +368,10 @@ __global__ void __launch_bounds__(1024) mm_ce_total_kernel(const float* __restri
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// The forward of few rows, in one launch or two: rows of W go by in vectors, one class a wave, and meet all rows of x
+// The forward of few rows, in one launch or two: rows of W go by in vectors, a few classes a wave, and meet all rows of x
 // (fp32 in LDS); every workgroup lists the rows by itself.  Bound by reading W: one row, 100,003 classes of 4096
-// bfloat16 values.  One workgroup finishes the losses (small heads), more leave partial sums to the rows' kernel.
+// bfloat16 values in 211 us, 3.9 TB/s.  One workgroup finishes the losses (small heads), more leave partial sums to the
+// rows' kernel.  Backward (D) takes the same logits and leaves d for the products.
 #define MM_CE_FEW 16     // rows, at most
 #define MM_CE_FEW_LDS 16384   // floats of x in LDS
 #define MM_CE_CLASSES 4  // of a wave at once
@@ -373,28 +381,46 @@ struct MMCeFew {
   long ldx, ignore;
   int T, D, V, targets64, reduction;
   int *count, *list, *y, *pos;
-  float *part, *picked, *lse, *loss;
+  float *part, *picked, *stats, *loss;
 };
 
-template <typename T, int ROWS, int TH>
-__global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a) {
+// D: d of the asked rows (nothing is listed) instead of the statistics, for classes v0 .. v0 + V of the head
+template <typename T>
+struct MMCeFewD {
+  typename MMCeType<T>::H *d, *dT;   // [rows][ldd], [V][64] (planes)
+  long ldd, plane, planeT;
+  int v0;
+  float scale;
+  MMCeScale by;
+};
+
+template <typename T, int ROWS, int TH, bool D>
+__global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b) {
   constexpr int N = MMVec<T>::N, W = TH / 64, C = MM_CE_CLASSES;
   extern __shared__ float mm_ce_x[];   // [T][D rounded up to whole vectors of a wave]
   __shared__ MMCeRow s_row[W][ROWS];
   __shared__ float s_hit[W][ROWS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, Dp = (a.D + 64 * N - 1) / (64 * N) * (64 * N);
-  // lane t of every wave: row t (rows that are left out are computed like the others and go nowhere)
-  const bool has = lane < a.T;
-  const long target = !has ? a.ignore : a.targets64 ? ((const long*)a.targets)[lane] : (long)((const int*)a.targets)[lane];
+  // lane t of every wave: row t (rows that are left out are computed like the others and go nowhere); D: asked row t
+  const int rows = D ? *a.count : a.T;
+  const bool has = lane < rows;
+  const long target = D || !has     ? a.ignore
+                      : a.targets64 ? ((const long*)a.targets)[lane]
+                                    : (long)((const int*)a.targets)[lane];
 #pragma unroll
   for (int t = 0; t < ROWS; ++t) {
-    if (t >= a.T) break;
-    for (int c = threadIdx.x; c < Dp; c += TH) mm_ce_x[t * Dp + c] = c < a.D ? (float)((const T*)a.x)[t * a.ldx + c] : 0.f;
+    if (t >= rows) break;
+    const long at = D ? a.list[t] : t;
+    for (int c = threadIdx.x; c < Dp; c += TH)
+      mm_ce_x[t * Dp + c] = c < a.D ? (float)((const T*)a.x)[at * a.ldx + c] : 0.f;
   }
   const unsigned long long asked = __ballot(target != a.ignore);
   const int at = __popcll(asked & ((1ull << lane) - 1)), n = __popcll(asked);
-  const int y = target >= 0 && target < a.V ? (int)target : -1;
-  if (blockIdx.x == 0 && wave == 0) {
+  const int y = D ? a.y[has ? lane : 0] : target >= 0 && target < a.V ? (int)target : -1;
+  const float top = D ? a.stats[has ? lane : 0] : 0.f, inv = D ? 1.f / a.stats[a.T + (has ? lane : 0)] : 0.f;
+  const float share = D ? b.by.share(has ? lane : 0) : 0.f;
+  const int end = D ? (int)mm_up(a.V, MM_NT_K) : a.V;   // D: zeros past the last class
+  if (!D && blockIdx.x == 0 && wave == 0) {
     if (target != a.ignore) {
       a.list[at] = lane;
       a.y[at] = y;
@@ -406,7 +432,7 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a) {
   __syncthreads();
   MMCeRow r{-INFINITY, 0.f};
   float hit = 0.f;
-  for (int v0 = (blockIdx.x * W + wave) * C; v0 < a.V; v0 += (int)gridDim.x * W * C) {
+  for (int v0 = (blockIdx.x * W + wave) * C; v0 < end; v0 += (int)gridDim.x * W * C) {
     float acc[ROWS][C] = {};
     const T* __restrict__ p[C];
 #pragma unroll
@@ -417,7 +443,7 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a) {
       for (int k = 0; k < C; ++k) mm_load_vec(p[k], c, end, w[k]);
 #pragma unroll
       for (int t = 0; t < ROWS; ++t) {
-        if (ROWS > 1 && t >= a.T) break;
+        if (ROWS > 1 && t >= rows) break;
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
           const floatx4 x = *(const floatx4*)(mm_ce_x + t * Dp + c + i);
@@ -433,19 +459,43 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a) {
 #pragma unroll 4
     for (; c < whole; c += 64 * N) add(c, c + N);
     if (whole < a.D && c < Dp) add(c, a.D);
+    float mine[C] = {};
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) {
-      if (ROWS > 1 && t >= a.T) break;
+      if (ROWS > 1 && t >= rows) break;
 #pragma unroll
       for (int k = 0; k < C; ++k) {
         const float l = mm_lanes_sum<64>(acc[t][k]);
-        if (lane == t && v0 + k < a.V) {
+        if constexpr (D) {
+          if (lane == t) mine[k] = l;
+        } else if (lane == t && v0 + k < a.V) {
           r = mm_ce_join(r, MMCeRow{l, 1.f});
           if (v0 + k == y) hit = l;
         }
       }
     }
+    if constexpr (D) {
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        const float p = __expf(mine[k] - top) * inv - (v0 + k + b.v0 == y ? 1.f : 0.f);
+        // a target out of range (loss NaN) makes the row NaN
+        mine[k] = has && v0 + k < a.V ? (y < 0 ? __builtin_nanf("") : p * b.scale) : 0.f;
+      }
+      if (has) mm_ce_put4<T>(b.d + lane * b.ldd + v0, b.plane, mine);
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        if (v0 + k >= a.V) break;
+        float v = mine[k] * share;
+#pragma unroll
+        for (int q = 0; q < MMCeType<T>::PLANES; ++q) {
+          const typename MMCeType<T>::H h = (typename MMCeType<T>::H)v;
+          b.dT[q * b.planeT + (long)(v0 + k) * 64 + lane] = has ? h : (typename MMCeType<T>::H)0.f;
+          v -= (float)h;
+        }
+      }
+    }
   }
+  if constexpr (D) return;
   if (gridDim.x > 1 && target != a.ignore && y >= 0 && y / C % (int)(gridDim.x * W) == (int)blockIdx.x * W + wave)
     a.picked[at] = hit;   // by the wave that has the target's class
   if (lane < ROWS) {
@@ -467,9 +517,9 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a) {
       p[1] = r.sum;
       return;
     }
-    const float z = r.top + logf(r.sum);
-    a.lse[at] = z;
-    l = y < 0 ? __builtin_nanf("") : z - hit;
+    a.stats[at] = r.top;
+    a.stats[a.T + at] = r.sum;
+    l = y < 0 ? __builtin_nanf("") : r.top - hit + logf(r.sum);
     if (a.reduction == 0) a.loss[lane] = l;
   }
   if (gridDim.x > 1 || a.reduction == 0) return;
@@ -518,14 +568,14 @@ mm_ce_d_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
 #pragma unroll
   for (int j = 0; j < Nt::FM; ++j) {
     const int m = m0 + t.row(j), at = min(m, count - 1), y = a.y[at];
-    const float lse = a.lse[at];
+    const float top = a.stats[at], inv = 1.f / a.stats[a.T + at];
     share[j] = a.by.share(at);
 #pragma unroll
     for (int i = 0; i < Nt::FN; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int n = n0 + t.col(i) + q;
-        const float p = __expf(t.acc[i][j][q] - lse) - (n + a.v0 == y ? 1.f : 0.f);
+        const float p = __expf(t.acc[i][j][q] - top) * inv - (n + a.v0 == y ? 1.f : 0.f);
         // a target out of range (loss NaN) makes the row NaN
         t.acc[i][j][q] = n < a.n && m < count ? (y < 0 ? __builtin_nanf("") : p * a.scale) : 0.f;
       }
@@ -556,7 +606,8 @@ mm_ce_d_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
     return;
   }
   H* const tile = (H*)mm_ce_lds;
-  mm_nt_store(t, tile, a.d + (long)m0 * a.ldd + n0, a.ldd, count - m0, cols - n0, [&](int i, int j) { return t.acc[i][j]; });
+  mm_nt_store(t, tile, a.d + (long)m0 * a.ldd + n0, a.ldd, count - m0, cols - n0,
+              [&](int i, int j) { return t.acc[i][j]; });
   mm_nt_store_transposed(t, tile, a.dT + (long)n0 * a.ldt + m0, a.ldt, rows - m0, a.n - n0,
                          [&](int i, int j) { return t.acc[i][j] * share[j]; });
 }
@@ -844,24 +895,30 @@ struct Tiles {
   }
 };
 
-template <typename T, int ROWS, int TH>
-bool launch_few(const MMCeFew& a, int wg, size_t lds, hipStream_t stream) {
-  if (!lds_granted<mm_ce_few_kernel<T, ROWS, TH>>((int)lds)) return false;
-  hipLaunchKernelGGL((mm_ce_few_kernel<T, ROWS, TH>), dim3(wg), dim3(TH), lds, stream, a);
+template <typename T, int ROWS, int TH, bool D>
+bool launch_few(const MMCeFew& a, const MMCeFewD<T>& b, int wg, hipStream_t stream) {
+  const size_t lds = (size_t)a.T * mm_up(a.D, 64 * MMVec<T>::N) * sizeof(float);
+  if (!lds_granted<mm_ce_few_kernel<T, ROWS, TH, D>>((int)lds)) return false;
+  hipLaunchKernelGGL((mm_ce_few_kernel<T, ROWS, TH, D>), dim3(wg), dim3(TH), lds, stream, a, b);
   return true;
+}
+
+template <typename T, bool D>
+bool few(const MMCeFew& a, const MMCeFewD<T>& b, int wg, hipStream_t stream) {
+  if (!D && wg == 1)
+    return a.T == 1 ? launch_few<T, 1, 1024, false>(a, b, 1, stream)
+                    : launch_few<T, MM_CE_FEW, 1024, false>(a, b, 1, stream);
+  return a.T == 1 ? launch_few<T, 1, 512, D>(a, b, wg, stream) : launch_few<T, MM_CE_FEW, 512, D>(a, b, wg, stream);
 }
 
 template <typename T>
 int forward_few(const Sizes& s, const MMCeFew& a, float* sums, hipStream_t stream) {
-  const int wg = few_workgroups(s), N = MMVec<T>::N;
-  const size_t lds = (size_t)s.T * mm_up(s.D, 64 * N) * sizeof(float);
-  bool ok;
-  if (wg == 1) ok = s.T == 1 ? launch_few<T, 1, 1024>(a, wg, lds, stream) : launch_few<T, MM_CE_FEW, 1024>(a, wg, lds, stream);
-  else ok = s.T == 1 ? launch_few<T, 1, 512>(a, wg, lds, stream) : launch_few<T, MM_CE_FEW, 512>(a, wg, lds, stream);
+  const int wg = few_workgroups(s);
+  const bool ok = few<T, false>(a, MMCeFewD<T>{}, wg, stream);
   if (!ok) return MM_ELAUNCH;
   if (wg > 1) {
     hipLaunchKernelGGL(mm_ce_rows_kernel, dim3(1), dim3(1024), 0, stream, a.part, s.T, wg, a.count, a.list, a.y,
-                       a.picked, a.lse, a.reduction == 0 ? a.loss : nullptr, a.reduction ? sums : nullptr);
+                       a.picked, a.stats, a.reduction == 0 ? a.loss : nullptr, a.reduction ? sums : nullptr);
     if (a.reduction)
       hipLaunchKernelGGL(mm_ce_total_kernel, dim3(1), dim3(1024), 0, stream, sums, a.count, a.reduction == MM_CE_MEAN,
                          a.loss);
@@ -870,7 +927,7 @@ int forward_few(const Sizes& s, const MMCeFew& a, float* sums, hipStream_t strea
 }
 
 template <typename T>
-int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, float* loss, float* lse,
+int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, float* loss, float* stats,
             const Forward& f, hipStream_t stream) {
   typedef typename MMCeType<T>::H H;
   if (s.T) {
@@ -891,7 +948,7 @@ int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int
     const int side = side_of(s.T, s.V, MMCeType<T>::P), tiles_n = (int)div_up(s.V, side);
     if (!Tiles<T>::template logits<false>(a, s.T, s.V, side, stream)) return MM_ELAUNCH;
     hipLaunchKernelGGL(mm_ce_rows_kernel, dim3((unsigned)div_up(s.T, 32)), dim3(1024), 0, stream, f.part, s.T, tiles_n,
-                       r.count, r.list, r.y, f.picked, lse, reduction == 0 ? loss : nullptr,
+                       r.count, r.list, r.y, f.picked, stats, reduction == 0 ? loss : nullptr,
                        reduction ? f.sums : nullptr);
   }
   if (reduction)
@@ -913,20 +970,22 @@ void join(const float* part, int splits, long part_rows, long rows, int N, const
 }
 
 template <typename T>
-int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, const float* lse,
+int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, const float* stats,
              const float* dloss, T* dx, T* dw, const Backward& b, hipStream_t stream) {
   typedef typename MMCeType<T>::H H;
   const float scale = s.dtype == MM_F16 ? HALF_SCALE : 1.f;
   const MMCeScale by{reduction ? nullptr : b.g, b.gmax, dloss, reduction == MM_CE_MEAN};
   if (!reduction)
     hipLaunchKernelGGL(mm_ce_grad_kernel, dim3(1), dim3(1024), 0, stream, dloss, r.count, r.list, b.g, b.gmax);
+  const bool few_d = few_rows(s);
   const bool direct = s.pieces == 1 && s.dx_splits == 1;   // dx without sums in memory
   for (long p = 0; p < s.pieces; ++p) {
     const long v0 = p * s.piece, n = s.V - v0 < s.piece ? s.V - v0 : s.piece, np = mm_up(n, MM_NT_K);
     MMPack px{x, r.list, r.count, b.x, b.xT, ldx, 0, s.Dp, s.Tp, s.T * s.Dp, s.D * s.Tp, (int)s.T, (int)s.D};
     if (p) px.out = px.outT = nullptr;   // once
-    const MMPack pw{w, nullptr, nullptr, b.w, b.wT, s.D, v0, s.Dp, s.piece_p, s.piece * s.Dp, s.D * s.piece_p, (int)n,
+    MMPack pw{w, nullptr, nullptr, b.w, b.wT, s.D, v0, s.Dp, s.piece_p, s.piece * s.Dp, s.D * s.piece_p, (int)n,
                     (int)s.D};
+    if (few_d) px.out = pw.out = nullptr;
     pack<T>(px, pw, MMZero{r.pos, direct ? dx : nullptr, s.T, (int)s.D}, stream);
     MMCeLogits<H> a{};
     a.x = MMNtOperand<H>{(const H*)b.x, s.Dp, s.T * s.Dp, 0};
@@ -936,7 +995,7 @@ int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, in
     a.y = r.y;
     a.K = (int)(s.Dp / MM_NT_K);
     a.T = s.T;
-    a.lse = lse;
+    a.stats = stats;
     a.by = by;
     a.d = (H*)b.d;
     a.dT = (H*)b.dT;
@@ -950,7 +1009,15 @@ int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, in
     // d in three planes, twice: its stores need another workgroup's products beside them (8598 rows, 59,192 classes: 2.9
     // ms against 3.5 with tiles of 256)
     const int side = side_of(s.T, n, MMCeType<T>::P);
-    bool ok = Tiles<T>::template logits<true>(a, s.T, n, MMCeType<T>::P > 1 && side > 128 ? 128 : side, stream);
+    bool ok;
+    if (few_d) {
+      const MMCeFew e{x, w + v0 * s.D, nullptr, ldx, 0, (int)s.T, (int)s.D, (int)n, 0, 0, r.count, r.list, r.y, r.pos,
+                      nullptr, nullptr, (float*)stats, nullptr};
+      const MMCeFewD<T> f{a.d, a.dT, a.ldd, a.plane, a.planeT, (int)v0, scale, by};
+      ok = few<T, true>(e, f, (int)clamp(div_up(np, 8 * MM_CE_CLASSES), 1, 512), stream);
+    } else {
+      ok = Tiles<T>::template logits<true>(a, s.T, n, MMCeType<T>::P > 1 && side > 128 ? 128 : side, stream);
+    }
     MMCeProduct<H> q{}, u{};
     if (dx) {
       q.a = MMNtOperand<H>{(const H*)b.d, s.piece_p, s.T * s.piece_p, 0};
@@ -1015,18 +1082,18 @@ extern "C" int mm_ce_workspace(long T, long D, long V, int dtype, const void* w,
 }
 
 extern "C" int mm_ce_fwd(const void* x, long ldx, int dtype, long T, long D, const void* w, long V, const void* targets,
-                         int targets64, long ignore, int reduction, float* loss, float* lse, int* rows, void* workspace,
+                         int targets64, long ignore, int reduction, float* loss, float* stats, int* rows, void* workspace,
                          hipStream_t stream) {
   MM_CE_CHECK("mm_ce_fwd");
   MM_CHECK_ARG(ldx >= 0 && reduction >= 0 && reduction <= 2, "bad reduction");
-  MM_CHECK_ARG(loss && rows && (T == 0 || (x && w && targets && lse && workspace)), "null pointer");
+  MM_CHECK_ARG(loss && rows && (T == 0 || (x && w && targets && stats && workspace)), "null pointer");
   Forward f;
   forward_space(s, (char*)workspace, &f);
   const Rows r = rows_of(rows, T);
   int rc = MM_OK;
   if (few_rows(s)) {
     const MMCeFew a{x, w, targets, ldx, ignore, (int)T, (int)D, (int)V, targets64, reduction, r.count, r.list, r.y, r.pos,
-                    f.part, f.picked, lse, loss};
+                    f.part, f.picked, stats, loss};
     MM_DISPATCH(dtype, rc = forward_few<T_>(s, a, f.sums, stream));
     return rc;
   }
@@ -1041,22 +1108,22 @@ extern "C" int mm_ce_fwd(const void* x, long ldx, int dtype, long T, long D, con
   };
   if (targets64) scan((const long*)targets);
   else scan((const int*)targets);
-  MM_DISPATCH(dtype, rc = forward<T_>(s, (const T_*)x, ldx, (const T_*)w, r, reduction, loss, lse, f, stream));
+  MM_DISPATCH(dtype, rc = forward<T_>(s, (const T_*)x, ldx, (const T_*)w, r, reduction, loss, stats, f, stream));
   return rc;
 }
 
 extern "C" int mm_ce_bwd(const void* x, long ldx, int dtype, long T, long D, const void* w, long V, int reduction,
-                         const float* lse, const int* rows, const float* dloss, void* dx, void* dw, void* workspace,
+                         const float* stats, const int* rows, const float* dloss, void* dx, void* dw, void* workspace,
                          hipStream_t stream) {
   MM_CE_CHECK("mm_ce_bwd");
   MM_CHECK_ARG(ldx >= 0 && reduction >= 0 && reduction <= 2, "bad reduction");
-  MM_CHECK_ARG(T > 0 && x && w && lse && rows && dloss && workspace, "null pointer");
+  MM_CHECK_ARG(T > 0 && x && w && stats && rows && dloss && workspace, "null pointer");
   if (!dx && !dw) return MM_OK;
   Backward b;
   backward_space(s, dx, dw, (char*)workspace, &b);
   const Rows r = rows_of((int*)rows, T);
   int rc = MM_OK;
-  MM_DISPATCH(dtype, rc = backward<T_>(s, (const T_*)x, ldx, (const T_*)w, r, reduction, lse, dloss, (T_*)dx, (T_*)dw, b,
+  MM_DISPATCH(dtype, rc = backward<T_>(s, (const T_*)x, ldx, (const T_*)w, r, reduction, stats, dloss, (T_*)dx, (T_*)dw, b,
                                        stream));
   return rc;
 }

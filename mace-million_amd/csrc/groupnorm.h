@@ -1,5 +1,6 @@
-// Group norm of rows of channels with an activation: what forward (groupnorm.hip) and backward (groupnorm_bwd.hip) share.  A structure is a run of rows, a group a run
-// of cg = C / groups channels; over the n = rows x cg values of a (structure, group):
+// Group norm of rows of channels with an activation: what forward (groupnorm.hip) and backward (groupnorm_bwd.hip)
+// share.  A structure is a run of rows, a group a run of cg = C / groups channels; over the n = rows x cg values of a
+// (structure, group):
 //     h = (x - mean) rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps),  z = h w + b,  y = act(z)
 //     dz = dy act'(z):  dw = sum_rows dz h,  db = sum_rows dz,  dx = rstd (dz w - mean(dz w) - h mean(dz w h))
 // Bound by HBM.  A thread keeps one vector of 16 bytes of channels for several rows, and sums go by channel first (over
@@ -372,7 +373,7 @@ struct Plan {
 };
 
 // Threads of a workgroup and values a thread.  Small structures by one wave: sums without barriers, and four times as
-// many of them at once (4096 structures of 22 rows of 128 channels, forward 64 -> 20 us).  1024 threads hold large ones.
+// many of them at once (4096 structures of 5 to 39 rows of 128 float values, forward 64 -> 36 us).  1024 threads hold large ones.
 struct Shape { int tpb, vals; };
 constexpr Shape kShapes[] = {{64, 64}, {256, 32}, {1024, 32}};
 
@@ -440,7 +441,8 @@ bool make_plan(const char* name, long rows, int structs, const int* offsets, int
 template <bool FWD>
 void join_tiles(const MMGroup& a, const float* part, float eps, float* out, hipStream_t stream) {
   if (a.structs < 256) {
-    hipLaunchKernelGGL((mm_groupnorm_join_kernel<FWD, 16>), dim3(a.structs, a.G), dim3(1024), 0, stream, a, part, eps, out);
+    hipLaunchKernelGGL((mm_groupnorm_join_kernel<FWD, 16>), dim3(a.structs, a.G), dim3(1024), 0, stream, a, part, eps,
+                       out);
   } else {
     const int n = a.structs / 4 + 1;
     hipLaunchKernelGGL((mm_groupnorm_join_kernel<FWD, 1>), dim3(n < 4096 ? n : 4096), dim3(256), 0, stream, a, part, eps,

@@ -126,7 +126,8 @@ extern "C" int mm_groupnorm_fwd(const void* x, long ldx, int dtype, long rows, i
       MM_GROUP_SHAPES(p.tile_tpb, mm_groupnorm_tile_stats_kernel, T_);
     });
     join_tiles<true>(p.a, workspace, eps, stats, stream);
-    MM_GROUP_DISPATCH(MM_GROUP_SHAPES, p.tile_tpb, mm_groupnorm_tile_fwd_kernel, grid, 0, p.a, (const T_*)x, ldx, w, b, p_dtype == MM_F32, (T_*)y,
+    MM_GROUP_DISPATCH(MM_GROUP_SHAPES, p.tile_tpb, mm_groupnorm_tile_fwd_kernel, grid, 0, p.a, (const T_*)x, ldx, w, b,
+                      p_dtype == MM_F32, (T_*)y,
                       ldy, p.n_tiles, stats);
   }
   return mm::launch_status("mm_groupnorm_fwd");

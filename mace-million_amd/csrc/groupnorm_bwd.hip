@@ -206,12 +206,14 @@ extern "C" int mm_groupnorm_bwd(const void* dy, long lddy, const void* x, long l
   if (part_rows && (dx || wpart)) {
     if (p.whole) {
       MM_GROUP_DISPATCH(MM_GROUP_WAVES, p.tpb, mm_groupnorm_whole_bwd_kernel, dim3(p.wg_whole, p.blocks), p.lds, p.a,
-                        (const T_*)dy, lddy, (const T_*)x, ldx, w, b, p_dtype == MM_F32, stats, (T_*)dx, lddx, wpart, part_rows);
+                        (const T_*)dy, lddy, (const T_*)x, ldx, w, b, p_dtype == MM_F32, stats, (T_*)dx, lddx, wpart,
+                         part_rows);
     }
     if (p.tiles) {
       const dim3 grid(p.wg_tiles, p.blocks);
       MM_GROUP_DISPATCH(MM_GROUP_SHAPES, p.tile_tpb, mm_groupnorm_tile_sums_kernel, grid, p.lds, p.a, (const T_*)dy, lddy,
-                        (const T_*)x, ldx, w, b, p_dtype == MM_F32, stats, p.n_tiles, dx ? part : nullptr, wpart, (long)p.wg_whole, part_rows);
+                        (const T_*)x, ldx, w, b, p_dtype == MM_F32, stats, p.n_tiles, dx ? part : nullptr, wpart,
+                        (long)p.wg_whole, part_rows);
       if (dx) {
         join_tiles<false>(p.a, part, 0.f, sums, stream);
         MM_GROUP_DISPATCH(MM_GROUP_SHAPES, p.tile_tpb, mm_groupnorm_tile_bwd_kernel, grid, 0, p.a, (const T_*)dy, lddy,

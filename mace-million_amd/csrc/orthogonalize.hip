@@ -39,7 +39,8 @@ __device__ __forceinline__ void mm_ortho_put4(_Float16* __restrict__ p, long pla
 
 // sums of squares of parts of matrix blockIdx.y
 template <typename T>
-__global__ void __launch_bounds__(256) mm_ortho_norm_kernel(const T* __restrict__ m, long size, double* __restrict__ part) {
+__global__ void __launch_bounds__(256)
+mm_ortho_norm_kernel(const T* __restrict__ m, long size, double* __restrict__ part) {
   constexpr int N = MMVec<T>::N;
   __shared__ double s[4];
   const T* __restrict__ p = m + (long)blockIdx.y * size;
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(64 * WAVES) mm_ortho_small_kernel(MMOrthoSmall
   // (89 of 201 x 137: 305 -> 137 us).
   constexpr bool GUARD = NT == 13 && PLANES == 2;
   const int mt = GUARD ? (a.side + 15) / 16 : MT, ms = GUARD ? (a.side + 31) / 32 : MS;
-  const int plane = ms * 32 * UNITS;   // units of a plane
+  constexpr int plane = MS * 32 * UNITS;   // units of a plane
   const bool work = !GUARD || wave * RT < mt;
   const bool wide = a.rows <= a.cols;
   auto row = [&](int t) { return 16 * (wave * RT + t) + i16; };
@@ -426,7 +427,8 @@ __global__ void __launch_bounds__(64 * WAVES) mm_ortho_small_kernel(MMOrthoSmall
     for (int q = 0; q < P; ++q)
 #pragma unroll
       for (int t = 0; t < RT; ++t)
-        c[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[mm_nt_first<P>(q)], v[t][mm_nt_second<P>(q)], c[t][i], 0, 0, 0);
+        c[t][i] =
+            __builtin_amdgcn_mfma_f32_16x16x32_f16(u[mm_nt_first<P>(q)], v[t][mm_nt_second<P>(q)], c[t][i], 0, 0, 0);
   };
 
   auto put_all = [&](const auto& v) {
@@ -462,7 +464,8 @@ __global__ void __launch_bounds__(64 * WAVES) mm_ortho_small_kernel(MMOrthoSmall
         for (int i = 0; i < AHEAD; ++i) read_rows(u[i], 16 * i, s);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          if (i + AHEAD < MT && (!GUARD || i + AHEAD < mt)) read_rows(u[(i + AHEAD) % (AHEAD + 1)], 16 * (i + AHEAD), s);
+          if (i + AHEAD < MT && (!GUARD || i + AHEAD < mt))
+            read_rows(u[(i + AHEAD) % (AHEAD + 1)], 16 * (i + AHEAD), s);
           __builtin_amdgcn_sched_barrier(0);
           if (!GUARD || i < mt) mma(acc, i, u[i % (AHEAD + 1)], v);
           __builtin_amdgcn_sched_barrier(0);
@@ -702,12 +705,10 @@ int check(const char* name, long batch, long rows, long cols, int dtype) {
   }
   return MM_OK;
 }
-}  // namespace
 
-namespace {
 // Matrices taken at once.  Up to 240 MB of workspace, so that their planes stay in the last cache (256 MB) between the
-// products, and a number whose tiles fill their rounds (64 bfloat16 matrices of 1024 x 1024: 64 at once 2900 us, 16 2800,
-// 14 2700).
+// products, and a number whose tiles fill their rounds (64 bfloat16 matrices of 1024 x 1024: 64 at once 2900 us, 16 2910,
+// 14 2540).
 int part_of(MMOrtho a, long batch, int dtype) {
   a.batch = 1;
   const long fits = 251658240L / (long)space(&a, dtype, nullptr), most = fits < 1 ? 1 : fits < batch ? fits : batch;

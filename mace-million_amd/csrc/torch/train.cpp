@@ -132,14 +132,14 @@ Tensor bytes_like(size_t n, const Tensor& like) { return at::empty({(int64_t)n},
 struct LossSizes { long T, D, V; };
 
 struct CrossEntropyFn : torch::autograd::Function<CrossEntropyFn> {
-  struct Result { Tensor loss, lse, rows; };
+  struct Result { Tensor loss, stats, rows; };
 
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& targets,
                         int64_t ignore, int64_t reduction, int64_t code) {
     auto [x2, ldx] = as_rows(x);
     const Tensor w = weight.contiguous();
     Result r = run(x2, ldx, w, targets, ignore, (int)reduction, (int)code);
-    ctx->save_for_backward({x2, w, r.lse, r.rows});
+    ctx->save_for_backward({x2, w, r.stats, r.rows});
     ctx->saved_data["args"] = std::vector<int64_t>{reduction, code, x2.size(0), x2.size(1), w.size(0)};
     ctx->saved_data["shape"] = x.sizes().vec();
     return r.loss;
@@ -149,13 +149,13 @@ struct CrossEntropyFn : torch::autograd::Function<CrossEntropyFn> {
                     int code) {
     const LossSizes n{x2.size(0), x2.size(1), w.size(0)};
     const Tensor y = targets.contiguous();
-    Result r{reduction ? f32({}, x2) : f32(targets.sizes(), x2), f32({n.T}, x2), i32({4 + 3 * n.T}, x2)};
+    Result r{reduction ? f32({}, x2) : f32(targets.sizes(), x2), f32({2, n.T}, x2), i32({4 + 3 * n.T}, x2)};
     size_t bytes = 0;
     done(mm_ce_workspace(n.T, n.D, n.V, code, ptr(w), 0, 0, &bytes));
     const Tensor ws = bytes_like(bytes, x2);
     if (n.T || reduction)
       done(mm_ce_fwd(ptr(x2), ldx, code, n.T, n.D, ptr(w), n.V, ptr(y), y.scalar_type() == at::kLong, ignore, reduction,
-                     fptr(r.loss), fptr(r.lse), iptr(r.rows), ptr(ws), stream()));
+                     fptr(r.loss), fptr(r.stats), iptr(r.rows), ptr(ws), stream()));
     return r;
   }
 
@@ -168,7 +168,7 @@ struct CrossEntropyFn : torch::autograd::Function<CrossEntropyFn> {
     const auto type = type_of(code);
     auto [x, ldx] = as_rows(unpacked(saved[0], {n.T, n.D}, type, dloss, "x"));
     const Tensor w = unpacked_dense(saved[1], {n.V, n.D}, type, dloss, "weight");
-    const Tensor lse = unpacked_dense(saved[2], {n.T}, at::kFloat, dloss, "log sums");
+    const Tensor stats = unpacked_dense(saved[2], {2, n.T}, at::kFloat, dloss, "statistics");
     const Tensor rows = unpacked_dense(saved[3], {4 + 3 * n.T}, at::kInt, dloss, "rows");
     Tensor dx, dw;
     if (ctx->needs_input_grad(0)) dx = at::empty(ctx->saved_data["shape"].toIntVector(), x.options());
@@ -177,7 +177,7 @@ struct CrossEntropyFn : torch::autograd::Function<CrossEntropyFn> {
       size_t bytes = 0;
       done(mm_ce_workspace(n.T, n.D, n.V, code, ptr(w), dx.defined(), dw.defined(), &bytes));
       const Tensor ws = bytes_like(bytes, x);
-      done(mm_ce_bwd(ptr(x), ldx, code, n.T, n.D, ptr(w), n.V, reduction, fptr(lse), iptr(rows), fptr(dloss), ptr(dx),
+      done(mm_ce_bwd(ptr(x), ldx, code, n.T, n.D, ptr(w), n.V, reduction, fptr(stats), iptr(rows), fptr(dloss), ptr(dx),
                      ptr(dw), ptr(ws), stream()));
     }
     variable_list out(6);

@@ -261,3 +261,32 @@ def test_refusals():
     (dx,) = torch.autograd.grad(f(xg, w, y), xg, create_graph=True)
     with pytest.raises(RuntimeError, match="once only"):
         dx.sum().backward()
+
+
+@pytest.mark.parametrize("T,V", [(1, 50), (5, 700), (16, 33), (17, 50), (130, 700), (600, 5000)])
+def test_probabilities_sum_to_one(T, V):
+    """sum_v dW[v] = g x sum_v d, and d of a row sums to 0 whatever the logits' roundings, if both directions take the
+    same logits: here near 2000, where a rounded log of the sum alone would be off by up to 2^-14.  One asked row, as
+    sums over rows have no roundings then.  E[depth] <= log V; sum |d| <= 2."""
+    from mace_onegpu.cross_entropy import linear_cross_entropy
+    g = torch.Generator().manual_seed(T + V)
+    base = torch.randn(33, generator=g)
+    w = base + 0.02 * torch.randn(V, 33, generator=g)
+    x = (2000 / base.square().sum() * base).expand(T, 33).contiguous()
+    y = torch.full((T,), -100)
+    y[T // 2] = V // 3
+    wg = w.cuda().requires_grad_()
+    loss = linear_cross_entropy(x.cuda(), wg, y.cuda(), reduction="sum")
+    dw, = torch.autograd.grad(loss, wg)
+    bound = U * x[0].double().abs() * (16 + 2 * torch.tensor(float(V)).log() + 64 + V / 64 + 2 * (6 + 16))
+    assert float(dw.abs().max()) > 0.01
+    assert bool((dw.double().sum(0).cpu().abs() <= bound).all()), float((dw.double().sum(0).cpu().abs() / bound).max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,D,V", [(1, 16, 8), (16, 1000, 3), (9, 77, 3000), (3, 5000, 65), (16, 40, 70001)])
+def test_few_rows_with_gradients(T, D, V, dtype):
+    x, w, y, dloss = _inputs(T, D, V, dtype, T + D + V)
+    for reduction in ("mean", "none"):
+        ref, bound = _reference(x.cuda(), w.cuda(), y.cuda(), dloss.cuda(), reduction, dtype)
+        _check(_run(x, w, y, dloss, reduction), ref, bound)
