@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
                                     : (long)((const int*)a.targets)[lane];
 #pragma unroll
   for (int t = 0; t < ROWS; ++t) {
-    if (t >= rows) break;
+    if (t >= rows) continue;
     const long at = D ? a.list[t] : t;
     for (int c = threadIdx.x; c < Dp; c += TH)
       mm_ce_x[t * Dp + c] = c < a.D ? (float)((const T*)a.x)[at * a.ldx + c] : 0.f;
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
       for (int k = 0; k < C; ++k) mm_load_vec(p[k], c, end, w[k]);
 #pragma unroll
       for (int t = 0; t < ROWS; ++t) {
-        if (ROWS > 1 && t >= rows) break;
+        if (ROWS > 1 && t >= rows) continue;   // not break, which would put acc into memory
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
           const floatx4 x = *(const floatx4*)(mm_ce_x + t * Dp + c + i);
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
     float mine[C] = {};
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) {
-      if (ROWS > 1 && t >= rows) break;
+      if (ROWS > 1 && t >= rows) continue;
 #pragma unroll
       for (int k = 0; k < C; ++k) {
         const float l = mm_lanes_sum<64>(acc[t][k]);
@@ -789,10 +789,18 @@ bool sizes_of(const char* name, long T, long D, long V, int dtype, const void* w
   return true;
 }
 
-// Few rows of a head: vectors of W without the matrix cores.
+// Few rows of a head: vectors of W without the matrix cores, where that takes less time.  Its adds and the sums over the
+// lanes take 0.09 + 0.00015 D ns a row and class where they exceed the reading of W (bfloat16, 16 rows, 100,003 classes of
+// 512 and 1024 values: 238 and 330 us; float, 10 rows, 50,000 of 1024: 122); tiles take four launches more, read W once if
+// it is an operand as it is (17 rows, 100,003 classes of 1024 values: 65 us in all), and three times its size if not
+// (float: packed and read in 16 bytes a value).
 bool few_rows(const Sizes& s) {
   const long Dp = mm_up(s.D, s.dtype == MM_F32 ? 256 : 512);
-  return s.T > 0 && s.T <= MM_CE_FEW && s.T * Dp <= MM_CE_FEW_LDS;
+  if (s.T == 0 || s.T > MM_CE_FEW || s.T * Dp > MM_CE_FEW_LDS) return false;
+  const double W = (double)s.V * s.D * (s.dtype == MM_F32 ? 4. : 2.);
+  const double few = (double)s.T * s.V * (0.09 + 0.00015 * s.D), reading = W / 4000.;   // ns
+  const double tiles = W * (s.dtype == MM_F32 ? 4. : s.D % MM_NT_K ? 3. : 1.) / 4200. + 25000.;
+  return (few > reading ? few : reading) <= tiles;
 }
 // one workgroup where W has up to 128 KB
 int few_workgroups(const Sizes& s) {
@@ -903,18 +911,18 @@ bool launch_few(const MMCeFew& a, const MMCeFewD<T>& b, int wg, hipStream_t stre
   return true;
 }
 
-template <typename T, bool D>
+template <typename T, int TH, bool D>
 bool few(const MMCeFew& a, const MMCeFewD<T>& b, int wg, hipStream_t stream) {
-  if (!D && wg == 1)
-    return a.T == 1 ? launch_few<T, 1, 1024, false>(a, b, 1, stream)
-                    : launch_few<T, MM_CE_FEW, 1024, false>(a, b, 1, stream);
-  return a.T == 1 ? launch_few<T, 1, 512, D>(a, b, wg, stream) : launch_few<T, MM_CE_FEW, 512, D>(a, b, wg, stream);
+  return a.T == 1   ? launch_few<T, 1, TH, D>(a, b, wg, stream)
+         : a.T <= 4 ? launch_few<T, 4, TH, D>(a, b, wg, stream)
+                    : launch_few<T, MM_CE_FEW, TH, D>(a, b, wg, stream);
 }
 
 template <typename T>
 int forward_few(const Sizes& s, const MMCeFew& a, float* sums, hipStream_t stream) {
   const int wg = few_workgroups(s);
-  const bool ok = few<T, false>(a, MMCeFewD<T>{}, wg, stream);
+  const MMCeFewD<T> none{};
+  const bool ok = wg == 1 ? few<T, 1024, false>(a, none, 1, stream) : few<T, 512, false>(a, none, wg, stream);
   if (!ok) return MM_ELAUNCH;
   if (wg > 1) {
     hipLaunchKernelGGL(mm_ce_rows_kernel, dim3(1), dim3(1024), 0, stream, a.part, s.T, wg, a.count, a.list, a.y,
@@ -1014,7 +1022,7 @@ int backward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, in
       const MMCeFew e{x, w + v0 * s.D, nullptr, ldx, 0, (int)s.T, (int)s.D, (int)n, 0, 0, r.count, r.list, r.y, r.pos,
                       nullptr, nullptr, (float*)stats, nullptr};
       const MMCeFewD<T> f{a.d, a.dT, a.ldd, a.plane, a.planeT, (int)v0, scale, by};
-      ok = few<T, true>(e, f, (int)clamp(div_up(np, 8 * MM_CE_CLASSES), 1, 512), stream);
+      ok = few<T, 512, true>(e, f, (int)clamp(div_up(np, 8 * MM_CE_CLASSES), 1, 512), stream);
     } else {
       ok = Tiles<T>::template logits<true>(a, s.T, n, MMCeType<T>::P > 1 && side > 128 ? 128 : side, stream);
     }
