@@ -255,6 +255,7 @@ struct MMCeLogits {
   float scale;
 };
 
+// 8192 rows, 131,072 classes of 2048 bfloat16 values: 4.24 ms, 1040 TFLOP/s; the matrix cores are busy 0.56 of it.
 template <typename T, typename Nt>
 __global__ void __launch_bounds__(Nt::TH, Nt::PER_CU)
 mm_ce_logits_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
@@ -351,11 +352,39 @@ mm_ce_rows_kernel(const float* __restrict__ part, long T, int tiles_n, const int
   sums[blockIdx.x] = t;
 }
 
-// sum (mean) of the blocks' sums
+// The same for few rows of many tiles: a row a workgroup, sums [rows] (16 rows, 1563 tiles: 20 -> 6 us).
+__global__ void __launch_bounds__(256)
+mm_ce_row_kernel(const float* __restrict__ part, long T, int tiles_n, const int* __restrict__ count,
+                 const int* __restrict__ list, const int* __restrict__ y, const float* __restrict__ picked,
+                 float* __restrict__ stats, float* __restrict__ loss, float* __restrict__ sums) {
+  __shared__ MMCeRow s[4];
+  const int i = blockIdx.x;
+  if (i >= *count) return;
+  MMCeRow r{-INFINITY, 0.f};
+#pragma unroll 4
+  for (int t = threadIdx.x; t < tiles_n; t += 256) {
+    const float2 p = *(const float2*)(part + ((long)t * T + i) * 2);
+    r = mm_ce_join(r, MMCeRow{p.x, p.y});
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) r = mm_ce_join(r, MMCeRow{__shfl_xor(r.top, d), __shfl_xor(r.sum, d)});
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = r;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < 4; ++w) r = mm_ce_join(r, s[w]);
+  stats[i] = r.top;
+  stats[T + i] = r.sum;
+  const float l = y[i] < 0 ? __builtin_nanf("") : r.top - picked[i] + logf(r.sum);
+  if (loss) loss[list[i]] = l;
+  if (sums) sums[i] = l;
+}
+
+// sum (mean) of the sums of `each` rows
 __global__ void __launch_bounds__(1024)
-mm_ce_total_kernel(const float* __restrict__ sums, const int* __restrict__ count, int mean, float* __restrict__ loss) {
+mm_ce_total_kernel(const float* __restrict__ sums, const int* __restrict__ count, int each, int mean,
+                   float* __restrict__ loss) {
   __shared__ double s[16];
-  const int n = *count, blocks = (n + 31) / 32;
+  const int n = *count, blocks = (n + each - 1) / each;
   double t = 0.;
   for (int i = threadIdx.x; i < blocks; i += 1024) t += (double)sums[i];
 #pragma unroll
@@ -549,6 +578,7 @@ __global__ void __launch_bounds__(1024) mm_ce_grad_kernel(const float* __restric
   *gmax = top;
 }
 
+// The same product, with 32 bits of d and its transpose to store: 291 us for 8192 classes of it, 945 TFLOP/s.
 template <typename T, typename Nt>
 __global__ void __launch_bounds__(Nt::TH, Nt::PER_CU)
 mm_ce_d_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
@@ -628,7 +658,8 @@ struct MMCeProduct {
   float inv;
 };
 
-// both in one launch, as neither fills the card by itself where rows and classes are few
+// both in one launch, as neither fills the card by itself where rows and classes are few (8192 rows and classes, 2048
+// bfloat16 values: 490 us, 1120 TFLOP/s)
 template <typename T, typename Nt>
 __global__ void __launch_bounds__(Nt::TH, Nt::PER_CU)
 mm_ce_product_kernel(MMCeProduct<typename MMCeType<T>::H> one, MMCeProduct<typename MMCeType<T>::H> two) {
@@ -789,11 +820,11 @@ bool sizes_of(const char* name, long T, long D, long V, int dtype, const void* w
   return true;
 }
 
-// Few rows of a head: vectors of W without the matrix cores, where that takes less time.  Its adds and the sums over the
-// lanes take 0.09 + 0.00015 D ns a row and class where they exceed the reading of W (bfloat16, 16 rows, 100,003 classes of
-// 512 and 1024 values: 238 and 330 us; float, 10 rows, 50,000 of 1024: 122); tiles take four launches more, read W once if
-// it is an operand as it is (17 rows, 100,003 classes of 1024 values: 65 us in all), and three times its size if not
-// (float: packed and read in 16 bytes a value).
+// Few rows of a head: vectors of W without the matrix cores, where that takes less time.  Its adds and the sums over
+// the lanes take 0.09 + 0.00015 D ns a row and class where they exceed the reading of W (bfloat16, 16 rows, 100,003
+// classes of 512 and 1024 values: 238 and 330 us; float, 10 rows, 50,000 of 1024: 122); tiles take four launches more,
+// read W once if it is an operand as it is (17 rows, 100,003 classes of 1024 values: 51 us in all), and three times its
+// size if not (float: packed and read in 16 bytes a value).
 bool few_rows(const Sizes& s) {
   const long Dp = mm_up(s.D, s.dtype == MM_F32 ? 256 : 512);
   if (s.T == 0 || s.T > MM_CE_FEW || s.T * Dp > MM_CE_FEW_LDS) return false;
@@ -808,6 +839,10 @@ int few_workgroups(const Sizes& s) {
   return (int)clamp(div_up(s.V, 8 * MM_CE_CLASSES), 2, 512);
 }
 
+// few rows of many tiles: a workgroup each
+#define MM_CE_ROW 256
+bool row_each(const Sizes& s, int tiles_n) { return s.T < MM_CE_ROW && tiles_n >= 64; }
+
 struct Forward {
   void *x, *w;
   float *part, *picked, *sums;
@@ -818,14 +853,14 @@ size_t forward_space(const Sizes& s, char* base, Forward* f) {
   if (few_rows(s)) {
     f->part = p.take<float>((size_t)few_workgroups(s) * s.T * 2);
     f->picked = p.take<float>(s.T);
-    f->sums = p.take<float>(1);
+    f->sums = p.take<float>(s.T);
     return p.used;
   }
   f->x = p.take<short>((size_t)s.planes * s.T * s.Dp);
   f->w = s.w_in_place ? nullptr : p.take<short>((size_t)s.planes * s.V * s.Dp);
   f->part = p.take<float>((size_t)div_up(s.V, BN) * s.T * 2);
   f->picked = p.take<float>(s.T);
-  f->sums = p.take<float>(div_up(s.T, 32));
+  f->sums = p.take<float>(s.T < MM_CE_ROW ? s.T : div_up(s.T, 32));
   f->counts = p.take<int>(div_up(s.T, 1024 * MM_CE_SCAN));
   return p.used;
 }
@@ -903,6 +938,25 @@ struct Tiles {
   }
 };
 
+// rows' statistics and losses from the tiles' (T > 0), then their sum or mean
+void finish(const Sizes& s, const Forward& f, int tiles_n, const Rows& r, int reduction, float* stats, float* loss,
+            hipStream_t stream) {
+  const bool one = row_each(s, tiles_n);
+  if (s.T) {
+    const dim3 grid((unsigned)(one ? s.T : div_up(s.T, 32)));
+    float *each = reduction == 0 ? loss : nullptr, *sums = reduction ? f.sums : nullptr;
+    if (one)
+      hipLaunchKernelGGL(mm_ce_row_kernel, grid, dim3(256), 0, stream, f.part, s.T, tiles_n, r.count, r.list, r.y, f.picked,
+                         stats, each, sums);
+    else
+      hipLaunchKernelGGL(mm_ce_rows_kernel, grid, dim3(1024), 0, stream, f.part, s.T, tiles_n, r.count, r.list, r.y,
+                         f.picked, stats, each, sums);
+  }
+  if (reduction)
+    hipLaunchKernelGGL(mm_ce_total_kernel, dim3(1), dim3(1024), 0, stream, f.sums, r.count, one ? 1 : 32,
+                       reduction == MM_CE_MEAN, loss);
+}
+
 template <typename T, int ROWS, int TH, bool D>
 bool launch_few(const MMCeFew& a, const MMCeFewD<T>& b, int wg, hipStream_t stream) {
   const size_t lds = (size_t)a.T * mm_up(a.D, 64 * MMVec<T>::N) * sizeof(float);
@@ -919,18 +973,12 @@ bool few(const MMCeFew& a, const MMCeFewD<T>& b, int wg, hipStream_t stream) {
 }
 
 template <typename T>
-int forward_few(const Sizes& s, const MMCeFew& a, float* sums, hipStream_t stream) {
+int forward_few(const Sizes& s, const MMCeFew& a, const Rows& r, const Forward& f, hipStream_t stream) {
   const int wg = few_workgroups(s);
   const MMCeFewD<T> none{};
   const bool ok = wg == 1 ? few<T, 1024, false>(a, none, 1, stream) : few<T, 512, false>(a, none, wg, stream);
   if (!ok) return MM_ELAUNCH;
-  if (wg > 1) {
-    hipLaunchKernelGGL(mm_ce_rows_kernel, dim3(1), dim3(1024), 0, stream, a.part, s.T, wg, a.count, a.list, a.y,
-                       a.picked, a.stats, a.reduction == 0 ? a.loss : nullptr, a.reduction ? sums : nullptr);
-    if (a.reduction)
-      hipLaunchKernelGGL(mm_ce_total_kernel, dim3(1), dim3(1024), 0, stream, sums, a.count, a.reduction == MM_CE_MEAN,
-                         a.loss);
-  }
+  if (wg > 1) finish(s, f, wg, r, a.reduction, a.stats, a.loss, stream);
   return mm::launch_status("mm_ce_fwd");
 }
 
@@ -938,6 +986,7 @@ template <typename T>
 int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, float* loss, float* stats,
             const Forward& f, hipStream_t stream) {
   typedef typename MMCeType<T>::H H;
+  const int side = side_of(s.T, s.V, MMCeType<T>::P), tiles_n = (int)div_up(s.V, side);
   if (s.T) {
     const MMPack px{x, r.list, r.count, f.x, nullptr, ldx, 0, s.Dp, 0, s.T * s.Dp, 0, (int)s.T, (int)s.D};
     const MMPack pw{w, nullptr, nullptr, f.w, nullptr, s.D, 0, s.Dp, 0, s.V * s.Dp, 0, (int)s.V, (int)s.D};
@@ -953,15 +1002,9 @@ int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int
     a.part = f.part;
     a.picked = f.picked;
     a.T = s.T;
-    const int side = side_of(s.T, s.V, MMCeType<T>::P), tiles_n = (int)div_up(s.V, side);
     if (!Tiles<T>::template logits<false>(a, s.T, s.V, side, stream)) return MM_ELAUNCH;
-    hipLaunchKernelGGL(mm_ce_rows_kernel, dim3((unsigned)div_up(s.T, 32)), dim3(1024), 0, stream, f.part, s.T, tiles_n,
-                       r.count, r.list, r.y, f.picked, stats, reduction == 0 ? loss : nullptr,
-                       reduction ? f.sums : nullptr);
   }
-  if (reduction)
-    hipLaunchKernelGGL(mm_ce_total_kernel, dim3(1), dim3(1024), 0, stream, f.sums, r.count, reduction == MM_CE_MEAN,
-                       loss);
+  finish(s, f, tiles_n, r, reduction, stats, loss, stream);
   return mm::launch_status("mm_ce_fwd");
 }
 
@@ -1102,7 +1145,7 @@ extern "C" int mm_ce_fwd(const void* x, long ldx, int dtype, long T, long D, con
   if (few_rows(s)) {
     const MMCeFew a{x, w, targets, ldx, ignore, (int)T, (int)D, (int)V, targets64, reduction, r.count, r.list, r.y, r.pos,
                     f.part, f.picked, stats, loss};
-    MM_DISPATCH(dtype, rc = forward_few<T_>(s, a, f.sums, stream));
+    MM_DISPATCH(dtype, rc = forward_few<T_>(s, a, r, f, stream));
     return rc;
   }
   const unsigned blocks = T ? (unsigned)div_up(T, 1024 * MM_CE_SCAN) : 1;

@@ -3,9 +3,10 @@
 // (structure, group):
 //     h = (x - mean) rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps),  z = h w + b,  y = act(z)
 //     dz = dy act'(z):  dw = sum_rows dz h,  db = sum_rows dz,  dx = rstd (dz w - mean(dz w) - h mean(dz w h))
-// Bound by HBM.  A thread keeps one vector of 16 bytes of channels for several rows, and sums go by channel first (over
-// a thread's rows, the lanes of a wave, the waves through LDS), then over the channels of a group: any group size works,
-// whether or not it holds whole vectors.
+// Bound by HBM (500,000 x 128 bfloat16 values in one structure, gelu: forward 115 us, backward 210, 3.1 TB/s; 4096
+// ragged structures of 90,001 x 128 floats, silu, whole: 37 and 43 us, 2.5 and 3.2 TB/s).  A thread keeps one vector of
+// 16 bytes of channels for several rows, and sums go by channel first (over a thread's rows, the lanes of a wave, the
+// waves through LDS), then over the channels of a group: any group size works, whether or not it holds whole vectors.
 //
 // Two ways, by the number of rows of a structure, which the host need not know:
 //   whole  a workgroup holds the structure (of its block of whole groups) in registers: every value is read once;
@@ -373,7 +374,8 @@ struct Plan {
 };
 
 // Threads of a workgroup and values a thread.  Small structures by one wave: sums without barriers, and four times as
-// many of them at once (4096 structures of 5 to 39 rows of 128 float values, forward 64 -> 36 us).  1024 threads hold large ones.
+// many of them at once (4096 structures of 5 to 39 rows of 128 float values, forward 64 -> 36 us).  1024 threads hold
+// large ones.
 struct Shape { int tpb, vals; };
 constexpr Shape kShapes[] = {{64, 64}, {256, 32}, {1024, 32}};
 

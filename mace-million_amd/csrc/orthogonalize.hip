@@ -172,6 +172,7 @@ __device__ __forceinline__ void mm_ortho_tiles_transposed(const Nt& t, uint4* ld
   }
 }
 
+// 4096 x 8192 bfloat16: 214 us for A (640 TFLOP/s of the half that is computed), 122 for B: 136 tiles on 256 CUs.
 // A = X X^T (WHAT 0) or B = b A + c A A (1): planes [side][lda], zeros past the last column.  Both are symmetric: tiles
 // below the diagonal are written twice, those above are not computed.
 template <int P, int WHAT, typename Nt>
@@ -269,6 +270,7 @@ __global__ void __launch_bounds__(256) mm_ortho_join_kernel(MMOrtho a) {
   mm_ortho_put4<PLANES>(a.a + ((long)e * a.side + m) * a.lda + n, a.pa, (const float*)&v);
 }
 
+// 4096 x 8192 bfloat16: 350 us, 785 TFLOP/s; the epilogue moves 16 bytes a value (X in fp32, both planes of halves).
 // X <- a X + B X (rows <= cols) or a X + X B; the last step writes out alone.  Other workgroups still read the operand
 // of X's planes: its new values go to a.next.
 template <typename T, typename Nt>
@@ -323,7 +325,8 @@ mm_ortho_step_kernel(MMOrtho a, int tiles_m, int tiles_n, int last) {
 //     W = b X + c (A X), which takes X's place in LDS;  X <- a X + A W, which takes it back
 // so that neither A nor B is stored (B X = A (b X + c A X)).  The order of an operand along the summed index is free as
 // long as both operands agree: 32 values are taken as k = 16 (e / 4) + 4 g + e % 4, the order in which a lane has its
-// results.  |W| stays below 16 where |X| does.  Bound by LDS (an operand read from it meets 16 rows only) and barriers.
+// results.  |W| stays below 16 where |X| does.  Bound by LDS (an operand read from it meets 16 rows only) and barriers:
+// float, 128 x 128 45 us for five steps, 89 of 201 x 137 123 - 138.
 struct MMOrthoSmall {
   const void* m;
   void* out;
