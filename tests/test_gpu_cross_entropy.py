@@ -290,3 +290,33 @@ def test_few_rows_with_gradients(T, D, V, dtype):
     for reduction in ("mean", "none"):
         ref, bound = _reference(x.cuda(), w.cuda(), y.cuda(), dloss.cuda(), reduction, dtype)
         _check(_run(x, w, y, dloss, reduction), ref, bound)
+
+
+@pytest.mark.parametrize("T,D,V,dtype", [(16, 64, 200, torch.float32), (1, 128, 20000, torch.bfloat16),
+                                         (3, 777, 5000, torch.float16), (200, 32, 20000, torch.bfloat16)])
+def test_few_rows_in_a_replayed_graph(T, D, V, dtype):
+    """Few rows of many classes; ignored rows hold NaN, and how many there are changes between the replays."""
+    from mace_onegpu.cross_entropy import linear_cross_entropy
+    x, w, y, dloss = (t.cuda() for t in _inputs(T, D, V, dtype, 10))
+    xs, ws, ys, up = x.clone().requires_grad_(), w.clone().requires_grad_(), y.clone(), dloss.clone()
+
+    def step():
+        loss = linear_cross_entropy(xs, ws, ys, reduction="none")
+        return (loss.detach(), *torch.autograd.grad(loss, (xs, ws), up))
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed, ignored in ((11, 0.0), (12, 0.5), (13, 1.0), (14, 0.3)):
+        a, b, c, d = (t.cuda() for t in _inputs(T, D, V, dtype, seed, ignored))
+        a[c < 0] = float("nan")
+        with torch.no_grad():
+            xs.copy_(a)
+            ws.copy_(b)
+        ys.copy_(c)
+        up.copy_(d)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(p, q) and bool(q.isfinite().all()) for p, q in zip(out, want))
+        assert not bool(out[1][c < 0].any())
