@@ -7,7 +7,7 @@
 // takes the logits again in the forward's order of sums: few rows by the kernel for few rows, more by tiles.
 // Rows whose target is ignored are taken out at the start: `list` has the asked rows in their order, and everything
 // runs over their number, which stays on the GPU.  (8192 rows, 131,072 classes of 2048 bfloat16 values, both gradients:
-// 16.3 ms, 807 TFLOP/s of the 13.2 T operations.  14,700 rows, 89 classes of 128 float values: 104 us, launches and
+// 16.3 ms, 807 TFLOP/s of the 13.2 T operations.  14,700 rows, 89 classes of 128 float values: 98 us, launches and
 // the six products of small tiles.)
 // Forward: tiles of logits in registers, of which every row's maximum, sum of exponentials and target's logit go out.
 // Backward: pieces of the vocabulary; the logits of a piece are taken again and become d, stored in 16 bits by rows
@@ -32,22 +32,23 @@ struct Rows {
 Rows rows_of(int* buf, long T) { return Rows{buf, buf + 4, buf + 4 + T, buf + 4 + 2 * T}; }
 }  // namespace
 
-#define MM_CE_SCAN 16   // rows of a thread: t0 + 1024 i
+// SCAN: rows of a thread, t0 + 1024 i.  16 where one workgroup lists them all, else 4 (98,304 rows, count and list: 16 ->
+// 9 us) up to 4 million rows (each workgroup sums the numbers of those before it).
 
 template <typename Y>
 __device__ __forceinline__ int mm_ce_asked(const Y* __restrict__ y, long t, long T, long ignore) {
   return t < T && (long)y[t] != ignore;
 }
 
-// asked rows of every 1024 x 16
-template <typename Y>
+// asked rows of every 1024 x SCAN
+template <typename Y, int SCAN>
 __global__ void __launch_bounds__(1024) mm_ce_count_kernel(const Y* __restrict__ y, long T, long ignore,
                                                            int* __restrict__ counts) {
   __shared__ int s[16];
-  const long t0 = (long)blockIdx.x * 1024 * MM_CE_SCAN + threadIdx.x;
+  const long t0 = (long)blockIdx.x * 1024 * SCAN + threadIdx.x;
   int n = 0;
 #pragma unroll
-  for (int i = 0; i < MM_CE_SCAN; ++i) n += mm_ce_asked(y, t0 + 1024 * i, T, ignore);
+  for (int i = 0; i < SCAN; ++i) n += mm_ce_asked(y, t0 + 1024 * i, T, ignore);
 #pragma unroll
   for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = n;
@@ -58,22 +59,22 @@ __global__ void __launch_bounds__(1024) mm_ce_count_kernel(const Y* __restrict__
 }
 
 // list, y, pos and the count; loss (nullable): 0 for ignored rows.  A target outside [0, V) becomes -1.  Rows are taken
-// 64 at a time by a wave, so that loads and stores are contiguous; the numbers of the 16 x 16 runs of 64 are summed by
+// 64 at a time by a wave, so that loads and stores are contiguous; the numbers of the SCAN x 16 runs of 64 are summed by
 // one wave.  (16 rows in a row for each thread: 25 us instead of 5 for 8192 rows.)
-template <typename Y>
+template <typename Y, int SCAN>
 __global__ void __launch_bounds__(1024) mm_ce_list_kernel(const Y* __restrict__ y, long T, int V, long ignore,
                                                           const int* __restrict__ counts, int* __restrict__ count,
                                                           int* __restrict__ list, int* __restrict__ yc,
                                                           int* __restrict__ pos, float* __restrict__ loss) {
-  __shared__ int s[MM_CE_SCAN * 16], s_all;
-  const long t0 = (long)blockIdx.x * 1024 * MM_CE_SCAN + threadIdx.x;
+  __shared__ int s[SCAN * 16], s_all;
+  const long t0 = (long)blockIdx.x * 1024 * SCAN + threadIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  long v[MM_CE_SCAN];
-  int at[MM_CE_SCAN];
+  long v[SCAN];
+  int at[SCAN];
 #pragma unroll
-  for (int i = 0; i < MM_CE_SCAN; ++i) v[i] = t0 + 1024 * i < T ? (long)y[t0 + 1024 * i] : ignore;
+  for (int i = 0; i < SCAN; ++i) v[i] = t0 + 1024 * i < T ? (long)y[t0 + 1024 * i] : ignore;
 #pragma unroll
-  for (int i = 0; i < MM_CE_SCAN; ++i) {
+  for (int i = 0; i < SCAN; ++i) {
     const unsigned long long asked = __ballot(v[i] != ignore);
     at[i] = __popcll(asked & ((1ull << lane) - 1));
     if (lane == 0) s[16 * i + wave] = __popcll(asked);
@@ -84,9 +85,10 @@ __global__ void __launch_bounds__(1024) mm_ce_list_kernel(const Y* __restrict__ 
     for (int b = lane; b < (int)blockIdx.x; b += 64) before += counts[b];
 #pragma unroll
     for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
-    int c[4], sum = 0;
+    constexpr int EACH = SCAN / 4;   // of a lane
+    int c[EACH], sum = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum += c[i] = s[4 * lane + i];
+    for (int i = 0; i < EACH; ++i) sum += c[i] = s[EACH * lane + i];
     int inc = sum;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -95,15 +97,15 @@ __global__ void __launch_bounds__(1024) mm_ce_list_kernel(const Y* __restrict__ 
     }
     int first = before + inc - sum;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[4 * lane + i] = first;
+    for (int i = 0; i < EACH; ++i) {
+      s[EACH * lane + i] = first;
       first += c[i];
     }
     if (lane == 63) s_all = first;
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < MM_CE_SCAN; ++i) {
+  for (int i = 0; i < SCAN; ++i) {
     const long t = t0 + 1024 * i;
     if (t >= T) break;
     if (v[i] != ignore) {
@@ -861,7 +863,7 @@ size_t forward_space(const Sizes& s, char* base, Forward* f) {
   f->part = p.take<float>((size_t)div_up(s.V, BN) * s.T * 2);
   f->picked = p.take<float>(s.T);
   f->sums = p.take<float>(s.T < MM_CE_ROW ? s.T : div_up(s.T, 32));
-  f->counts = p.take<int>(div_up(s.T, 1024 * MM_CE_SCAN));
+  f->counts = p.take<int>(div_up(s.T, 1024 * 4));
   return p.used;
 }
 
@@ -1148,14 +1150,18 @@ extern "C" int mm_ce_fwd(const void* x, long ldx, int dtype, long T, long D, con
     MM_DISPATCH(dtype, rc = forward_few<T_>(s, a, r, f, stream));
     return rc;
   }
-  const unsigned blocks = T ? (unsigned)div_up(T, 1024 * MM_CE_SCAN) : 1;
-  auto scan = [&](auto y) {
+  auto list = [&](auto y, auto each) {
+    typedef std::remove_const_t<std::remove_pointer_t<decltype(y)>> Y;
+    constexpr int SCAN = decltype(each)::value;
+    const unsigned blocks = T ? (unsigned)div_up(T, 1024 * SCAN) : 1;
     if (blocks > 1)
-      hipLaunchKernelGGL((mm_ce_count_kernel<std::remove_const_t<std::remove_pointer_t<decltype(y)>>>), dim3(blocks),
-                         dim3(1024), 0, stream, y, T, ignore, f.counts);
-    hipLaunchKernelGGL((mm_ce_list_kernel<std::remove_const_t<std::remove_pointer_t<decltype(y)>>>), dim3(blocks),
-                       dim3(1024), 0, stream, y, T, (int)V, ignore, f.counts, r.count, r.list, r.y, r.pos,
-                       reduction == 0 ? loss : nullptr);
+      hipLaunchKernelGGL((mm_ce_count_kernel<Y, SCAN>), dim3(blocks), dim3(1024), 0, stream, y, T, ignore, f.counts);
+    hipLaunchKernelGGL((mm_ce_list_kernel<Y, SCAN>), dim3(blocks), dim3(1024), 0, stream, y, T, (int)V, ignore, f.counts,
+                       r.count, r.list, r.y, r.pos, reduction == 0 ? loss : nullptr);
+  };
+  auto scan = [&](auto y) {
+    if (T > 16384 && T <= 4194304) list(y, std::integral_constant<int, 4>{});
+    else list(y, std::integral_constant<int, 16>{});
   };
   if (targets64) scan((const long*)targets);
   else scan((const int*)targets);

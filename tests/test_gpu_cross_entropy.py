@@ -320,3 +320,15 @@ def test_few_rows_in_a_replayed_graph(T, D, V, dtype):
         want = step()
         assert all(torch.equal(p, q) and bool(q.isfinite().all()) for p, q in zip(out, want))
         assert not bool(out[1][c < 0].any())
+
+
+@pytest.mark.parametrize("T", [16384, 16385, 70001, 4194304 + 5000])
+def test_lists_of_many_rows(T):
+    """Every row's loss and gradient, where the asked rows are listed by one workgroup, by many, by larger ones."""
+    from mace_onegpu.cross_entropy import linear_cross_entropy
+    x, w, y, dloss = (t.cuda() for t in _inputs(T, 4, 5, torch.float32, T, 0.7))
+    ref, bound = _reference(x, w, y, dloss, "none", torch.float32)
+    got = linear_cross_entropy(x, w, y.int(), reduction="none")
+    xs = x.requires_grad_()
+    dx, = torch.autograd.grad(linear_cross_entropy(xs, w, y, reduction="none"), xs, dloss)
+    _check(dict(loss=got, dx=dx), ref, bound)
