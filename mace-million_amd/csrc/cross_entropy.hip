@@ -1,10 +1,13 @@
 // Cross entropy of linear logits, without keeping them:
-//     l[t, v] = x[t] . W[v],  top[t] = max_v l[t, v],  s[t] = sum_v exp(l[t, v] - top[t])
-//     loss[t] = top[t] - l[t, y[t]] + log s[t]
+//     l[t, v] = x[t] . W[v],  top[t] = max_v l[t, v],  rest[t] = sum over v != y[t] of exp(l[t, v] - top[t])
+//     s[t] = rest[t] + exp(l[t, y[t]] - top[t]),  loss[t] = top[t] - l[t, y[t]] + log s[t]
 //     d[t, v] = exp(l[t, v] - top[t]) / s[t] - [v = y[t]]:  dx[t] = g[t] d[t] W,  dW = sum_t g[t] d[t]^T x[t]
-// top and s are kept, not log sum exp: its rounding (2^-24 of it) would be a relative error of a whole row of
-// probabilities, and d of a row that is certain of its class is their difference from 1.  For the same reason backward
-// takes the logits again in the forward's order of sums: few rows by the kernel for few rows, more by tiles.
+// A row that is certain of its class has s = 1 + rest with a small rest: rounding s would leave 2^-24 of 1 in the loss and in
+// d, whatever their size (1.5e-5 of a loss of 0.004).  So the sums leave the target out, and where it is the largest logit,
+// loss = log1p(rest) and its d = -rest / (1 + rest), both as near as the exponentials.
+// top and s (or rest) are kept, not log sum exp: its rounding (2^-24 of it) would be a relative error of a whole row of
+// probabilities.  For the same reason backward takes the logits again in the forward's order of sums: few rows by the
+// kernel for few rows, more by tiles.
 // Rows whose target is ignored are taken out at the start: `list` has the asked rows in their order, and everything
 // runs over their number, which stays on the GPU.  (8192 rows, 131,072 classes of 2048 bfloat16 values, both gradients:
 // 16.3 ms, 807 TFLOP/s of the 13.2 T operations.  14,700 rows, 89 classes of 128 float values: 98 us, launches and
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(256) mm_ce_pack_kernel(MMPack first, MMPack se
 
 // ------------------------------------------------------------------------------------------------ logits
 struct MMCeRow {
-  float top, sum;   // sum of exp(l - top)
+  float top, sum;   // sum of exp(l - top) over the classes other than the target
 };
 
 __device__ __forceinline__ MMCeRow mm_ce_join(MMCeRow a, MMCeRow b) {
@@ -226,6 +229,38 @@ __device__ __forceinline__ MMCeRow mm_ce_join(MMCeRow a, MMCeRow b) {
   if (top == -INFINITY) return MMCeRow{top, a.sum + b.sum};   // nothing yet, or -inf alone
   return MMCeRow{top, a.sum * __expf(a.top - top) + b.sum * __expf(b.top - top)};
 }
+
+// Loss of a row whose target's logit is `picked` (bad: target out of range), and what the backward keeps of its sums: s, or
+// -rest where the target is the largest logit (-0 at least: the sign tells the two).
+__device__ __forceinline__ float mm_ce_loss(const MMCeRow& r, float picked, bool bad, float* keep) {
+  if (bad) {
+    *keep = r.sum;
+    return __builtin_nanf("");
+  }
+  const float gap = r.top - picked;
+  if (gap == 0.f) {
+    *keep = -r.sum;
+    return log1pf(r.sum);
+  }
+  const float s = r.sum + __expf(-gap);   // NaN where logits are infinite
+  *keep = s;
+  return gap + logf(s);
+}
+
+// d of a row from what is kept: exp(l - top) inv, at the target times `by` plus `add`
+struct MMCeD {
+  float inv, by, add;
+  __device__ __forceinline__ explicit MMCeD(float keep) {
+    const bool sure = __builtin_signbitf(keep);
+    inv = 1.f / (sure ? 1.f - keep : keep);
+    by = sure ? 0.f : 1.f;
+    add = sure ? keep * inv : -1.f;
+  }
+  __device__ __forceinline__ float operator()(float l, float top, bool target) const {
+    const float p = __expf(l - top) * inv;
+    return target ? fmaf(p, by, add) : p;
+  }
+};
 
 // The incoming gradient: of every row's loss (g of the asked rows and the largest finite |g|), or (g null) of their sum
 // or mean, dloss [1].
@@ -249,7 +284,7 @@ struct MMCeLogits {
   float *part, *picked;  // [tiles of columns][T][2], [T]
   long T;
   // backward: columns v0 .. v0 + n
-  const float* stats;            // [2][T]: top, s
+  const float* stats;            // [2][T]: top, s or -rest
   MMCeScale by;
   H *d, *dT;                     // [T][ldd], [n][ldt] (planes)
   long ldd, ldt, plane, planeT;
@@ -288,6 +323,7 @@ mm_ce_logits_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
         if (n == y) {
           hit = t.acc[i][j][q];
           has = true;
+          t.acc[i][j][q] = -INFINITY;   // stays out of the sum
         }
       }
     if (has && m < count) a.picked[m] = hit;
@@ -340,8 +376,7 @@ mm_ce_rows_kernel(const float* __restrict__ part, long T, int tiles_n, const int
   float l = 0.f;
   if (i < n && (threadIdx.x & 31) == 0) {
     stats[i] = r.top;
-    stats[T + i] = r.sum;
-    l = y[i] < 0 ? __builtin_nanf("") : r.top - picked[i] + logf(r.sum);
+    l = mm_ce_loss(r, picked[i], y[i] < 0, stats + T + i);
     if (loss) loss[list[i]] = l;
   }
   if (!sums) return;
@@ -375,8 +410,7 @@ mm_ce_row_kernel(const float* __restrict__ part, long T, int tiles_n, const int*
   if (threadIdx.x) return;
   for (int w = 1; w < 4; ++w) r = mm_ce_join(r, s[w]);
   stats[i] = r.top;
-  stats[T + i] = r.sum;
-  const float l = y[i] < 0 ? __builtin_nanf("") : r.top - picked[i] + logf(r.sum);
+  const float l = mm_ce_loss(r, picked[i], y[i] < 0, stats + T + i);
   if (loss) loss[list[i]] = l;
   if (sums) sums[i] = l;
 }
@@ -448,7 +482,8 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
   const unsigned long long asked = __ballot(target != a.ignore);
   const int at = __popcll(asked & ((1ull << lane) - 1)), n = __popcll(asked);
   const int y = D ? a.y[has ? lane : 0] : target >= 0 && target < a.V ? (int)target : -1;
-  const float top = D ? a.stats[has ? lane : 0] : 0.f, inv = D ? 1.f / a.stats[a.T + (has ? lane : 0)] : 0.f;
+  const float top = D ? a.stats[has ? lane : 0] : 0.f;
+  const MMCeD d_of(D ? a.stats[a.T + (has ? lane : 0)] : 1.f);
   const float share = D ? b.by.share(has ? lane : 0) : 0.f;
   const int end = D ? (int)mm_up(a.V, MM_NT_K) : a.V;   // D: zeros past the last class
   if (!D && blockIdx.x == 0 && wave == 0) {
@@ -500,7 +535,7 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
         if constexpr (D) {
           if (lane == t) mine[k] = l;
         } else if (lane == t && v0 + k < a.V) {
-          r = mm_ce_join(r, MMCeRow{l, 1.f});
+          r = mm_ce_join(r, MMCeRow{l, v0 + k == y ? 0.f : 1.f});
           if (v0 + k == y) hit = l;
         }
       }
@@ -508,7 +543,7 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
     if constexpr (D) {
 #pragma unroll
       for (int k = 0; k < C; ++k) {
-        const float p = __expf(mine[k] - top) * inv - (v0 + k + b.v0 == y ? 1.f : 0.f);
+        const float p = d_of(mine[k], top, v0 + k + b.v0 == y);
         // a target out of range (loss NaN) makes the row NaN
         mine[k] = has && v0 + k < a.V ? (y < 0 ? __builtin_nanf("") : p * b.scale) : 0.f;
       }
@@ -549,8 +584,7 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
       return;
     }
     a.stats[at] = r.top;
-    a.stats[a.T + at] = r.sum;
-    l = y < 0 ? __builtin_nanf("") : r.top - hit + logf(r.sum);
+    l = mm_ce_loss(r, hit, y < 0, a.stats + a.T + at);
     if (a.reduction == 0) a.loss[lane] = l;
   }
   if (gridDim.x > 1 || a.reduction == 0) return;
@@ -600,14 +634,15 @@ mm_ce_d_kernel(MMCeLogits<typename MMCeType<T>::H> a, int tiles_n) {
 #pragma unroll
   for (int j = 0; j < Nt::FM; ++j) {
     const int m = m0 + t.row(j), at = min(m, count - 1), y = a.y[at];
-    const float top = a.stats[at], inv = 1.f / a.stats[a.T + at];
+    const float top = a.stats[at];
+    const MMCeD d_of(a.stats[a.T + at]);
     share[j] = a.by.share(at);
 #pragma unroll
     for (int i = 0; i < Nt::FN; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int n = n0 + t.col(i) + q;
-        const float p = __expf(t.acc[i][j][q] - top) * inv - (n + a.v0 == y ? 1.f : 0.f);
+        const float p = d_of(t.acc[i][j][q], top, n + a.v0 == y);
         // a target out of range (loss NaN) makes the row NaN
         t.acc[i][j][q] = n < a.n && m < count ? (y < 0 ? __builtin_nanf("") : p * a.scale) : 0.f;
       }

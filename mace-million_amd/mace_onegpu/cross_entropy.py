@@ -5,9 +5,11 @@
 x [..., D] and weight [classes, D]: float32, bfloat16 or float16, both of one type; rows of x may be strided and are read
 in place where the last axis is contiguous.  targets [...]: int32 or int64 classes; rows whose target is ignore_index are
 taken out (loss 0, zero gradient, whatever stands in them); any other target outside [0, classes) makes the row's loss
-and the gradients NaN.  The logits live in registers alone: forward keeps one number a row, backward takes them again in
-pieces of the classes.  float32 products are taken from three bfloat16 parts of each operand at float32 accuracy (values
-from 3.396e38 on give NaN); logits, exponentials and all sums are float32, in a fixed order: the same bits in every run.
+and the gradients NaN.  The logits live in registers alone: forward keeps two numbers a row, backward takes them again in
+pieces of the classes.  Losses and gradients of rows that are certain of their class keep their digits: they come from the
+sum over the other classes, which is never added to 1.  float32 products are taken from three bfloat16 parts of each
+operand at float32 accuracy (values from 3.396e38 on give NaN); logits, exponentials and all sums are float32, in a fixed
+order: the same bits in every run.
 Runs on torch's current stream without reading anything back, can be captured into a HIP graph, and needs the GPU: there
 is no CPU path.  The reference has no counterpart.
 """
