@@ -225,8 +225,8 @@ struct MMCeRow {
 };
 
 __device__ __forceinline__ MMCeRow mm_ce_join(MMCeRow a, MMCeRow b) {
-  const float top = fmaxf(a.top, b.top);
-  if (top == -INFINITY) return MMCeRow{top, a.sum + b.sum};   // nothing yet, or -inf alone
+  const float top = fmaxf(a.top, b.top);   // drops a NaN, which has to reach the sum
+  if (a.top == -INFINITY && b.top == -INFINITY) return MMCeRow{top, a.sum + b.sum};   // nothing yet, or -inf alone
   return MMCeRow{top, a.sum * __expf(a.top - top) + b.sum * __expf(b.top - top)};
 }
 
