@@ -41,8 +41,9 @@ class Muon(torch.optim.Optimizer):
         p <- (1 - lr weight_decay) p - lr 0.2 sqrt(max(rows, columns)) orthogonalize(u)
 
     The factor gives an update a root mean square of about 0.2, what Adam's has, so that learning rates carry over and
-    neither axis has to be the input's.  buf is float32; u is rounded to the parameter's type.  Vectors and scalars
-    belong to another optimizer."""
+    neither axis has to be the input's.  buf is float32; so is u, but for bfloat16 parameters, to whose type it is rounded
+    (of the same range; float16's would overflow, or lose small gradients).  Vectors and scalars belong to another
+    optimizer."""
 
     def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
                  coefficients=COEFFICIENTS, eps=1e-7):
@@ -83,7 +84,8 @@ class Muon(torch.optim.Optimizer):
                 buf = state["momentum_buffer"]
                 buf.mul_(group["momentum"]).add_(g)
                 u = g.add(buf, alpha=group["momentum"]) if group["nesterov"] else buf
-                o = orthogonalize(u.to(p.dtype), group["steps"], group["coefficients"], group["eps"])
+                u = u if p.dtype == torch.float16 else u.to(p.dtype)
+                o = orthogonalize(u, group["steps"], group["coefficients"], group["eps"])
                 if group["weight_decay"]:
                     p.mul_(1 - group["lr"] * group["weight_decay"])
                 p.add_(o, alpha=-group["lr"] * 0.2 * math.sqrt(max(p.shape[-2:])))
