@@ -462,6 +462,7 @@ struct MMCeFewD {
 template <typename T, int ROWS, int TH, bool D>
 __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b) {
   constexpr int N = MMVec<T>::N, W = TH / 64, C = MM_CE_CLASSES;
+  constexpr bool SPLIT = MMCeType<T>::PLANES > 1;   // what the planes of more rows cannot hold gives NaN here too
   extern __shared__ float mm_ce_x[];   // [T][D rounded up to whole vectors of a wave]
   __shared__ MMCeRow s_row[W][ROWS];
   __shared__ float s_hit[W][ROWS];
@@ -476,8 +477,10 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
   for (int t = 0; t < ROWS; ++t) {
     if (t >= rows) continue;
     const long at = D ? a.list[t] : t;
-    for (int c = threadIdx.x; c < Dp; c += TH)
-      mm_ce_x[t * Dp + c] = c < a.D ? (float)((const T*)a.x)[at * a.ldx + c] : 0.f;
+    for (int c = threadIdx.x; c < Dp; c += TH) {
+      const float v = c < a.D ? (float)((const T*)a.x)[at * a.ldx + c] : 0.f;
+      mm_ce_x[t * Dp + c] = SPLIT && fabsf(v) >= MM_SPLIT_LIMIT ? __builtin_nanf("") : v;
+    }
   }
   const unsigned long long asked = __ballot(target != a.ignore);
   const int at = __popcll(asked & ((1ull << lane) - 1)), n = __popcll(asked);
@@ -499,7 +502,7 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
   MMCeRow r{-INFINITY, 0.f};
   float hit = 0.f;
   for (int v0 = (blockIdx.x * W + wave) * C; v0 < end; v0 += (int)gridDim.x * W * C) {
-    float acc[ROWS][C] = {};
+    float acc[ROWS][C] = {}, large[C] = {};   // the largest |w| (a NaN is in acc anyway)
     const T* __restrict__ p[C];
 #pragma unroll
     for (int k = 0; k < C; ++k) p[k] = (const T*)a.w + (size_t)min(v0 + k, a.V - 1) * a.D;
@@ -507,6 +510,12 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
       float w[C][N];
 #pragma unroll
       for (int k = 0; k < C; ++k) mm_load_vec(p[k], c, end, w[k]);
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+#pragma unroll
+          for (int i = 0; i < N; ++i) large[k] = fmaxf(large[k], fabsf(w[k][i]));
+      }
 #pragma unroll
       for (int t = 0; t < ROWS; ++t) {
         if (ROWS > 1 && t >= rows) continue;   // not break, which would put acc into memory
@@ -525,6 +534,12 @@ __global__ void __launch_bounds__(TH) mm_ce_few_kernel(MMCeFew a, MMCeFewD<T> b)
 #pragma unroll 4
     for (; c < whole; c += 64 * N) add(c, c + N);
     if (whole < a.D && c < Dp) add(c, a.D);
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int t = 0; t < ROWS; ++t)
+#pragma unroll
+        for (int k = 0; k < C; ++k) acc[t][k] = large[k] >= MM_SPLIT_LIMIT ? __builtin_nanf("") : acc[t][k];
+    }
     float mine[C] = {};
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) {

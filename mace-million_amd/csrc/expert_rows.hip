@@ -289,9 +289,6 @@ struct MMFew {
   int k, M, D, F, E;
 };
 
-// the least float that rounds to infinity in bfloat16
-#define MM_SPLIT_LIMIT 0x1.ffp127f
-
 template <typename T, int LC>
 __global__ void __launch_bounds__(256) mm_expert_few_kernel(MMFew a, T* __restrict__ y) {
   constexpr int N = MMVec<T>::N, G = 256 / LC;

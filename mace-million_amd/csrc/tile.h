@@ -46,6 +46,9 @@ struct MMRaw<float> {
   float x[8];
 };
 
+// the least float that rounds to infinity in bfloat16
+#define MM_SPLIT_LIMIT 0x1.ffp127f
+
 // float operands may be scaled on the way
 template <typename T, bool SCALED = false>
 __device__ __forceinline__ MMFrag<T> mm_operand(const MMRaw<T>& r, float scale = 1.f) {

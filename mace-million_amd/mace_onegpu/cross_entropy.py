@@ -8,8 +8,9 @@ taken out (loss 0, zero gradient, whatever stands in them); any other target out
 and the gradients NaN.  The logits live in registers alone: forward keeps two numbers a row, backward takes them again in
 pieces of the classes.  Losses and gradients of rows that are certain of their class keep their digits: they come from the
 sum over the other classes, which is never added to 1.  float32 products are taken from three bfloat16 parts of each
-operand at float32 accuracy (values from 3.396e38 on give NaN); logits, exponentials and all sums are float32, in a fixed
-order: the same bits in every run.
+operand at float32 accuracy (values from 3.396e38 on, infinity among them, give NaN, for one row as for many; 16-bit
+infinities give what their sums do); logits, exponentials and all sums are float32, in a fixed order: the same bits in
+every run.
 Runs on torch's current stream without reading anything back, can be captured into a HIP graph, and needs the GPU: there
 is no CPU path.  The reference has no counterpart.
 """
