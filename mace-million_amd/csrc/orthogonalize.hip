@@ -125,9 +125,17 @@ __global__ void __launch_bounds__(256) mm_ortho_start_kernel(MMOrtho a, int step
   }
 }
 
+// one value, as mm_ortho_put4
+__device__ __forceinline__ void mm_ortho_put1(_Float16* p, long plane, float v) {
+  const _Float16 h = (_Float16)v;
+  p[0] = h;
+  p[plane] = (_Float16)(v - (float)h);
+}
+
 // out = f acc as planes, rows (or, transposed, columns) of it: one plane through LDS in whole lines, two from the
-// registers (their tiles are small, and LDS would take two barriers for each plane)
-template <int PLANES, typename Nt>
+// registers (their tiles are small, and LDS would take two barriers for each plane).  HALF: of a tile on the diagonal,
+// what lies on and below it (transposed: what lies below it).
+template <int PLANES, bool HALF = false, typename Nt>
 __device__ __forceinline__ void mm_ortho_tiles(const Nt& t, uint4* lds, _Float16* out, long ld, long plane, int rows,
                                                int cols, float f) {
   if constexpr (PLANES == 1) {
@@ -138,13 +146,21 @@ __device__ __forceinline__ void mm_ortho_tiles(const Nt& t, uint4* lds, _Float16
 #pragma unroll
       for (int i = 0; i < Nt::FN; ++i) {
         const floatx4 v = t.acc[i][j] * f;
-        if (t.row(j) < rows && t.col(i) < cols)
-          mm_ortho_put4<2>(out + (long)t.row(j) * ld + t.col(i), plane, (const float*)&v);
+        const int m = t.row(j), n = t.col(i);
+        _Float16* const p = out + (long)m * ld + n;
+        if (m >= rows || n >= cols) continue;
+        if (!HALF || n + 3 <= m) {
+          mm_ortho_put4<2>(p, plane, (const float*)&v);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 3; ++q)
+            if (n + q <= m) mm_ortho_put1(p + q, plane, v[q]);
+        }
       }
   }
 }
 
-template <int PLANES, typename Nt>
+template <int PLANES, bool HALF = false, typename Nt>
 __device__ __forceinline__ void mm_ortho_tiles_transposed(const Nt& t, uint4* lds, _Float16* out, long ld, long plane,
                                                           int rows, int cols, float f) {
   if constexpr (PLANES == 1) {
@@ -164,9 +180,18 @@ __device__ __forceinline__ void mm_ortho_tiles_transposed(const Nt& t, uint4* ld
         }
         mm_quad_transpose(h);
         mm_quad_transpose(l);
-        if (m < rows && n < cols) {
-          *(halfx4*)(out + (long)n * ld + m) = halfx4{h[0], h[1], h[2], h[3]};
-          *(halfx4*)(out + plane + (long)n * ld + m) = halfx4{l[0], l[1], l[2], l[3]};
+        if (m >= rows || n >= cols) continue;
+        _Float16* const p = out + (long)n * ld + m;
+        if (!HALF || m > n) {
+          *(halfx4*)p = halfx4{h[0], h[1], h[2], h[3]};
+          *(halfx4*)(p + plane) = halfx4{l[0], l[1], l[2], l[3]};
+        } else {
+#pragma unroll
+          for (int q = 1; q < 4; ++q)
+            if (m + q > n) {
+              p[q] = h[q];
+              p[plane + q] = l[q];
+            }
         }
       }
   }
@@ -174,7 +199,9 @@ __device__ __forceinline__ void mm_ortho_tiles_transposed(const Nt& t, uint4* ld
 
 // 4096 x 8192 bfloat16: 214 us for A (640 TFLOP/s of the half that is computed), 122 for B: 136 tiles on 256 CUs.
 // A = X X^T (WHAT 0) or B = b A + c A A (1): planes [side][lda], zeros past the last column.  Both are symmetric: tiles
-// below the diagonal are written twice, those above are not computed.
+// below the diagonal are written twice, those above are not computed.  Two planes' products (high x low, low x high) come
+// in the other order above the diagonal, so there a tile on it is written twice as well: a result then has the same bits
+// whatever the tiles, which the number of matrices decides.
 template <int P, int WHAT, typename Nt>
 __global__ void __launch_bounds__(Nt::TH, Nt::PER_CU) mm_ortho_square_kernel(MMOrtho a, int tiles) {
   constexpr int PLANES = P == 1 ? 1 : 2;
@@ -241,6 +268,12 @@ __global__ void __launch_bounds__(Nt::TH, Nt::PER_CU) mm_ortho_square_kernel(MMO
     }
   }
   const int left = (int)a.lda - n0, low = (int)a.lda - m0;   // columns with their zeros
+  if (PLANES > 1 && tm == tn) {
+    mm_ortho_tiles<PLANES, true>(t, mm_ortho_lds, out + (long)m0 * a.lda + n0, a.lda, a.pa, a.side - m0, left, 1.f);
+    mm_ortho_tiles_transposed<PLANES, true>(t, mm_ortho_lds, out + (long)n0 * a.lda + m0, a.lda, a.pa, low, a.side - n0,
+                                            1.f);
+    return;
+  }
   mm_ortho_tiles<PLANES>(t, mm_ortho_lds, out + (long)m0 * a.lda + n0, a.lda, a.pa, a.side - m0, left, 1.f);
   if (tm != tn)
     mm_ortho_tiles_transposed<PLANES>(t, mm_ortho_lds, out + (long)n0 * a.lda + m0, a.lda, a.pa, low, a.side - n0, 1.f);
