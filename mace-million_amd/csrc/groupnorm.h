@@ -60,26 +60,38 @@ __device__ __forceinline__ int mm_group_find(const MMGroup& a, long r) {
   return lo;
 }
 
-// Distribution function of the normal distribution, given e = exp(-z^2 / 2): Hastings' approximation of erf (Abramowitz
-// and Stegun 7.1.26), off by 0.75e-7 at most.  With it the activation shares its one exponential with the derivative; erff
-// and expf bound the backward by their instructions.
+// Distribution function of the normal distribution, given e = exp(-z^2 / 2).  The tail beyond |z| is e R(|z|), where R is
+// a polynomial in t = 1 / (1 + p |z|), fitted here for the least largest relative error over |z| <= 14 (with fp32's
+// roundings 5.2 x 2^-24; with two terms less 20 x 2^-24, for 16-bit rows, which then round to 2^-12 at best): the tail
+// keeps its digits however small it is.  With it the activation shares its one exponential with the derivative; erff
+// and expf bound the backward by their instructions (500,000 x 128 bfloat16 values: 309 us with nine terms, 303 with
+// seven).
+template <typename T>
 __device__ __forceinline__ float mm_normal(float z, float e) {
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
-                           0.254829592f);
-  const float half = 0.5f * p * e;   // of the tail beyond |z|
-  return z > 0.f ? 1.f - half : half;
+  constexpr bool FLOAT = sizeof(T) == 4;
+  constexpr int TERMS = FLOAT ? 9 : 7;
+  constexpr float p = FLOAT ? 0.35f : 0.36f;
+  constexpr float nine[] = {0.139621407f, 0.139861852f, 0.119833007f, 0.105507337f, -0.0231080018f,
+                            0.15917109f,  -0.255711198f, 0.143970042f, -0.0291455518f};
+  constexpr float seven[] = {0.143713027f, 0.141772658f,  0.139718115f, 0.0265525803f,
+                             0.180949137f, -0.179760993f, 0.0470551737f};
+  const float t = __builtin_amdgcn_rcpf(fmaf(p, fabsf(z), 1.f));
+  float r = 0.f;
+#pragma unroll
+  for (int i = TERMS - 1; i >= 0; --i) r = fmaf(r, t, FLOAT ? nine[i] : seven[i < 7 ? i : 0]);
+  const float tail = r * t * e;
+  return z > 0.f ? 1.f - tail : tail;
 }
 
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ float mm_act(float z) {
   if constexpr (ACT == MM_GROUP_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
-  if constexpr (ACT == MM_GROUP_ACT_GELU) return z * mm_normal(z, __expf(-0.5f * z * z));
+  if constexpr (ACT == MM_GROUP_ACT_GELU) return z * mm_normal<T>(z, __expf(-0.5f * z * z));
   return z;
 }
 
 // derivative at z
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ float mm_act_slope(float z) {
   if constexpr (ACT == MM_GROUP_ACT_SILU) {
     const float q = __builtin_amdgcn_rcpf(1.f + __expf(-z));
@@ -87,7 +99,7 @@ __device__ __forceinline__ float mm_act_slope(float z) {
   }
   if constexpr (ACT == MM_GROUP_ACT_GELU) {
     const float e = __expf(-0.5f * z * z);
-    return fmaf(z * 0.39894228f, e, mm_normal(z, e));
+    return fmaf(z * 0.39894228f, e, mm_normal<T>(z, e));
   }
   return 1.f;
 }

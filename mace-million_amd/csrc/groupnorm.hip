@@ -29,7 +29,7 @@ mm_groupnorm_whole_fwd_kernel(MMGroup a, const T* __restrict__ x, long ldx, cons
         for (int j = 0; j < R; ++j) {
           const int r = l.sub + j * l.nsub;
 #pragma unroll
-          for (int i = 0; i < N; ++i) v[j][i] = mm_act<ACT>(fmaf(v[j][i] * rs[0][i], wv[i], bv[i]));
+          for (int i = 0; i < N; ++i) v[j][i] = mm_act<T, ACT>(fmaf(v[j][i] * rs[0][i], wv[i], bv[i]));
           if (r < q.n && l.on) l.store(y, ldy, q.first + r, v[j]);
         }
       });
@@ -81,7 +81,7 @@ mm_groupnorm_tile_fwd_kernel(MMGroup a, const T* __restrict__ x, long ldx, const
         float v[N];
         l.get(x, ldx, first + r, v);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = mm_act<ACT>(fmaf((v[i] - mu[i]) * rs[i], wv[i], bv[i]));
+        for (int i = 0; i < N; ++i) v[i] = mm_act<T, ACT>(fmaf((v[i] - mu[i]) * rs[i], wv[i], bv[i]));
         l.store(y, ldy, first + r, v);
       }
     });

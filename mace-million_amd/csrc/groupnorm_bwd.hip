@@ -63,7 +63,7 @@ mm_groupnorm_whole_bwd_kernel(MMGroup a, const T* __restrict__ dy, long lddy, co
         for (int i = 0; i < N; ++i) {
           h[j][i] = (h[j][i] - mu[i]) * rs[i];
           const bool has = l.sub + j * l.nsub < q.n;
-          const float dz = has ? g[j][i] * mm_act_slope<ACT>(fmaf(h[j][i], wv[i], bv[i])) : 0.f;
+          const float dz = has ? g[j][i] * mm_act_slope<T, ACT>(fmaf(h[j][i], wv[i], bv[i])) : 0.f;
           sum[1][i] = has ? fmaf(dz, h[j][i], sum[1][i]) : sum[1][i];
           sum[0][i] += dz;
           g[j][i] = dz;
@@ -128,7 +128,7 @@ mm_groupnorm_tile_sums_kernel(MMGroup a, const T* __restrict__ dy, long lddy, co
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             h[i] = (h[i] - mu[i]) * rs[i];
-            const float dz = g[i] * mm_act_slope<ACT>(fmaf(h[i], wv[i], bv[i]));
+            const float dz = g[i] * mm_act_slope<T, ACT>(fmaf(h[i], wv[i], bv[i]));
             sum[0][i] += dz;
             sum[1][i] = fmaf(dz, h[i], sum[1][i]);
           }
@@ -180,7 +180,7 @@ mm_groupnorm_tile_bwd_kernel(MMGroup a, const T* __restrict__ dy, long lddy, con
         l.get(dy, lddy, first + r, g);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const float h = (v[i] - mu[i]) * rs[i], dz = g[i] * mm_act_slope<ACT>(fmaf(h, wv[i], bv[i]));
+          const float h = (v[i] - mu[i]) * rs[i], dz = g[i] * mm_act_slope<T, ACT>(fmaf(h, wv[i], bv[i]));
           g[i] = rs[i] * (fmaf(dz, wv[i], -m0[i]) - h * m1[i]);
         }
         l.store(dx, lddx, first + r, g);
