@@ -895,6 +895,9 @@ int few_workgroups(const Sizes& s) {
 #define MM_CE_ROW 256
 bool row_each(const Sizes& s, int tiles_n) { return s.T < MM_CE_ROW && tiles_n >= 64; }
 
+// tiles of the forward's logits
+int logits_side(const Sizes& s) { return side_of(s.T, s.V, s.dtype == MM_F32 ? 6 : 1); }
+
 struct Forward {
   void *x, *w;
   float *part, *picked, *sums;
@@ -910,7 +913,7 @@ size_t forward_space(const Sizes& s, char* base, Forward* f) {
   }
   f->x = p.take<short>((size_t)s.planes * s.T * s.Dp);
   f->w = s.w_in_place ? nullptr : p.take<short>((size_t)s.planes * s.V * s.Dp);
-  f->part = p.take<float>((size_t)div_up(s.V, BN) * s.T * 2);
+  f->part = p.take<float>((size_t)div_up(s.V, logits_side(s)) * s.T * 2);
   f->picked = p.take<float>(s.T);
   f->sums = p.take<float>(s.T < MM_CE_ROW ? s.T : div_up(s.T, 32));
   f->counts = p.take<int>(div_up(s.T, 1024 * 4));
@@ -1038,7 +1041,7 @@ template <typename T>
 int forward(const Sizes& s, const T* x, long ldx, const T* w, const Rows& r, int reduction, float* loss, float* stats,
             const Forward& f, hipStream_t stream) {
   typedef typename MMCeType<T>::H H;
-  const int side = side_of(s.T, s.V, MMCeType<T>::P), tiles_n = (int)div_up(s.V, side);
+  const int side = logits_side(s), tiles_n = (int)div_up(s.V, side);
   if (s.T) {
     const MMPack px{x, r.list, r.count, f.x, nullptr, ldx, 0, s.Dp, 0, s.T * s.Dp, 0, (int)s.T, (int)s.D};
     const MMPack pw{w, nullptr, nullptr, f.w, nullptr, s.D, 0, s.Dp, 0, s.V * s.Dp, 0, (int)s.V, (int)s.D};
