@@ -422,6 +422,8 @@ int mm_ce_bwd(const void* x, long ldx, int dtype, long T, long D, const void* w,
 /* out = X after `steps` of A = X X^T, X <- a X + (b A + c A A) X (on the shorter side) from X = m / (|m| + eps), for every
  * matrix of m [batch, rows, cols]; coefficients HOST [steps][3]; at most 65535 matrices of 65536 rows and columns */
 int mm_orthogonalize_workspace(long batch, long rows, long cols, int dtype, size_t* bytes /* HOST */);
+/* for this number of steps: 256 bytes where one workgroup holds a matrix through all of them (otherwise as above) */
+int mm_orthogonalize_workspace_steps(long batch, long rows, long cols, int dtype, int steps, size_t* bytes /* HOST */);
 int mm_orthogonalize(const void* m, int dtype, long batch, long rows, long cols, int steps,
                      const float* coefficients /* HOST */, float eps, void* out, void* workspace, mm_stream_t stream);
 

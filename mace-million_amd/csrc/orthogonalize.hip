@@ -778,6 +778,16 @@ extern "C" int mm_orthogonalize_workspace(long batch, long rows, long cols, int 
   return MM_OK;
 }
 
+extern "C" int mm_orthogonalize_workspace_steps(long batch, long rows, long cols, int dtype, int steps, size_t* bytes) {
+  const int rc = check("mm_orthogonalize_workspace_steps", batch, rows, cols, dtype);
+  if (rc != MM_OK) return rc;
+  MM_CHECK_ARG(steps >= 0 && bytes, "bad steps or no result");
+  if (batch == 0 || !held(rows, cols, dtype, steps).rows)
+    return mm_orthogonalize_workspace(batch, rows, cols, dtype, bytes);
+  *bytes = 256;   // not touched
+  return MM_OK;
+}
+
 extern "C" int mm_orthogonalize(const void* m, int dtype, long batch, long rows, long cols, int steps,
                                 const float* coefficients, float eps, void* out, void* workspace, hipStream_t stream) {
   const int rc = check("mm_orthogonalize", batch, rows, cols, dtype);

@@ -241,7 +241,7 @@ Tensor orthogonalize(const Tensor& m0, const std::vector<float>& coefficients, d
   for (long i = 0; i < batch; i += 65535) {   // of a launch's grid
     const long n = std::min(batch - i, 65535L);
     size_t bytes = 0;
-    done(mm_orthogonalize_workspace(n, rows, cols, code, &bytes));
+    done(mm_orthogonalize_workspace_steps(n, rows, cols, code, (int)(coefficients.size() / 3), &bytes));
     if (!ws.defined() || bytes > (size_t)ws.numel()) ws = bytes_like(bytes, m);
     done(mm_orthogonalize((const char*)ptr(m) + i * step, code, n, rows, cols, (int)(coefficients.size() / 3),
                           coefficients.data(), (float)eps, (char*)ptr(out) + i * step, ptr(ws), stream()));

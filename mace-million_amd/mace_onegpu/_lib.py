@@ -113,6 +113,7 @@ SIGNATURES = {
     "mm_ce_fwd": [P, L, I, L, L, P, L, P, I, L, I, P, P, P, P, P],
     "mm_ce_bwd": [P, L, I, L, L, P, L, I, P, P, P, P, P, P, P],
     "mm_orthogonalize_workspace": [L, L, L, I, P],
+    "mm_orthogonalize_workspace_steps": [L, L, L, I, I, P],
     "mm_orthogonalize": [P, I, L, L, L, I, P, F, P, P, P],
     # tables
     "mm_radial_mlp_f64": [I, P, P, P, P, P, I, I, I, D, I, D, P, P],
