@@ -830,8 +830,10 @@ struct Space {
 int tiles(long m, long n, int side) { return (int)(div_up(m, side) * div_up(n, side)); }
 int side_of(long m, long n, int P) { return mm_tile_side(P, tiles(m, n, 256), tiles(m, n, 128), tiles(m, n, 64)); }
 
-// Tile and parts of the summed index K of an m x n product by the same rule, no part below 512 values; a part costs its
-// sums' way through memory.
+// Tile and parts of the summed index K of an m x n product by the same rule, no part below 512 values; a part costs
+// its sums' way through memory.  Whole passes with one side and number of parts for both products, us: 14,700 float
+// rows, 89 classes of 128 values: 64 x 1 311, x 8 127, x 64 314 (each by its own: 87); 1000 x 3000 float of 512: 64 x
+// 1 155, 128 x 4 144, x 64 376 (153); 8192 x 8192 bfloat16 of 2048: 256 x 1 1059, x 2 1143, x 8 1469 (1067).
 int splits_of(long m, long n, long K, int P, int* side) {
   const long most = clamp(K / 512, 1, 64);
   const MMTileRates r = mm_tile_rates(P);

@@ -410,7 +410,11 @@ __device__ __forceinline__ bool mm_nt_lower(int b, int batch, int tiles, int* e,
 __host__ __device__ inline long mm_up(long n, long size) { return (n + size - 1) / size * size; }
 
 // Tiles of 256, 128 and 64 for P products: how many run at once, and the time of such a round where one tile of 256 on
-// every CU takes 1, by the rates that products of 1024 and more reach (planes leave room for fewer workgroups on a CU).
+// every CU takes 1, by the rates that products of 1024 and more reach (planes leave room for fewer workgroups on a
+// CU).  Logits of 1024 values and their sums, us by tiles of 256 | 128 | 64: bfloat16 1024 x 1024 47 | 32 | 27, 2048 x
+// 8192 56 | 60 | 75, 4096 x 16,384 159 | 170 | 224; float (P = 6) 174 | 62 | 42, 212 | 214 | 259, 735 | 753 | 940.  P
+// = 3, five steps of float matrices: 1024 x 1024 1545 | 582 | 278, 14 of them 3222 | 1829 | 1856 (in parts by their
+// own tiles 1643).
 struct MMTileRates {
   int side[3] = {256, 128, 64}, slots[3];
   double round[3];

@@ -6,9 +6,10 @@
 // X is carried in fp32 and a X is added in fp32: small singular values, which grow by a in every step, keep its bits.
 // The products take float16 operands, scaled by powers of two (X and A by 2^12, B = b A + c A A by 2^10) into the middle
 // of its range: one plane for bfloat16 matrices (2^-12 of an operand, against 2^-9 of the result's own rounding), two
-// planes and three products (2^-22) for float and float16.  |X| and |A| have to stay below 16, |B| below 64: the norm of
-// M bounds them by 1 and the usual coefficients keep them below 3; what passes them becomes infinite or NaN.
-// Norms are summed in 64 bits, so that neither large nor tiny values leave the range.
+// planes and three products (2^-22) for float and float16.  Entries of X, A and W (of the small matrices, below) have
+// to stay below 16, of B below 64: the norm of M bounds X and A by 1 at first, and the usual coefficients keep all of
+// them below 3; what passes becomes infinite or NaN.  Norms are summed in 64 bits, so that neither large nor tiny
+// values leave the range.
 #include "nt.h"
 
 #include <utility>
@@ -358,8 +359,9 @@ mm_ortho_step_kernel(MMOrtho a, int tiles_m, int tiles_n, int last) {
 //     W = b X + c (A X), which takes X's place in LDS;  X <- a X + A W, which takes it back
 // so that neither A nor B is stored (B X = A (b X + c A X)).  The order of an operand along the summed index is free as
 // long as both operands agree: 32 values are taken as k = 16 (e / 4) + 4 g + e % 4, the order in which a lane has its
-// results.  |W| stays below 16 where |X| does.  Bound by LDS (an operand read from it meets 16 rows only) and barriers:
-// float, 128 x 128 45 us for five steps, 89 of 201 x 137 123 - 138.
+// results.  W has the scale of X (of a singular value s it makes b s + c s^3: where X stays below 2, W stays below 16
+// with the usual coefficients).  Bound by LDS (an operand read from it meets 16 rows only) and barriers: float, 128 x
+// 128 45 us for five steps, 89 of 201 x 137 123 - 138.
 struct MMOrthoSmall {
   const void* m;
   void* out;
@@ -631,8 +633,10 @@ size_t space(MMOrtho* a, int dtype, char* base) {
   a->a = p.take<_Float16>(planes * a->pa);
   a->b = p.take<_Float16>(planes * a->pa);
   a->next = p.take<_Float16>(planes * (a->rows <= a->cols ? a->pv : a->pu));
-  // A long side is summed in parts of 512 values or more where A has few tiles.  The rule looks at the matrix alone, so
-  // that its result does not depend on how many stand beside it.
+  // A long side is summed in parts of 512 values or more where A has few tiles.  The rule looks at the matrix alone,
+  // so that its result does not depend on how many stand beside it.  (Five steps, us in 1 | 4 | 8 parts: 192 x 4096
+  // float 348 | 189 | 196, bfloat16 237 | 140 | 157, 64 of the float ones 2369 | 1974 | 2104; 192 x 16,384 float 1074
+  // | 411 | 339; 192 x 768 in one part 148, in two 138; 256 x 4096, not split, 359 | 209 | 211.)
   const long other = a->rows < a->cols ? a->cols : a->rows;
   a->splits = a->side <= 192 && other >= 1024 ? (int)(other / 512 < 8 ? other / 512 : 8) : 1;
   a->sums = a->splits > 1 ? p.take<float>(a->splits * a->pa) : nullptr;
@@ -670,7 +674,10 @@ bool small(const MMOrthoSmall& a, int batch, int lds, hipStream_t stream) {
   return true;
 }
 
-// rows, tiles of columns and LDS of the workgroup that holds a matrix (rows 0: none does)
+// rows, tiles of columns and LDS of the workgroup that holds a matrix (rows 0: none does).  Five float steps, us held
+// | by tiles: one of 128 x 128 44 | 98, of 128 x 256 106 | 107, of 160 x 208 122 | 117; 89 of 201 x 137 122 | 301, of
+// 160 x 208 127 | 312; 300 of 128 x 256 255 | 457.  bfloat16: one of 160 x 208 56 | 90, 300 of them 120 | 364.  Larger
+// shapes were not built, as a single float one gains nothing already (by tiles 89 of 176 x 176 258, of 160 x 256 311).
 struct Held { int rows, nt, lds; };
 Held held(long rows, long cols, int dtype, int steps) {
   const long side = rows < cols ? rows : cols, other = rows < cols ? cols : rows;

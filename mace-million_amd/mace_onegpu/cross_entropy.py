@@ -11,8 +11,9 @@ sum over the other classes, which is never added to 1.  float32 products are tak
 operand at float32 accuracy (values from 3.396e38 on, infinity among them, give NaN, for one row as for many; 16-bit
 infinities give what their sums do); logits, exponentials and all sums are float32, in a fixed order: the same bits in
 every run.
-Runs on torch's current stream without reading anything back, can be captured into a HIP graph, and needs the GPU: there
-is no CPU path.  The reference has no counterpart.
+Sizes from 2^31 - 2^16 on are refused, and so are rows times classes, or their sum times D, from about 2^36 (6.8e10)
+on: the launches' tiles of 64 x 64.  Runs on torch's current stream without reading anything back, can be captured into
+a HIP graph, and needs the GPU: there is no CPU path.  The reference has no counterpart.
 """
 from ._ops import ops
 

@@ -6,9 +6,11 @@ on every matrix of m [..., rows, columns] (expert blocks [E, D, F] are a batch),
 coefficients five steps bring the singular values of m into about 0.7 .. 1.2 and leave its singular vectors: the update
 of a step then moves all directions alike.  float32, bfloat16 or float16; norms are summed in 64 bits, iterates are
 carried in float32, products take float16 operands (of float32 and float16 matrices two parts of each, 22 bits).
-Iterates whose entries pass 16 become infinite or NaN (coefficients that make them grow); a matrix with infinite or NaN
-entries gives NaN and leaves the others alone; a matrix of zeros stays one.  Runs on torch's current stream, can be
-captured into a HIP graph, and needs the GPU: there is no CPU path.  The reference has no counterpart.
+Where entries of X, of A or of b X + c A X pass 16, or those of b A + c A A 64, the result is infinite or NaN (the usual
+coefficients keep all of them below 3; others may make singular values grow past 2).  A matrix with infinite or NaN
+entries gives NaN and leaves the others alone; a matrix of zeros stays one.  A matrix's result has the same bits
+whatever stands beside it.  Runs on torch's current stream, can be captured into a HIP graph, and needs the GPU: there
+is no CPU path.  The reference has no counterpart.
 """
 import math
 
