@@ -65,8 +65,8 @@ class Muon(torch.optim.Optimizer):
         # torch casts a state to its parameter's type, which would round the float32 buffers of 16-bit parameters
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             for p, i in zip(group["params"], saved["params"]):
-                if i in state_dict["state"]:
-                    buf = state_dict["state"][i]["momentum_buffer"]
+                buf = state_dict["state"].get(i, {}).get("momentum_buffer")
+                if buf is not None:
                     self.state[p]["momentum_buffer"] = buf.detach().to(p.device, torch.float32, copy=True)
 
     @torch.no_grad()
