@@ -58,6 +58,7 @@ class Muon(torch.optim.Optimizer):
         super().add_param_group(group)
         for p in self.param_groups[-1]["params"]:
             if p.dim() < 2:
+                del self.param_groups[-1]
                 raise ValueError(f"Muon takes matrices and batches of them, got a parameter {tuple(p.shape)}")
 
     def load_state_dict(self, state_dict):

@@ -1,5 +1,18 @@
 """Muon's parameter groups and saved state (no GPU: nothing is stepped)."""
+import pytest
 import torch
+
+
+def test_a_refused_group_is_not_kept():
+    from mace_onegpu.muon import Muon
+    good, vector = torch.nn.Parameter(torch.zeros(3, 4)), torch.nn.Parameter(torch.zeros(4))
+    opt = Muon([good])
+    for group in (dict(params=[vector]), dict(params=vector), dict(params=[torch.nn.Parameter(torch.zeros(2, 2)), vector])):
+        with pytest.raises(ValueError, match="matrices"):
+            opt.add_param_group(group)
+        assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2, 3, 4))], lr=0.5))
+    assert [g["lr"] for g in opt.param_groups] == [1e-3, 0.5]
 
 
 def test_state_of_parameters_that_had_no_gradient():
