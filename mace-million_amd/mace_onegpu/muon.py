@@ -45,7 +45,8 @@ class Muon(torch.optim.Optimizer):
     The factor gives an update a root mean square of about 0.2, what Adam's has, so that learning rates carry over and
     neither axis has to be the input's.  buf is float32; so is u, but for bfloat16 parameters, to whose type it is rounded
     (of the same range; float16's would overflow, or lose small gradients).  Vectors and scalars belong to another
-    optimizer."""
+    optimizer.  A step may be captured into a HIP graph once every parameter has taken one (RuntimeError before); the
+    graph keeps lr and the other numbers of its capture."""
 
     def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
                  coefficients=COEFFICIENTS, eps=1e-7):
@@ -80,8 +81,11 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                g = p.grad.float()
                 state = self.state[p]
+                if not state and p.is_cuda and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("Muon takes a step before it is captured: a momentum made inside a graph would be "
+                                       "cleared by every replay")
+                g = p.grad.float()
                 if not state:
                     state["momentum_buffer"] = torch.zeros_like(g)
                 buf = state["momentum_buffer"]
