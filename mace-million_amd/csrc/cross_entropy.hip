@@ -2,23 +2,23 @@
 //     l[t, v] = x[t] . W[v],  top[t] = max_v l[t, v],  rest[t] = sum over v != y[t] of exp(l[t, v] - top[t])
 //     s[t] = rest[t] + exp(l[t, y[t]] - top[t]),  loss[t] = top[t] - l[t, y[t]] + log s[t]
 //     d[t, v] = exp(l[t, v] - top[t]) / s[t] - [v = y[t]]:  dx[t] = g[t] d[t] W,  dW = sum_t g[t] d[t]^T x[t]
-// A row that is certain of its class has s = 1 + rest with a small rest: rounding s would leave 2^-24 of 1 in the loss and in
-// d, whatever their size (1.5e-5 of a loss of 0.004).  So the sums leave the target out, and where it is the largest logit,
-// loss = log1p(rest) and its d = -rest / (1 + rest), both as near as the exponentials.
+// A row that is certain of its class has s = 1 + rest with a small rest: rounding s would leave 2^-24 of 1 in the loss
+// and in d, whatever their size (1.5e-5 of a loss of 0.004).  So the sums leave the target out, and where it is the
+// largest logit, loss = log1p(rest) and its d = -rest / (1 + rest), both as near as the exponentials.
 // top and s (or rest) are kept, not log sum exp: its rounding (2^-24 of it) would be a relative error of a whole row of
 // probabilities.  For the same reason backward takes the logits again in the forward's order of sums: few rows by the
 // kernel for few rows, more by tiles.
 // Rows whose target is ignored are taken out at the start: `list` has the asked rows in their order, and everything
-// runs over their number, which stays on the GPU.  (8192 rows, 131,072 classes of 2048 bfloat16 values, both gradients:
-// 16.3 ms, 807 TFLOP/s of the 13.2 T operations.  14,700 rows, 89 classes of 128 float values: 98 us, launches and
-// the six products of small tiles.)
+// runs over their number, which stays on the GPU.  (8192 rows, 131,072 classes of 2048 bfloat16 values, both
+// gradients: 16.5 ms, 800 TFLOP/s of the 13.2 T operations.  14,700 rows, 89 classes of 128 float values: 97 us,
+// launches and the six products of small tiles.)
 // Forward: tiles of logits in registers, of which every row's maximum, sum of exponentials and target's logit go out.
 // Backward: pieces of the vocabulary; the logits of a piece are taken again and become d, stored in 16 bits by rows
 // and transposed, and two products give the piece's part of dx (kept in fp32 over the pieces) and its rows of dW.
 // Bound by the matrix cores: 2 T D V operations forward, 6 T D V backward.
 //
 // Operands (nt.h): 16-bit types as they are; float as three bfloat16 planes (six products, fp32 accuracy).  d is rounded
-// to the type (relative error 2^-9 in bfloat16, 2^-12 in float16, of each of the many terms of dx and dW, as the
+// to the type (relative error 2^-8 in bfloat16, 2^-11 in float16, of each of the many terms of dx and dW, as the
 // operands themselves are); in float16 it is scaled by 2^14 first, so that probabilities down to 2^-28 keep all their
 // bits and none above 2^-39 vanishes.  The incoming gradient g stays out of d in dx (applied in fp32 at the end) and
 // enters the transposed d as g / max|g|.  All sums are fp32 and in a fixed order.
@@ -230,8 +230,8 @@ __device__ __forceinline__ MMCeRow mm_ce_join(MMCeRow a, MMCeRow b) {
   return MMCeRow{top, a.sum * __expf(a.top - top) + b.sum * __expf(b.top - top)};
 }
 
-// Loss of a row whose target's logit is `picked` (bad: target out of range), and what the backward keeps of its sums: s, or
-// -rest where the target is the largest logit (-0 at least: the sign tells the two).
+// Loss of a row whose target's logit is `picked` (bad: target out of range), and what the backward keeps of its sums:
+// s, or -rest where the target is the largest logit (-0 at least: the sign tells the two).
 __device__ __forceinline__ float mm_ce_loss(const MMCeRow& r, float picked, bool bad, float* keep) {
   if (bad) {
     *keep = r.sum;

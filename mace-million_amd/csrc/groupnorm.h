@@ -62,7 +62,7 @@ __device__ __forceinline__ int mm_group_find(const MMGroup& a, long r) {
 
 // Distribution function of the normal distribution, given e = exp(-z^2 / 2).  The tail beyond |z| is e R(|z|), where R is
 // a polynomial in t = 1 / (1 + p |z|), fitted here for the least largest relative error over |z| <= 14 (with fp32's
-// roundings 5.2 x 2^-24; with two terms less 20 x 2^-24, for 16-bit rows, which then round to 2^-12 at best): the tail
+// roundings 5.2 x 2^-24; with two terms less 20 x 2^-24, for 16-bit rows, which then round to 2^-11 at best): the tail
 // keeps its digits however small it is.  With it the activation shares its one exponential with the derivative; erff
 // and expf bound the backward by their instructions (500,000 x 128 bfloat16 values: 309 us with nine terms, 303 with
 // seven).

@@ -5,7 +5,7 @@
 //
 // X is carried in fp32 and a X is added in fp32: small singular values, which grow by a in every step, keep its bits.
 // The products take float16 operands, scaled by powers of two (X and A by 2^12, B = b A + c A A by 2^10) into the middle
-// of its range: one plane for bfloat16 matrices (2^-12 of an operand, against 2^-9 of the result's own rounding), two
+// of its range: one plane for bfloat16 matrices (2^-11 of an operand, against 2^-8 of the result's own rounding), two
 // planes and three products (2^-22) for float and float16.  Entries of X, A and W (of the small matrices, below) have
 // to stay below 16, of B below 64: the norm of M bounds X and A by 1 at first, and the usual coefficients keep all of
 // them below 3; what passes becomes infinite or NaN.  Norms are summed in 64 bits, so that neither large nor tiny

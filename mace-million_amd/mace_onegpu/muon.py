@@ -18,7 +18,7 @@ import torch
 
 from ._ops import ops
 
-COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # as published with this optimizer (K. Jordan and others, 2024)
 
 
 def orthogonalize(m, steps=5, coefficients=COEFFICIENTS, eps=1e-7):

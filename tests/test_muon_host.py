@@ -7,7 +7,8 @@ def test_a_refused_group_is_not_kept():
     from mace_onegpu.muon import Muon
     good, vector = torch.nn.Parameter(torch.zeros(3, 4)), torch.nn.Parameter(torch.zeros(4))
     opt = Muon([good])
-    for group in (dict(params=[vector]), dict(params=vector), dict(params=[torch.nn.Parameter(torch.zeros(2, 2)), vector])):
+    for group in (dict(params=[vector]), dict(params=vector),
+                  dict(params=[torch.nn.Parameter(torch.zeros(2, 2)), vector])):
         with pytest.raises(ValueError, match="matrices"):
             opt.add_param_group(group)
         assert len(opt.param_groups) == 1
